@@ -273,6 +273,30 @@ int kq_mx_linear_mm(int w_fmt, const void* a, int a_dtype, int64_t lda, const vo
                     const uint8_t* w_scale, int64_t m, int64_t n, int64_t k, int out_dtype, void* c,
                     int64_t ldc, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------- products grouped by expert -- */
+
+/* y[r] = W_g x[r] for the rows r of group g, dense 16-bit weights (no kquant
+ * counterpart: its closures loop over experts with F.linear, as
+ * scripts/closure_exl3_layer.py:557-598 does).  dtype: KQ_DT_BF16 or KQ_DT_F16,
+ * of every operand and result.  Group g owns rows [offsets[g], offsets[g + 1])
+ * of x [rows, k] (row stride ldx) and of y [rows, n] (row stride ldy); offsets
+ * (device int64 [groups + 1], not decreasing) are clamped to [0, rows], and
+ * rows of no group are written as zeros.  w [groups, n, k] contiguous.
+ * Products accumulate in fp32 and round once.  n, k and the strides are
+ * multiples of 8 (strides up to 2^22), groups <= 4096; x, w, y 16-byte aligned,
+ * y aliases neither.  Deterministic; no workspace. */
+int kq_grouped_linear(int dtype, const void* x, int64_t ldx, int64_t rows, const int64_t* offsets, int groups,
+                      const void* w, int64_t n, int64_t k, void* y, int64_t ldy, void* stream);
+
+/* dx[r] = W_g^T dy[r], with the same operands (rows of no group: zeros). */
+int kq_grouped_linear_dx(int dtype, const void* dy, int64_t lddy, int64_t rows, const int64_t* offsets, int groups,
+                         const void* w, int64_t n, int64_t k, void* dx, int64_t lddx, void* stream);
+
+/* dw[g] = sum over the group's rows of dy[r] x[r]^T ([groups, n, k]; zeros for
+ * an empty group). */
+int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows,
+                         const int64_t* offsets, int groups, int64_t n, int64_t k, void* dw, void* stream);
+
 /* -------------------------------------------------------------- Hessian -- */
 
 /* acc += X^T diag(w) X for X [n, k] (row stride ld elements, k % 8 == 0,

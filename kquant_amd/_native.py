@@ -9,6 +9,7 @@ on the host (as kquant's CPU helpers do) still run the GPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from collections.abc import Iterable
 
@@ -119,6 +120,9 @@ SIGNATURES: dict[str, list] = {
                            _INT, _VP, _INT, _VP, _I64, _VP, _I64, _VP],
     "kq_qsrt_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _I64, _I64, _INT, _VP, _VP, _VP, _VP, _INT, _VP, _I64,
                        _VP, _I64, _VP],
+    "kq_grouped_linear": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
+    "kq_grouped_linear_dx": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
+    "kq_grouped_linear_dw": [_INT, _VP, _I64, _VP, _I64, _I64, _VP, _INT, _I64, _I64, _VP, _VP],
 }
 QSRT_TRANSPOSED = 1
 LDL_ZERO_DIAGONAL = 1
@@ -202,6 +206,14 @@ def stream_handle(device: torch.device) -> int:
 
 def stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream_handle(device))
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (none needed if it is)."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_gpu() -> torch.device:

@@ -1,0 +1,232 @@
+// Matrix products grouped by expert with ragged sizes: rows sorted by group
+// times that group's dense 16-bit weight, and both gradients.
+//
+//   forward  y[r]  = W_g x[r]                 for the rows r of group g
+//   dx       dx[r] = W_g^T dy[r]
+//   dw       dW_g  = sum over r of dy[r] x[r]^T
+//
+// All three run on the tiles of kq_mm16.h: the weight is read along its rows in
+// the forward pass and across them for dx, and dw contracts over the rows of a
+// group, both operands read across.  Group sizes stay on the device (offsets),
+// so each workgroup numbers the tiles itself: the groups' row tiles are summed
+// in LDS and a tile's group follows from its number.
+#include "kq_internal.h"
+#include "kq_mm16.h"
+
+namespace kq {
+namespace grouped {
+
+constexpr int MAX_GROUPS = 4096;
+enum { FORWARD = 0, DX = 1, DW = 2 };
+
+struct Args {
+  const char* rows_in;    // x (forward), dy (dx, dw)
+  const char* other;      // w, or x (dw)
+  char* out;              // y, dx, dw
+  uint32_t ld_in, ld_other, ld_out;  // bytes
+  const int64_t* offsets;
+  int64_t rows;
+  int groups, n, k;
+};
+
+__shared__ __attribute__((aligned(16))) unsigned char lds[mm16::LDS_BYTES];
+__shared__ int first_tile[MAX_GROUPS + 1];  // forward, dx: tiles before each group
+__shared__ int part_sum[mm16::THREADS];
+
+// Offsets are device data: clamped to the rows there are, so that no value of
+// them reads or writes outside.
+__device__ __forceinline__ int64_t clamped(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+template <int MODE, bool F16>
+struct Problem {
+  Args g;
+  int mtiles, ntiles, tiles;  // dw: of one group
+
+  __device__ __forceinline__ void range(int e, int64_t& beg, int& n) const {
+    beg = clamped(g.offsets[e], 0, g.rows);
+    n = (int)(clamped(g.offsets[e + 1], beg, g.rows) - beg);
+  }
+  __device__ __forceinline__ int total() const { return tiles; }
+
+  // Numbers the tiles; every thread of the workgroup calls it.
+  __device__ __forceinline__ void setup() {
+    const int cols = MODE == FORWARD ? g.n : g.k;
+    ntiles = (cols + mm16::BN - 1) / mm16::BN;
+    mtiles = MODE == DW ? (g.n + mm16::BM - 1) / mm16::BM : 0;
+    if (MODE == DW) {
+      tiles = g.groups * mtiles * ntiles;
+      return;
+    }
+    const int t = threadIdx.x, per = (g.groups + mm16::THREADS - 1) / mm16::THREADS;
+    const int e0 = min(t * per, g.groups), e1 = min(e0 + per, g.groups);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) {
+      int64_t beg;
+      int n;
+      range(e, beg, n);
+      first_tile[e] = sum;
+      sum += (n + mm16::BM - 1) / mm16::BM * ntiles;
+    }
+    part_sum[t] = sum;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < mm16::THREADS; ++i) {
+      const int v = part_sum[i];
+      before += i < t ? v : 0;
+      all += v;
+    }
+    for (int e = e0; e < e1; ++e) first_tile[e] += before;
+    if (t == 0) first_tile[g.groups] = all;
+    __syncthreads();
+    tiles = __builtin_amdgcn_readfirstlane(all);
+  }
+
+  // Group and position of tile t; hint is the group of this caller's last tile.
+  __device__ __forceinline__ void find(int t, int& hint, int& mt, int& nt) const {
+    if (MODE == DW) {
+      const int per = mtiles * ntiles;
+      hint = t / per;
+      mm16::tile_mn(t - hint * per, mtiles, ntiles, mt, nt);
+    } else {
+      int e = hint;
+      while (__builtin_amdgcn_readfirstlane(first_tile[e + 1]) <= t) ++e;
+      hint = e;
+      const int f = __builtin_amdgcn_readfirstlane(first_tile[e]);
+      const int m = (__builtin_amdgcn_readfirstlane(first_tile[e + 1]) - f) / ntiles;
+      mm16::tile_mn(t - f, m, ntiles, mt, nt);
+    }
+  }
+
+  __device__ __forceinline__ mm16::Tile tile(int t, int& hint) const {
+    int mt, nt, n;
+    int64_t beg;
+    find(t, hint, mt, nt);
+    range(hint, beg, n);
+    const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
+    mm16::Tile r;
+    r.a.ld = g.ld_in;
+    r.b.ld = g.ld_other;
+    if (MODE == DW) {
+      r.kc = n;
+      r.rows = min(mm16::BM, g.n - m0);
+      r.a.base = g.rows_in + beg * g.ld_in + 2 * (int64_t)m0;
+      r.a.width = 2u * (uint32_t)(g.n - m0);
+      r.b.base = g.other + beg * g.ld_other + 2 * (int64_t)n0;
+      r.b.width = 2u * (uint32_t)(g.k - n0);
+      r.a.rows = r.b.rows = 0;
+    } else {
+      r.kc = MODE == FORWARD ? g.k : g.n;
+      r.rows = min(mm16::BM, n - m0);
+      r.a.base = g.rows_in + (beg + m0) * g.ld_in;
+      r.a.rows = r.rows;
+      r.a.width = 0;
+      const char* w = g.other + (int64_t)hint * g.n * g.ld_other;
+      if (MODE == FORWARD) {
+        r.b.base = w + (int64_t)n0 * g.ld_other;
+        r.b.rows = min(mm16::BN, g.n - n0);
+        r.b.width = 0;
+      } else {
+        r.b.base = w + 2 * (int64_t)n0;
+        r.b.rows = 0;
+        r.b.width = 2u * (uint32_t)(g.k - n0);
+      }
+    }
+    return r;
+  }
+
+  template <int NB, int WN>
+  __device__ __forceinline__ void epilogue(const mm16::Tile& tl, int t, int hint, int wm, int wn,
+                                           const float16_t (&acc)[NB][WN], int lane) const {
+    int mt, nt, n;
+    int64_t beg;
+    find(t, hint, mt, nt);
+    range(hint, beg, n);
+    const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
+    const int64_t row0 = MODE == DW ? (int64_t)hint * g.n + m0 : beg + m0;
+    mm16::store16<NB, WN, F16>(g.out + row0 * g.ld_out + 2 * (int64_t)n0, g.ld_out, tl.rows,
+                               (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, acc, lane);
+  }
+};
+
+// Rows that belong to no group are zeros.
+__device__ __forceinline__ void zero_rows(const Args& g, int cols) {
+  const int64_t beg = clamped(g.offsets[0], 0, g.rows), end = clamped(g.offsets[g.groups], beg, g.rows);
+  const int64_t before = beg, after = g.rows - end;
+  for (int64_t i = blockIdx.x; i < before + after; i += gridDim.x) {
+    char* p = g.out + (i < before ? i : end + i - before) * g.ld_out;
+    for (int c = (int)threadIdx.x * 8; c < cols; c += mm16::THREADS * 8)
+      *reinterpret_cast<mm16::u32x4_t*>(p + 2 * (int64_t)c) = mm16::u32x4_t{0u, 0u, 0u, 0u};
+  }
+}
+
+template <int MODE, bool F16>
+__global__ __launch_bounds__(mm16::THREADS, 1) void grouped_kernel(Args g) {
+  Problem<MODE, F16> p{g, 0, 0, 0};
+  p.setup();
+  if (MODE != DW) zero_rows(g, MODE == FORWARD ? g.n : g.k);
+  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE != DW, Problem<MODE, F16>> core(p, lds);
+  core.run();
+}
+
+template <int MODE>
+static hipError_t launch(int dtype, const Args& g, hipStream_t st) {
+  int dev = 0, cus = 0;
+  hipError_t e = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
+  if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+  if (e != hipSuccess) return e;
+  const unsigned grid = cus >= 8 ? (unsigned)(cus / 8 * 8) : 8u;
+  if (dtype == KQ_DT_F16) grouped_kernel<MODE, true><<<grid, mm16::THREADS, 0, st>>>(g);
+  else grouped_kernel<MODE, false><<<grid, mm16::THREADS, 0, st>>>(g);
+  return hipGetLastError();
+}
+
+static int check(const char* fn, int dtype, int64_t rows, int groups, int64_t n, int64_t k, int64_t ld_n, int64_t ld_k,
+                 const int64_t* offsets, const void* a, const void* b, const void* c) {
+  if (dtype != KQ_DT_BF16 && dtype != KQ_DT_F16) return kq_fail(KQ_ERR_INVALID, "%s: dtype must be bf16 or f16", fn);
+  if (rows < 0 || groups < 1 || n <= 0 || k <= 0 || n % 8 || k % 8 || ld_n < n || ld_k < k || ld_n % 8 || ld_k % 8)
+    return kq_fail(KQ_ERR_INVALID,
+                   "%s: need groups >= 1, n %% 8 == 0, k %% 8 == 0, row strides of at least n and k, multiples of 8 "
+                   "(rows=%lld groups=%d n=%lld k=%lld strides %lld, %lld)",
+                   fn, (long long)rows, groups, (long long)n, (long long)k, (long long)ld_n, (long long)ld_k);
+  const int64_t tiles_n = (n + 255) / 256, tiles_k = (k + 255) / 256;
+  if (groups > MAX_GROUPS || rows > INT32_MAX / 2 || ld_n > mm16::MAX_LD || ld_k > mm16::MAX_LD ||
+      (int64_t)groups * tiles_n * tiles_k > INT32_MAX / 2 ||
+      (rows / 256 + groups) * (tiles_n > tiles_k ? tiles_n : tiles_k) > INT32_MAX / 2)
+    return kq_fail(KQ_ERR_LIMIT, "%s: at most %d groups, 2^30 rows and tiles, rows of 2^22 elements", fn, MAX_GROUPS);
+  if (!offsets || kq_misaligned(offsets, 8)) return kq_fail(KQ_ERR_INVALID, "%s: offsets must be int64 on the device", fn);
+  if (kq_misaligned(a, 16) || kq_misaligned(b, 16) || kq_misaligned(c, 16))
+    return kq_fail(KQ_ERR_INVALID, "%s: operands must be 16-byte aligned", fn);
+  return KQ_OK;
+}
+
+}  // namespace grouped
+}  // namespace kq
+
+using namespace kq;
+
+extern "C" int kq_grouped_linear(int dtype, const void* x, int64_t ldx, int64_t rows, const int64_t* offsets, int groups,
+                                 const void* w, int64_t n, int64_t k, void* y, int64_t ldy, void* stream) {
+  if (int rc = grouped::check("kq_grouped_linear", dtype, rows, groups, n, k, ldy, ldx, offsets, x, w, y)) return rc;
+  if (rows == 0) return KQ_OK;
+  const grouped::Args g{(const char*)x, (const char*)w, (char*)y, (uint32_t)(2 * ldx), (uint32_t)(2 * k),
+                        (uint32_t)(2 * ldy), offsets, rows, groups, (int)n, (int)k};
+  return kq_check_launch(grouped::launch<grouped::FORWARD>(dtype, g, (hipStream_t)stream), "kq_grouped_linear");
+}
+
+extern "C" int kq_grouped_linear_dx(int dtype, const void* dy, int64_t lddy, int64_t rows, const int64_t* offsets,
+                                    int groups, const void* w, int64_t n, int64_t k, void* dx, int64_t lddx,
+                                    void* stream) {
+  if (int rc = grouped::check("kq_grouped_linear_dx", dtype, rows, groups, n, k, lddy, lddx, offsets, dy, w, dx)) return rc;
+  if (rows == 0) return KQ_OK;
+  const grouped::Args g{(const char*)dy, (const char*)w, (char*)dx, (uint32_t)(2 * lddy), (uint32_t)(2 * k),
+                        (uint32_t)(2 * lddx), offsets, rows, groups, (int)n, (int)k};
+  return kq_check_launch(grouped::launch<grouped::DX>(dtype, g, (hipStream_t)stream), "kq_grouped_linear_dx");
+}
+
+extern "C" int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows,
+                                    const int64_t* offsets, int groups, int64_t n, int64_t k, void* dw, void* stream) {
+  if (int rc = grouped::check("kq_grouped_linear_dw", dtype, rows, groups, n, k, lddy, ldx, offsets, dy, x, dw)) return rc;
+  const grouped::Args g{(const char*)dy, (const char*)x, (char*)dw, (uint32_t)(2 * lddy), (uint32_t)(2 * ldx),
+                        (uint32_t)(2 * k), offsets, rows, groups, (int)n, (int)k};
+  return kq_check_launch(grouped::launch<grouped::DW>(dtype, g, (hipStream_t)stream), "kq_grouped_linear_dw");
+}
