@@ -33,6 +33,10 @@ enum {
 
 /* element formats */
 enum { KQ_FMT_MXFP8_E4M3 = 0, KQ_FMT_MXFP4_E2M1 = 1 };
+/* dense bf16 rows without scales, where an entry point says that it takes them */
+enum { KQ_FMT_BF16 = 2 };
+/* reductions of a loss */
+enum { KQ_LOSS_NONE = 0, KQ_LOSS_MEAN = 1, KQ_LOSS_SUM = 2 };
 /* dense element types */
 enum { KQ_DT_BF16 = 0, KQ_DT_F16 = 1, KQ_DT_F32 = 2 };
 /* flags */
@@ -296,6 +300,43 @@ int kq_grouped_linear_dx(int dtype, const void* dy, int64_t lddy, int64_t rows, 
  * an empty group). */
 int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows,
                          const int64_t* offsets, int groups, int64_t n, int64_t k, void* dw, void* stream);
+
+/* --------------------------------------------------- vocabulary head loss -- */
+
+/* Softmax cross entropy of a vocabulary head without keeping its logits (no
+ * kquant counterpart: the quality measure of a quantized head, and the loss of
+ * its recovery).  With z[t][v] = h_t . w_v in fp32,
+ *   lse[t] = log sum_v exp z[t][v],  losses[t] = lse[t] - z[t][target[t]],
+ * both fp32 [tokens] and 0 where target[t] == ignore_index; a target outside
+ * [0, vocab) gives a NaN loss.  sums: fp32 [2], the losses' sum and their mean
+ * over the counted tokens (NaN if none).
+ * h bf16 [tokens, k] (row stride ldh elements, ldh % 8 == 0).  w_fmt: the head
+ * as KQ_FMT_BF16 [vocab, k] (k % 8 == 0, w_scale NULL), or MXFP8 / MXFP4 rows
+ * with E8M0 scales [vocab, k/32] (k % 64 == 0).  target: device int64.
+ * tokens <= 2^20, vocab <= 2^24, k <= 2^16.  workspace: 256-byte aligned,
+ * uninitialised; it holds the counted rows and 16 bytes per token and 256
+ * vocabulary rows, of an MX head an expanded piece (the size functions plan
+ * for the current device).  Deterministic. */
+int64_t kq_linear_cross_entropy_workspace_size(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, int backward);
+int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
+                            const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target,
+                            int64_t ignore_index, float* losses, float* lse, float* sums, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Its gradients.  grad (fp32, device): one value per token with KQ_LOSS_NONE,
+ * else one value, the gradient of the mean or the sum.  With
+ *   d[t][v] = g_t (exp(z[t][v] - lse[t]) - [v == target[t]]),
+ * g_t zero for ignored tokens: dh = d w (bf16 [tokens, k], row stride lddh, or
+ * NULL) and, for a bf16 head, dw = d^T h (bf16 [vocab, k], or NULL).  lse is
+ * kq_linear_cross_entropy's.  d is formed in fp32 piece by piece of the
+ * vocabulary (at most 1 GiB of it at once) and rounded to bf16 as an operand.
+ * Ignored tokens' rows of h reach nothing; their dh is zero.  Deterministic.
+ * workspace: kq_linear_cross_entropy_workspace_size(..., backward = 1). */
+int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
+                                     const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target,
+                                     int64_t ignore_index, const float* lse, const float* grad, int reduction,
+                                     void* dh, int64_t lddh, void* dw, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
 
 /* -------------------------------------------------------------- Hessian -- */
 

@@ -24,6 +24,10 @@ KQ_ERR_HIP = -2
 KQ_ERR_LIMIT = -3
 FMT_MXFP8_E4M3 = 0
 FMT_MXFP4_E2M1 = 1
+FMT_BF16 = 2
+LOSS_NONE = 0
+LOSS_MEAN = 1
+LOSS_SUM = 2
 DT_BF16 = 0
 DT_F16 = 1
 DT_F32 = 2
@@ -123,6 +127,10 @@ SIGNATURES: dict[str, list] = {
     "kq_grouped_linear": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dx": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dw": [_INT, _VP, _I64, _VP, _I64, _I64, _VP, _INT, _I64, _I64, _VP, _VP],
+    "kq_linear_cross_entropy_workspace_size": [_INT, _I64, _I64, _I64, _INT],
+    "kq_linear_cross_entropy": [_INT, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _VP],
+    "kq_linear_cross_entropy_backward": [_INT, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _INT, _VP,
+                                         _I64, _VP, _VP, _I64, _VP],
 }
 QSRT_TRANSPOSED = 1
 LDL_ZERO_DIAGONAL = 1

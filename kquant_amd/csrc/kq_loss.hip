@@ -1,0 +1,683 @@
+// Softmax cross entropy of a vocabulary head without keeping the logits.
+//
+//   z[t][v] = h_t . w_v          loss_t = lse_t - z[t][y_t],  lse_t = log sum_v exp z[t][v]
+//   d[t][v] = g_t (exp(z[t][v] - lse_t) - [v = y_t])
+//   dh_t = sum_v d[t][v] w_v     dw_v = sum_t d[t][v] h_t
+//
+// What bounds it: the matrix products (2 T V K flop forward, 6 T V K backward,
+// a third of which recomputes z); at few tokens, the head's bytes.  The
+// logits never reach memory in the forward pass: a tile's epilogue reduces its
+// 128 vocabulary rows per wave to a running maximum and a sum of exponentials
+// per token, and picks the target's logit.  The product is taken as W H^T, so
+// a lane holds one token's logits and reduces them in registers.  The
+// backward pass walks the vocabulary in pieces whose gradient d^T (bf16) fits
+// a bounded workspace; a piece recomputes its logits, and its d^T then is an
+// operand of both gradients' products, for dh across its rows and for dw along
+// them.
+//
+// Tokens whose target is ignore_index are left out of every product: the
+// counted rows are first gathered (their number stays on the device), so their
+// values, NaN and Inf among them, reach nothing, and cost nothing.
+//
+// Precision: products of bf16 values are exact and sum in fp32, as do the
+// exponentials, their sums and dh's planes; d is rounded to bf16 to be an
+// operand (half a step, 2^-8 relative, of each term of sums that are themselves
+// rounded to bf16).  Heads in MXFP8 / MXFP4 are expanded piece by piece to bf16,
+// which holds their values exactly.
+#include "kq_internal.h"
+#include "kq_mm16.h"
+
+namespace kq {
+namespace loss {
+
+using mm16::Tile;
+using mm16::u32x4_t;
+
+enum { NONE = 0, MEAN = 1, SUM = 2 };
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+
+__shared__ __attribute__((aligned(16))) unsigned char lds[mm16::LDS_BYTES];
+
+// Counted tokens in order: rows[i] the i-th one's row, place[t] its i or -1.
+__global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict__ target, int64_t ignore_index,
+                                                       int tokens, int* __restrict__ rows, int* __restrict__ place,
+                                                       int* __restrict__ count) {
+  __shared__ int wave_sum[16];
+  constexpr int PER = 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int t0 = 0; t0 < tokens; t0 += 1024 * PER) {
+    const int first = t0 + tid * PER;
+    int mine = 0, keep = 0;
+    for (int q = 0; q < PER; ++q)
+      if (first + q < tokens && target[first + q] != ignore_index) {
+        keep |= 1 << q;
+        ++mine;
+      }
+    int upto = mine;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    if (lane == 63) wave_sum[wave] = upto;
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      before += w < wave ? wave_sum[w] : 0;
+      all += wave_sum[w];
+    }
+    int at = before + upto - mine;
+    for (int q = 0; q < PER; ++q)
+      if (first + q < tokens) {
+        const bool k = keep >> q & 1;
+        place[first + q] = k ? at : -1;
+        if (k) rows[at++] = first + q;
+      }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) *count = base;
+}
+
+struct Gather {
+  const char* h;
+  int64_t ldh;  // bytes
+  const int64_t* target;
+  const int* place;
+  const int* count;
+  int tokens, k;
+  int64_t vocab;
+  char* hc;      // counted rows, then zero rows up to a multiple of 8
+  int* target_c;  // -1 where the target is outside the vocabulary
+  // backward
+  const float* lse;
+  const float* grad;
+  int reduction;
+  float* lse_c;
+  float* g_c;
+  char* dh;
+  int64_t lddh;  // bytes
+};
+
+// One workgroup per token row: a counted one goes to its place, an ignored
+// one's gradient is zero.
+__global__ __launch_bounds__(256) void gather_kernel(Gather g) {
+  const int t = blockIdx.x, count = *g.count;
+  if (t >= g.tokens) {  // the zero rows behind the counted ones
+    const int row = count + t - g.tokens;
+    if (row < (count + 7) / 8 * 8)
+      for (int c = (int)threadIdx.x * 8; c < g.k; c += 2048)
+        *reinterpret_cast<u32x4_t*>(g.hc + ((int64_t)row * g.k + c) * 2) = u32x4_t{0u, 0u, 0u, 0u};
+    return;
+  }
+  const int at = g.place[t];
+  if (at >= 0) {
+    for (int c = (int)threadIdx.x * 8; c < g.k; c += 2048)
+      *reinterpret_cast<u32x4_t*>(g.hc + ((int64_t)at * g.k + c) * 2) =
+          *reinterpret_cast<const u32x4_t*>(g.h + t * g.ldh + 2 * (int64_t)c);
+    if (threadIdx.x == 0) {
+      const int64_t y = g.target[t];
+      const bool ok = y >= 0 && y < g.vocab;
+      g.target_c[at] = ok ? (int)y : -1;
+      if (g.lse_c) {
+        const float up = g.reduction == NONE ? g.grad[t] : g.reduction == MEAN ? g.grad[0] / (float)count : g.grad[0];
+        g.lse_c[at] = g.lse[t];
+        g.g_c[at] = ok ? up : __builtin_nanf("");
+      }
+    }
+  } else if (g.dh) {
+    for (int c = (int)threadIdx.x * 8; c < g.k; c += 2048)
+      *reinterpret_cast<u32x4_t*>(g.dh + t * g.lddh + 2 * (int64_t)c) = u32x4_t{0u, 0u, 0u, 0u};
+  }
+}
+
+// A running (maximum, sum of exp(z - maximum)) joined with another.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2), ref = top == -__builtin_inff() ? 0.0f : top;
+  s = s * __builtin_amdgcn_exp2f((m - ref) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * LOG2E);
+  m = top;
+}
+
+// The logits of a vocabulary piece: W rows [first, first + rows) x counted
+// tokens.  Forward: partial maxima and sums, part[(2 tile + wave row)][token],
+// and the targets' logits.  GRAD: d^T, row stride ldg elements, zero in the
+// token columns from count up to a multiple of 8.
+struct LogitArgs {
+  const char* w;  // bf16 rows of the piece
+  const char* hc;
+  const int* count;
+  const int* target_c;
+  int first, rows, k, tokens;
+  float2_t* part;
+  int part0;  // tiles of the pieces before
+  float* z_target;
+  const float* lse_c;
+  const float* g_c;
+  __bf16* dt;
+  int ldg;
+};
+
+template <bool GRAD>
+struct LogitProblem {
+  LogitArgs g;
+  int count, mtiles, ntiles;
+
+  __device__ __forceinline__ int total() const { return mtiles * ntiles; }
+  __device__ __forceinline__ Tile tile(int t, int&) const {
+    int mt, nt;
+    mm16::tile_mn(t, mtiles, ntiles, mt, nt);
+    const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
+    Tile r;
+    r.kc = g.k;
+    r.rows = min(mm16::BM, g.rows - m0);
+    r.a = {g.w + (int64_t)m0 * g.k * 2, (uint32_t)g.k * 2u, r.rows, 0u};
+    r.b = {g.hc + (int64_t)n0 * g.k * 2, (uint32_t)g.k * 2u, min(mm16::BN, count - n0), 0u};
+    return r;
+  }
+  template <int NB, int WN>
+  __device__ __forceinline__ void epilogue(const Tile& tl, int t, int, int wm, int wn, const float16_t (&acc)[NB][WN],
+                                           int lane) const {
+    int mt, nt;
+    mm16::tile_mn(t, mtiles, ntiles, mt, nt);
+    const int v0 = g.first + mt * mm16::BM, n0 = nt * mm16::BN;
+    if (GRAD) {
+      int tgt[WN];
+      float lse[WN], up[WN];
+#pragma unroll
+      for (int j = 0; j < WN; ++j) {
+        const int c = n0 + wn + 32 * j + (lane & 31);
+        const bool live = c < count;
+        tgt[j] = live ? g.target_c[c] - v0 : -1;
+        lse[j] = live ? g.lse_c[c] : 0.0f;
+        up[j] = live ? g.g_c[c] : 0.0f;
+      }
+      __bf16* out = g.dt + (int64_t)mt * mm16::BM * g.ldg + n0;
+      const int cols = min((count + 7) / 8 * 8 - n0, mm16::BN);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = wm + 4 * (lane >> 5) + 32 * i + 8 * (r >> 2) + (r & 3);
+          if (at < tl.rows) {
+#pragma unroll
+            for (int j = 0; j < WN; ++j) {
+              const int c = wn + 32 * j + (lane & 31);
+              const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
+              if (c < cols) out[(int64_t)at * g.ldg + c] = (__bf16)(n0 + c < count ? up[j] * p : 0.0f);
+            }
+          }
+        }
+      return;
+    }
+    const int row = wm + 4 * (lane >> 5);  // this lane's rows: row + 32 i + 8 (r / 4) + r % 4
+    const bool whole = tl.rows >= wm + 32 * NB;
+#pragma unroll
+    for (int j = 0; j < WN; ++j) {
+      float m = -__builtin_inff(), s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (whole || row + 32 * i + 8 * (r >> 2) + (r & 3) < tl.rows) m = fmaxf(m, acc[i][j][r]);
+      const float ref = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (whole || row + 32 * i + 8 * (r >> 2) + (r & 3) < tl.rows)
+            s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * LOG2E);
+      join(m, s, __shfl_xor(m, 32), __shfl_xor(s, 32));
+      const int c = n0 + wn + 32 * j + (lane & 31);
+      const bool live = c < count;
+      if (live && lane < 32) {
+        float2_t v;
+        v[0] = m;
+        v[1] = s;
+        g.part[(int64_t)(2 * (g.part0 + mt) + (wm >> 7)) * g.tokens + c] = v;
+      }
+      const int at = live ? g.target_c[c] - v0 - row : -1;
+      if (__any(at >= 0 && at < 32 * NB && !(at & 4))) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (at == 32 * i + 8 * (r >> 2) + (r & 3)) g.z_target[c] = acc[i][j][r];
+      }
+    }
+  }
+};
+
+template <bool GRAD>
+__global__ __launch_bounds__(mm16::THREADS, 1) void logit_kernel(LogitArgs g) {
+  LogitProblem<GRAD> p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
+  p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
+  p.ntiles = (p.count + mm16::BN - 1) / mm16::BN;
+  mm16::Core<false, false, false, false, LogitProblem<GRAD>> core(p, lds);
+  core.run();
+}
+
+// dh: d (its transpose, read across) x the piece's rows (read across), the
+// vocabulary cut into slices.  One slice of one piece stores dh itself, at the
+// tokens' own rows; else slices add up in fp32 planes [slice][token][k].
+struct DhArgs {
+  const char* dt;
+  int ldg;
+  const char* w;
+  const int* count;
+  const int* rows_of;
+  int rows, k, slices, tokens;
+  char* dh;  // or null
+  int64_t lddh;  // bytes
+  float* planes;
+  int add;  // to the planes of the pieces before
+};
+
+struct DhProblem {
+  DhArgs g;
+  int count, mtiles, ntiles;
+
+  __device__ __forceinline__ int total() const { return mtiles * ntiles * g.slices; }
+  __device__ __forceinline__ Tile tile(int t, int&) const {
+    int mt, nt;
+    const int per = mtiles * ntiles, sl = t / per;
+    mm16::tile_mn(t - sl * per, mtiles, ntiles, mt, nt);
+    const int m0 = mt * mm16::BM, n0 = nt * mm16::BN, steps = (g.rows + mm16::BK - 1) / mm16::BK;
+    const int v0 = sl * steps / g.slices * mm16::BK;  // slices <= 16, steps <= 2^18
+    const int v1 = min((sl + 1) * steps / g.slices * mm16::BK, g.rows);
+    Tile r;
+    r.kc = v1 - v0;
+    r.rows = min(mm16::BM, count - m0);
+    r.a = {g.dt + ((int64_t)v0 * g.ldg + m0) * 2, (uint32_t)g.ldg * 2u, 0, (uint32_t)((count + 7) / 8 * 8 - m0) * 2u};
+    r.b = {g.w + ((int64_t)v0 * g.k + n0) * 2, (uint32_t)g.k * 2u, 0, (uint32_t)(g.k - n0) * 2u};
+    return r;
+  }
+  template <int NB, int WN>
+  __device__ __forceinline__ void epilogue(const Tile& tl, int t, int, int wm, int wn, const float16_t (&acc)[NB][WN],
+                                           int lane) const {
+    int mt, nt;
+    const int per = mtiles * ntiles, sl = t / per;
+    mm16::tile_mn(t - sl * per, mtiles, ntiles, mt, nt);
+    const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
+    if (g.dh) {
+      const int* map = g.rows_of + m0;
+      char* out = g.dh + 2 * (int64_t)n0;
+      mm16::each(tl.rows, g.k - n0, wm, wn, acc, lane, [&](int r, int c, float v) {
+        *reinterpret_cast<__bf16*>(out + map[r] * g.lddh + 2 * (int64_t)c) = (__bf16)v;
+      });
+    } else {
+      float* out = g.planes + ((int64_t)sl * g.tokens + m0) * g.k + n0;
+      const uint32_t ld = (uint32_t)g.k;
+      if (g.add)
+        mm16::each(tl.rows, g.k - n0, wm, wn, acc, lane,
+                   [&](int r, int c, float v) { out[(uint32_t)r * ld + (uint32_t)c] += v; });
+      else
+        mm16::each(tl.rows, g.k - n0, wm, wn, acc, lane,
+                   [&](int r, int c, float v) { out[(uint32_t)r * ld + (uint32_t)c] = v; });
+    }
+  }
+};
+
+__global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
+  DhProblem p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
+  p.mtiles = (p.count + mm16::BM - 1) / mm16::BM;
+  p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
+  mm16::Core<true, true, false, true, DhProblem> core(p, lds);
+  core.run();
+}
+
+// dh at the tokens' own rows = the sum of the planes, in slice order.
+__global__ __launch_bounds__(256) void dh_sum_kernel(const float* __restrict__ planes, int slices, int tokens, int k,
+                                                     const int* __restrict__ place, char* __restrict__ dh,
+                                                     int64_t lddh) {
+  const int t = blockIdx.x, at = place[t];
+  if (at < 0) return;
+  for (int c = (int)threadIdx.x * 4; c < k; c += 1024) {
+    const float* p = planes + (int64_t)at * k + c;
+    float4_t v = *reinterpret_cast<const float4_t*>(p);
+    for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const float4_t*>(p + (int64_t)s * tokens * k);
+    uint32_t* o = reinterpret_cast<uint32_t*>(dh + t * lddh + 2 * (int64_t)c);
+    o[0] = f32x2_to_bf16x2_bits(v[0], v[1]);
+    o[1] = f32x2_to_bf16x2_bits(v[2], v[3]);
+  }
+}
+
+// dw rows of the piece: d^T (along its rows) x the counted tokens (across).
+struct DwArgs {
+  const char* dt;
+  int ldg;
+  const char* hc;
+  const int* count;
+  int rows, k;
+  char* dw;
+};
+
+struct DwProblem {
+  DwArgs g;
+  int count, mtiles, ntiles;  // count: rounded up to 8, the rows behind it are zero
+
+  __device__ __forceinline__ int total() const { return mtiles * ntiles; }
+  __device__ __forceinline__ Tile tile(int t, int&) const {
+    int mt, nt;
+    mm16::tile_mn(t, mtiles, ntiles, mt, nt);
+    const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
+    Tile r;
+    r.kc = count;
+    r.rows = min(mm16::BM, g.rows - m0);
+    r.a = {g.dt + (int64_t)m0 * g.ldg * 2, (uint32_t)g.ldg * 2u, r.rows, 0u};
+    r.b = {g.hc + (int64_t)n0 * 2, (uint32_t)g.k * 2u, 0, (uint32_t)(g.k - n0) * 2u};
+    return r;
+  }
+  template <int NB, int WN>
+  __device__ __forceinline__ void epilogue(const Tile& tl, int t, int, int wm, int wn, const float16_t (&acc)[NB][WN],
+                                           int lane) const {
+    int mt, nt;
+    mm16::tile_mn(t, mtiles, ntiles, mt, nt);
+    const int n0 = nt * mm16::BN;
+    mm16::store16<NB, WN, false>(g.dw + ((int64_t)mt * mm16::BM * g.k + n0) * 2, (uint32_t)g.k * 2u, tl.rows, g.k - n0,
+                                 wm, wn, acc, lane);
+  }
+};
+
+__global__ __launch_bounds__(mm16::THREADS, 1) void dw_kernel(DwArgs g) {
+  DwProblem p{g, (__builtin_amdgcn_readfirstlane(*g.count) + 7) / 8 * 8, 0, 0};
+  p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
+  p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
+  mm16::Core<false, true, false, false, DwProblem> core(p, lds);
+  core.run();
+}
+
+// lse and loss of every token from its partial maxima and sums (nparts rows of
+// `tokens`), 16 tokens a workgroup; 0 for the ignored ones, NaN where the
+// target is outside the vocabulary.
+__global__ __launch_bounds__(1024) void combine_kernel(const float2_t* __restrict__ part, int nparts, int tokens,
+                                                       const int* __restrict__ place, const int* __restrict__ target_c,
+                                                       const float* __restrict__ z_target, float* __restrict__ losses,
+                                                       float* __restrict__ lse) {
+  __shared__ float ms[64][17], ss[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, t = blockIdx.x * 16 + x;
+  const int at = t < tokens ? place[t] : -1;
+  float m = -__builtin_inff(), s = 0.0f;
+  if (at >= 0)
+    for (int p = y; p < nparts; p += 64) {
+      const float2_t v = part[(int64_t)p * tokens + at];
+      join(m, s, v[0], v[1]);
+    }
+  ms[y][x] = m;
+  ss[y][x] = s;
+  __syncthreads();
+  if (y != 0 || t >= tokens) return;
+  for (int q = 1; q < 64; ++q) join(m, s, ms[q][x], ss[q][x]);
+  const float l = m + LN2 * __builtin_amdgcn_logf(s);
+  lse[t] = at < 0 ? 0.0f : l;
+  losses[t] = at < 0 ? 0.0f : target_c[at] < 0 ? __builtin_nanf("") : l - z_target[at];
+}
+
+// sums[0] = the losses' sum, sums[1] = their mean over the counted tokens (NaN
+// if there are none), added in 64 bits.
+__global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ losses, int tokens,
+                                                   const int* __restrict__ count, float* __restrict__ sums) {
+  __shared__ double red[1024];
+  double s = 0.0;
+  for (int t = threadIdx.x; t < tokens; t += 1024) s += (double)losses[t];
+  red[threadIdx.x] = s;
+  for (int w = 512; w > 0; w >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+  }
+  if (threadIdx.x == 0) {
+    sums[0] = (float)red[0];
+    sums[1] = (float)(red[0] / (double)*count);
+  }
+}
+
+// ------------------------------------------------------------------- host --
+
+constexpr int64_t PIECE_BYTES = 1ll << 30;  // of a piece's d^T, and of its expanded rows
+
+struct Plan {
+  int64_t piece, pieces;       // vocabulary rows
+  int slices;                  // of dh's contraction
+  int64_t ldg;
+  int64_t o_rows, o_place, o_count, o_target, o_lse, o_g, o_z, o_part, o_hc, o_w, o_dt, o_planes, bytes;
+};
+
+static int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backward, int cus) {
+  Plan p{};
+  const bool mx = w_fmt != KQ_FMT_BF16;
+  p.ldg = up(tokens > 0 ? tokens : 1, 8);
+  int64_t most = vocab;
+  if (mx) most = PIECE_BYTES / (2 * k);
+  if (backward && PIECE_BYTES / (2 * p.ldg) < most) most = PIECE_BYTES / (2 * p.ldg);
+  if (most < 1024) most = 1024;
+  most = most / 256 * 256;
+  p.pieces = most >= vocab ? 1 : (vocab + most - 1) / most;
+  p.piece = p.pieces == 1 ? vocab : up((vocab + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (vocab + p.piece - 1) / p.piece;
+  // dh: slices of the vocabulary until its tiles fill the CUs; a slice's plane is written and read once (5 TB/s),
+  // a 64-row step of a tile takes 1.3 us
+  p.slices = 1;
+  if (backward) {
+    const int64_t tiles = ((tokens + 255) / 256) * ((k + 255) / 256), steps = (p.piece + 63) / 64;
+    double best = 1e30;
+    for (int64_t s = 1; s <= 16 && (s == 1 || s * 4 <= steps); ++s) {
+      const double t = (double)((tiles * s + cus - 1) / cus) * (double)((steps + s - 1) / s) * 1.3 +
+                       (s > 1 || p.pieces > 1 ? 5.0 + (double)(s * tokens * k * 8) / 5e6 : 0.0);
+      if (t < best) {
+        best = t;
+        p.slices = (int)s;
+      }
+    }
+  }
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up(bytes, 256);
+    return o;
+  };
+  p.o_rows = take(tokens * 4);
+  p.o_place = take(tokens * 4);
+  p.o_count = take(4);
+  p.o_target = take(tokens * 4);
+  p.o_hc = take(up(tokens, 8) * k * 2);
+  if (mx) p.o_w = take(p.piece * k * 2);
+  if (backward) {
+    p.o_lse = take(tokens * 4);
+    p.o_g = take(tokens * 4);
+    p.o_dt = take(p.piece * p.ldg * 2);
+    if (p.slices > 1 || p.pieces > 1) p.o_planes = take(p.slices * tokens * k * 4);
+  } else {
+    p.o_z = take(tokens * 4);
+    p.o_part = take(2 * p.pieces * ((p.piece + 255) / 256) * tokens * 8);
+  }
+  p.bytes = at;
+  return p;
+}
+
+static hipError_t stream_cus(hipStream_t st, int* cus) {
+  int dev = 0;
+  hipError_t e = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
+  if (e == hipSuccess) e = hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev);
+  return e;
+}
+
+static int check(const char* fn, int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
+                 const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target, int reduction) {
+  const bool mx = w_fmt == KQ_FMT_MXFP8_E4M3 || w_fmt == KQ_FMT_MXFP4_E2M1;
+  if (!mx && w_fmt != KQ_FMT_BF16) return kq_fail(KQ_ERR_INVALID, "%s: unknown head format %d", fn, w_fmt);
+  if (reduction < NONE || reduction > SUM) return kq_fail(KQ_ERR_INVALID, "%s: unknown reduction %d", fn, reduction);
+  if (tokens < 0 || vocab <= 0 || k <= 0 || k % (mx ? 64 : 8) || ldh < k || ldh % 8)
+    return kq_fail(KQ_ERR_INVALID,
+                   "%s: need k %% %d == 0, ldh >= k, ldh %% 8 == 0, vocab >= 1 (tokens=%lld vocab=%lld k=%lld ldh=%lld)", fn,
+                   mx ? 64 : 8, (long long)tokens, (long long)vocab, (long long)k, (long long)ldh);
+  if (tokens > 1 << 20 || vocab > 1 << 24 || k > 1 << 16)
+    return kq_fail(KQ_ERR_LIMIT, "%s: at most 2^20 tokens, 2^24 vocabulary rows and k = 2^16", fn);
+  if (mx && !w_scale) return kq_fail(KQ_ERR_INVALID, "%s: a block-scaled head needs its scales", fn);
+  if (kq_misaligned(h, 16) || kq_misaligned(w, 16) || kq_misaligned(target, 8) || kq_misaligned(w_scale, 2))
+    return kq_fail(KQ_ERR_INVALID, "%s: h and w must be 16-byte aligned", fn);
+  return KQ_OK;
+}
+
+// The piece's rows in bf16: the head's own, or expanded into the workspace.
+static int piece_rows(int w_fmt, const void* w, const uint8_t* w_scale, int64_t first, int64_t rows, int64_t k,
+                      char* expanded, const char** out, void* stream) {
+  if (w_fmt == KQ_FMT_BF16) {
+    *out = (const char*)w + first * k * 2;
+    return KQ_OK;
+  }
+  *out = expanded;
+  const int64_t row = w_fmt == KQ_FMT_MXFP8_E4M3 ? k : k / 2;
+  return kq_mx_dequant(w_fmt, (const char*)w + first * row, w_scale + first * (k / 32), rows, k, KQ_DT_BF16, expanded, 0,
+                       stream);
+}
+
+static unsigned persistent_grid(int cus) { return cus >= 8 ? (unsigned)(cus / 8 * 8) : 8u; }
+
+}  // namespace loss
+}  // namespace kq
+
+using namespace kq;
+
+extern "C" int64_t kq_linear_cross_entropy_workspace_size(int w_fmt, int64_t tokens, int64_t vocab, int64_t k,
+                                                          int backward) {
+  if (tokens < 0 || vocab <= 0 || k <= 0 || tokens > 1 << 20 || vocab > 1 << 24 || k > 1 << 16) return -1;
+  int cus = 0;
+  if (loss::stream_cus(nullptr, &cus) != hipSuccess || cus <= 0) cus = 256;
+  return loss::plan(w_fmt, tokens, vocab, k, backward != 0, cus).bytes;
+}
+
+extern "C" int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
+                                       const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target,
+                                       int64_t ignore_index, float* losses, float* lse, float* sums, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
+  const char* fn = "kq_linear_cross_entropy";
+  if (int rc = loss::check(fn, w_fmt, h, ldh, tokens, w, w_scale, vocab, k, target, loss::NONE)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  int cus = 0;
+  if (int rc = kq_check_launch(loss::stream_cus(st, &cus), fn)) return rc;
+  const loss::Plan p = loss::plan(w_fmt, tokens, vocab, k, false, cus);
+  if (workspace_bytes < p.bytes || kq_misaligned(workspace, 256))
+    return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", fn, (long long)p.bytes);
+  char* ws = (char*)workspace;
+  int* count = (int*)(ws + p.o_count);
+  loss::compact_kernel<<<1, 1024, 0, st>>>(target, ignore_index, (int)tokens, (int*)(ws + p.o_rows),
+                                           (int*)(ws + p.o_place), count);
+  if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+  if (tokens > 0) {
+    loss::Gather g{};
+    g.h = (const char*)h;
+    g.ldh = 2 * ldh;
+    g.target = target;
+    g.place = (int*)(ws + p.o_place);
+    g.count = count;
+    g.tokens = (int)tokens;
+    g.k = (int)k;
+    g.vocab = vocab;
+    g.hc = ws + p.o_hc;
+    g.target_c = (int*)(ws + p.o_target);
+    loss::gather_kernel<<<(unsigned)tokens, 256, 0, st>>>(g);
+    if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+    loss::LogitArgs a{};
+    a.hc = ws + p.o_hc;
+    a.count = count;
+    a.target_c = g.target_c;
+    a.k = (int)k;
+    a.tokens = (int)tokens;
+    a.part = (float2_t*)(ws + p.o_part);
+    a.z_target = (float*)(ws + p.o_z);
+    for (int64_t first = 0; first < vocab; first += p.piece) {
+      a.first = (int)first;
+      a.rows = (int)(vocab - first < p.piece ? vocab - first : p.piece);
+      if (int rc = loss::piece_rows(w_fmt, w, w_scale, first, a.rows, k, ws + p.o_w, &a.w, stream)) return rc;
+      loss::logit_kernel<false><<<loss::persistent_grid(cus), mm16::THREADS, 0, st>>>(a);
+      if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+      a.part0 += (a.rows + mm16::BM - 1) / mm16::BM;
+    }
+    loss::combine_kernel<<<(unsigned)((tokens + 15) / 16), 1024, 0, st>>>(a.part, 2 * a.part0, (int)tokens, g.place,
+                                                                         g.target_c, a.z_target, losses, lse);
+    if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+  }
+  loss::sum_kernel<<<1, 1024, 0, st>>>(losses, (int)tokens, count, sums);
+  return kq_check_launch(hipGetLastError(), fn);
+}
+
+extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
+                                                const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target,
+                                                int64_t ignore_index, const float* lse, const float* grad, int reduction,
+                                                void* dh, int64_t lddh, void* dw, void* workspace,
+                                                int64_t workspace_bytes, void* stream) {
+  const char* fn = "kq_linear_cross_entropy_backward";
+  if (int rc = loss::check(fn, w_fmt, h, ldh, tokens, w, w_scale, vocab, k, target, reduction)) return rc;
+  if (dw && w_fmt != KQ_FMT_BF16) return kq_fail(KQ_ERR_INVALID, "%s: only a bf16 head has a gradient", fn);
+  if (lddh < k || lddh % 8 || kq_misaligned(dh, 16) || kq_misaligned(dw, 16))
+    return kq_fail(KQ_ERR_INVALID, "%s: need lddh >= k, lddh %% 8 == 0, dh and dw 16-byte aligned", fn);
+  hipStream_t st = (hipStream_t)stream;
+  int cus = 0;
+  if (int rc = kq_check_launch(loss::stream_cus(st, &cus), fn)) return rc;
+  const loss::Plan p = loss::plan(w_fmt, tokens, vocab, k, true, cus);
+  if (workspace_bytes < p.bytes || kq_misaligned(workspace, 256))
+    return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", fn, (long long)p.bytes);
+  char* ws = (char*)workspace;
+  int* count = (int*)(ws + p.o_count);
+  loss::compact_kernel<<<1, 1024, 0, st>>>(target, ignore_index, (int)tokens, (int*)(ws + p.o_rows),
+                                           (int*)(ws + p.o_place), count);
+  if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+  if (tokens == 0 && !dw) return KQ_OK;
+  loss::Gather g{};
+  g.h = (const char*)h;
+  g.ldh = 2 * ldh;
+  g.target = target;
+  g.place = (int*)(ws + p.o_place);
+  g.count = count;
+  g.tokens = (int)tokens;
+  g.k = (int)k;
+  g.vocab = vocab;
+  g.hc = ws + p.o_hc;
+  g.target_c = (int*)(ws + p.o_target);
+  g.lse = lse;
+  g.grad = grad;
+  g.reduction = reduction;
+  g.lse_c = (float*)(ws + p.o_lse);
+  g.g_c = (float*)(ws + p.o_g);
+  g.dh = (char*)dh;
+  g.lddh = 2 * lddh;
+  loss::gather_kernel<<<(unsigned)tokens + 8, 256, 0, st>>>(g);
+  if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+  const unsigned grid = loss::persistent_grid(cus);
+  loss::LogitArgs a{};
+  a.hc = g.hc;
+  a.count = count;
+  a.target_c = g.target_c;
+  a.k = (int)k;
+  a.tokens = (int)tokens;
+  a.lse_c = g.lse_c;
+  a.g_c = g.g_c;
+  a.dt = (__bf16*)(ws + p.o_dt);
+  a.ldg = (int)p.ldg;
+  const bool planes = p.slices > 1 || p.pieces > 1;
+  for (int64_t first = 0; first < vocab; first += p.piece) {
+    a.first = (int)first;
+    a.rows = (int)(vocab - first < p.piece ? vocab - first : p.piece);
+    if (int rc = loss::piece_rows(w_fmt, w, w_scale, first, a.rows, k, ws + p.o_w, &a.w, stream)) return rc;
+    loss::logit_kernel<true><<<grid, mm16::THREADS, 0, st>>>(a);
+    if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+    if (dh) {
+      const loss::DhArgs d{(const char*)a.dt, (int)p.ldg, a.w, count, (int*)(ws + p.o_rows), a.rows, (int)k, p.slices,
+                           (int)tokens, planes ? nullptr : (char*)dh, 2 * lddh, (float*)(ws + p.o_planes), first > 0};
+      loss::dh_kernel<<<grid, mm16::THREADS, 0, st>>>(d);
+      if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+    }
+    if (dw) {
+      const loss::DwArgs d{(const char*)a.dt, (int)p.ldg, g.hc, count, a.rows, (int)k, (char*)dw + first * k * 2};
+      loss::dw_kernel<<<grid, mm16::THREADS, 0, st>>>(d);
+      if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+    }
+  }
+  if (dh && planes && tokens > 0) {
+    loss::dh_sum_kernel<<<(unsigned)tokens, 256, 0, st>>>((const float*)(ws + p.o_planes), p.slices, (int)tokens, (int)k,
+                                                         g.place, (char*)dh, 2 * lddh);
+    if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
+  }
+  return KQ_OK;
+}

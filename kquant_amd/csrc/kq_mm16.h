@@ -73,6 +73,17 @@ struct Tile {
   int rows;  // rows of the tile that are stored
 };
 
+// The same in every lane, in scalar registers.
+__device__ __forceinline__ void make_scalar(Operand& o) {
+  const uint64_t a = reinterpret_cast<uint64_t>(o.base);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  o.base = reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
+  o.ld = (uint32_t)__builtin_amdgcn_readfirstlane((int)o.ld);
+  o.rows = __builtin_amdgcn_readfirstlane(o.rows);
+  o.width = (uint32_t)__builtin_amdgcn_readfirstlane((int)o.width);
+}
+
 // Tile tl of an mtiles x ntiles grid, in groups of GROUP_M row tiles.
 __device__ __forceinline__ void tile_mn(int tl, int mtiles, int ntiles, int& mt, int& nt) {
   const int per = GROUP_M * ntiles, g = tl / per, rem = tl - g * per;
@@ -160,29 +171,37 @@ __device__ __forceinline__ float16_t mfma(u32x4_t a, u32x4_t b, float16_t c) {
                                                  0, 0);
 }
 
-// Stores a wave's blocks to out (row stride ld bytes), rows below `rows` and
-// columns below `cols` of the tile, rounded to nearest even.
-template <int NB, int WN, bool F16>
-__device__ __forceinline__ void store16(char* out, uint32_t ld, int rows, int cols, int wm, int wn,
-                                        const float16_t (&acc)[NB][WN], int lane) {
-  const int row = wm + 4 * (lane >> 5), col = wn + (lane & 31);
-  // opaque, so that the offsets of every element are not kept (and spilled) from tile to tile
-  asm volatile("" : "+s"(ld));
+// The elements of a wave's blocks, f(row, column, value) for rows below `rows`
+// and columns below `cols` of the tile.  The row is made opaque, so that the
+// offsets of the elements are not kept (and spilled) from tile to tile.
+template <int NB, int WN, class F>
+__device__ __forceinline__ void each(int rows, int cols, int wm, int wn, const float16_t (&acc)[NB][WN], int lane,
+                                     F&& f) {
+  int row = wm + 4 * (lane >> 5);
+  const int col = wn + (lane & 31);
+  asm volatile("" : "+v"(row));
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int at = row + 32 * i + 8 * (r >> 2) + (r & 3);
       if (at < rows) {
-        const uint32_t off = (uint32_t)at * ld + 2u * (uint32_t)col;
 #pragma unroll
         for (int j = 0; j < WN; ++j)
-          if (col + 32 * j < cols) {
-            if (F16) *reinterpret_cast<_Float16*>(out + off + 64 * j) = (_Float16)acc[i][j][r];
-            else *reinterpret_cast<__bf16*>(out + off + 64 * j) = (__bf16)acc[i][j][r];
-          }
+          if (col + 32 * j < cols) f(at, col + 32 * j, acc[i][j][r]);
       }
     }
+}
+
+// Stores a wave's blocks to out (row stride ld bytes), rounded to nearest even.
+template <int NB, int WN, bool F16>
+__device__ __forceinline__ void store16(char* out, uint32_t ld, int rows, int cols, int wm, int wn,
+                                        const float16_t (&acc)[NB][WN], int lane) {
+  each(rows, cols, wm, wn, acc, lane, [&](int r, int c, float v) {
+    char* q = out + ((uint32_t)r * ld + 2u * (uint32_t)c);
+    if (F16) *reinterpret_cast<_Float16*>(q) = (_Float16)v;
+    else *reinterpret_cast<__bf16*>(q) = (__bf16)v;
+  });
 }
 
 // The tiles of problem P, worker by worker.  P has
@@ -214,6 +233,9 @@ struct Core {
     lk = 0;
     if (lt < p.total()) {
       ld = p.tile(lt, lhint);
+      make_scalar(ld.a);
+      make_scalar(ld.b);
+      ld.kc = __builtin_amdgcn_readfirstlane(ld.kc);
       la.set(ld.a, lw, lane);
       lb.set(ld.b, lw, lane);
     } else {

@@ -1,0 +1,324 @@
+"""Softmax cross entropy of a vocabulary head against its formulas in float64.
+
+Tolerances.  With B[t][v] = sum_k |h| |w| and E = K 2^-24 B an fp32 logit's
+distance from the exact one (exact products, each of at most K additions
+rounds by half a step of a partial sum), a loss is within 2 max_v E, plus what
+the exponentials add: the argument z - m is rounded twice and exp2 and log2
+are within two steps (8 2^-24 (1 + |z - m|) relative to a term, terms of
+|z - m| > 30 being nothing next to the sum), sums of at most 400 additions in a
+row, and the roundings of lse and the loss themselves.  A gradient's term d is
+off by p times that, plus half a bf16 step; its fp32 sum and the result's
+rounding come on top."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from kquant_amd import mxfp4, mxfp8
+from kquant_amd.io import mxfp4 as mxfp4_io
+from kquant_amd.loss import linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+U24, U8 = 2.0 ** -24, 2.0 ** -8
+
+
+def formula(h, w, target, ignore=-100):
+    """losses, their tolerance, and d per unit upstream gradient with its tolerance, in 64 bits."""
+    h, w = h.double(), w.double()
+    counted = target != ignore
+    h = torch.where(counted[:, None], h, torch.zeros_like(h))
+    column = torch.where(counted, target, torch.zeros_like(target))[:, None]
+    z = h @ w.T
+    err = h.shape[1] * U24 * (h.abs() @ w.abs().T).amax(1)
+    lse = torch.logsumexp(z, 1)
+    losses = torch.where(counted, lse - z.gather(1, column)[:, 0], torch.zeros_like(lse))
+    rel = 2 * err + U24 * (8 * 31 + 400)
+    tol = rel + U24 * 4 * (lse.abs() + z.abs().amax(1) + losses.abs())
+    d = torch.exp(z - lse[:, None])
+    dtol = d * (tol + rel)[:, None]
+    d.scatter_add_(1, column, -torch.ones_like(column, dtype=d.dtype))
+    d, dtol = d * counted[:, None], (dtol + 4 * U24) * counted[:, None]
+    return losses, tol, d, dtol
+
+
+def check_sum(got, d, dtol, other):
+    """got bf16 [m, n] against d [m, l] @ other [l, n], d an operand rounded to bf16."""
+    other = other.double()
+    want = d @ other
+    size = d.abs() @ other.abs()
+    tol = dtol @ other.abs() * (1 + U8) + U8 * size + d.shape[1] * U24 * size * (1 + U8)
+    tol = tol + U8 * (want.abs() + tol) + 2.0 ** -126 * (1 + other.abs().sum(0)[None])
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} outside, first at {bad.nonzero()[0].tolist()}"
+
+
+def near(got, want, tol):
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), f"{int(bad.sum())} outside, first {bad.nonzero()[0].tolist()}"
+
+
+def inputs(tokens, vocab, k, gpu, seed=0, ignored=0.2, spread=3.0):
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    h = torch.randn(tokens, k, generator=g, device=gpu).to(torch.bfloat16)
+    w = (torch.randn(vocab, k, generator=g, device=gpu) * (spread / math.sqrt(k))).to(torch.bfloat16)
+    target = torch.randint(0, vocab, (tokens,), generator=g, device=gpu)
+    target[torch.rand(tokens, generator=g, device=gpu) < ignored] = -100
+    return h, w, target
+
+
+def check(h, w, target, values=None, scale=None, reduction="mean", up=None):
+    """values: the head in float64 (w itself by default)."""
+    values = w if values is None else values
+    losses, tol, d, dtol = formula(h, values, target)
+    counted = int((target != -100).sum())
+    dense = scale is None
+    h = h.detach().requires_grad_()
+    w = w.detach().requires_grad_() if dense else w
+    got = linear_cross_entropy(h, w, target, scale, reduction=reduction)
+    assert got.dtype == torch.float32
+    if reduction == "none":
+        near(got.detach(), losses, tol)
+        up = torch.ones_like(got) if up is None else up
+        g = up.double()
+    else:
+        total, ttol = losses.sum(), tol[target != -100].sum()
+        share = 1 / counted if reduction == "mean" else 1.0
+        near(got.detach()[None], total[None] * share, (ttol * share + 2 * U24 * (total.abs() * share + 1))[None])
+        up = torch.ones_like(got) if up is None else up
+        g = (up.double() * share).expand(h.shape[0])
+    grads = torch.autograd.grad(got, (h, w) if dense else (h,), up)
+    d = d * g[:, None]
+    dtol = dtol * g.abs()[:, None] + 4 * U24 * d.abs()
+    check_sum(grads[0], d, dtol, values)
+    if dense:
+        check_sum(grads[1], d.T, dtol.T, torch.where((target != -100)[:, None], h.detach(), torch.zeros_like(h)))
+    return (got.detach(), *grads)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 32, 33, 64, 65, 300])
+@pytest.mark.parametrize("vocab,k", [(1, 8), (7, 72), (256, 64), (257, 264), (1000, 520)])
+def test_sizes(gpu, tokens, vocab, k):
+    h, w, target = inputs(tokens, vocab, k, gpu, seed=tokens)
+    target[-1] = vocab - 1
+    check(h, w, target)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("ignored", [0.0, 0.5, 0.97])
+def test_reductions(gpu, reduction, ignored):
+    h, w, target = inputs(150, 777, 136, gpu, ignored=ignored)
+    target[3] = 5
+    up = torch.randn(150, device=gpu) if reduction == "none" else torch.tensor(-2.5, device=gpu)
+    check(h, w, target, reduction=reduction, up=up)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("tokens,vocab,k", [(1, 100, 64), (5, 1003, 256), (40, 513, 192), (300, 2049, 448)])
+def test_block_scaled_heads(gpu, fmt, tokens, vocab, k):
+    h, w, target = inputs(tokens, vocab, k, gpu)
+    target[0] = vocab - 1
+    if fmt == "mxfp8":
+        q, s = mxfp8.mxfp8_quantize(w)
+        values = mxfp8.mxfp8_dequantize(q, s)
+    else:
+        q, s = mxfp4.mxfp4_quantize(w)
+        values = mxfp4_io.dequant(q, s)
+    check(h, q, target, values=values, scale=s)
+    if fmt == "mxfp8":
+        again = linear_cross_entropy(h, q.view(torch.uint8), target, s)
+        assert torch.equal(again, linear_cross_entropy(h, q, target, s))
+
+
+def test_large_logits(gpu):
+    """Logits of some hundreds, a certain target and an impossible one: no overflow, and losses near 0 and far from it."""
+    h, w, target = inputs(40, 300, 64, gpu, spread=150.0, ignored=0.0)
+    z = h.float() @ w.float().T
+    target[:20] = z.argmax(1)[:20]
+    target[20:] = z.argmin(1)[20:]
+    check(h, w, target, reduction="none")
+
+
+def test_ignored_rows_reach_nothing(gpu):
+    """NaN and Inf in ignored rows change no loss and no gradient; their own gradient is zero."""
+    h, w, target = inputs(90, 500, 72, gpu, ignored=0.4)
+    target[0] = 3
+    want = check(h, w, target)
+    bad = h.clone()
+    gone = target == -100
+    bad[gone] = float("nan")
+    bad[gone.nonzero()[0]] = float("inf")
+    x, y = bad.requires_grad_(), w.clone().requires_grad_()
+    loss = linear_cross_entropy(x, y, target)
+    dh, dw = torch.autograd.grad(loss, (x, y))
+    assert torch.equal(loss.detach(), want[0]) and torch.equal(dh, want[1]) and torch.equal(dw, want[2])
+    assert not dh[gone].any()
+
+
+def test_nothing_counted(gpu):
+    h, w, target = inputs(70, 300, 64, gpu)
+    target[:] = 9
+    for reduction, value in (("mean", math.nan), ("sum", 0.0)):
+        x, y = h.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = linear_cross_entropy(x, y, target, ignore_index=9, reduction=reduction)
+        assert torch.equal(loss.detach().cpu(), torch.tensor(value)) or (loss.isnan() and math.isnan(value))
+        for grad in torch.autograd.grad(loss, (x, y)):
+            assert not grad.any()
+    x, y = h[:0].clone().requires_grad_(), w.clone().requires_grad_()
+    loss = linear_cross_entropy(x, y, target[:0], reduction="none")
+    dh, dw = torch.autograd.grad(loss, (x, y), torch.empty(0, device=gpu))
+    assert loss.shape == (0,) and dh.shape == (0, 64) and not dw.any()
+
+
+def test_target_outside_the_vocabulary(gpu):
+    for tokens in (6, 80):
+        h, w, target = inputs(tokens, 100, 64, gpu, ignored=0.0)
+        clean = linear_cross_entropy(h, w, target, reduction="none")
+        target[2], target[4] = 100, -1
+        losses = linear_cross_entropy(h, w, target, reduction="none")
+        assert losses[[2, 4]].isnan().all()
+        rest = [i for i in range(tokens) if i not in (2, 4)]
+        assert torch.equal(losses[rest], clean[rest])
+
+
+def test_nonfinite_logits(gpu):
+    """A row of NaN makes its own loss NaN; a head row of -inf logits takes no part in the others."""
+    for tokens in (6, 80):
+        h, w, target = inputs(tokens, 300, 64, gpu, ignored=0.0)
+        h[1] = float("nan")
+        losses = linear_cross_entropy(h, w, target, reduction="none")
+        assert losses[1].isnan() and not losses[2:].isnan().any()
+        h, w, target = inputs(tokens, 300, 64, gpu, ignored=0.0)
+        h[:, 0], w[:, 0] = 1.0, 0.0
+        target[target == 7] = 8
+        w[7] = 0.0
+        w[7, 0] = float("-inf")
+        losses = linear_cross_entropy(h, w, target, reduction="none")
+        keep = [v for v in range(300) if v != 7]
+        moved = torch.where(target > 7, target - 1, target)
+        want, tol, _, _ = formula(h, w[keep], moved)
+        near(losses, want, tol)
+
+
+def test_vocabulary_pieces(gpu):
+    """More tokens x vocabulary than one piece of the backward pass holds, and dh summed over pieces."""
+    tokens, vocab, k = 9000, 70001, 64
+    h, w, target = inputs(tokens, vocab, k, gpu, ignored=0.1)
+    x, y = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = linear_cross_entropy(x, y, target, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (x, y))
+    some = torch.arange(0, tokens, 150, device=gpu)
+    losses, tol, d, dtol = formula(h[some], w, target[some])
+    check_sum(dh[some], d, dtol, w)
+    near(linear_cross_entropy(h, w, target, reduction="none")[some], losses, tol)
+    del d, dtol
+    lse = torch.logsumexp((h.double() @ w.double().T), 1)
+    cols = torch.tensor([0, 1, 255, 256, 30000, 59391, 59392, vocab - 1], device=gpu)
+    hd = torch.where((target != -100)[:, None], h, torch.zeros_like(h)).double()
+    z = h.double() @ w[cols].double().T
+    counted = (target != -100)[:, None]
+    p = torch.exp(z - lse[:, None]) * counted
+    d = p - (target[:, None] == cols[None]).double()
+    err = k * U24 * (h.double().abs() @ w.double().abs().T).amax(1)
+    dtol = p * (4 * err[:, None] + U24 * 1400) + 4 * U24 * counted
+    check_sum(dw[cols], d.T, dtol.T, hd)
+
+
+def test_shapes_and_strides(gpu):
+    """[batch, length, K] states as a slice of a wider buffer, a strided target."""
+    h, w, target = inputs(60, 321, 64, gpu)
+    wide = torch.full((4, 15, 100), float("nan"), dtype=torch.bfloat16, device=gpu)
+    wide[..., 8:72] = h.reshape(4, 15, 64)
+    strided = torch.stack([target.reshape(4, 15), torch.zeros(4, 15, dtype=torch.int64, device=gpu)], -1)[..., 0]
+    x = wide.requires_grad_()
+    losses = linear_cross_entropy(x[..., 8:72], w, strided, reduction="none")
+    assert losses.shape == (4, 15)
+    (dx,) = torch.autograd.grad(losses.sum(), x)
+    want = check(h, w, target, reduction="sum")
+    assert torch.equal(losses.reshape(-1).detach(), linear_cross_entropy(h, w, target, reduction="none"))
+    assert torch.equal(dx[..., 8:72].reshape(60, 64), want[1]) and not dx[..., :8].any() and not dx[..., 72:].any()
+
+
+def test_gradient_against_differences(gpu):
+    """Central differences along a direction: the truncation is at most a sixth
+    of the third derivative, itself at most the cube of the spread of the
+    logits' change."""
+    g = torch.Generator(device=gpu).manual_seed(3)
+    h = (torch.randint(-8, 9, (50, 64), generator=g, device=gpu) / 8).to(torch.bfloat16)
+    w = (torch.randint(-8, 9, (200, 64), generator=g, device=gpu) / 16).to(torch.bfloat16)
+    target = torch.randint(0, 200, (50,), generator=g, device=gpu)
+    x, y = h.clone().requires_grad_(), w.clone().requires_grad_()
+    dh, dw = torch.autograd.grad(linear_cross_entropy(x, y, target, reduction="sum"), (x, y))
+    for leaf, grad, which in ((h, dh, 0), (w, dw, 1)):
+        e = (torch.randint(-1, 2, leaf.shape, generator=g, device=gpu) / 64).to(torch.bfloat16)
+        hi, lo = (leaf.float() + e.float()).to(torch.bfloat16), (leaf.float() - e.float()).to(torch.bfloat16)
+        assert torch.equal(hi.float() - lo.float(), 2 * e.float())
+        at = [linear_cross_entropy(*((t, w) if which == 0 else (h, t)), target, reduction="none").double() for t in (hi, lo)]
+        dz = e.double() @ w.double().T if which == 0 else h.double() @ e.double().T
+        spread = dz.amax(1) - dz.amin(1)
+        _, tol, d, dtol = formula(h, w, target)
+        rounded = ((dtol + U8 * d.abs()) * dz.abs()).sum() + U8 * (grad.double().abs() * e.double().abs()).sum()
+        got, want = ((at[0] - at[1]) / 2).sum(), (grad.double() * e.double()).sum()
+        assert (got - want).abs() <= (spread ** 3 / 6).sum() + 2 * tol.sum() + 2 * rounded
+
+
+@pytest.mark.parametrize("tokens", [9, 200])
+def test_repeated_and_captured(gpu, tokens):
+    h, w, target = inputs(tokens, 700, 136, gpu)
+    target[0] = 1
+
+    def step(h, w, target):
+        loss = linear_cross_entropy(h, w, target)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    x, y = h.clone().requires_grad_(), w.clone().requires_grad_()
+    for a, b in zip(step(x, y, target), step(x, y, target)):
+        assert torch.equal(a, b)
+    sx, sy, st = h.clone().requires_grad_(), w.clone().requires_grad_(), target.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(sx, sy, st)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(sx, sy, st)
+    for seed in range(3):
+        nh, _, nt = inputs(tokens, 700, 136, gpu, seed=10 + seed, ignored=0.4 * seed)
+        nt[-1] = 0
+        with torch.no_grad():
+            sx.copy_(nh)
+            st.copy_(nt)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(nh.requires_grad_(), y, nt)):
+            assert torch.equal(a, b)
+
+
+def test_streams(gpu):
+    h, w, target = inputs(300, 900, 136, gpu)
+    _, _, other = inputs(300, 900, 136, gpu, seed=4)
+    want = [linear_cross_entropy(h, w, t, reduction="none") for t in (target, other)]
+    torch.cuda.synchronize()
+    got = []
+    for t in (target, other):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got.append(linear_cross_entropy(h, w, t, reduction="none"))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_cpu_tensors(gpu):
+    h, w, target = inputs(50, 200, 64, gpu)
+    x, y = h.cpu().requires_grad_(), w.cpu().requires_grad_()
+    loss = linear_cross_entropy(x, y, target.cpu())
+    grads = torch.autograd.grad(loss, (x, y))
+    gx, gy = h.clone().requires_grad_(), w.clone().requires_grad_()
+    want = linear_cross_entropy(gx, gy, target)
+    assert loss.device.type == "cpu" and torch.equal(loss.detach(), want.detach().cpu())
+    for a, b in zip(grads, torch.autograd.grad(want, (gx, gy))):
+        assert torch.equal(a, b.cpu())

@@ -1,0 +1,113 @@
+"""Arguments that the grouped products, the head loss and the linears'
+epilogues refuse, before anything reaches a GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from kquant_amd import _native as N
+from kquant_amd.grouped import grouped_linear
+from kquant_amd.loss import linear_cross_entropy
+
+BF16 = torch.bfloat16
+
+
+def bf16(*shape):
+    return torch.zeros(*shape, dtype=BF16)
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(x=torch.zeros(4, 16)), TypeError, "bfloat16 or both float16"),
+    (dict(w=torch.zeros(2, 8, 16, dtype=torch.float16)), TypeError, "both"),
+    (dict(offsets=torch.zeros(3)), TypeError, "int64 or int32"),
+    (dict(x=bf16(4)), ValueError, r"\[rows, K\]"),
+    (dict(w=bf16(8, 16)), ValueError, r"\[groups, N, K\]"),
+    (dict(x=bf16(4, 24)), ValueError, "expects K=16"),
+    (dict(w=bf16(2, 9, 16)), ValueError, "multiples of 8"),
+    (dict(x=bf16(4, 12), w=bf16(2, 8, 12)), ValueError, "multiples of 8"),
+    (dict(w=bf16(2, 0, 16)), ValueError, "multiples of 8"),
+    (dict(w=bf16(0, 8, 16), offsets=torch.zeros(1, dtype=torch.int64)), ValueError, "groups=0"),
+    (dict(w=bf16(4097, 8, 16), offsets=torch.zeros(4098, dtype=torch.int64)), ValueError, "groups=4097"),
+    (dict(offsets=torch.zeros(2, dtype=torch.int64)), ValueError, "offsets shape"),
+])
+def test_grouped_linear(change, error, text):
+    args = dict(x=bf16(4, 16), w=bf16(2, 8, 16), offsets=torch.zeros(3, dtype=torch.int64)) | change
+    with pytest.raises(error, match=text):
+        grouped_linear(args["x"], args["w"], args["offsets"])
+
+
+def test_grouped_c_entries():
+    lib = N.library()
+    p = ctypes.c_void_p(256)  # never read: validation fails first
+    ok = [N.DT_BF16, p, 64, 10, p, 3, p, 32, 64, p, 32, None]
+    for at, value, text in ((0, N.DT_F32, b"bf16 or f16"), (2, 56, b"strides"), (2, 68, b"multiples of 8"), (3, -1, b"groups"),
+                            (5, 0, b"groups >= 1"), (7, 30, b"n % 8"), (8, 60, b"k % 8"), (10, 24, b"strides"),
+                            (4, None, b"offsets"), (1, ctypes.c_void_p(264), b"16-byte"), (6, ctypes.c_void_p(8), b"16-byte"),
+                            (9, ctypes.c_void_p(2), b"16-byte")):
+        args = list(ok)
+        args[at] = value
+        assert lib.kq_grouped_linear(*args) == N.KQ_ERR_INVALID and text in lib.kq_last_error(), (at, lib.kq_last_error())
+    for at, value in ((5, 4097), (2, 1 << 23), (3, 1 << 31)):
+        args = list(ok)
+        args[at] = value
+        assert lib.kq_grouped_linear(*args) == N.KQ_ERR_LIMIT
+    dx = list(ok)
+    dx[2], dx[10] = 24, 64
+    assert lib.kq_grouped_linear_dx(*dx) == N.KQ_ERR_INVALID
+    dw = [N.DT_BF16, p, 32, p, 24, 10, p, 3, 32, 64, p, None]
+    assert lib.kq_grouped_linear_dw(*dw) == N.KQ_ERR_INVALID and b"strides" in lib.kq_last_error()
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(reduction="max"), ValueError, "reduction"),
+    (dict(h=torch.zeros(4, 64)), TypeError, "hidden must be bfloat16"),
+    (dict(h=torch.zeros(4, 64, dtype=torch.float16)), TypeError, "hidden must be bfloat16"),
+    (dict(target=torch.zeros(4, dtype=torch.int32)), TypeError, "int64"),
+    (dict(target=torch.zeros(5, dtype=torch.int64)), ValueError, "target shape"),
+    (dict(w=torch.zeros(9, 64)), TypeError, "without scales must be bfloat16"),
+    (dict(w=bf16(9, 32)), ValueError, "does not match K=64"),
+    (dict(w=bf16(0, 64)), ValueError, "does not match"),
+    (dict(w=bf16(64)), ValueError, r"\[V, K\]"),
+    (dict(h=bf16(4, 60), w=bf16(9, 60)), ValueError, "multiple of 8"),
+    (dict(scale=torch.zeros(9, 2, dtype=torch.uint8)), TypeError, "block-scaled head"),
+    (dict(w=torch.zeros(9, 64, dtype=torch.uint8), scale=torch.zeros(9, 2)), TypeError, "E8M0"),
+    (dict(w=torch.zeros(9, 64, dtype=torch.uint8), scale=torch.zeros(9, 3, dtype=torch.uint8)), ValueError, "scale shape"),
+    (dict(w=torch.zeros(9, 48, dtype=torch.uint8), scale=torch.zeros(9, 2, dtype=torch.uint8)), ValueError, "does not match"),
+    (dict(h=bf16(4, 32), w=torch.zeros(9, 32, dtype=torch.uint8), scale=torch.zeros(9, 1, dtype=torch.uint8)), ValueError,
+     "multiple of 64"),
+])
+def test_linear_cross_entropy(change, error, text):
+    args = dict(h=bf16(4, 64), w=bf16(9, 64), target=torch.zeros(4, dtype=torch.int64), scale=None, reduction="mean") | change
+    with pytest.raises(error, match=text):
+        linear_cross_entropy(args["h"], args["w"], args["target"], args["scale"], reduction=args["reduction"])
+
+
+def test_loss_c_entries():
+    lib = N.library()
+    p = ctypes.c_void_p(256)
+    ok = [N.FMT_BF16, p, 64, 10, p, None, 99, 64, p, -100, p, p, p, p, 1 << 30, None]
+    for at, value, text in ((0, 7, b"head format"), (2, 56, b"ldh >= k"), (2, 68, b"ldh % 8"), (3, -1, b"tokens=-1"),
+                            (6, 0, b"vocab >= 1"), (7, 60, b"k % 8"), (1, ctypes.c_void_p(264), b"16-byte"),
+                            (0, N.FMT_MXFP8_E4M3, b"needs its scales")):
+        args = list(ok)
+        args[at] = value
+        assert lib.kq_linear_cross_entropy(*args) == N.KQ_ERR_INVALID and text in lib.kq_last_error(), (at, lib.kq_last_error())
+    for at, value in ((3, (1 << 20) + 1), (6, (1 << 24) + 1)):
+        args = list(ok)
+        args[at] = value
+        assert lib.kq_linear_cross_entropy(*args) == N.KQ_ERR_LIMIT
+    back = [N.FMT_MXFP8_E4M3, p, 64, 10, p, p, 99, 64, p, -100, p, p, N.LOSS_MEAN, p, 64, p, p, 1 << 30, None]
+    assert lib.kq_linear_cross_entropy_backward(*back) == N.KQ_ERR_INVALID and b"only a bf16 head" in lib.kq_last_error()
+    back[0], back[5], back[12] = N.FMT_BF16, None, 3
+    assert lib.kq_linear_cross_entropy_backward(*back) == N.KQ_ERR_INVALID and b"reduction" in lib.kq_last_error()
+    back[12], back[14] = N.LOSS_SUM, 56
+    assert lib.kq_linear_cross_entropy_backward(*back) == N.KQ_ERR_INVALID and b"lddh" in lib.kq_last_error()
+    size = lib.kq_linear_cross_entropy_workspace_size
+    assert size(N.FMT_BF16, -1, 10, 64, 0) == -1 and size(N.FMT_BF16, 10, 0, 64, 0) == -1
+    assert size(N.FMT_BF16, 0, 10, 64, 0) > 0 and size(N.FMT_BF16, 0, 10, 64, 1) > 0
+    # no [tokens, vocabulary] array forward; at most 1 GiB of it backward
+    assert size(N.FMT_BF16, 4096, 131072, 4096, 0) < 4096 * 131072 // 4
+    assert size(N.FMT_BF16, 16384, 131072, 64, 1) < (1 << 30) + (1 << 28)
