@@ -35,6 +35,9 @@ enum {
 enum { KQ_FMT_MXFP8_E4M3 = 0, KQ_FMT_MXFP4_E2M1 = 1 };
 /* dense bf16 rows without scales, where an entry point says that it takes them */
 enum { KQ_FMT_BF16 = 2 };
+/* activations of a linear's epilogue: max(x, 0), x sigmoid(x), x Phi(x) and
+   its tanh form x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 */
+enum { KQ_LIN_NONE = 0, KQ_LIN_RELU = 1, KQ_LIN_SILU = 2, KQ_LIN_GELU = 3, KQ_LIN_GELU_TANH = 4 };
 /* reductions of a loss */
 enum { KQ_LOSS_NONE = 0, KQ_LOSS_MEAN = 1, KQ_LOSS_SUM = 2 };
 /* dense element types */
@@ -276,6 +279,20 @@ int64_t kq_mx_linear_mm_workspace_size(int64_t m, int64_t n, int64_t k);
 int kq_mx_linear_mm(int w_fmt, const void* a, int a_dtype, int64_t lda, const void* w_q,
                     const uint8_t* w_scale, int64_t m, int64_t n, int64_t k, int out_dtype, void* c,
                     int64_t ldc, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* kq_mx_linear_ws (a_dtype KQ_DT_BF16) or kq_mx_linear_f32 (KQ_DT_F32, out_dtype
+ * KQ_DT_F32) with an epilogue on the fp32 accumulators, rounded once:
+ *   C = activation(A dequant(W)^T + bias) + residual
+ * (no kquant counterpart: its closures apply them as torch ops on the linear's
+ * rounded result).  activation: KQ_LIN_*.  bias: [n] bf16 or f32 (bias_dtype),
+ * or NULL.  residual: [m, n] of out_dtype, row stride ldr >= n, or NULL; it may
+ * be c itself (ldr == ldc), and aliases nothing else.  The erf of the
+ * exact GELU is within 1.5e-7 (Abramowitz and Stegun 7.1.26).  Other arguments
+ * and the workspace are those of the entry point it extends. */
+int kq_mx_linear_epilogue(int w_fmt, int a_dtype, const void* a, int64_t lda, const void* w_q, const uint8_t* w_scale,
+                          int64_t m, int64_t n, int64_t k, int activation, const void* bias, int bias_dtype,
+                          const void* residual, int64_t ldr, int out_dtype, void* c, int64_t ldc, void* workspace,
+                          int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------- products grouped by expert -- */
 

@@ -25,6 +25,7 @@ KQ_ERR_LIMIT = -3
 FMT_MXFP8_E4M3 = 0
 FMT_MXFP4_E2M1 = 1
 FMT_BF16 = 2
+LIN_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 LOSS_NONE = 0
 LOSS_MEAN = 1
 LOSS_SUM = 2
@@ -124,6 +125,8 @@ SIGNATURES: dict[str, list] = {
                            _INT, _VP, _INT, _VP, _I64, _VP, _I64, _VP],
     "kq_qsrt_linear": [_VP, _INT, _I64, _I64, _VP, _I64, _I64, _I64, _INT, _VP, _VP, _VP, _VP, _INT, _VP, _I64,
                        _VP, _I64, _VP],
+    "kq_mx_linear_epilogue": [_INT, _INT, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _INT, _VP, _INT, _VP, _I64, _INT, _VP,
+                              _I64, _VP, _I64, _VP],
     "kq_grouped_linear": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dx": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dw": [_INT, _VP, _I64, _VP, _I64, _I64, _VP, _INT, _I64, _I64, _VP, _VP],

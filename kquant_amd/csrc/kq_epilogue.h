@@ -1,0 +1,86 @@
+// The linear's epilogue: c = act(x W^T + bias) + residual, in fp32 on the
+// accumulated product and rounded once.
+//
+// The activations fall in three classes, so that a kernel whose epilogue is
+// unrolled over its accumulators needs three forms and no branch per element:
+//   none, relu       x below `low` becomes `low` (-inf or 0; NaN stays)
+//   silu, gelu_tanh  x sigmoid(x (c1 + c3 x^2)): c = (1, 0), or (2 sqrt(2/pi),
+//                    0.044715 times that), since (1 + tanh u) / 2 = sigmoid(2u)
+//   gelu             x Phi(x), Phi by the rational-exponential approximation of
+//                    Abramowitz and Stegun 7.1.26 for erf (|error| <= 1.5e-7)
+#pragma once
+
+#include "kq_act.h"
+#include "kq_common.h"
+
+namespace kq {
+
+enum { EPI_OFF = 0, EPI_CLAMP = 1, EPI_SIGMOID = 2, EPI_ERF = 3 };
+
+struct Epilogue {
+  int kind;              // EPI_*
+  float low, c1, c3;
+  const void* bias;      // [n] or null
+  int bias_f32;
+  const void* residual;  // [m, n] of the output's type, or null
+  int64_t ldr;
+};
+
+template <int KIND>
+__device__ __forceinline__ float epi_activate(const Epilogue& e, float x) {
+  if (KIND == EPI_CLAMP) return x < e.low ? e.low : x;
+  // arguments end where the sigmoid is 0 or 1 and the exponential 0: exp_act of an infinity is NaN
+  if (KIND == EPI_SIGMOID) {
+    const float s = x * fmaf(e.c3, fminf(x * x, 1e30f), e.c1);
+    return x * sigmoid_act(fminf(fmaxf(s, -200.0f), 200.0f));
+  }
+  if (KIND == EPI_ERF) {
+    const float a = fabsf(x) * 0.70710678f;
+    const float t = rcp_act(fmaf(0.3275911f, a, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float tail = 0.5f * p * t * exp_act(-fminf(a * a, 200.0f));  // (1 - erf(|x| / sqrt 2)) / 2
+    return x * (x < 0.0f ? tail : 1.0f - tail);
+  }
+  return x;
+}
+
+// the class decided at run time
+__device__ __forceinline__ float epi_activate_any(const Epilogue& e, float x) {
+  return e.kind == EPI_SIGMOID ? epi_activate<EPI_SIGMOID>(e, x)
+         : e.kind == EPI_ERF   ? epi_activate<EPI_ERF>(e, x)
+                               : epi_activate<EPI_CLAMP>(e, x);
+}
+
+__device__ __forceinline__ float epi_bias(const Epilogue& e, int64_t n) {
+  if (!e.bias) return 0.0f;
+  return e.bias_f32 ? static_cast<const float*>(e.bias)[n]
+                    : bf16_bits_to_f32(static_cast<const uint16_t*>(e.bias)[n]);
+}
+
+// OUT: KQ_DT_BF16 or KQ_DT_F32, the output's and so the residual's type.
+template <int OUT>
+__device__ __forceinline__ float epi_residual(const Epilogue& e, int64_t m, int64_t n) {
+  if (!e.residual) return 0.0f;
+  const int64_t at = m * e.ldr + n;
+  return OUT == KQ_DT_F32 ? static_cast<const float*>(e.residual)[at]
+                          : bf16_bits_to_f32(static_cast<const uint16_t*>(e.residual)[at]);
+}
+
+// The value at (m, n) of the matrix from its accumulated product.
+template <int OUT>
+__device__ __forceinline__ float epi_apply(const Epilogue& e, float x, int64_t m, int64_t n) {
+  return epi_activate_any(e, x + epi_bias(e, n)) + epi_residual<OUT>(e, m, n);
+}
+
+// The epilogue of the rows from m0 and the columns from n0 on.
+template <int OUT>
+static inline Epilogue epi_at(Epilogue e, int64_t m0, int64_t n0) {
+  if (e.bias) e.bias = static_cast<const char*>(e.bias) + n0 * (e.bias_f32 ? 4 : 2);
+  if (e.residual) e.residual = static_cast<const char*>(e.residual) + (m0 * e.ldr + n0) * (OUT == KQ_DT_F32 ? 4 : 2);
+  return e;
+}
+
+}  // namespace kq

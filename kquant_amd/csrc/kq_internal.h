@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/kquant_amd.h"
+#include "kq_epilogue.h"
 
 // Record a printf-style message as this thread's last error and return code.
 int kq_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
@@ -70,6 +71,7 @@ struct SkinnyArgs {
   void* c;
   int64_t ldc;
   int m, n, k;
+  Epilogue epi = {};  // bf16 and fp32 rows
 };
 hipError_t mx_skinny_bf16(int fmt, bool out_f32, const SkinnyArgs& args, hipStream_t st);
 hipError_t mx_skinny_f32(int fmt, const SkinnyArgs& args, hipStream_t st);

@@ -10,8 +10,11 @@
 // K step 64, LDS double buffered.  Weights are staged in LDS still packed
 // (E4M3: 64 B per row and step, E2M1: 32 B) and expanded to bf16 per fragment.
 #include "kq_dma.h"
+#include "kq_epilogue.h"
 #include "kq_gemm.h"
 #include "kq_internal.h"
+
+#include <type_traits>
 
 namespace kq {
 
@@ -30,10 +33,11 @@ using gemm::bf16x8_t;
 using gemm::u32x2_t;
 using gemm::u32x4_t;
 
-template <int FMT, int OUT, bool SPLIT>
+template <int FMT, int OUT, bool SPLIT, bool EPI = false>
 __global__ __launch_bounds__(512, 1) void mx_linear_kernel(
     const uint16_t* __restrict__ a, int64_t lda, const uint8_t* __restrict__ wq,
-    const uint8_t* __restrict__ ws, void* __restrict__ c, int64_t ldc, int M, int N, int K, int KB, int64_t plane) {
+    const uint8_t* __restrict__ ws, void* __restrict__ c, int64_t ldc, int M, int N, int K, int KB, int64_t plane,
+    Epilogue epi) {
   using namespace lin;
   constexpr int BROW = b_row<FMT>();
   constexpr int WBYTES = FMT == 0 ? BK : BK / 2;  // packed bytes per row per step
@@ -165,6 +169,7 @@ __global__ __launch_bounds__(512, 1) void mx_linear_kernel(
         const int gm = m0 + wm + i * 32 + 8 * (r >> 2) + 4 * fk + (r & 3);
         const int gn = n0 + wn + j * 32 + frow;
         if (gm < M && gn < N) {
+          if (EPI) acc[i][j][r] = epi_apply<OUT>(epi, acc[i][j][r], gm, gn);
           if (OUT == 2) static_cast<float*>(c)[z * plane + (int64_t)gm * ldc + gn] = acc[i][j][r];
           else static_cast<__bf16*>(c)[(int64_t)gm * ldc + gn] = (__bf16)acc[i][j][r];
         }
@@ -211,6 +216,10 @@ __global__ __launch_bounds__(512, 1) void mx_linear_kernel(
 //    [s steps / slices, (s + 1) steps / slices) of tile t into plane s of c
 //    (c + s plane); the caller sums the planes.  Needs slices <= steps.
 //  * UNIT: every E8M0 scale is 127 (x 1); no scale array is read.
+//  * EPI: the epilogue's class (kq_epilogue.h), EPI_OFF none.  It runs on the
+//    accumulators before they are stored; a 32-row block's 64 residual values
+//    are all loaded before the first is used, since nothing else runs on the
+//    SIMD meanwhile.
 namespace lin3 {
 constexpr int NSTAGE = 3;
 constexpr int A_BYTES = lin::BM * lin::BK * 2;                      // 32 KiB
@@ -231,11 +240,11 @@ __device__ __forceinline__ void tile_mn(int tl, int mtiles, int ntiles, int& mt,
 
 __shared__ __attribute__((aligned(16))) unsigned char lin3_lds[lin3::NSTAGE * lin3::stage<0>()];
 
-template <int FMT, int OUT, bool UNIT = false>
+template <int FMT, int OUT, bool UNIT = false, int EPI = EPI_OFF>
 __global__ __launch_bounds__(256, 1) void mx_linear_dma_kernel(
     const uint16_t* __restrict__ a, int64_t lda, uint32_t a_bytes, const uint8_t* __restrict__ wq,
     const uint8_t* __restrict__ ws, uint32_t w_bytes, uint32_t s_bytes, void* __restrict__ c,
-    int64_t ldc, int M, int N, int K, int KB, int slices, int64_t plane) {
+    int64_t ldc, int M, int N, int K, int KB, int slices, int64_t plane, Epilogue epi) {
   using namespace lin3;
   using dma::i32x4_t;
   constexpr int WQ = FMT == 0 ? 4 : 2;  // weight loads per wave per stage
@@ -489,7 +498,47 @@ __global__ __launch_bounds__(256, 1) void mx_linear_dma_kernel(
       cslot = nslot;
     }
 
-    if (active) {
+    if (EPI != EPI_OFF && active) {
+      float bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bias[j] = epi_bias(epi, min(n0 + wn + j * 32 + frow, N - 1));
+      using out_t = typename std::conditional<OUT == 2, float, __bf16>::type;
+      out_t* ct = static_cast<out_t*>(c) + (int64_t)(m0 + wm) * ldc + n0 + wn;
+      const out_t* rt = epi.residual ? static_cast<const out_t*>(epi.residual) + (int64_t)(m0 + wm) * epi.ldr + n0 + wn
+                                     : nullptr;
+      const int rows = M - m0 - wm, cols = N - n0 - wn;  // of this wave's part
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // opaque: the offsets of a block are made when it is stored, not kept through the K loop
+        int row = i * 32 + 4 * f, col = frow;
+        asm volatile("" : "+v"(row), "+v"(col));
+        float res[16][4];
+        if (rt) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const out_t* p = rt + min(row + 8 * (r >> 2) + (r & 3), rows - 1) * epi.ldr;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) res[r][j] = (float)p[min(col + j * 32, cols - 1)];
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) res[r][j] = 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = row + 8 * (r >> 2) + (r & 3);
+          out_t* p = ct + at * ldc;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = epi_activate<EPI>(epi, acc[i][j][r] + bias[j]) + res[r][j];
+            if (at < rows && col + j * 32 < cols) p[col + j * 32] = (out_t)v;
+          }
+        }
+      }
+    }
+    if (EPI == EPI_OFF && active) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -781,9 +830,10 @@ __global__ __launch_bounds__(256) void scale_dwords_t_kernel(const uint32_t* __r
 
 // C = the sum of the K slices' fp32 planes [slices][m, ldp] in slice order,
 // four columns (ldp % 4 == 0) per thread.
-template <int OUT>
+template <int OUT, bool EPI = false>
 __global__ __launch_bounds__(256) void plane_sum_kernel(const float* __restrict__ planes, int slices, int64_t plane,
-                                                        int ldp, int m, int n, void* __restrict__ c, int64_t ldc) {
+                                                        int ldp, int m, int n, void* __restrict__ c, int64_t ldc,
+                                                        Epilogue epi) {
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per_row = ldp / 4;
   const int64_t row = q / per_row;
@@ -792,6 +842,11 @@ __global__ __launch_bounds__(256) void plane_sum_kernel(const float* __restrict_
   const float* p = planes + row * ldp + col;
   float4_t v = *reinterpret_cast<const float4_t*>(p);
   for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const float4_t*>(p + s * plane);
+  if (EPI) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < n) v[j] = epi_apply<OUT>(epi, v[j], row, col + j);
+  }
   const int64_t at = row * ldc + col;
   if (col + 4 <= n && (reinterpret_cast<uintptr_t>(c) + at * (OUT == 2 ? 4 : 2)) % (OUT == 2 ? 16 : 8) == 0) {
     if (OUT == 2) *reinterpret_cast<float4_t*>(static_cast<float*>(c) + at) = v;
@@ -901,10 +956,11 @@ static hipError_t stream_cus(hipStream_t st, int* cus) {
 
 template <int OUT>
 static hipError_t sum_planes(const SplitPlan& p, const void* planes, int m, int n, void* c, int64_t ldc,
-                             hipStream_t st) {
+                             hipStream_t st, const Epilogue& epi = Epilogue{}) {
   const int64_t quads = m * (p.ldp / 4);
-  plane_sum_kernel<OUT><<<(unsigned)((quads + 255) / 256), 256, 0, st>>>(
-      static_cast<const float*>(planes), p.slices, p.plane, (int)p.ldp, m, n, c, ldc);
+  auto kern = epi.kind == EPI_OFF ? plane_sum_kernel<OUT, false> : plane_sum_kernel<OUT, true>;
+  kern<<<(unsigned)((quads + 255) / 256), 256, 0, st>>>(static_cast<const float*>(planes), p.slices, p.plane, (int)p.ldp,
+                                                        m, n, c, ldc, epi);
   return hipGetLastError();
 }
 
@@ -914,7 +970,8 @@ static hipError_t sum_planes(const SplitPlan& p, const void* planes, int m, int 
 template <int FMT, int OUT, bool UNIT = false>
 static hipError_t launch_linear_dma(const uint16_t* a, int64_t lda, const uint8_t* wq,
                                     const uint8_t* ws, void* c, int64_t ldc, int M, int N, int K,
-                                    int KB, hipStream_t st, int slices = 1, int64_t plane = 0) {
+                                    int KB, hipStream_t st, int slices = 1, int64_t plane = 0,
+                                    const Epilogue& epi = Epilogue{}) {
   int dev = 0, cus = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
@@ -931,9 +988,15 @@ static hipError_t launch_linear_dma(const uint16_t* a, int64_t lda, const uint8_
       if (grid > (tiles + 7) / 8 * 8) grid = (tiles + 7) / 8 * 8;
       void* cp = OUT == 2 ? (void*)(static_cast<float*>(c) + m0 * ldc + n0)
                           : (void*)(static_cast<uint16_t*>(c) + m0 * ldc + n0);
-      mx_linear_dma_kernel<FMT, OUT, UNIT><<<grid, 256, 0, st>>>(
-          a + m0 * lda, lda, (uint32_t)(mc * lda * 2), wq + n0 * kw, ws + n0 * ks,
-          (uint32_t)(nc * kw), (uint32_t)(nc * ks), cp, ldc, mc, nc, K, KB, slices, plane);
+      auto kern = mx_linear_dma_kernel<FMT, OUT, UNIT>;
+      if constexpr (!UNIT) {
+        if (epi.kind == EPI_CLAMP) kern = mx_linear_dma_kernel<FMT, OUT, false, EPI_CLAMP>;
+        if (epi.kind == EPI_SIGMOID) kern = mx_linear_dma_kernel<FMT, OUT, false, EPI_SIGMOID>;
+        if (epi.kind == EPI_ERF) kern = mx_linear_dma_kernel<FMT, OUT, false, EPI_ERF>;
+      }
+      kern<<<grid, 256, 0, st>>>(a + m0 * lda, lda, (uint32_t)(mc * lda * 2), wq + n0 * kw, ws + n0 * ks,
+                                 (uint32_t)(nc * kw), (uint32_t)(nc * ks), cp, ldc, mc, nc, K, KB, slices, plane,
+                                 epi_at<OUT>(epi, m0, n0));
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
   }
@@ -995,15 +1058,17 @@ static bool one_range(int64_t lda_bytes, int64_t w_row_bytes, int64_t m, int64_t
 template <int FMT, int OUT>
 static hipError_t launch_linear(const uint16_t* a, int64_t lda, const uint8_t* wq, const uint8_t* ws,
                                 void* c, int64_t ldc, int M, int N, int K, int KB, hipStream_t st, int slices = 1,
-                                int64_t plane = 0) {
+                                int64_t plane = 0, const Epilogue& epi = Epilogue{}) {
   if (takes_dma(FMT, lda, ws, KB))
-    return launch_linear_dma<FMT, OUT>(a, lda, wq, ws, c, ldc, M, N, K, KB, st, slices, plane);
+    return launch_linear_dma<FMT, OUT>(a, lda, wq, ws, c, ldc, M, N, K, KB, st, slices, plane, epi);
   const size_t lds = 2 * (size_t)lin::stage_bytes<FMT>();
-  auto kern = OUT == 2 && slices > 1 ? mx_linear_kernel<FMT, 2, true> : mx_linear_kernel<FMT, OUT, false>;
+  auto kern = OUT == 2 && slices > 1  ? mx_linear_kernel<FMT, 2, true>
+              : epi.kind == EPI_OFF ? mx_linear_kernel<FMT, OUT, false>
+                                    : mx_linear_kernel<FMT, OUT, false, true>;
   hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e != hipSuccess) return e;
   dim3 grid((N + lin::BN - 1) / lin::BN, (M + lin::BM - 1) / lin::BM, slices);
-  kern<<<grid, lin::THREADS, lds, st>>>(a, lda, wq, ws, c, ldc, M, N, K, KB, plane);
+  kern<<<grid, lin::THREADS, lds, st>>>(a, lda, wq, ws, c, ldc, M, N, K, KB, plane, epi);
   return hipGetLastError();
 }
 
@@ -1011,10 +1076,10 @@ static hipError_t launch_linear(const uint16_t* a, int64_t lda, const uint8_t* w
 template <int FMT, int OUT>
 static hipError_t launch_linear_split(const uint16_t* a, int64_t lda, const uint8_t* wq, const uint8_t* ws, void* c,
                                       int64_t ldc, int M, int N, int K, int KB, const SplitPlan& p, void* planes,
-                                      hipStream_t st) {
-  if (p.slices <= 1) return launch_linear<FMT, OUT>(a, lda, wq, ws, c, ldc, M, N, K, KB, st);
+                                      hipStream_t st, const Epilogue& epi) {
+  if (p.slices <= 1) return launch_linear<FMT, OUT>(a, lda, wq, ws, c, ldc, M, N, K, KB, st, 1, 0, epi);
   const hipError_t e = launch_linear<FMT, 2>(a, lda, wq, ws, planes, p.ldp, M, N, K, KB, st, p.slices, p.plane);
-  return e == hipSuccess ? sum_planes<OUT>(p, planes, M, N, c, ldc, st) : e;
+  return e == hipSuccess ? sum_planes<OUT>(p, planes, M, N, c, ldc, st, epi) : e;
 }
 
 static int current_cus() {
@@ -1149,30 +1214,24 @@ extern "C" int64_t kq_mx_linear_workspace_size(int64_t m, int64_t n, int64_t k) 
              ? 0 : p.bytes;
 }
 
-extern "C" int kq_mx_linear(int w_fmt, const void* a, int64_t lda, const void* w_q,
-                            const uint8_t* w_scale, int64_t m, int64_t n, int64_t k,
-                            int out_dtype, void* c, int64_t ldc, void* stream) {
-  return kq_mx_linear_ws(w_fmt, a, lda, w_q, w_scale, m, n, k, out_dtype, c, ldc, nullptr, 0, stream);
-}
-
-extern "C" int kq_mx_linear_ws(int w_fmt, const void* a, int64_t lda, const void* w_q, const uint8_t* w_scale,
-                               int64_t m, int64_t n, int64_t k, int out_dtype, void* c, int64_t ldc,
-                               void* workspace, int64_t workspace_bytes, void* stream) {
+static int linear_bf16(const char* fn, int w_fmt, const void* a, int64_t lda, const void* w_q, const uint8_t* w_scale,
+                       int64_t m, int64_t n, int64_t k, const Epilogue& epi, int out_dtype, void* c, int64_t ldc,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
   if (w_fmt != KQ_FMT_MXFP8_E4M3 && w_fmt != KQ_FMT_MXFP4_E2M1)
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear: unknown weight format %d", w_fmt);
+    return kq_fail(KQ_ERR_INVALID, "%s: unknown weight format %d", fn, w_fmt);
   if (out_dtype != KQ_DT_BF16 && out_dtype != KQ_DT_F32)
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear: output dtype must be bf16 or f32");
+    return kq_fail(KQ_ERR_INVALID, "%s: output dtype must be bf16 or f32", fn);
   if (m < 0 || n < 0 || k <= 0 || k % 64 != 0 || lda < k || lda % 8 != 0 || ldc < n)
     return kq_fail(KQ_ERR_INVALID,
-                   "kq_mx_linear: need k %% 64 == 0, lda >= k, lda %% 8 == 0, ldc >= n "
+                   "%s: need k %% 64 == 0, lda >= k, lda %% 8 == 0, ldc >= n "
                    "(m=%lld n=%lld k=%lld lda=%lld ldc=%lld)",
-                   (long long)m, (long long)n, (long long)k, (long long)lda, (long long)ldc);
+                   fn, (long long)m, (long long)n, (long long)k, (long long)lda, (long long)ldc);
   if (m > INT32_MAX / 2 || n > INT32_MAX / 2 || k > INT32_MAX / 2)
-    return kq_fail(KQ_ERR_LIMIT, "kq_mx_linear: dimension too large");
+    return kq_fail(KQ_ERR_LIMIT, "%s: dimension too large", fn);
   if (kq_misaligned(a, 16) || kq_misaligned(w_q, 16) || kq_misaligned(w_scale, 2))
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear: a and w_q must be 16-byte aligned");
+    return kq_fail(KQ_ERR_INVALID, "%s: a and w_q must be 16-byte aligned", fn);
   if (kq_misaligned(workspace, 16))
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear: workspace must be 16-byte aligned");
+    return kq_fail(KQ_ERR_INVALID, "%s: workspace must be 16-byte aligned", fn);
   if (m == 0 || n == 0) return KQ_OK;
   if (!workspace) workspace_bytes = 0;
   hipStream_t st = (hipStream_t)stream;
@@ -1184,7 +1243,7 @@ extern "C" int kq_mx_linear_ws(int w_fmt, const void* a, int64_t lda, const void
   SplitPlan p;
   if (!skinny) {
     int cus = 0;
-    if ((e = stream_cus(st, &cus)) != hipSuccess) return kq_check_launch(e, "kq_mx_linear");
+    if ((e = stream_cus(st, &cus)) != hipSuccess) return kq_check_launch(e, fn);
     const double step = step_us(takes_dma(w_fmt == KQ_FMT_MXFP8_E4M3 ? 0 : 1, lda, w_scale, k));
     p = plan_within(plan_split(m, n, k, step, cus), workspace_bytes,
                     one_range(2 * lda, w_fmt == KQ_FMT_MXFP8_E4M3 ? k : k / 2, m, n));
@@ -1192,16 +1251,29 @@ extern "C" int kq_mx_linear_ws(int w_fmt, const void* a, int64_t lda, const void
   }
   if (skinny)
     return kq_check_launch(mx_skinny_bf16(w_fmt, out_dtype == KQ_DT_F32,
-                                          {a, nullptr, lda, wp, w_scale, c, ldc, (int)m, (int)n, (int)k}, st),
-                           "kq_mx_linear");
+                                          {a, nullptr, lda, wp, w_scale, c, ldc, (int)m, (int)n, (int)k, epi}, st),
+                           fn);
   auto run = [&](auto launch) {
-    return launch(ap, lda, wp, w_scale, c, ldc, (int)m, (int)n, (int)k, (int)k, p, workspace, st);
+    return launch(ap, lda, wp, w_scale, c, ldc, (int)m, (int)n, (int)k, (int)k, p, workspace, st, epi);
   };
   if (w_fmt == KQ_FMT_MXFP8_E4M3)
     e = out_dtype == KQ_DT_BF16 ? run(launch_linear_split<0, 0>) : run(launch_linear_split<0, 2>);
   else
     e = out_dtype == KQ_DT_BF16 ? run(launch_linear_split<1, 0>) : run(launch_linear_split<1, 2>);
-  return kq_check_launch(e, "kq_mx_linear");
+  return kq_check_launch(e, fn);
+}
+
+extern "C" int kq_mx_linear_ws(int w_fmt, const void* a, int64_t lda, const void* w_q, const uint8_t* w_scale,
+                               int64_t m, int64_t n, int64_t k, int out_dtype, void* c, int64_t ldc,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
+  return linear_bf16("kq_mx_linear", w_fmt, a, lda, w_q, w_scale, m, n, k, Epilogue{}, out_dtype, c, ldc, workspace,
+                     workspace_bytes, stream);
+}
+
+extern "C" int kq_mx_linear(int w_fmt, const void* a, int64_t lda, const void* w_q,
+                            const uint8_t* w_scale, int64_t m, int64_t n, int64_t k,
+                            int out_dtype, void* c, int64_t ldc, void* stream) {
+  return kq_mx_linear_ws(w_fmt, a, lda, w_q, w_scale, m, n, k, out_dtype, c, ldc, nullptr, 0, stream);
 }
 
 extern "C" int64_t kq_mx_linear_f32_workspace_size(int64_t m, int64_t k) {
@@ -1224,25 +1296,24 @@ extern "C" int64_t kq_mx_linear_f32_split_workspace_size(int64_t m, int64_t n, i
              ? m * 3 * k * 2 : f32_planes_offset(m, k) + p.bytes;
 }
 
-extern "C" int kq_mx_linear_f32(int w_fmt, const float* a, int64_t lda, const void* w_q,
-                                const uint8_t* w_scale, int64_t m, int64_t n, int64_t k, float* c,
-                                int64_t ldc, void* workspace, int64_t workspace_bytes,
-                                void* stream) {
+static int linear_f32(const char* fn, int w_fmt, const float* a, int64_t lda, const void* w_q, const uint8_t* w_scale,
+                      int64_t m, int64_t n, int64_t k, const Epilogue& epi, float* c, int64_t ldc, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
   if (w_fmt != KQ_FMT_MXFP8_E4M3 && w_fmt != KQ_FMT_MXFP4_E2M1)
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear_f32: unknown weight format %d", w_fmt);
+    return kq_fail(KQ_ERR_INVALID, "%s: unknown weight format %d", fn, w_fmt);
   if (m < 0 || n < 0 || k <= 0 || k % 64 != 0 || lda < k || lda % 4 != 0 || ldc < n)
     return kq_fail(KQ_ERR_INVALID,
-                   "kq_mx_linear_f32: need k %% 64 == 0, lda >= k, lda %% 4 == 0, ldc >= n "
+                   "%s: need k %% 64 == 0, lda >= k, lda %% 4 == 0, ldc >= n "
                    "(m=%lld n=%lld k=%lld lda=%lld ldc=%lld)",
-                   (long long)m, (long long)n, (long long)k, (long long)lda, (long long)ldc);
+                   fn, (long long)m, (long long)n, (long long)k, (long long)lda, (long long)ldc);
   if (m > INT32_MAX / 2 || n > INT32_MAX / 2 || 3 * k > INT32_MAX / 2)
-    return kq_fail(KQ_ERR_LIMIT, "kq_mx_linear_f32: dimension too large");
+    return kq_fail(KQ_ERR_LIMIT, "%s: dimension too large", fn);
   if (workspace_bytes < m * 3 * k * 2)
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear_f32: workspace needs %lld bytes",
+    return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes", fn,
                    (long long)(m * 3 * k * 2));
   if (kq_misaligned(a, 16) || kq_misaligned(w_q, 16) || kq_misaligned(w_scale, 2) ||
       kq_misaligned(workspace, 16))
-    return kq_fail(KQ_ERR_INVALID, "kq_mx_linear_f32: a, w_q and workspace must be 16-byte aligned");
+    return kq_fail(KQ_ERR_INVALID, "%s: a, w_q and workspace must be 16-byte aligned", fn);
   if (m == 0 || n == 0) return KQ_OK;
   hipStream_t st = (hipStream_t)stream;
   const int64_t off = f32_planes_offset(m, k), w_row = w_fmt == KQ_FMT_MXFP8_E4M3 ? k : k / 2;
@@ -1251,24 +1322,66 @@ extern "C" int kq_mx_linear_f32(int w_fmt, const float* a, int64_t lda, const vo
   SplitPlan p;
   if (!skinny) {
     int cus = 0;
-    if (int rc = kq_check_launch(stream_cus(st, &cus), "kq_mx_linear_f32")) return rc;
+    if (int rc = kq_check_launch(stream_cus(st, &cus), fn)) return rc;
     const double step = step_us(takes_dma(w_fmt == KQ_FMT_MXFP8_E4M3 ? 0 : 1, 3 * k, w_scale, k));
     p = plan_within(plan_split(m, n, 3 * k, step, cus), workspace_bytes - off, one_range(6 * k, w_row, m, n));
     skinny = takes_skinny(form, m, n, k, w_scale, p, step, cus);
   }
   if (skinny)
     return kq_check_launch(mx_skinny_f32(w_fmt, {a, nullptr, lda, (const uint8_t*)w_q, w_scale, c, ldc, (int)m, (int)n,
-                                                 (int)k}, st),
-                           "kq_mx_linear_f32");
+                                                 (int)k, epi}, st),
+                           fn);
   uint16_t* a3 = static_cast<uint16_t*>(workspace);
   const int64_t quads = m * (k / 4);
   split3_bf16_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, st>>>(a, lda, m, k, a3);
-  if (int rc = kq_check_launch(hipGetLastError(), "kq_mx_linear_f32")) return rc;
+  if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   const uint8_t* wp = (const uint8_t*)w_q;
   auto* launch = w_fmt == KQ_FMT_MXFP8_E4M3 ? launch_linear_split<0, 2> : launch_linear_split<1, 2>;
   const hipError_t e = launch(a3, 3 * k, wp, w_scale, c, ldc, (int)m, (int)n, (int)(3 * k), (int)k, p,
-                              static_cast<char*>(workspace) + off, st);
-  return kq_check_launch(e, "kq_mx_linear_f32");
+                              static_cast<char*>(workspace) + off, st, epi);
+  return kq_check_launch(e, fn);
+}
+
+extern "C" int kq_mx_linear_f32(int w_fmt, const float* a, int64_t lda, const void* w_q,
+                                const uint8_t* w_scale, int64_t m, int64_t n, int64_t k, float* c,
+                                int64_t ldc, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  return linear_f32("kq_mx_linear_f32", w_fmt, a, lda, w_q, w_scale, m, n, k, Epilogue{}, c, ldc, workspace,
+                    workspace_bytes, stream);
+}
+
+extern "C" int kq_mx_linear_epilogue(int w_fmt, int a_dtype, const void* a, int64_t lda, const void* w_q,
+                                     const uint8_t* w_scale, int64_t m, int64_t n, int64_t k, int activation,
+                                     const void* bias, int bias_dtype, const void* residual, int64_t ldr, int out_dtype,
+                                     void* c, int64_t ldc, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* fn = "kq_mx_linear_epilogue";
+  if (a_dtype != KQ_DT_BF16 && a_dtype != KQ_DT_F32)
+    return kq_fail(KQ_ERR_INVALID, "%s: input dtype must be bf16 or f32", fn);
+  if (a_dtype == KQ_DT_F32 && out_dtype != KQ_DT_F32)
+    return kq_fail(KQ_ERR_INVALID, "%s: f32 rows give f32 results", fn);
+  if (activation < KQ_LIN_NONE || activation > KQ_LIN_GELU_TANH)
+    return kq_fail(KQ_ERR_INVALID, "%s: unknown activation %d", fn, activation);
+  if (bias && bias_dtype != KQ_DT_BF16 && bias_dtype != KQ_DT_F32)
+    return kq_fail(KQ_ERR_INVALID, "%s: bias dtype must be bf16 or f32", fn);
+  if (residual && ldr < n) return kq_fail(KQ_ERR_INVALID, "%s: need ldr >= n", fn);
+  if (kq_misaligned(bias, bias_dtype == KQ_DT_F32 ? 4 : 2) || kq_misaligned(residual, out_dtype == KQ_DT_F32 ? 4 : 2))
+    return kq_fail(KQ_ERR_INVALID, "%s: bias and residual must be aligned to their type", fn);
+  Epilogue e{};
+  e.kind = activation == KQ_LIN_GELU                                             ? EPI_ERF
+           : activation == KQ_LIN_SILU || activation == KQ_LIN_GELU_TANH ? EPI_SIGMOID
+                                                                                 : EPI_CLAMP;
+  e.low = activation == KQ_LIN_RELU ? 0.0f : -__builtin_inff();
+  constexpr double C = 1.5957691216057308;  // 2 sqrt(2 / pi)
+  e.c1 = activation == KQ_LIN_GELU_TANH ? (float)C : 1.0f;
+  e.c3 = activation == KQ_LIN_GELU_TANH ? (float)(0.044715 * C) : 0.0f;
+  e.bias = bias;
+  e.bias_f32 = bias_dtype == KQ_DT_F32;
+  e.residual = residual;
+  e.ldr = ldr;
+  return a_dtype == KQ_DT_F32 ? linear_f32(fn, w_fmt, static_cast<const float*>(a), lda, w_q, w_scale, m, n, k, e,
+                                           static_cast<float*>(c), ldc, workspace, workspace_bytes, stream)
+                              : linear_bf16(fn, w_fmt, a, lda, w_q, w_scale, m, n, k, e, out_dtype, c, ldc, workspace,
+                                            workspace_bytes, stream);
 }
 
 static int check_linear_mx(const char* fn, int a_fmt, int w_fmt, int64_t lda, int64_t m, int64_t n, int64_t k,

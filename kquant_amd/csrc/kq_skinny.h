@@ -24,6 +24,7 @@
 // Rows past M or N are read at the last valid row and not stored.
 #pragma once
 
+#include "kq_epilogue.h"
 #include "kq_gemm.h"
 
 namespace kq {
@@ -57,11 +58,11 @@ __device__ __forceinline__ u32x4_t load16_nt(const void* p) {
 // FMT: weight format; AT: activation rows; OUT: KQ_DT_BF16 / KQ_DT_F32;
 // MB x 16 activation rows and R x 16 weight rows per workgroup, P windows in
 // flight; HALF: K % 128 == 64 (2-byte aligned scale rows, a half window at
-// the end).
-template <int FMT, int AT, int OUT, int MB, int R, int P, bool HALF>
+// the end); EPI: with the linear's epilogue.
+template <int FMT, int AT, int OUT, int MB, int R, int P, bool HALF, bool EPI>
 __global__ __launch_bounds__(512) void mx_skinny_kernel(
     const void* __restrict__ a, const uint8_t* __restrict__ a_scale, int64_t lda, const uint8_t* __restrict__ wq,
-    const uint8_t* __restrict__ ws, void* __restrict__ c, int64_t ldc, int M, int N, int K, int mtiles) {
+    const uint8_t* __restrict__ ws, void* __restrict__ c, int64_t ldc, int M, int N, int K, int mtiles, Epilogue epi) {
   static_assert(AT != A_MXFP8 || (FMT == 0 && !HALF), "MXFP8 rows take E4M3 weights and whole windows");
   using Win = Window<FMT, AT, MB, R>;
   extern __shared__ __attribute__((aligned(16))) float skinny_red[];
@@ -283,6 +284,7 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
     const int at = ((m >> 4) * R + (n >> 4)) * 256 + (16 * ((m & 15) >> 2) + (n & 15)) * 4 + (m & 3);
     float sum = skinny_red[at];
     for (int w = 1; w < waves; ++w) sum += skinny_red[w * TILE + at];
+    if (EPI) sum = epi_apply<OUT>(epi, sum, m0 + m, n0 + n);
     if (OUT == 2) static_cast<float*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = sum;
     else static_cast<__bf16*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = (__bf16)sum;
   }

@@ -11,14 +11,16 @@ static hipError_t launch(const SkinnyArgs& s, hipStream_t st) {
   const int nwin = (s.k + WIN - 1) / WIN;
   const int waves = nwin < 8 ? nwin : 8;
   const size_t lds = (size_t)waves * MB * R * 1024;
-  auto kern = mx_skinny_kernel<FMT, AT, OUT, MB, R, P, HALF>;
+  auto kern = mx_skinny_kernel<FMT, AT, OUT, MB, R, P, HALF, false>;
+  if constexpr (AT != A_MXFP8)
+    if (s.epi.kind != EPI_OFF) kern = mx_skinny_kernel<FMT, AT, OUT, MB, R, P, HALF, true>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
   const int64_t mtiles = (s.m + 16 * MB - 1) / (16 * MB), ntiles = ((int64_t)s.n + 16 * R - 1) / (16 * R);
   kern<<<(unsigned)(mtiles * ((ntiles + 7) / 8 * 8)), waves * 64, lds, st>>>(
-      s.a, s.a_scale, s.lda, s.wq, s.ws, s.c, s.ldc, s.m, s.n, s.k, (int)mtiles);
+      s.a, s.a_scale, s.lda, s.wq, s.ws, s.c, s.ldc, s.m, s.n, s.k, (int)mtiles, s.epi);
   return hipGetLastError();
 }
 

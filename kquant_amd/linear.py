@@ -29,8 +29,26 @@ import torch
 from . import _native as N
 
 
+def _check_epilogue(bias, activation, residual, lead, n: int, f32: bool, out_dtype: torch.dtype) -> None:
+    if activation not in N.LIN_ACTIVATIONS:
+        raise ValueError(f"activation must be None, relu, silu, gelu or gelu_tanh, got {activation!r}")
+    if f32 and out_dtype != torch.float32:
+        raise TypeError("a float32 source with an epilogue gives a float32 result")
+    if bias is not None:
+        if bias.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"bias must be bfloat16 or float32, got {bias.dtype}")
+        if tuple(bias.shape) != (n,):
+            raise ValueError(f"bias shape {tuple(bias.shape)} != {(n,)}")
+    if residual is not None:
+        if residual.dtype != out_dtype:
+            raise TypeError(f"residual must have the result's type {out_dtype}, got {residual.dtype}")
+        if tuple(residual.shape) != (*lead, n):
+            raise ValueError(f"residual shape {tuple(residual.shape)} != {(*lead, n)}")
+
+
 def _linear(fmt: int, source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
-            out_dtype: torch.dtype | None) -> torch.Tensor:
+            out_dtype: torch.dtype | None, bias: torch.Tensor | None = None, activation: str | None = None,
+            residual: torch.Tensor | None = None) -> torch.Tensor:
     if out_dtype is None:
         out_dtype = torch.float32 if source.dtype == torch.float32 else torch.bfloat16
     if source.ndim < 1:
@@ -53,9 +71,15 @@ def _linear(fmt: int, source: torch.Tensor, weight: torch.Tensor, scale: torch.T
     exact_f32 = a.dtype == torch.float32
     if not exact_f32 and a.dtype != torch.bfloat16:
         a = a.to(torch.bfloat16)
-    (a, w, s), gpu, host = N.to_gpu([a, weight.view(torch.uint8), scale])
+    epilogue = bias is not None or activation is not None or residual is not None
+    if epilogue:
+        _check_epilogue(bias, activation, residual, lead, n, exact_f32, out_dtype)
+        residual = None if residual is None else residual.reshape(-1, n)
+    (a, w, s, bias, residual), gpu, host = N.to_gpu([a, weight.view(torch.uint8), scale, bias, residual])
     a, w, s = N.aligned(a), N.aligned(w), N.aligned(s)
     m = a.shape[0]
+    if epilogue:
+        return _linear_epilogue(fmt, a, w, s, out_dtype, bias, activation, residual, lead, gpu, host)
     if exact_f32:
         out = torch.empty(m, n, dtype=torch.float32, device=gpu)
         ws = torch.empty(max(int(N.library().kq_mx_linear_f32_split_workspace_size(m, n, k)), 16),
@@ -73,26 +97,55 @@ def _linear(fmt: int, source: torch.Tensor, weight: torch.Tensor, scale: torch.T
     return out if host is None else out.to(host)
 
 
+def _linear_epilogue(fmt, a, w, s, out_dtype, bias, activation, residual, lead, gpu, host) -> torch.Tensor:
+    m, k = a.shape
+    n = w.shape[0]
+    f32 = a.dtype == torch.float32
+    if bias is not None:
+        bias = bias.contiguous()
+    if residual is not None and (residual.stride(1) != 1 or residual.stride(0) < n):
+        residual = residual.contiguous()
+    with N.on_device(gpu):
+        size = N.library().kq_mx_linear_f32_split_workspace_size if f32 else N.library().kq_mx_linear_workspace_size
+        need = max(int(size(m, n, k)), 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=gpu) if need else None
+        out = torch.empty(m, n, dtype=out_dtype, device=gpu)
+        N.call("kq_mx_linear_epilogue", fmt, N.DTYPE_CODES[a.dtype], N.ptr(a), k, N.ptr(w), N.ptr(s), m, n, k,
+               N.LIN_ACTIVATIONS[activation], N.ptr(bias), N.DT_BF16 if bias is None else N.DTYPE_CODES[bias.dtype],
+               N.ptr(residual), n if residual is None else residual.stride(0), N.DTYPE_CODES[out_dtype], N.ptr(out), n,
+               N.ptr(ws), need, N.stream(gpu))
+    out = out.reshape(*lead, n)
+    return out if host is None else out.to(host)
+
+
 def mxfp8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, *,
-                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                 bias: torch.Tensor | None = None, activation: str | None = None,
+                 residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``source [..., K] @ dequant(weight E4M3 [N, K], scale [N, K/32]).T``.
 
     Output dtype defaults to fp32 for fp32 sources and bf16 otherwise.
+
+    ``bias`` [N] (bf16 or fp32), ``activation`` ("relu", "silu", "gelu", its
+    tanh form "gelu_tanh", or None) and ``residual`` (of the result's shape and
+    type) are applied in the kernel's epilogue on the fp32 sums, which are then
+    rounded once: ``activation(source @ W.T + bias) + residual``.
     """
     if weight.dtype not in (torch.float8_e4m3fn, torch.uint8):
         raise TypeError(f"MXFP8 weight must be float8_e4m3fn, got {weight.dtype}")
-    return _linear(N.FMT_MXFP8_E4M3, source, weight, scale, out_dtype)
+    return _linear(N.FMT_MXFP8_E4M3, source, weight, scale, out_dtype, bias, activation, residual)
 
 
 def mxfp4_linear(source: torch.Tensor, packed: torch.Tensor, scale: torch.Tensor, *,
-                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                 bias: torch.Tensor | None = None, activation: str | None = None,
+                 residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``source [..., K] @ dequant(packed [N, K/2], scale [N, K/32]).T``.
 
-    Output dtype defaults to fp32 for fp32 sources and bf16 otherwise.
+    Output dtype defaults to fp32 for fp32 sources and bf16 otherwise; bias,
+    activation and residual as in ``mxfp8_linear``.
     """
     if packed.dtype != torch.uint8:
         raise TypeError(f"expected uint8, got {packed.dtype}")
-    return _linear(N.FMT_MXFP4_E2M1, source, packed, scale, out_dtype)
+    return _linear(N.FMT_MXFP4_E2M1, source, packed, scale, out_dtype, bias, activation, residual)
 
 
 MX_LINEAR_K_ALIGN = 128  # the MXFP8 x MXFP8 kernel's K granule

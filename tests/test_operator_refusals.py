@@ -10,6 +10,7 @@ import torch
 
 from kquant_amd import _native as N
 from kquant_amd.grouped import grouped_linear
+from kquant_amd.linear import mxfp4_linear, mxfp8_linear
 from kquant_amd.loss import linear_cross_entropy
 
 BF16 = torch.bfloat16
@@ -111,3 +112,34 @@ def test_loss_c_entries():
     # no [tokens, vocabulary] array forward; at most 1 GiB of it backward
     assert size(N.FMT_BF16, 4096, 131072, 4096, 0) < 4096 * 131072 // 4
     assert size(N.FMT_BF16, 16384, 131072, 64, 1) < (1 << 30) + (1 << 28)
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(activation="tanh"), ValueError, "activation"),
+    (dict(bias=torch.zeros(9, dtype=torch.float16)), TypeError, "bias must be"),
+    (dict(bias=torch.zeros(8)), ValueError, "bias shape"),
+    (dict(residual=torch.zeros(4, 9)), TypeError, "result's type"),
+    (dict(residual=bf16(4, 8)), ValueError, "residual shape"),
+    (dict(source=torch.zeros(4, 64), activation="relu", out_dtype=BF16), TypeError, "float32 result"),
+])
+def test_linear_epilogue(change, error, text):
+    args = dict(source=bf16(4, 64), bias=None, activation=None, residual=None, out_dtype=None) | change
+    source = args.pop("source")
+    scale = torch.zeros(9, 2, dtype=torch.uint8)
+    with pytest.raises(error, match=text):
+        mxfp8_linear(source, torch.zeros(9, 64, dtype=torch.uint8), scale, **args)
+    with pytest.raises(error, match=text):
+        mxfp4_linear(source, torch.zeros(9, 32, dtype=torch.uint8), scale, **args)
+
+
+def test_linear_epilogue_c_entry():
+    lib = N.library()
+    p = ctypes.c_void_p(256)
+    ok = [N.FMT_MXFP8_E4M3, N.DT_BF16, p, 64, p, p, 4, 9, 64, 0, p, N.DT_F32, p, 9, N.DT_BF16, p, 9, None, 0, None]
+    for at, value, text in ((0, N.FMT_BF16, b"weight format"), (1, N.DT_F16, b"input dtype"), (1, N.DT_F32, b"f32 results"),
+                            (9, 5, b"activation 5"), (9, -1, b"activation"), (11, N.DT_F16, b"bias dtype"), (13, 8, b"ldr >= n"),
+                            (14, N.DT_F16, b"output dtype"), (10, ctypes.c_void_p(2), b"aligned to their type"),
+                            (12, ctypes.c_void_p(1), b"aligned to their type"), (16, 8, b"ldc >= n"), (8, 60, b"k % 64")):
+        args = list(ok)
+        args[at] = value
+        assert lib.kq_mx_linear_epilogue(*args) == N.KQ_ERR_INVALID and text in lib.kq_last_error(), (at, lib.kq_last_error())
