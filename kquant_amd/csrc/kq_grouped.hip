@@ -143,8 +143,10 @@ struct Problem {
     range(hint, beg, n);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     const int64_t row0 = MODE == DW ? (int64_t)hint * g.n + m0 : beg + m0;
-    mm16::store16<NB, WN, F16>(g.out + row0 * g.ld_out + 2 * (int64_t)n0, g.ld_out, tl.rows,
-                               (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, acc, lane);
+    char* out = g.out + row0 * g.ld_out + 2 * (int64_t)n0;
+    mm16::store16<NB, WN, F16>([&](int r) { return out + r * (int64_t)g.ld_out; }, tl.rows,
+                               (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, lane,
+                               [&](int i, int j, int r) { return acc[i][j][r]; });
   }
 };
 

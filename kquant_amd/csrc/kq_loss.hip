@@ -4,6 +4,11 @@
 //   d[t][v] = g_t (exp(z[t][v] - lse_t) - [v = y_t])
 //   dh_t = sum_v d[t][v] w_v     dw_v = sum_t d[t][v] h_t
 //
+// with g_t = alpha u_t: alpha (one upstream gradient, over the token count for a
+// mean; else the largest magnitude of the tokens' gradients) multiplies the fp32
+// sums, so that the -1 of a target enters the products exactly and not as a
+// rounded 1 / count, whose error all tokens would share.
+//
 // What bounds it: the matrix products (2 T V K flop forward, 6 T V K backward,
 // a third of which recomputes z); at few tokens, the head's bytes.  The
 // logits never reach memory in the forward pass: a tile's epilogue reduces its
@@ -79,6 +84,29 @@ __global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict
   if (tid == 0) *count = base;
 }
 
+// alpha of the upstream gradients (see above); 1 where they are all zero.
+__global__ __launch_bounds__(1024) void alpha_kernel(const float* __restrict__ grad, int reduction, int tokens,
+                                                     const int* __restrict__ place, const int* __restrict__ count,
+                                                     float* __restrict__ alpha) {
+  __shared__ float wave_max[16];
+  if (reduction != NONE) {
+    if (threadIdx.x == 0) *alpha = reduction == SUM ? grad[0] : *count > 0 ? grad[0] / (float)*count : 0.0f;
+    return;
+  }
+  float m = 0.0f;  // the largest finite one: another leaves u infinite or NaN, as it should
+  for (int t = threadIdx.x; t < tokens; t += 1024) {
+    const float v = fabsf(grad[t]);
+    if (place[t] >= 0 && v < __builtin_inff()) m = fmaxf(m, v);
+  }
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, wave_max[w]);
+    *alpha = m > 0.0f ? m : 1.0f;
+  }
+}
+
 struct Gather {
   const char* h;
   int64_t ldh;  // bytes
@@ -93,8 +121,9 @@ struct Gather {
   const float* lse;
   const float* grad;
   int reduction;
+  const float* alpha;
   float* lse_c;
-  float* g_c;
+  float* u_c;  // upstream gradients over alpha
   char* dh;
   int64_t lddh;  // bytes
 };
@@ -120,9 +149,8 @@ __global__ __launch_bounds__(256) void gather_kernel(Gather g) {
       const bool ok = y >= 0 && y < g.vocab;
       g.target_c[at] = ok ? (int)y : -1;
       if (g.lse_c) {
-        const float up = g.reduction == NONE ? g.grad[t] : g.reduction == MEAN ? g.grad[0] / (float)count : g.grad[0];
         g.lse_c[at] = g.lse[t];
-        g.g_c[at] = ok ? up : __builtin_nanf("");
+        g.u_c[at] = ok ? (g.reduction == NONE ? g.grad[t] / *g.alpha : 1.0f) : __builtin_nanf("");
       }
     }
   } else if (g.dh) {
@@ -152,8 +180,8 @@ struct LogitArgs {
   int part0;  // tiles of the pieces before
   float* z_target;
   const float* lse_c;
-  const float* g_c;
-  __bf16* dt;
+  const float* u_c;
+  char* dt;
   int ldg;
 };
 
@@ -189,24 +217,16 @@ struct LogitProblem {
         const bool live = c < count;
         tgt[j] = live ? g.target_c[c] - v0 : -1;
         lse[j] = live ? g.lse_c[c] : 0.0f;
-        up[j] = live ? g.g_c[c] : 0.0f;
+        up[j] = live ? g.u_c[c] : 0.0f;
       }
-      __bf16* out = g.dt + (int64_t)mt * mm16::BM * g.ldg + n0;
-      const int cols = min((count + 7) / 8 * 8 - n0, mm16::BN);
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = wm + 4 * (lane >> 5) + 32 * i + 8 * (r >> 2) + (r & 3);
-          if (at < tl.rows) {
-#pragma unroll
-            for (int j = 0; j < WN; ++j) {
-              const int c = wn + 32 * j + (lane & 31);
-              const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
-              if (c < cols) out[(int64_t)at * g.ldg + c] = (__bf16)(n0 + c < count ? up[j] * p : 0.0f);
-            }
-          }
-        }
+      char* out = g.dt + ((int64_t)mt * mm16::BM * g.ldg + n0) * 2;
+      const int row = wm + 4 * (lane >> 5);
+      mm16::store16<NB, WN, false>([&](int r) { return out + r * (int64_t)g.ldg * 2; }, tl.rows,
+                                   (count + 7) / 8 * 8 - n0, wm, wn, lane, [&](int i, int j, int r) {
+        const int at = row + 32 * i + 8 * (r >> 2) + (r & 3);
+        const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
+        return n0 + wn + 32 * j + (lane & 31) < count ? up[j] * p : 0.0f;
+      });
       return;
     }
     const int row = wm + 4 * (lane >> 5);  // this lane's rows: row + 32 i + 8 (r / 4) + r % 4
@@ -266,6 +286,7 @@ struct DhArgs {
   const int* count;
   const int* rows_of;
   int rows, k, slices, tokens;
+  const float* alpha;
   char* dh;  // or null
   int64_t lddh;  // bytes
   float* planes;
@@ -301,9 +322,9 @@ struct DhProblem {
     if (g.dh) {
       const int* map = g.rows_of + m0;
       char* out = g.dh + 2 * (int64_t)n0;
-      mm16::each(tl.rows, g.k - n0, wm, wn, acc, lane, [&](int r, int c, float v) {
-        *reinterpret_cast<__bf16*>(out + map[r] * g.lddh + 2 * (int64_t)c) = (__bf16)v;
-      });
+      const float alpha = *g.alpha;
+      mm16::store16<NB, WN, false>([&](int r) { return out + map[r] * g.lddh; }, tl.rows, g.k - n0, wm, wn, lane,
+                                   [&](int i, int j, int r) { return alpha * acc[i][j][r]; });
     } else {
       float* out = g.planes + ((int64_t)sl * g.tokens + m0) * g.k + n0;
       const uint32_t ld = (uint32_t)g.k;
@@ -327,17 +348,19 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
 
 // dh at the tokens' own rows = the sum of the planes, in slice order.
 __global__ __launch_bounds__(256) void dh_sum_kernel(const float* __restrict__ planes, int slices, int tokens, int k,
-                                                     const int* __restrict__ place, char* __restrict__ dh,
+                                                     const int* __restrict__ place,
+                                                     const float* __restrict__ alpha_at, char* __restrict__ dh,
                                                      int64_t lddh) {
   const int t = blockIdx.x, at = place[t];
   if (at < 0) return;
+  const float alpha = *alpha_at;
   for (int c = (int)threadIdx.x * 4; c < k; c += 1024) {
     const float* p = planes + (int64_t)at * k + c;
     float4_t v = *reinterpret_cast<const float4_t*>(p);
     for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const float4_t*>(p + (int64_t)s * tokens * k);
     uint32_t* o = reinterpret_cast<uint32_t*>(dh + t * lddh + 2 * (int64_t)c);
-    o[0] = f32x2_to_bf16x2_bits(v[0], v[1]);
-    o[1] = f32x2_to_bf16x2_bits(v[2], v[3]);
+    o[0] = f32x2_to_bf16x2_bits(alpha * v[0], alpha * v[1]);
+    o[1] = f32x2_to_bf16x2_bits(alpha * v[2], alpha * v[3]);
   }
 }
 
@@ -347,6 +370,7 @@ struct DwArgs {
   int ldg;
   const char* hc;
   const int* count;
+  const float* alpha;
   int rows, k;
   char* dw;
 };
@@ -373,8 +397,10 @@ struct DwProblem {
     int mt, nt;
     mm16::tile_mn(t, mtiles, ntiles, mt, nt);
     const int n0 = nt * mm16::BN;
-    mm16::store16<NB, WN, false>(g.dw + ((int64_t)mt * mm16::BM * g.k + n0) * 2, (uint32_t)g.k * 2u, tl.rows, g.k - n0,
-                                 wm, wn, acc, lane);
+    char* out = g.dw + ((int64_t)mt * mm16::BM * g.k + n0) * 2;
+    const float alpha = *g.alpha;
+    mm16::store16<NB, WN, false>([&](int r) { return out + r * (int64_t)g.k * 2; }, tl.rows, g.k - n0, wm, wn, lane,
+                                 [&](int i, int j, int r) { return alpha * acc[i][j][r]; });
   }
 };
 
@@ -438,7 +464,7 @@ struct Plan {
   int64_t piece, pieces;       // vocabulary rows
   int slices;                  // of dh's contraction
   int64_t ldg;
-  int64_t o_rows, o_place, o_count, o_target, o_lse, o_g, o_z, o_part, o_hc, o_w, o_dt, o_planes, bytes;
+  int64_t o_rows, o_place, o_count, o_target, o_lse, o_u, o_alpha, o_z, o_part, o_hc, o_w, o_dt, o_planes, bytes;
 };
 
 static int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
@@ -484,7 +510,8 @@ static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backw
   if (mx) p.o_w = take(p.piece * k * 2);
   if (backward) {
     p.o_lse = take(tokens * 4);
-    p.o_g = take(tokens * 4);
+    p.o_u = take(tokens * 4);
+    p.o_alpha = take(4);
     p.o_dt = take(p.piece * p.ldg * 2);
     if (p.slices > 1 || p.pieces > 1) p.o_planes = take(p.slices * tokens * k * 4);
   } else {
@@ -638,10 +665,14 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
   g.lse = lse;
   g.grad = grad;
   g.reduction = reduction;
+  float* alpha = (float*)(ws + p.o_alpha);
+  g.alpha = alpha;
   g.lse_c = (float*)(ws + p.o_lse);
-  g.g_c = (float*)(ws + p.o_g);
+  g.u_c = (float*)(ws + p.o_u);
   g.dh = (char*)dh;
   g.lddh = 2 * lddh;
+  loss::alpha_kernel<<<1, 1024, 0, st>>>(grad, reduction, (int)tokens, g.place, count, alpha);
+  if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   loss::gather_kernel<<<(unsigned)tokens + 8, 256, 0, st>>>(g);
   if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   const unsigned grid = loss::persistent_grid(cus);
@@ -652,8 +683,8 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
   a.k = (int)k;
   a.tokens = (int)tokens;
   a.lse_c = g.lse_c;
-  a.g_c = g.g_c;
-  a.dt = (__bf16*)(ws + p.o_dt);
+  a.u_c = g.u_c;
+  a.dt = ws + p.o_dt;
   a.ldg = (int)p.ldg;
   const bool planes = p.slices > 1 || p.pieces > 1;
   for (int64_t first = 0; first < vocab; first += p.piece) {
@@ -663,20 +694,20 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
     loss::logit_kernel<true><<<grid, mm16::THREADS, 0, st>>>(a);
     if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
     if (dh) {
-      const loss::DhArgs d{(const char*)a.dt, (int)p.ldg, a.w, count, (int*)(ws + p.o_rows), a.rows, (int)k, p.slices,
-                           (int)tokens, planes ? nullptr : (char*)dh, 2 * lddh, (float*)(ws + p.o_planes), first > 0};
+      const loss::DhArgs d{a.dt, (int)p.ldg, a.w, count, (int*)(ws + p.o_rows), a.rows, (int)k, p.slices, (int)tokens,
+                           alpha, planes ? nullptr : (char*)dh, 2 * lddh, (float*)(ws + p.o_planes), first > 0};
       loss::dh_kernel<<<grid, mm16::THREADS, 0, st>>>(d);
       if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
     }
     if (dw) {
-      const loss::DwArgs d{(const char*)a.dt, (int)p.ldg, g.hc, count, a.rows, (int)k, (char*)dw + first * k * 2};
+      const loss::DwArgs d{a.dt, (int)p.ldg, g.hc, count, alpha, a.rows, (int)k, (char*)dw + first * k * 2};
       loss::dw_kernel<<<grid, mm16::THREADS, 0, st>>>(d);
       if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
     }
   }
   if (dh && planes && tokens > 0) {
     loss::dh_sum_kernel<<<(unsigned)tokens, 256, 0, st>>>((const float*)(ws + p.o_planes), p.slices, (int)tokens, (int)k,
-                                                         g.place, (char*)dh, 2 * lddh);
+                                                         g.place, alpha, (char*)dh, 2 * lddh);
     if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   }
   return KQ_OK;

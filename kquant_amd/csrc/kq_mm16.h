@@ -53,6 +53,7 @@ constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
 constexpr int64_t MAX_LD = 1 << 22;    // elements: 256 rows stay below OUT_OF_RANGE
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -193,15 +194,49 @@ __device__ __forceinline__ void each(int rows, int cols, int wm, int wn, const f
     }
 }
 
-// Stores a wave's blocks to out (row stride ld bytes), rounded to nearest even.
-template <int NB, int WN, bool F16>
-__device__ __forceinline__ void store16(char* out, uint32_t ld, int rows, int cols, int wm, int wn,
-                                        const float16_t (&acc)[NB][WN], int lane) {
-  each(rows, cols, wm, wn, acc, lane, [&](int r, int c, float v) {
-    char* q = out + ((uint32_t)r * ld + 2u * (uint32_t)c);
-    if (F16) *reinterpret_cast<_Float16*>(q) = (_Float16)v;
-    else *reinterpret_cast<__bf16*>(q) = (__bf16)v;
-  });
+// Two 16-bit values of a row pair, rounded to nearest even.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  return F16 ? f32x2_to_f16x2_bits(lo, hi) : f32x2_to_bf16x2_bits(lo, hi);
+}
+
+// Stores a wave's blocks in 16 bits: rows below `rows`, columns below `cols` (a
+// multiple of 4) of the tile, f(i, j, r) the value of element r of block (i,
+// j), address(row) the 8-byte aligned address of a row's column 0 (asked for rows
+// below `rows` only).  A lane holds four rows of one column and
+// exchanges them with its quad for four columns of one row, in 10 instructions
+// of its registers, so it stores 8 bytes: a store instruction takes as long for
+// 2 bytes a lane.
+template <int NB, int WN, bool F16, class At, class F>
+__device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm, int wn, int lane, F&& f) {
+  const int t = lane & 3;
+  int row = wm + 4 * (lane >> 5) + t, col = wn + (lane & 28);
+  asm volatile("" : "+v"(row), "+v"(col));  // the elements' offsets are not kept (and spilled) from tile to tile
+  // even lanes: the low halves of (own, partner), odd lanes: the high halves of (partner, own)
+  const uint32_t sel = t & 1 ? 0x03020706u : 0x05040100u;
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int at = row + 32 * i + 8 * g;
+      char* p = address(min(at, rows - 1)) + 2 * (int64_t)col;
+#pragma unroll
+      for (int j = 0; j < WN; ++j) {
+        uint32_t q[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t own = pack16<F16>(f(i, j, 4 * g + 2 * h), f(i, j, 4 * g + 2 * h + 1));
+          const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+          q[h] = __builtin_amdgcn_perm(other, own, sel);
+        }
+        const uint32_t send = t & 2 ? q[0] : q[1];
+        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)send, 0x4e, 0xf, 0xf, true);  // lane ^ 2
+        u32x2_t v;
+        v[0] = t & 2 ? got : q[0];
+        v[1] = t & 2 ? q[1] : got;
+        if (at < rows && col + 32 * j < cols) *reinterpret_cast<u32x2_t*>(p + 64 * j) = v;
+      }
+    }
 }
 
 // The tiles of problem P, worker by worker.  P has
