@@ -8,8 +8,7 @@
 // All three run on the tiles of kq_mm16.h: the weight is read along its rows in
 // the forward pass and across them for dx, and dw contracts over the rows of a
 // group, both operands read across.  Group sizes stay on the device (offsets),
-// so each workgroup numbers the tiles itself: the groups' row tiles are summed
-// in LDS and a tile's group follows from its number.
+// so each workgroup numbers the tiles itself.
 #include "kq_internal.h"
 #include "kq_mm16.h"
 
@@ -29,9 +28,9 @@ struct Args {
   int groups, n, k;
 };
 
+constexpr int TABLE = 4;  // 64 tiles of a worker each
+
 __shared__ __attribute__((aligned(16))) unsigned char lds[mm16::LDS_BYTES];
-__shared__ int first_tile[MAX_GROUPS + 1];  // forward, dx: tiles before each group
-__shared__ int part_sum[mm16::THREADS];
 
 // Offsets are device data: clamped to the rows there are, so that no value of
 // them reads or writes outside.
@@ -40,87 +39,117 @@ __device__ __forceinline__ int64_t clamped(int64_t v, int64_t lo, int64_t hi) { 
 template <int MODE, bool F16>
 struct Problem {
   Args g;
-  int mtiles, ntiles, tiles;  // dw: of one group
+  int mtiles, ntiles, count;
+  // lane l of entry q: this worker's tile 64 q + l (forward, dx)
+  int group_nt[TABLE], mt_of[TABLE];
 
-  __device__ __forceinline__ void range(int e, int64_t& beg, int& n) const {
-    beg = clamped(g.offsets[e], 0, g.rows);
-    n = (int)(clamped(g.offsets[e + 1], beg, g.rows) - beg);
+  __device__ __forceinline__ void range(int e, int& beg, int& n) const {
+    const int64_t b = clamped(g.offsets[e], 0, g.rows);
+    beg = (int)b;
+    n = (int)(clamped(g.offsets[e + 1], b, g.rows) - b);
   }
-  __device__ __forceinline__ int total() const { return tiles; }
+  __device__ __forceinline__ int tiles() const { return count; }
 
-  // Numbers the tiles; every thread of the workgroup calls it.
+  // Numbers the tiles; every thread of the workgroup calls it, before the slabs
+  // use LDS.  The groups' tiles are summed in LDS, then every lane looks one of
+  // the worker's tiles up, so the K loops find theirs in a register.
   __device__ __forceinline__ void setup() {
     const int cols = MODE == FORWARD ? g.n : g.k;
     ntiles = (cols + mm16::BN - 1) / mm16::BN;
-    mtiles = MODE == DW ? (g.n + mm16::BM - 1) / mm16::BM : 0;
+    mtiles = (g.n + mm16::BM - 1) / mm16::BM;
     if (MODE == DW) {
-      tiles = g.groups * mtiles * ntiles;
+      count = mm16::worker_tiles(g.groups * mtiles * ntiles);
       return;
     }
+    int* first = reinterpret_cast<int*>(lds);  // [groups + 1]
+    int* part = first + MAX_GROUPS + 1;
     const int t = threadIdx.x, per = (g.groups + mm16::THREADS - 1) / mm16::THREADS;
     const int e0 = min(t * per, g.groups), e1 = min(e0 + per, g.groups);
     int sum = 0;
     for (int e = e0; e < e1; ++e) {
-      int64_t beg;
-      int n;
+      int beg, n;
       range(e, beg, n);
-      first_tile[e] = sum;
+      first[e] = sum;
       sum += (n + mm16::BM - 1) / mm16::BM * ntiles;
     }
-    part_sum[t] = sum;
+    part[t] = sum;
     __syncthreads();
     int before = 0, all = 0;
     for (int i = 0; i < mm16::THREADS; ++i) {
-      const int v = part_sum[i];
+      const int v = part[i];
       before += i < t ? v : 0;
       all += v;
     }
-    for (int e = e0; e < e1; ++e) first_tile[e] += before;
-    if (t == 0) first_tile[g.groups] = all;
+    for (int e = e0; e < e1; ++e) first[e] += before;
+    if (t == 0) first[g.groups] = all;
     __syncthreads();
-    tiles = __builtin_amdgcn_readfirstlane(all);
-  }
-
-  // Group and position of tile t; hint is the group of this caller's last tile.
-  __device__ __forceinline__ void find(int t, int& hint, int& mt, int& nt) const {
-    if (MODE == DW) {
-      const int per = mtiles * ntiles;
-      hint = t / per;
-      mm16::tile_mn(t - hint * per, mtiles, ntiles, mt, nt);
-    } else {
-      int e = hint;
-      while (__builtin_amdgcn_readfirstlane(first_tile[e + 1]) <= t) ++e;
-      hint = e;
-      const int f = __builtin_amdgcn_readfirstlane(first_tile[e]);
-      const int m = (__builtin_amdgcn_readfirstlane(first_tile[e + 1]) - f) / ntiles;
-      mm16::tile_mn(t - f, m, ntiles, mt, nt);
+    all = __builtin_amdgcn_readfirstlane(all);
+    count = mm16::worker_tiles(all);
+#pragma unroll
+    for (int q = 0; q < TABLE; ++q) {
+      const int tile = mm16::worker_number() + (64 * q + (t & 63)) * (int)gridDim.x;
+      group_nt[q] = mt_of[q] = 0;
+      if (tile < all) {
+        int lo = 0, hi = g.groups;  // first[lo] <= tile < first[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (first[mid] <= tile) lo = mid;
+          else hi = mid;
+        }
+        int nt;
+        mm16::tile_mn(tile - first[lo], (first[lo + 1] - first[lo]) / ntiles, ntiles, mt_of[q], nt);
+        group_nt[q] = lo << 16 | nt;
+      }
     }
+    __syncthreads();  // the slabs' loads overwrite the sums
   }
 
-  __device__ __forceinline__ mm16::Tile tile(int t, int& hint) const {
-    int mt, nt, n;
-    int64_t beg;
-    find(t, hint, mt, nt);
-    range(hint, beg, n);
+  __device__ __forceinline__ int entry(const int (&v)[TABLE], int i) const {
+    const int q = i >> 6, l = i & 63;
+    int r = __builtin_amdgcn_readlane(v[0], l);
+#pragma unroll
+    for (int x = 1; x < TABLE; ++x) r = q == x ? __builtin_amdgcn_readlane(v[x], l) : r;
+    return r;
+  }
+
+  // Group, first row and row count of it, and position of this worker's tile i.
+  __device__ __forceinline__ void find(int i, int& e, int& beg, int& n, int& mt, int& nt) const {
+    if (MODE == DW) {
+      const int t = mm16::worker_number() + i * (int)gridDim.x, per = mtiles * ntiles;
+      e = t / per;
+      mm16::tile_mn(t - e * per, mtiles, ntiles, mt, nt);
+    } else {
+      const int en = entry(group_nt, i);
+      e = en >> 16;
+      nt = en & 0xffff;
+      mt = entry(mt_of, i);
+    }
+    range(e, beg, n);
+  }
+
+  __device__ __forceinline__ mm16::Tile tile(int i) const {
+    int e, beg, n, mt, nt;
+    find(i, e, beg, n, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     mm16::Tile r;
     r.a.ld = g.ld_in;
     r.b.ld = g.ld_other;
+    r.cols = mm16::BN;
     if (MODE == DW) {
       r.kc = n;
       r.rows = min(mm16::BM, g.n - m0);
-      r.a.base = g.rows_in + beg * g.ld_in + 2 * (int64_t)m0;
+      r.a.base = g.rows_in + (int64_t)beg * g.ld_in + 2 * (int64_t)m0;
       r.a.width = 2u * (uint32_t)(g.n - m0);
-      r.b.base = g.other + beg * g.ld_other + 2 * (int64_t)n0;
+      r.b.base = g.other + (int64_t)beg * g.ld_other + 2 * (int64_t)n0;
       r.b.width = 2u * (uint32_t)(g.k - n0);
       r.a.rows = r.b.rows = 0;
     } else {
       r.kc = MODE == FORWARD ? g.k : g.n;
       r.rows = min(mm16::BM, n - m0);
-      r.a.base = g.rows_in + (beg + m0) * g.ld_in;
+      r.a.base = g.rows_in + (int64_t)(beg + m0) * g.ld_in;
       r.a.rows = r.rows;
       r.a.width = 0;
-      const char* w = g.other + (int64_t)hint * g.n * g.ld_other;
+      const char* w = g.other + (int64_t)e * g.n * g.ld_other;
       if (MODE == FORWARD) {
         r.b.base = w + (int64_t)n0 * g.ld_other;
         r.b.rows = min(mm16::BN, g.n - n0);
@@ -135,18 +164,16 @@ struct Problem {
   }
 
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const mm16::Tile& tl, int t, int hint, int wm, int wn,
+  __device__ __forceinline__ void epilogue(const mm16::Tile& tl, int i, int wm, int wn,
                                            const float16_t (&acc)[NB][WN], int lane) const {
-    int mt, nt, n;
-    int64_t beg;
-    find(t, hint, mt, nt);
-    range(hint, beg, n);
+    int e, beg, n, mt, nt;
+    find(i, e, beg, n, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
-    const int64_t row0 = MODE == DW ? (int64_t)hint * g.n + m0 : beg + m0;
+    const int64_t row0 = MODE == DW ? (int64_t)e * g.n + m0 : beg + m0;
     char* out = g.out + row0 * g.ld_out + 2 * (int64_t)n0;
     mm16::store16<NB, WN, F16>([&](int r) { return out + r * (int64_t)g.ld_out; }, tl.rows,
                                (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, lane,
-                               [&](int i, int j, int r) { return acc[i][j][r]; });
+                               [&](int x, int y, int r) { return acc[x][y][r]; });
   }
 };
 
@@ -163,10 +190,11 @@ __device__ __forceinline__ void zero_rows(const Args& g, int cols) {
 
 template <int MODE, bool F16>
 __global__ __launch_bounds__(mm16::THREADS, 1) void grouped_kernel(Args g) {
-  Problem<MODE, F16> p{g, 0, 0, 0};
+  Problem<MODE, F16> p;
+  p.g = g;
   p.setup();
   if (MODE != DW) zero_rows(g, MODE == FORWARD ? g.n : g.k);
-  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE != DW, Problem<MODE, F16>> core(p, lds);
+  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE == DW ? mm16::WHOLE : mm16::SMALL_ROWS, Problem<MODE, F16>> core(p, lds);
   core.run();
 }
 
@@ -176,9 +204,14 @@ static hipError_t launch(int dtype, const Args& g, hipStream_t st) {
   hipError_t e = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
   if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   if (e != hipSuccess) return e;
-  const unsigned grid = cus >= 8 ? (unsigned)(cus / 8 * 8) : 8u;
-  if (dtype == KQ_DT_F16) grouped_kernel<MODE, true><<<grid, mm16::THREADS, 0, st>>>(g);
-  else grouped_kernel<MODE, false><<<grid, mm16::THREADS, 0, st>>>(g);
+  int64_t grid = cus >= 8 ? cus / 8 * 8 : 8;
+  if (MODE != DW) {  // a worker's table holds 256 tiles: more workers where there may be more
+    const int64_t most = (g.rows / mm16::BM + (g.rows < g.groups ? g.rows : g.groups)) *
+                         (((MODE == FORWARD ? g.n : g.k) + mm16::BN - 1) / mm16::BN);
+    grid *= (most + grid * 64 * TABLE - 1) / (grid * 64 * TABLE);
+  }
+  if (dtype == KQ_DT_F16) grouped_kernel<MODE, true><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
+  else grouped_kernel<MODE, false><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
   return hipGetLastError();
 }
 

@@ -107,6 +107,8 @@ __global__ __launch_bounds__(1024) void alpha_kernel(const float* __restrict__ g
   }
 }
 
+__device__ __forceinline__ int tile_number(int i) { return mm16::worker_number() + i * (int)gridDim.x; }
+
 struct Gather {
   const char* h;
   int64_t ldh;  // bytes
@@ -190,12 +192,14 @@ struct LogitProblem {
   LogitArgs g;
   int count, mtiles, ntiles;
 
-  __device__ __forceinline__ int total() const { return mtiles * ntiles; }
-  __device__ __forceinline__ Tile tile(int t, int&) const {
+  __device__ __forceinline__ int tiles() const { return mm16::worker_tiles(mtiles * ntiles); }
+  __device__ __forceinline__ Tile tile(int x) const {
+    const int t = tile_number(x);
     int mt, nt;
     mm16::tile_mn(t, mtiles, ntiles, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     Tile r;
+    r.cols = mm16::BN;
     r.kc = g.k;
     r.rows = min(mm16::BM, g.rows - m0);
     r.a = {g.w + (int64_t)m0 * g.k * 2, (uint32_t)g.k * 2u, r.rows, 0u};
@@ -203,8 +207,9 @@ struct LogitProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int t, int, int wm, int wn, const float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, const float16_t (&acc)[NB][WN],
                                            int lane) const {
+    const int t = tile_number(x);
     int mt, nt;
     mm16::tile_mn(t, mtiles, ntiles, mt, nt);
     const int v0 = g.first + mt * mm16::BM, n0 = nt * mm16::BN;
@@ -272,7 +277,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void logit_kernel(LogitArgs g) {
   LogitProblem<GRAD> p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (p.count + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, false, false, false, LogitProblem<GRAD>> core(p, lds);
+  mm16::Core<false, false, false, mm16::WHOLE, LogitProblem<GRAD>> core(p, lds);
   core.run();
 }
 
@@ -297,8 +302,9 @@ struct DhProblem {
   DhArgs g;
   int count, mtiles, ntiles;
 
-  __device__ __forceinline__ int total() const { return mtiles * ntiles * g.slices; }
-  __device__ __forceinline__ Tile tile(int t, int&) const {
+  __device__ __forceinline__ int tiles() const { return mm16::worker_tiles(mtiles * ntiles * g.slices); }
+  __device__ __forceinline__ Tile tile(int x) const {
+    const int t = tile_number(x);
     int mt, nt;
     const int per = mtiles * ntiles, sl = t / per;
     mm16::tile_mn(t - sl * per, mtiles, ntiles, mt, nt);
@@ -306,6 +312,7 @@ struct DhProblem {
     const int v0 = sl * steps / g.slices * mm16::BK;  // slices <= 16, steps <= 2^18
     const int v1 = min((sl + 1) * steps / g.slices * mm16::BK, g.rows);
     Tile r;
+    r.cols = mm16::BN;
     r.kc = v1 - v0;
     r.rows = min(mm16::BM, count - m0);
     r.a = {g.dt + ((int64_t)v0 * g.ldg + m0) * 2, (uint32_t)g.ldg * 2u, 0, (uint32_t)((count + 7) / 8 * 8 - m0) * 2u};
@@ -313,8 +320,9 @@ struct DhProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int t, int, int wm, int wn, const float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, const float16_t (&acc)[NB][WN],
                                            int lane) const {
+    const int t = tile_number(x);
     int mt, nt;
     const int per = mtiles * ntiles, sl = t / per;
     mm16::tile_mn(t - sl * per, mtiles, ntiles, mt, nt);
@@ -342,7 +350,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
   DhProblem p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (p.count + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
-  mm16::Core<true, true, false, true, DhProblem> core(p, lds);
+  mm16::Core<true, true, false, mm16::SMALL_ROWS, DhProblem> core(p, lds);
   core.run();
 }
 
@@ -379,12 +387,14 @@ struct DwProblem {
   DwArgs g;
   int count, mtiles, ntiles;  // count: rounded up to 8, the rows behind it are zero
 
-  __device__ __forceinline__ int total() const { return mtiles * ntiles; }
-  __device__ __forceinline__ Tile tile(int t, int&) const {
+  __device__ __forceinline__ int tiles() const { return mm16::worker_tiles(mtiles * ntiles); }
+  __device__ __forceinline__ Tile tile(int x) const {
+    const int t = tile_number(x);
     int mt, nt;
     mm16::tile_mn(t, mtiles, ntiles, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     Tile r;
+    r.cols = mm16::BN;
     r.kc = count;
     r.rows = min(mm16::BM, g.rows - m0);
     r.a = {g.dt + (int64_t)m0 * g.ldg * 2, (uint32_t)g.ldg * 2u, r.rows, 0u};
@@ -392,8 +402,9 @@ struct DwProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int t, int, int wm, int wn, const float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, const float16_t (&acc)[NB][WN],
                                            int lane) const {
+    const int t = tile_number(x);
     int mt, nt;
     mm16::tile_mn(t, mtiles, ntiles, mt, nt);
     const int n0 = nt * mm16::BN;
@@ -408,7 +419,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dw_kernel(DwArgs g) {
   DwProblem p{g, (__builtin_amdgcn_readfirstlane(*g.count) + 7) / 8 * 8, 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, true, false, false, DwProblem> core(p, lds);
+  mm16::Core<false, true, false, mm16::WHOLE, DwProblem> core(p, lds);
   core.run();
 }
 

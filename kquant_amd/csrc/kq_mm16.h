@@ -13,23 +13,29 @@
 // v_mfma_f32_32x32x16 (2048 cycles), while LDS moves 128 KiB of fragment reads
 // and 64 KiB of new operands for it (1536 cycles).  So everything else has a
 // fixed place between two MFMAs (sched_barrier pins it):
-//  * operands go HBM -> LDS by 16-byte direct loads into two stages of 64 KiB.
-//    A stage is whole 128-byte lines of rows (contraction-major) or 512-byte
-//    runs of 64 contraction rows (the other form), XOR-swizzled so that the
-//    lanes of a read fall on distinct banks.
+//  * operands go HBM -> LDS by 16-byte direct loads, a step's share of one
+//    operand a slab of 32 KiB, and all of LDS is five slabs: A and B of the step
+//    in use and of the next one, and A of the step after.  A slab is whole
+//    128-byte lines of rows (contraction-major) or 512-byte runs of 64
+//    contraction rows (the other form), XOR-swizzled so that the lanes of a read
+//    fall on distinct banks.
 //  * a step's fragments are read one step ahead: block b of 16 MFMAs (k16
 //    block b) reads the fragments of k16 block (b + 3) % 4, of this step in
 //    block 0 and of the next one after it.  Operands across the contraction
 //    are read transposed (ds_read_b64_tr_b16).
 //  * one barrier a step, after block 0: every wave then holds all of the
-//    current stage in registers, so the stage is free and the loads of the
-//    step after next go into it, in block 1.
+//    current slabs in registers, so both are free.  B of the step after next is
+//    loaded in block 1, A of the one after that in blocks 2 and 3: a direct
+//    load takes 16 cycles of the CU's address unit, so 64 of them in one block
+//    of 512 cycles held its MFMAs up (two stages of both operands, all loads in
+//    block 1: 3325 cycles a step at 4096 x 12288 x 7168).
 //  * a resource is rebased every step, and ends with the operand's last valid
 //    row and column: rows past a ragged group or a matrix read as zero without
 //    touching memory, and offsets stay below 2^31 whatever the matrix's size.
 // Row tiles of at most 128 rows (the ragged end of a group) run as four waves
 // side by side over the columns, 32 NB rows x 64 columns each, so rows that
-// are not there cost no MFMA beyond the next 32, 64 or 128.
+// are not there cost no MFMA beyond the next 32, 64 or 128; narrow column tiles
+// run as four waves down the rows.
 //
 // The kernels are persistent: a problem P numbers its tiles, worker w takes
 // w, w + G, ... with the workers of one XCD numbered consecutively, so the 32
@@ -44,10 +50,10 @@ namespace kq {
 namespace mm16 {
 
 constexpr int BM = 256, BN = 256, BK = 64, THREADS = 256;
-constexpr int SLAB = 256 * BK * 2;     // one operand of a stage
-constexpr int STAGE = 2 * SLAB;
-constexpr int LDS_BYTES = 2 * STAGE;
-constexpr int LOADS = 8;               // direct loads per wave, operand and stage
+constexpr int SLAB = 256 * BK * 2;     // one operand of a step
+constexpr int SLOTS = 5;               // slabs in LDS
+constexpr int LDS_BYTES = SLOTS * SLAB;
+constexpr int LOADS = 8;               // direct loads per wave and slab
 constexpr int GROUP_M = 4;             // row tiles per group of the tile order
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
 constexpr int64_t MAX_LD = 1 << 22;    // elements: 256 rows stay below OUT_OF_RANGE
@@ -72,6 +78,7 @@ struct Tile {
   Operand a, b;
   int kc;    // contraction length (0 gives zeros)
   int rows;  // rows of the tile that are stored
+  int cols;  // and columns
 };
 
 // The same in every lane, in scalar registers.
@@ -239,75 +246,74 @@ __device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm
     }
 }
 
+// One operand's loads, slab after slab, across this worker's tiles.
+template <bool ACROSS>
+struct Side {
+  Operand o;
+  Loader<ACROSS> l;
+  int i, k, kc;  // tile (of this worker's), contraction index of the next slab, the tile's contraction length
+
+  template <class P, class Pick>
+  __device__ __forceinline__ void set(const P& p, int tiles, int lw, int lane, Pick&& pick) {
+    k = 0;
+    kc = 0;  // loads past the last tile read zeros and touch nothing
+    if (i < tiles) {
+      const Tile t = p.tile(i);
+      o = pick(t);
+      make_scalar(o);
+      kc = __builtin_amdgcn_readfirstlane(t.kc);
+      l.set(o, lw, lane);
+    }
+  }
+  __device__ __forceinline__ dma::i32x4_t resource() const { return Loader<ACROSS>::resource(o, k, kc); }
+  // load u (0..7) of the slab at k into LDS slot base `slot`
+  __device__ __forceinline__ void issue(int u, const dma::i32x4_t& r, uint32_t slot, int lw) const {
+    dma::load_to_lds16(r, l.offset(u, kc - k), slot + (uint32_t)((4 * u + lw) * 1024));
+  }
+};
+
+enum { WHOLE = 0, SMALL_ROWS = 1, SMALL_COLS = 2 };  // which tiles may be narrow
+
 // The tiles of problem P, worker by worker.  P has
-//   int total()                         tiles
-//   Tile tile(int t, int& hint)         tile t (hint: this caller's, 0 at first; t never falls)
-//   epilogue<NB, WN>(const Tile&, int t, int hint, int wm, int wn, const float16_t (&acc)[NB][WN], int lane)
-// with element r of acc[i][j] at row wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4,
-// column wn + 32 j + lane % 32 of the tile.  SMALL: row tiles of up to 128
-// rows occur.
-template <bool AA, bool BA, bool F16, bool SMALL, class P>
+//   int tiles()          this worker's number of them
+//   Tile tile(int i)     its i-th
+//   epilogue<NB, WN>(const Tile&, int i, int wm, int wn, const float16_t (&acc)[NB][WN], int lane)
+// with element r of acc[a][b] at row wm + 32 a + 8 (r / 4) + 4 (lane / 32) + r % 4,
+// column wn + 32 b + lane % 32 of the tile.
+template <bool AA, bool BA, bool F16, int NARROW, class P>
 struct Core {
   const P& p;
   uint32_t lds0;
-  int lane, lw, G;
-  // load side: item lt's tile and the next stage's contraction index and slot
-  int lt, lk, lslot, lhint;
-  Tile ld;
-  Loader<AA> la;
-  Loader<BA> lb;
-  int cslot;  // stage in use
+  int lane, lw, tiles;
+  Side<AA> sa;
+  Side<BA> sb;
+  int ca, cb;  // slots of the slabs in use
 
   __device__ __forceinline__ Core(const P& prob, unsigned char* l) : p(prob) {
     lane = threadIdx.x & 63;
     lw = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     lds0 = dma::lds_offset_of(l);
-    G = gridDim.x;
   }
-  __device__ __forceinline__ void set_load_tile() {
-    lk = 0;
-    if (lt < p.total()) {
-      ld = p.tile(lt, lhint);
-      make_scalar(ld.a);
-      make_scalar(ld.b);
-      ld.kc = __builtin_amdgcn_readfirstlane(ld.kc);
-      la.set(ld.a, lw, lane);
-      lb.set(ld.b, lw, lane);
-    } else {
-      ld.kc = 0;  // loads past the end read zeros and touch nothing
+  static __device__ __forceinline__ int after(int slot) { return slot >= SLOTS - 2 ? slot - (SLOTS - 2) : slot + 2; }
+  __device__ __forceinline__ uint32_t slot(int c) const { return lds0 + (uint32_t)(c * SLAB); }
+  __device__ __forceinline__ void set_a() { sa.set(p, tiles, lw, lane, [](const Tile& t) { return t.a; }); }
+  __device__ __forceinline__ void set_b() { sb.set(p, tiles, lw, lane, [](const Tile& t) { return t.b; }); }
+  __device__ __forceinline__ void next_a() {
+    if ((sa.k += BK) >= sa.kc) {
+      ++sa.i;
+      set_a();
     }
   }
-  // load u of the next stage: 0..7 operand A, 8..15 operand B
-  __device__ __forceinline__ void issue_one(int u, const dma::i32x4_t& ra, const dma::i32x4_t& rb) {
-    const uint32_t base = lds0 + (uint32_t)(lslot * STAGE);
-    if (u < LOADS)
-      dma::load_to_lds16(ra, la.offset(u, ld.kc - lk), base + (uint32_t)((4 * u + lw) * 1024));
-    else
-      dma::load_to_lds16(rb, lb.offset(u - LOADS, ld.kc - lk), base + (uint32_t)(SLAB + (4 * (u - LOADS) + lw) * 1024));
-  }
-  __device__ __forceinline__ void resources(dma::i32x4_t& ra, dma::i32x4_t& rb) {
-    ra = Loader<AA>::resource(ld.a, lk, ld.kc);
-    rb = Loader<BA>::resource(ld.b, lk, ld.kc);
-  }
-  __device__ __forceinline__ void advance() {
-    lslot ^= 1;
-    lk += BK;
-    if (lk >= ld.kc) {
-      lt += G;
-      set_load_tile();
+  __device__ __forceinline__ void next_b() {
+    if ((sb.k += BK) >= sb.kc) {
+      ++sb.i;
+      set_b();
     }
-  }
-  __device__ __forceinline__ void issue_stage() {
-    dma::i32x4_t ra, rb;
-    resources(ra, rb);
-#pragma unroll
-    for (int u = 0; u < 2 * LOADS; ++u) issue_one(u, ra, rb);
-    advance();
   }
 
   // Wave tile of NB x WN blocks at (wm, wn): this item's steps, then its epilogue.
   template <int NB, int WN>
-  __device__ __forceinline__ void item(const Tile& tl, int t, int hint, int wm, int wn) {
+  __device__ __forceinline__ void item(const Tile& tl, int it, int wm, int wn) {
     Reader<AA, NB> fa;
     Reader<BA, WN> fb;
     int l = lane;
@@ -323,22 +329,19 @@ struct Core {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     // fragment f of k16 block kk: 0..NB-1 of A, then B
-    auto read_one = [&](uint32_t st, int kk, int f) {
-      if (f < NB) a[kk][f] = fa.read(st, kk, f);
-      else b[kk][f - NB] = fb.read(st + SLAB, kk, f - NB);
+    auto read_one = [&](uint32_t as, uint32_t bs, int kk, int f) {
+      if (f < NB) a[kk][f] = fa.read(as, kk, f);
+      else b[kk][f - NB] = fb.read(bs, kk, f - NB);
     };
     const int steps = steps_of(tl.kc);
-    {  // this item's first stage has landed: in run() or at the last barrier of the item before
-
-      const uint32_t st = lds0 + (uint32_t)(cslot * STAGE);
+    // this item's first slabs have landed: in run() or at the last barrier of the item before
 #pragma unroll
-      for (int kk = 0; kk < 3; ++kk)
+    for (int kk = 0; kk < 3; ++kk)
 #pragma unroll
-        for (int f = 0; f < NB + WN; ++f) read_one(st, kk, f);
-    }
+      for (int f = 0; f < NB + WN; ++f) read_one(slot(ca), slot(cb), kk, f);
     constexpr int NM = NB * WN;  // MFMAs of a k16 block
     for (int s = 0; s < steps; ++s) {
-      const uint32_t cur = lds0 + (uint32_t)(cslot * STAGE), nxt = lds0 + (uint32_t)((cslot ^ 1) * STAGE);
+      const uint32_t acur = slot(ca), bcur = slot(cb), anxt = slot(after(ca)), bnxt = slot(after(cb));
       dma::i32x4_t ra, rb;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
@@ -346,54 +349,85 @@ struct Core {
         for (int m = 0; m < NM; ++m) {
           const int i = m / WN, j = m % WN;
           acc[i][j] = mfma<F16>(a[kk][i], b[kk][j], acc[i][j]);
-          // fragments of k16 block (kk + 3) % 4 and, in block 1, the loads
 #pragma unroll
           for (int f = m * (NB + WN) / NM; f < (m + 1) * (NB + WN) / NM; ++f)
-            read_one(kk == 0 ? cur : nxt, (kk + 3) & 3, f);
-          if (kk == 1) {
+            read_one(kk == 0 ? acur : anxt, kk == 0 ? bcur : bnxt, (kk + 3) & 3, f);
+          if (kk == 1) {  // B of the step after next, into A's slot
 #pragma unroll
-            for (int u = m * 2 * LOADS / NM; u < (m + 1) * 2 * LOADS / NM; ++u) issue_one(u, ra, rb);
+            for (int u = m * LOADS / NM; u < (m + 1) * LOADS / NM; ++u) sb.issue(u, rb, acur, lw);
+          }
+          if (kk >= 2) {  // A of the step after that, into B's slot
+#pragma unroll
+            for (int u = ((kk - 2) * NM + m) * LOADS / (2 * NM); u < ((kk - 2) * NM + m + 1) * LOADS / (2 * NM); ++u)
+              sa.issue(u, ra, bcur, lw);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
         if (kk == 0) {
-          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): no read of the current stage is in flight
-          dma::wait_and_barrier<0>();          // the next stage has landed, the current one is free
-          resources(ra, rb);
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): no read of the current slabs is in flight
+          dma::wait_and_barrier<LOADS>();      // the next ones have landed, the current ones are free
+          rb = sb.resource();
+          ra = sa.resource();
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (kk == 1) advance();
+        if (kk == 1) next_b();
+        if (kk == 3) next_a();
       }
-      cslot ^= 1;
+      ca = after(ca);
+      cb = after(cb);
     }
-    p.template epilogue<NB, WN>(tl, t, hint, wm, wn, acc, l);
+    p.template epilogue<NB, WN>(tl, it, wm, wn, acc, l);
   }
 
   __device__ __forceinline__ void run() {
-    const int worker = (int)(blockIdx.x % 8) * (G / 8) + (int)(blockIdx.x / 8);
-    const int total = p.total();
-    if (worker >= total) return;
-    lt = worker;
-    lslot = cslot = 0;
-    lhint = 0;
-    set_load_tile();
-    issue_stage();
-    issue_stage();
-    dma::wait_and_barrier<2 * LOADS>();
-    int hint = 0;
-    for (int t = worker; t < total; t += G) {
-      const Tile tl = p.tile(t, hint);
-      if (SMALL && tl.rows <= 128) {
-        if (tl.rows <= 32) item<1, 2>(tl, t, hint, 0, 64 * lw);
-        else if (tl.rows <= 64) item<2, 2>(tl, t, hint, 0, 64 * lw);
-        else item<4, 2>(tl, t, hint, 0, 64 * lw);
+    tiles = p.tiles();
+    if (tiles <= 0) return;
+    sa.i = sb.i = 0;
+    ca = 0;
+    cb = 1;
+    set_a();
+    set_b();
+#pragma unroll
+    for (int q = 0; q < SLOTS; ++q) {  // A, B, A, B, A
+      if (q & 1) {
+        const dma::i32x4_t r = sb.resource();
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) sb.issue(u, r, slot(q), lw);
+        next_b();
       } else {
-        item<4, 4>(tl, t, hint, (lw >> 1) * 128, (lw & 1) * 128);
+        const dma::i32x4_t r = sa.resource();
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) sa.issue(u, r, slot(q), lw);
+        next_a();
+      }
+    }
+    dma::wait_and_barrier<(SLOTS - 2) * LOADS>();
+    for (int i = 0; i < tiles; ++i) {
+      const Tile tl = p.tile(i);
+      if (NARROW == SMALL_ROWS && tl.rows <= 128) {
+        if (tl.rows <= 32) item<1, 2>(tl, i, 0, 64 * lw);
+        else if (tl.rows <= 64) item<2, 2>(tl, i, 0, 64 * lw);
+        else item<4, 2>(tl, i, 0, 64 * lw);
+      } else if (NARROW == SMALL_COLS && tl.cols <= 128) {
+        if (tl.cols <= 32) item<2, 1>(tl, i, 64 * lw, 0);
+        else if (tl.cols <= 64) item<2, 2>(tl, i, 64 * lw, 0);
+        else item<2, 4>(tl, i, 64 * lw, 0);
+      } else {
+        item<4, 4>(tl, i, (lw >> 1) * 128, (lw & 1) * 128);
       }
     }
     __builtin_amdgcn_s_waitcnt(dma::waitcnt_vm(0));  // no load may land after the workgroup ends
   }
 };
+
+// Workers of one XCD (workgroup b runs on XCD b % 8) are numbered consecutively.
+__device__ __forceinline__ int worker_number() {
+  return (int)(blockIdx.x % 8) * ((int)gridDim.x / 8) + (int)(blockIdx.x / 8);
+}
+__device__ __forceinline__ int worker_tiles(int total) {
+  const int w = worker_number(), g = (int)gridDim.x;
+  return total > w ? (total - w - 1) / g + 1 : 0;
+}
 
 }  // namespace mm16
 }  // namespace kq
