@@ -44,9 +44,11 @@ struct Problem {
   int group_nt[TABLE], mt_of[TABLE];
 
   __device__ __forceinline__ void range(int e, int& beg, int& n) const {
-    const int64_t b = clamped(g.offsets[e], 0, g.rows);
+    // constant memory: the scalar loads of a group that is the same in every lane
+    const auto* o = (const __attribute__((address_space(4))) int64_t*)g.offsets + e;
+    const int64_t b = clamped(o[0], 0, g.rows);
     beg = (int)b;
-    n = (int)(clamped(g.offsets[e + 1], b, g.rows) - b);
+    n = (int)(clamped(o[1], b, g.rows) - b);
   }
   __device__ __forceinline__ int tiles() const { return count; }
 
@@ -165,15 +167,15 @@ struct Problem {
 
   template <int NB, int WN>
   __device__ __forceinline__ void epilogue(const mm16::Tile& tl, int i, int wm, int wn,
-                                           const float16_t (&acc)[NB][WN], int lane) const {
+                                           float16_t (&acc)[NB][WN], int lane) const {
     int e, beg, n, mt, nt;
     find(i, e, beg, n, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     const int64_t row0 = MODE == DW ? (int64_t)e * g.n + m0 : beg + m0;
     char* out = g.out + row0 * g.ld_out + 2 * (int64_t)n0;
     mm16::store16<NB, WN, F16>([&](int r) { return out + r * (int64_t)g.ld_out; }, tl.rows,
-                               (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, lane,
-                               [&](int x, int y, int r) { return acc[x][y][r]; });
+                               (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, acc, lane,
+                               [](int, int, int, float v) { return v; });
   }
 };
 

@@ -12,7 +12,7 @@
 // What bounds it: the matrix products (2 T V K flop forward, 6 T V K backward,
 // a third of which recomputes z); at few tokens, the head's bytes.  The
 // logits never reach memory in the forward pass: a tile's epilogue reduces its
-// 128 vocabulary rows per wave to a running maximum and a sum of exponentials
+// 64 or 128 vocabulary rows per wave to a running maximum and a sum of exponentials
 // per token, and picks the target's logit.  The product is taken as W H^T, so
 // a lane holds one token's logits and reduces them in registers.  The
 // backward pass walks the vocabulary in pieces whose gradient d^T (bf16) fits
@@ -169,8 +169,8 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // The logits of a vocabulary piece: W rows [first, first + rows) x counted
-// tokens.  Forward: partial maxima and sums, part[(2 tile + wave row)][token],
-// and the targets' logits.  GRAD: d^T, row stride ldg elements, zero in the
+// tokens.  Forward: partial maxima and sums of 64 vocabulary rows each,
+// part[4 tile + row / 64][token], and the targets' logits.  GRAD: d^T, row stride ldg elements, zero in the
 // token columns from count up to a multiple of 8.
 struct LogitArgs {
   const char* w;  // bf16 rows of the piece
@@ -199,7 +199,7 @@ struct LogitProblem {
     mm16::tile_mn(t, mtiles, ntiles, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     Tile r;
-    r.cols = mm16::BN;
+    r.cols = min(mm16::BN, count - n0);
     r.kc = g.k;
     r.rows = min(mm16::BM, g.rows - m0);
     r.a = {g.w + (int64_t)m0 * g.k * 2, (uint32_t)g.k * 2u, r.rows, 0u};
@@ -207,7 +207,7 @@ struct LogitProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, const float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
                                            int lane) const {
     const int t = tile_number(x);
     int mt, nt;
@@ -227,46 +227,75 @@ struct LogitProblem {
       char* out = g.dt + ((int64_t)mt * mm16::BM * g.ldg + n0) * 2;
       const int row = wm + 4 * (lane >> 5);
       mm16::store16<NB, WN, false>([&](int r) { return out + r * (int64_t)g.ldg * 2; }, tl.rows,
-                                   (count + 7) / 8 * 8 - n0, wm, wn, lane, [&](int i, int j, int r) {
+                                   (count + 7) / 8 * 8 - n0, wm, wn, acc, lane, [&](int i, int j, int r, float z) {
         const int at = row + 32 * i + 8 * (r >> 2) + (r & 3);
-        const float p = __builtin_amdgcn_exp2f((acc[i][j][r] - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
+        const float p = __builtin_amdgcn_exp2f((z - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
         return n0 + wn + 32 * j + (lane & 31) < count ? up[j] * p : 0.0f;
       });
       return;
     }
     const int row = wm + 4 * (lane >> 5);  // this lane's rows: row + 32 i + 8 (r / 4) + r % 4
-    const bool whole = tl.rows >= wm + 32 * NB;
+    float m[WN], s[WN], hit[WN];
+    int at[WN];  // the target's position from this lane's first row
+    bool some = false;
 #pragma unroll
     for (int j = 0; j < WN; ++j) {
-      float m = -__builtin_inff(), s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (whole || row + 32 * i + 8 * (r >> 2) + (r & 3) < tl.rows) m = fmaxf(m, acc[i][j][r]);
-      const float ref = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (whole || row + 32 * i + 8 * (r >> 2) + (r & 3) < tl.rows)
-            s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * LOG2E);
-      join(m, s, __shfl_xor(m, 32), __shfl_xor(s, 32));
+      m[j] = -__builtin_inff();
+      s[j] = hit[j] = 0.0f;
       const int c = n0 + wn + 32 * j + (lane & 31);
-      const bool live = c < count;
-      if (live && lane < 32) {
-        float2_t v;
-        v[0] = m;
-        v[1] = s;
-        g.part[(int64_t)(2 * (g.part0 + mt) + (wm >> 7)) * g.tokens + c] = v;
+      at[j] = c < count ? g.target_c[c] - v0 - row : -1;
+      some |= at[j] >= 0 && at[j] < 32 * NB;
+    }
+    // one pass, 16 logits at a time: the sums so far are rescaled to a new maximum
+    const bool any = __any(some);
+    const int left = tl.rows - row;  // of this lane's rows, where the vocabulary ends in them
+    const bool cut = tl.rows < wm + 32 * NB;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      mm16::in_place(acc, i);
+#pragma unroll
+      for (int j = 0; j < WN; ++j) {
+        float z[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = acc[i][j][r];
+        if (any) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) hit[j] = at[j] == 32 * i + 8 * (r >> 2) + (r & 3) ? z[r] : hit[j];
+        }
+        if (cut) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[r] = 32 * i + 8 * (r >> 2) + (r & 3) < left ? z[r] : -__builtin_inff();
+        }
+        float top = m[j];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, z[r]);
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        float sum = s[j] * __builtin_amdgcn_exp2f((m[j] - ref) * LOG2E);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((z[r] - ref) * LOG2E);
+        m[j] = top;
+        s[j] = sum;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const int at = live ? g.target_c[c] - v0 - row : -1;
-      if (__any(at >= 0 && at < 32 * NB && !(at & 4))) {
+    }
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (at == 32 * i + 8 * (r >> 2) + (r & 3)) g.z_target[c] = acc[i][j][r];
+    for (int j = 0; j < WN; ++j) {
+      join(m[j], s[j], __shfl_xor(m[j], 32), __shfl_xor(s[j], 32));
+      const int c = n0 + wn + 32 * j + (lane & 31);
+      if (c < count) {
+        if (lane < 32) {
+          float2_t* part = g.part + (int64_t)(4 * (g.part0 + mt) + (wm >> 6)) * g.tokens + c;
+          float2_t v;
+          v[0] = m[j];
+          v[1] = s[j];
+          part[0] = v;
+          if (NB == 4) {  // 128 rows at once: nothing is left for the second 64
+            v[0] = -__builtin_inff();
+            v[1] = 0.0f;
+            part[g.tokens] = v;
+          }
+        }
+        if (at[j] >= 0 && at[j] < 32 * NB && !(at[j] & 4)) g.z_target[c] = hit[j];
       }
     }
   }
@@ -277,7 +306,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void logit_kernel(LogitArgs g) {
   LogitProblem<GRAD> p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (p.count + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, false, false, mm16::WHOLE, LogitProblem<GRAD>> core(p, lds);
+  mm16::Core<false, false, false, mm16::SMALL_COLS, LogitProblem<GRAD>> core(p, lds);
   core.run();
 }
 
@@ -320,7 +349,7 @@ struct DhProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, const float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
                                            int lane) const {
     const int t = tile_number(x);
     int mt, nt;
@@ -331,8 +360,8 @@ struct DhProblem {
       const int* map = g.rows_of + m0;
       char* out = g.dh + 2 * (int64_t)n0;
       const float alpha = *g.alpha;
-      mm16::store16<NB, WN, false>([&](int r) { return out + map[r] * g.lddh; }, tl.rows, g.k - n0, wm, wn, lane,
-                                   [&](int i, int j, int r) { return alpha * acc[i][j][r]; });
+      mm16::store16<NB, WN, false>([&](int r) { return out + map[r] * g.lddh; }, tl.rows, g.k - n0, wm, wn, acc, lane,
+                                   [&](int, int, int, float v) { return alpha * v; });
     } else {
       float* out = g.planes + ((int64_t)sl * g.tokens + m0) * g.k + n0;
       const uint32_t ld = (uint32_t)g.k;
@@ -402,7 +431,7 @@ struct DwProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, const float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
                                            int lane) const {
     const int t = tile_number(x);
     int mt, nt;
@@ -410,8 +439,8 @@ struct DwProblem {
     const int n0 = nt * mm16::BN;
     char* out = g.dw + ((int64_t)mt * mm16::BM * g.k + n0) * 2;
     const float alpha = *g.alpha;
-    mm16::store16<NB, WN, false>([&](int r) { return out + r * (int64_t)g.k * 2; }, tl.rows, g.k - n0, wm, wn, lane,
-                                 [&](int i, int j, int r) { return alpha * acc[i][j][r]; });
+    mm16::store16<NB, WN, false>([&](int r) { return out + r * (int64_t)g.k * 2; }, tl.rows, g.k - n0, wm, wn, acc, lane,
+                                 [&](int, int, int, float v) { return alpha * v; });
   }
 };
 
@@ -527,7 +556,7 @@ static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backw
     if (p.slices > 1 || p.pieces > 1) p.o_planes = take(p.slices * tokens * k * 4);
   } else {
     p.o_z = take(tokens * 4);
-    p.o_part = take(2 * p.pieces * ((p.piece + 255) / 256) * tokens * 8);
+    p.o_part = take(4 * p.pieces * ((p.piece + 255) / 256) * tokens * 8);
   }
   p.bytes = at;
   return p;
@@ -632,7 +661,7 @@ extern "C" int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, in
       if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
       a.part0 += (a.rows + mm16::BM - 1) / mm16::BM;
     }
-    loss::combine_kernel<<<(unsigned)((tokens + 15) / 16), 1024, 0, st>>>(a.part, 2 * a.part0, (int)tokens, g.place,
+    loss::combine_kernel<<<(unsigned)((tokens + 15) / 16), 1024, 0, st>>>(a.part, 4 * a.part0, (int)tokens, g.place,
                                                                          g.target_c, a.z_target, losses, lse);
     if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   }

@@ -102,42 +102,6 @@ __device__ __forceinline__ void tile_mn(int tl, int mtiles, int ntiles, int& mt,
 
 __device__ __forceinline__ int steps_of(int kc) { return kc > BK ? (kc + BK - 1) / BK : 1; }
 
-// The direct loads of one operand: this lane's offset in a stage, and the
-// resource of the stage that starts at contraction index k0.
-template <bool ACROSS>
-struct Loader {
-  uint32_t off, step;
-  int col;  // contraction-major: this lane's first contraction index in a stage
-
-  __device__ __forceinline__ void set(const Operand& o, int lw, int lane) {
-    if (ACROSS) {
-      const int row = 2 * lw + (lane >> 5);
-      off = (uint32_t)row * o.ld + (uint32_t)(((lane & 31) ^ (4 * (row & 3))) * 16);
-      step = 8 * o.ld;
-      col = 0;
-    } else {
-      const int row = 8 * lw + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
-      off = (uint32_t)row * o.ld + (uint32_t)(ch * 16);
-      step = 32 * o.ld;
-      col = 8 * ch;
-    }
-  }
-  // load u (0..7) goes to LDS offset (4 u + lw) * 1024 of the operand's slab
-  __device__ __forceinline__ uint32_t offset(int u, int left) const {
-    return (ACROSS || col < left ? off : OUT_OF_RANGE) + (uint32_t)u * step;
-  }
-  static __device__ __forceinline__ dma::i32x4_t resource(const Operand& o, int k0, int kc) {
-    const int left = kc - k0;
-    if (ACROSS) {
-      const int rows = left < BK ? left : BK;
-      return dma::make_rsrc(o.base + (int64_t)k0 * o.ld, rows > 0 ? (uint32_t)(rows - 1) * o.ld + o.width : 0u);
-    }
-    const int wide = left < BK ? left : BK;
-    return dma::make_rsrc(o.base + 2 * (int64_t)k0,
-                          o.rows > 0 && left > 0 ? (uint32_t)(o.rows - 1) * o.ld + 2u * (uint32_t)wide : 0u);
-  }
-};
-
 // This lane's LDS offsets of the fragments of NB 32-row blocks from row0 (a
 // multiple of 64).
 template <bool ACROSS, int NB>
@@ -179,17 +143,26 @@ __device__ __forceinline__ float16_t mfma(u32x4_t a, u32x4_t b, float16_t c) {
                                                  0, 0);
 }
 
+// Keeps block row i of the accumulators where the MFMAs left them until here:
+// moved to other registers all at once after the K loop they would not fit, and
+// a spill's wait for memory would stand in the loop.
+template <int NB, int WN>
+__device__ __forceinline__ void in_place(float16_t (&acc)[NB][WN], int i) {
+#pragma unroll
+  for (int j = 0; j < WN; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
 // The elements of a wave's blocks, f(row, column, value) for rows below `rows`
 // and columns below `cols` of the tile.  The row is made opaque, so that the
 // offsets of the elements are not kept (and spilled) from tile to tile.
 template <int NB, int WN, class F>
-__device__ __forceinline__ void each(int rows, int cols, int wm, int wn, const float16_t (&acc)[NB][WN], int lane,
-                                     F&& f) {
+__device__ __forceinline__ void each(int rows, int cols, int wm, int wn, float16_t (&acc)[NB][WN], int lane, F&& f) {
   int row = wm + 4 * (lane >> 5);
   const int col = wn + (lane & 31);
   asm volatile("" : "+v"(row));
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i) {
+    in_place(acc, i);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int at = row + 32 * i + 8 * (r >> 2) + (r & 3);
@@ -199,6 +172,7 @@ __device__ __forceinline__ void each(int rows, int cols, int wm, int wn, const f
           if (col + 32 * j < cols) f(at, col + 32 * j, acc[i][j][r]);
       }
     }
+  }
 }
 
 // Two 16-bit values of a row pair, rounded to nearest even.
@@ -208,21 +182,23 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 
 // Stores a wave's blocks in 16 bits: rows below `rows`, columns below `cols` (a
-// multiple of 4) of the tile, f(i, j, r) the value of element r of block (i,
-// j), address(row) the 8-byte aligned address of a row's column 0 (asked for rows
-// below `rows` only).  A lane holds four rows of one column and
+// multiple of 4) of the tile, f(i, j, r, v) the value stored for element r of
+// block (i, j), v the accumulated one, and address(row) the 8-byte aligned
+// address of a row's column 0 (asked for rows below `rows` only).  A lane holds four rows of one column and
 // exchanges them with its quad for four columns of one row, in 10 instructions
 // of its registers, so it stores 8 bytes: a store instruction takes as long for
 // 2 bytes a lane.
 template <int NB, int WN, bool F16, class At, class F>
-__device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm, int wn, int lane, F&& f) {
+__device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm, int wn, float16_t (&acc)[NB][WN],
+                                        int lane, F&& f) {
   const int t = lane & 3;
   int row = wm + 4 * (lane >> 5) + t, col = wn + (lane & 28);
   asm volatile("" : "+v"(row), "+v"(col));  // the elements' offsets are not kept (and spilled) from tile to tile
   // even lanes: the low halves of (own, partner), odd lanes: the high halves of (partner, own)
   const uint32_t sel = t & 1 ? 0x03020706u : 0x05040100u;
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i) {
+    in_place(acc, i);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int at = row + 32 * i + 8 * g;
@@ -232,7 +208,8 @@ __device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm
         uint32_t q[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t own = pack16<F16>(f(i, j, 4 * g + 2 * h), f(i, j, 4 * g + 2 * h + 1));
+          const int r = 4 * g + 2 * h;
+          const uint32_t own = pack16<F16>(f(i, j, r, acc[i][j][r]), f(i, j, r + 1, acc[i][j][r + 1]));
           const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xb1, 0xf, 0xf, true);  // lane ^ 1
           q[h] = __builtin_amdgcn_perm(other, own, sel);
         }
@@ -243,32 +220,75 @@ __device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm
         v[1] = t & 2 ? q[1] : got;
         if (at < rows && col + 32 * j < cols) *reinterpret_cast<u32x2_t*>(p + 64 * j) = v;
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  }
 }
 
-// One operand's loads, slab after slab, across this worker's tiles.
+// One operand's loads, slab after slab, across this worker's tiles.  The
+// resource of the next slab is made when the last one's loads are out, in a few
+// scalar instructions: 64 contraction indices on, and only a tile's last slab
+// is shorter.
 template <bool ACROSS>
 struct Side {
-  Operand o;
-  Loader<ACROSS> l;
-  int i, k, kc;  // tile (of this worker's), contraction index of the next slab, the tile's contraction length
+  dma::i32x4_t r;
+  int i, k, kc;       // tile (of this worker's), contraction index of the next slab, the tile's contraction length
+  uint32_t inc;       // bytes from slab to slab
+  uint32_t ld, rows;  // the tile's row stride and valid rows (contraction-major)
+  uint32_t width;     // its valid bytes of a row (across)
+  uint32_t off, at, step;  // this lane's offset in a slab, in this slab, and from load to load
+  int col;            // contraction-major: this lane's first contraction index in a slab
 
+  // what the slab at k ends with: rows and columns past it read as zero
+  __device__ __forceinline__ void limit() {
+    const int left = kc - k, n = left < BK ? left : BK;
+    if (ACROSS) {
+      r[2] = n > 0 ? (int)((uint32_t)(n - 1) * ld + width) : 0;
+    } else {
+      r[2] = n > 0 && rows > 0 ? (int)((rows - 1) * ld + 2u * (uint32_t)n) : 0;
+      at = col < left ? off : OUT_OF_RANGE;
+    }
+  }
   template <class P, class Pick>
   __device__ __forceinline__ void set(const P& p, int tiles, int lw, int lane, Pick&& pick) {
     k = 0;
     kc = 0;  // loads past the last tile read zeros and touch nothing
     if (i < tiles) {
       const Tile t = p.tile(i);
-      o = pick(t);
+      Operand o = pick(t);
       make_scalar(o);
       kc = __builtin_amdgcn_readfirstlane(t.kc);
-      l.set(o, lw, lane);
+      r = dma::make_rsrc(o.base, 0);
+      ld = o.ld;
+      rows = (uint32_t)o.rows;
+      width = o.width;
+      inc = ACROSS ? BK * o.ld : BK * 2;
+      if (ACROSS) {
+        const int row = 2 * lw + (lane >> 5);
+        off = at = (uint32_t)row * o.ld + (uint32_t)(((lane & 31) ^ (4 * (row & 3))) * 16);
+        step = 8 * o.ld;
+      } else {
+        const int row = 8 * lw + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
+        off = (uint32_t)row * o.ld + (uint32_t)(ch * 16);
+        step = 32 * o.ld;
+        col = 8 * ch;
+      }
     }
+    limit();
   }
-  __device__ __forceinline__ dma::i32x4_t resource() const { return Loader<ACROSS>::resource(o, k, kc); }
-  // load u (0..7) of the slab at k into LDS slot base `slot`
-  __device__ __forceinline__ void issue(int u, const dma::i32x4_t& r, uint32_t slot, int lw) const {
-    dma::load_to_lds16(r, l.offset(u, kc - k), slot + (uint32_t)((4 * u + lw) * 1024));
+  // load u (0..7) of the slab at k into LDS slot base `slot`: 1 KiB at (4 u + lw) * 1024
+  __device__ __forceinline__ void issue(int u, uint32_t slot, int lw) const {
+    dma::load_to_lds16(r, at + (uint32_t)u * step, slot + (uint32_t)((4 * u + lw) * 1024));
+  }
+  // the next slab of this tile; false at its end
+  __device__ __forceinline__ bool next() {
+    k += BK;
+    if (k >= kc) return false;
+    const uint32_t lo = (uint32_t)r[0] + inc;
+    r[1] += lo < inc ? 1 : 0;
+    r[0] = (int)lo;
+    if (kc - k < BK) limit();
+    return true;
   }
 };
 
@@ -277,7 +297,7 @@ enum { WHOLE = 0, SMALL_ROWS = 1, SMALL_COLS = 2 };  // which tiles may be narro
 // The tiles of problem P, worker by worker.  P has
 //   int tiles()          this worker's number of them
 //   Tile tile(int i)     its i-th
-//   epilogue<NB, WN>(const Tile&, int i, int wm, int wn, const float16_t (&acc)[NB][WN], int lane)
+//   epilogue<NB, WN>(const Tile&, int i, int wm, int wn, float16_t (&acc)[NB][WN], int lane)
 // with element r of acc[a][b] at row wm + 32 a + 8 (r / 4) + 4 (lane / 32) + r % 4,
 // column wn + 32 b + lane % 32 of the tile.
 template <bool AA, bool BA, bool F16, int NARROW, class P>
@@ -299,13 +319,13 @@ struct Core {
   __device__ __forceinline__ void set_a() { sa.set(p, tiles, lw, lane, [](const Tile& t) { return t.a; }); }
   __device__ __forceinline__ void set_b() { sb.set(p, tiles, lw, lane, [](const Tile& t) { return t.b; }); }
   __device__ __forceinline__ void next_a() {
-    if ((sa.k += BK) >= sa.kc) {
+    if (!sa.next()) {
       ++sa.i;
       set_a();
     }
   }
   __device__ __forceinline__ void next_b() {
-    if ((sb.k += BK) >= sb.kc) {
+    if (!sb.next()) {
       ++sb.i;
       set_b();
     }
@@ -342,32 +362,33 @@ struct Core {
     constexpr int NM = NB * WN;  // MFMAs of a k16 block
     for (int s = 0; s < steps; ++s) {
       const uint32_t acur = slot(ca), bcur = slot(cb), anxt = slot(after(ca)), bnxt = slot(after(cb));
-      dma::i32x4_t ra, rb;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
           const int i = m / WN, j = m % WN;
           acc[i][j] = mfma<F16>(a[kk][i], b[kk][j], acc[i][j]);
+          // block 0 reads in its first half, so that nothing is in flight at the barrier
+          constexpr int HALF = NM > 1 ? NM / 2 : 1;
+          const int rn = kk == 0 ? HALF : NM;
 #pragma unroll
-          for (int f = m * (NB + WN) / NM; f < (m + 1) * (NB + WN) / NM; ++f)
-            read_one(kk == 0 ? acur : anxt, kk == 0 ? bcur : bnxt, (kk + 3) & 3, f);
+          for (int f = 0; f < NB + WN; ++f)
+            if (f * rn / (NB + WN) == m)
+              read_one(kk == 0 ? acur : anxt, kk == 0 ? bcur : bnxt, (kk + 3) & 3, f);
           if (kk == 1) {  // B of the step after next, into A's slot
 #pragma unroll
-            for (int u = m * LOADS / NM; u < (m + 1) * LOADS / NM; ++u) sb.issue(u, rb, acur, lw);
+            for (int u = m * LOADS / NM; u < (m + 1) * LOADS / NM; ++u) sb.issue(u, acur, lw);
           }
           if (kk >= 2) {  // A of the step after that, into B's slot
 #pragma unroll
             for (int u = ((kk - 2) * NM + m) * LOADS / (2 * NM); u < ((kk - 2) * NM + m + 1) * LOADS / (2 * NM); ++u)
-              sa.issue(u, ra, bcur, lw);
+              sa.issue(u, bcur, lw);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
         if (kk == 0) {
           __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): no read of the current slabs is in flight
           dma::wait_and_barrier<LOADS>();      // the next ones have landed, the current ones are free
-          rb = sb.resource();
-          ra = sa.resource();
           __builtin_amdgcn_sched_barrier(0);
         }
         if (kk == 1) next_b();
@@ -377,10 +398,13 @@ struct Core {
       cb = after(cb);
     }
     p.template epilogue<NB, WN>(tl, it, wm, wn, acc, l);
+    // an epilogue that ends in a lane's branch must not be the tile loop's last statement: the loop would be taken
+    // for one of divergent exit, and its scalars (the loads' resources) would be kept in vector registers
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   __device__ __forceinline__ void run() {
-    tiles = p.tiles();
+    tiles = __builtin_amdgcn_readfirstlane(p.tiles());
     if (tiles <= 0) return;
     sa.i = sb.i = 0;
     ca = 0;
@@ -390,20 +414,21 @@ struct Core {
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {  // A, B, A, B, A
       if (q & 1) {
-        const dma::i32x4_t r = sb.resource();
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) sb.issue(u, r, slot(q), lw);
+        for (int u = 0; u < LOADS; ++u) sb.issue(u, slot(q), lw);
         next_b();
       } else {
-        const dma::i32x4_t r = sa.resource();
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) sa.issue(u, r, slot(q), lw);
+        for (int u = 0; u < LOADS; ++u) sa.issue(u, slot(q), lw);
         next_a();
       }
     }
     dma::wait_and_barrier<(SLOTS - 2) * LOADS>();
     for (int i = 0; i < tiles; ++i) {
-      const Tile tl = p.tile(i);
+      Tile tl = p.tile(i);
+      tl.kc = __builtin_amdgcn_readfirstlane(tl.kc);
+      tl.rows = __builtin_amdgcn_readfirstlane(tl.rows);
+      tl.cols = __builtin_amdgcn_readfirstlane(tl.cols);
       if (NARROW == SMALL_ROWS && tl.rows <= 128) {
         if (tl.rows <= 32) item<1, 2>(tl, i, 0, 64 * lw);
         else if (tl.rows <= 64) item<2, 2>(tl, i, 0, 64 * lw);
