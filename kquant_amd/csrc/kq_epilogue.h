@@ -26,6 +26,16 @@ struct Epilogue {
   int64_t ldr;
 };
 
+// Instead of storing the results, the softmax of the rows: part[row][column /
+// 16] = (maximum, sum of exp(z - maximum)) of 16 columns, parts = ceil(n / 16),
+// and z_target[row] = z[row][target[row]] where the target is a column.
+struct LossTail {
+  const int64_t* target;
+  float2_t* part;
+  int64_t parts;
+  float* z_target;
+};
+
 template <int KIND>
 __device__ __forceinline__ float epi_activate(const Epilogue& e, float x) {
   if (KIND == EPI_CLAMP) return x < e.low ? e.low : x;

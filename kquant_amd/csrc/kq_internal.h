@@ -73,6 +73,8 @@ struct SkinnyArgs {
   int m, n, k;
   Epilogue epi = {};  // bf16 and fp32 rows
 };
+// Instead of storing the results, their rows' softmax.
+hipError_t mx_skinny_loss(int fmt, const SkinnyArgs& args, const LossTail& loss, hipStream_t st);
 hipError_t mx_skinny_bf16(int fmt, bool out_f32, const SkinnyArgs& args, hipStream_t st);
 hipError_t mx_skinny_f32(int fmt, const SkinnyArgs& args, hipStream_t st);
 hipError_t mx_skinny_mx(bool out_f32, const SkinnyArgs& args, hipStream_t st);

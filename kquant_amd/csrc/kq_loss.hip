@@ -478,21 +478,62 @@ __global__ __launch_bounds__(1024) void combine_kernel(const float2_t* __restric
   losses[t] = at < 0 ? 0.0f : target_c[at] < 0 ? __builtin_nanf("") : l - z_target[at];
 }
 
+// The few-token form: the maxima and sums of 16 columns each, part[token][nparts],
+// one workgroup a token.
+__global__ __launch_bounds__(1024) void combine_few_kernel(const float2_t* __restrict__ part, int64_t nparts,
+                                                           const int64_t* __restrict__ target, int64_t ignore_index,
+                                                           int64_t vocab, const float* __restrict__ z_target,
+                                                           float* __restrict__ losses, float* __restrict__ lse) {
+  __shared__ float ms[16], ss[16];
+  const int t = blockIdx.x;
+  const int64_t y = target[t];
+  if (y == ignore_index) {
+    if (threadIdx.x == 0) losses[t] = lse[t] = 0.0f;
+    return;
+  }
+  float m = -__builtin_inff(), s = 0.0f;
+  for (int64_t p = threadIdx.x; p < nparts; p += 1024) {
+    const float2_t v = part[t * nparts + p];
+    join(m, s, v[0], v[1]);
+  }
+  for (int d = 1; d < 64; d <<= 1) join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+  if ((threadIdx.x & 63) == 0) {
+    ms[threadIdx.x >> 6] = m;
+    ss[threadIdx.x >> 6] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) join(m, s, ms[w], ss[w]);
+  const float l = m + LN2 * __builtin_amdgcn_logf(s);
+  lse[t] = l;
+  losses[t] = y >= 0 && y < vocab ? l - z_target[t] : __builtin_nanf("");
+}
+
 // sums[0] = the losses' sum, sums[1] = their mean over the counted tokens (NaN
 // if there are none), added in 64 bits.
 __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ losses, int tokens,
-                                                   const int* __restrict__ count, float* __restrict__ sums) {
+                                                   const int64_t* __restrict__ target, int64_t ignore_index,
+                                                   float* __restrict__ sums) {
   __shared__ double red[1024];
+  __shared__ int counts[1024];
   double s = 0.0;
-  for (int t = threadIdx.x; t < tokens; t += 1024) s += (double)losses[t];
+  int n = 0;
+  for (int t = threadIdx.x; t < tokens; t += 1024) {
+    s += (double)losses[t];
+    n += target[t] != ignore_index ? 1 : 0;
+  }
   red[threadIdx.x] = s;
+  counts[threadIdx.x] = n;
   for (int w = 512; w > 0; w >>= 1) {
     __syncthreads();
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    if ((int)threadIdx.x < w) {
+      red[threadIdx.x] += red[threadIdx.x + w];
+      counts[threadIdx.x] += counts[threadIdx.x + w];
+    }
   }
   if (threadIdx.x == 0) {
     sums[0] = (float)red[0];
-    sums[1] = (float)(red[0] / (double)*count);
+    sums[1] = (float)(red[0] / (double)counts[0]);
   }
 }
 
@@ -501,6 +542,7 @@ __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ los
 constexpr int64_t PIECE_BYTES = 1ll << 30;  // of a piece's d^T, and of its expanded rows
 
 struct Plan {
+  bool few;                    // the one-pass kernel of kq_skinny.hip
   int64_t piece, pieces;       // vocabulary rows
   int slices;                  // of dh's contraction
   int64_t ldg;
@@ -512,6 +554,15 @@ static int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backward, int cus) {
   Plan p{};
   const bool mx = w_fmt != KQ_FMT_BF16;
+  // A block-scaled head at few tokens is read as it is, once (5 tokens, V = 129280, K = 7168 E4M3: FEW_US; expanded
+  // to bf16 and multiplied in tiles 835 us).  A bf16 head's tiles stream it at the chip's rate at any count.
+  p.few = mx && !backward && tokens >= 1 && tokens <= 64;
+  if (p.few) {
+    p.o_z = 0;
+    p.o_part = up(tokens * 4, 256);
+    p.bytes = p.o_part + up(tokens * ((vocab + 15) / 16) * 8, 256);
+    return p;
+  }
   p.ldg = up(tokens > 0 ? tokens : 1, 8);
   int64_t most = vocab;
   if (mx) most = PIECE_BYTES / (2 * k);
@@ -627,6 +678,21 @@ extern "C" int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, in
   if (workspace_bytes < p.bytes || kq_misaligned(workspace, 256))
     return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", fn, (long long)p.bytes);
   char* ws = (char*)workspace;
+  if (p.few) {
+    const LossTail tail{target, (float2_t*)(ws + p.o_part), (vocab + 15) / 16, (float*)(ws + p.o_z)};
+    hipError_t e = mx_skinny_loss(w_fmt, {h, nullptr, ldh, (const uint8_t*)w, w_scale, nullptr, 0, (int)tokens,
+                                          (int)vocab, (int)k}, tail, st);
+    if (e == hipSuccess) {
+      loss::combine_few_kernel<<<(unsigned)tokens, 1024, 0, st>>>(tail.part, tail.parts, target, ignore_index, vocab,
+                                                                  tail.z_target, losses, lse);
+      e = hipGetLastError();
+    }
+    if (e == hipSuccess) {
+      loss::sum_kernel<<<1, 1024, 0, st>>>(losses, (int)tokens, target, ignore_index, sums);
+      e = hipGetLastError();
+    }
+    return kq_check_launch(e, fn);
+  }
   int* count = (int*)(ws + p.o_count);
   loss::compact_kernel<<<1, 1024, 0, st>>>(target, ignore_index, (int)tokens, (int*)(ws + p.o_rows),
                                            (int*)(ws + p.o_place), count);
@@ -665,7 +731,7 @@ extern "C" int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, in
                                                                          g.target_c, a.z_target, losses, lse);
     if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   }
-  loss::sum_kernel<<<1, 1024, 0, st>>>(losses, (int)tokens, count, sums);
+  loss::sum_kernel<<<1, 1024, 0, st>>>(losses, (int)tokens, target, ignore_index, sums);
   return kq_check_launch(hipGetLastError(), fn);
 }
 

@@ -58,11 +58,13 @@ __device__ __forceinline__ u32x4_t load16_nt(const void* p) {
 // FMT: weight format; AT: activation rows; OUT: KQ_DT_BF16 / KQ_DT_F32;
 // MB x 16 activation rows and R x 16 weight rows per workgroup, P windows in
 // flight; HALF: K % 128 == 64 (2-byte aligned scale rows, a half window at
-// the end); EPI: with the linear's epilogue.
-template <int FMT, int AT, int OUT, int MB, int R, int P, bool HALF, bool EPI>
+// the end); TAIL: what becomes of the sums.
+enum { TAIL_STORE = 0, TAIL_EPILOGUE = 1, TAIL_LOSS = 2 };
+template <int FMT, int AT, int OUT, int MB, int R, int P, bool HALF, int TAIL>
 __global__ __launch_bounds__(512) void mx_skinny_kernel(
     const void* __restrict__ a, const uint8_t* __restrict__ a_scale, int64_t lda, const uint8_t* __restrict__ wq,
-    const uint8_t* __restrict__ ws, void* __restrict__ c, int64_t ldc, int M, int N, int K, int mtiles, Epilogue epi) {
+    const uint8_t* __restrict__ ws, void* __restrict__ c, int64_t ldc, int M, int N, int K, int mtiles, Epilogue epi,
+    LossTail loss) {
   static_assert(AT != A_MXFP8 || (FMT == 0 && !HALF), "MXFP8 rows take E4M3 weights and whole windows");
   using Win = Window<FMT, AT, MB, R>;
   extern __shared__ __attribute__((aligned(16))) float skinny_red[];
@@ -280,13 +282,32 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
   __syncthreads();
   for (int e = (int)threadIdx.x; e < TILE; e += (int)blockDim.x) {
     const int n = e % (16 * R), m = e / (16 * R);
-    if (m0 + m >= M || n0 + n >= N) continue;
+    const bool in = m0 + m < M && n0 + n < N;
+    if (TAIL != TAIL_LOSS && !in) continue;
     const int at = ((m >> 4) * R + (n >> 4)) * 256 + (16 * ((m & 15) >> 2) + (n & 15)) * 4 + (m & 3);
     float sum = skinny_red[at];
     for (int w = 1; w < waves; ++w) sum += skinny_red[w * TILE + at];
-    if (EPI) sum = epi_apply<OUT>(epi, sum, m0 + m, n0 + n);
-    if (OUT == 2) static_cast<float*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = sum;
-    else static_cast<__bf16*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = (__bf16)sum;
+    if constexpr (TAIL == TAIL_LOSS) {
+      // logits of 16 columns of one row in 16 lanes (whole waves run: TILE is a multiple of 64)
+      if (in && loss.target[m0 + m] == n0 + n) loss.z_target[m0 + m] = sum;
+      float top = in ? sum : -__builtin_inff();
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      float total = in ? __builtin_amdgcn_exp2f((sum - ref) * 1.44269504f) : 0.0f;
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) total += __shfl_xor(total, d);
+      if (in && (n & 15) == 0) {
+        float2_t v;
+        v[0] = top;
+        v[1] = total;
+        loss.part[(int64_t)(m0 + m) * loss.parts + (n0 + n) / 16] = v;
+      }
+    } else {
+      if (TAIL == TAIL_EPILOGUE) sum = epi_apply<OUT>(epi, sum, m0 + m, n0 + n);
+      if (OUT == 2) static_cast<float*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = sum;
+      else static_cast<__bf16*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = (__bf16)sum;
+    }
   }
 }
 
