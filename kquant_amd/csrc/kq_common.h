@@ -165,4 +165,19 @@ __device__ __forceinline__ float quad_max(float v) {
   return fmaxf(v, __int_as_float(y));
 }
 
+// 4 x 4 transpose of 16-bit elements over a quad of lanes: element s of lane t
+// becomes element t of lane s (two elements a word), in 8 instructions.
+__device__ __forceinline__ void quad_transpose16(uint32_t& w0, uint32_t& w1) {
+  const int t = (int)threadIdx.x & 3;
+  // even lanes: the low halves of (own, partner), odd lanes: the high halves of (partner, own)
+  const uint32_t sel = t & 1 ? 0x03020706u : 0x05040100u;
+  const uint32_t p0 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w0, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+  const uint32_t p1 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w1, 0xb1, 0xf, 0xf, true);
+  const uint32_t q0 = __builtin_amdgcn_perm(p0, w0, sel), q1 = __builtin_amdgcn_perm(p1, w1, sel);
+  const uint32_t send = t & 2 ? q0 : q1;
+  const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)send, 0x4e, 0xf, 0xf, true);  // lane ^ 2
+  w0 = t & 2 ? got : q0;
+  w1 = t & 2 ? q1 : got;
+}
+
 }  // namespace kq

@@ -24,6 +24,7 @@ struct Epilogue {
   int bias_f32;
   const void* residual;  // [m, n] of the output's type, or null
   int64_t ldr;
+  int quads;             // bf16 results of 8-byte aligned groups of 4 columns (n, ldc, ldr, c, residual)
 };
 
 // Instead of storing the results, the softmax of the rows: part[row][column /

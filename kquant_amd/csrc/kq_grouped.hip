@@ -41,10 +41,10 @@ struct Problem {
   Args g;
   int mtiles, ntiles, count;
   // lane l of entry q: this worker's tile 64 q + l (forward, dx)
-  int group_nt[TABLE], mt_of[TABLE];
+  int group_nt[TABLE], mt_of[TABLE], beg_of[TABLE], n_of[TABLE];
 
   __device__ __forceinline__ void range(int e, int& beg, int& n) const {
-    // constant memory: the scalar loads of a group that is the same in every lane
+    // constant memory, so that a group that is the same in every lane takes scalar loads
     const auto* o = (const __attribute__((address_space(4))) int64_t*)g.offsets + e;
     const int64_t b = clamped(o[0], 0, g.rows);
     beg = (int)b;
@@ -71,18 +71,26 @@ struct Problem {
     for (int e = e0; e < e1; ++e) {
       int beg, n;
       range(e, beg, n);
-      first[e] = sum;
       sum += (n + mm16::BM - 1) / mm16::BM * ntiles;
     }
-    part[t] = sum;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < mm16::THREADS; ++i) {
-      const int v = part[i];
-      before += i < t ? v : 0;
-      all += v;
+    int upto = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(upto, d);
+      if ((t & 63) >= d) upto += v;
     }
-    for (int e = e0; e < e1; ++e) first[e] += before;
+    if ((t & 63) == 63) part[t >> 6] = upto;
+    __syncthreads();
+    int all = 0, at = upto - sum;
+    for (int w = 0; w < mm16::THREADS / 64; ++w) {
+      at += w < t >> 6 ? part[w] : 0;
+      all += part[w];
+    }
+    for (int e = e0; e < e1; ++e) {
+      int beg, n;
+      range(e, beg, n);
+      first[e] = at;
+      at += (n + mm16::BM - 1) / mm16::BM * ntiles;
+    }
     if (t == 0) first[g.groups] = all;
     __syncthreads();
     all = __builtin_amdgcn_readfirstlane(all);
@@ -90,7 +98,7 @@ struct Problem {
 #pragma unroll
     for (int q = 0; q < TABLE; ++q) {
       const int tile = mm16::worker_number() + (64 * q + (t & 63)) * (int)gridDim.x;
-      group_nt[q] = mt_of[q] = 0;
+      group_nt[q] = mt_of[q] = beg_of[q] = n_of[q] = 0;
       if (tile < all) {
         int lo = 0, hi = g.groups;  // first[lo] <= tile < first[hi]
         while (hi - lo > 1) {
@@ -101,6 +109,7 @@ struct Problem {
         int nt;
         mm16::tile_mn(tile - first[lo], (first[lo + 1] - first[lo]) / ntiles, ntiles, mt_of[q], nt);
         group_nt[q] = lo << 16 | nt;
+        range(lo, beg_of[q], n_of[q]);
       }
     }
     __syncthreads();  // the slabs' loads overwrite the sums
@@ -120,13 +129,15 @@ struct Problem {
       const int t = mm16::worker_number() + i * (int)gridDim.x, per = mtiles * ntiles;
       e = t / per;
       mm16::tile_mn(t - e * per, mtiles, ntiles, mt, nt);
+      range(e, beg, n);
     } else {
       const int en = entry(group_nt, i);
       e = en >> 16;
       nt = en & 0xffff;
       mt = entry(mt_of, i);
+      beg = entry(beg_of, i);
+      n = entry(n_of, i);
     }
-    range(e, beg, n);
   }
 
   __device__ __forceinline__ mm16::Tile tile(int i) const {

@@ -507,33 +507,79 @@ __global__ __launch_bounds__(256, 1) void mx_linear_dma_kernel(
       const out_t* rt = epi.residual ? static_cast<const out_t*>(epi.residual) + (int64_t)(m0 + wm) * epi.ldr + n0 + wn
                                      : nullptr;
       const int rows = M - m0 - wm, cols = N - n0 - wn;  // of this wave's part
+      if (OUT != 2 && epi.quads) {
+        // A lane's four rows of one column, exchanged over its quad for four columns of one row: residual loads and
+        // stores of 8 bytes a lane, a quarter of the instructions.  The next 32 rows' residual is in flight while
+        // these are worked on.
+        const int t = lane & 3;
+        u32x2_t res[2][4][4];
+        auto fetch = [&](int i, u32x2_t (&to)[4][4]) {
+          int row = i * 32 + 4 * f + t, col = lane & 28;
+          asm volatile("" : "+v"(row), "+v"(col));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // opaque: the offsets of a block are made when it is stored, not kept through the K loop
-        int row = i * 32 + 4 * f, col = frow;
-        asm volatile("" : "+v"(row), "+v"(col));
-        float res[16][4];
-        if (rt) {
+          for (int g = 0; g < 4; ++g) {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(rt) + min(row + 8 * g, rows - 1) * epi.ldr;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[g][j] = *reinterpret_cast<const u32x2_t*>(p + min(col + j * 32, cols - 4));
+          }
+        };
+        if (rt) fetch(0, res[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (rt && i < 3) fetch(i + 1, res[(i + 1) & 1]);
+          int row = i * 32 + 4 * f + t, col = lane & 28;
+          asm volatile("" : "+v"(row), "+v"(col));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint16_t* p = reinterpret_cast<uint16_t*>(ct) + (row + 8 * g) * ldc;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[2] = {0u, 0u};
+              if (rt) {
+                w[0] = res[i & 1][g][j][0];
+                w[1] = res[i & 1][g][j][1];
+                quad_transpose16(w[0], w[1]);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                w[h] = f32x2_to_bf16x2_bits(
+                    epi_activate<EPI>(epi, acc[i][j][4 * g + 2 * h] + bias[j]) + __uint_as_float(w[h] << 16),
+                    epi_activate<EPI>(epi, acc[i][j][4 * g + 2 * h + 1] + bias[j]) + __uint_as_float(w[h] & 0xffff0000u));
+              quad_transpose16(w[0], w[1]);
+              if (row + 8 * g < rows && col + j * 32 < cols) *reinterpret_cast<u32x2_t*>(p + col + j * 32) = u32x2_t{w[0], w[1]};
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // opaque: the offsets of a block are made when it is stored, not kept through the K loop
+          int row = i * 32 + 4 * f, col = frow;
+          asm volatile("" : "+v"(row), "+v"(col));
+          float res[16][4];
+          if (rt) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const out_t* p = rt + min(row + 8 * (r >> 2) + (r & 3), rows - 1) * epi.ldr;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) res[r][j] = (float)p[min(col + j * 32, cols - 1)];
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) res[r][j] = 0.0f;
+          }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const out_t* p = rt + min(row + 8 * (r >> 2) + (r & 3), rows - 1) * epi.ldr;
+            const int at = row + 8 * (r >> 2) + (r & 3);
+            out_t* p = ct + at * ldc;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) res[r][j] = (float)p[min(col + j * 32, cols - 1)];
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) res[r][j] = 0.0f;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = row + 8 * (r >> 2) + (r & 3);
-          out_t* p = ct + at * ldc;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = epi_activate<EPI>(epi, acc[i][j][r] + bias[j]) + res[r][j];
-            if (at < rows && col + j * 32 < cols) p[col + j * 32] = (out_t)v;
+            for (int j = 0; j < 4; ++j) {
+              const float v = epi_activate<EPI>(epi, acc[i][j][r] + bias[j]) + res[r][j];
+              if (at < rows && col + j * 32 < cols) p[col + j * 32] = (out_t)v;
+            }
           }
         }
       }
@@ -1378,6 +1424,8 @@ extern "C" int kq_mx_linear_epilogue(int w_fmt, int a_dtype, const void* a, int6
   e.bias_f32 = bias_dtype == KQ_DT_F32;
   e.residual = residual;
   e.ldr = ldr;
+  e.quads = out_dtype == KQ_DT_BF16 && n % 4 == 0 && ldc % 4 == 0 && !kq_misaligned(c, 8) &&
+            (!residual || (ldr % 4 == 0 && !kq_misaligned(residual, 8)));
   return a_dtype == KQ_DT_F32 ? linear_f32(fn, w_fmt, static_cast<const float*>(a), lda, w_q, w_scale, m, n, k, e,
                                            static_cast<float*>(c), ldc, workspace, workspace_bytes, stream)
                               : linear_bf16(fn, w_fmt, a, lda, w_q, w_scale, m, n, k, e, out_dtype, c, ldc, workspace,

@@ -194,8 +194,6 @@ __device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm
   const int t = lane & 3;
   int row = wm + 4 * (lane >> 5) + t, col = wn + (lane & 28);
   asm volatile("" : "+v"(row), "+v"(col));  // the elements' offsets are not kept (and spilled) from tile to tile
-  // even lanes: the low halves of (own, partner), odd lanes: the high halves of (partner, own)
-  const uint32_t sel = t & 1 ? 0x03020706u : 0x05040100u;
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     in_place(acc, i);
@@ -205,19 +203,16 @@ __device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm
       char* p = address(min(at, rows - 1)) + 2 * (int64_t)col;
 #pragma unroll
       for (int j = 0; j < WN; ++j) {
-        uint32_t q[2];
+        uint32_t w[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 4 * g + 2 * h;
-          const uint32_t own = pack16<F16>(f(i, j, r, acc[i][j][r]), f(i, j, r + 1, acc[i][j][r + 1]));
-          const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)own, 0xb1, 0xf, 0xf, true);  // lane ^ 1
-          q[h] = __builtin_amdgcn_perm(other, own, sel);
+          w[h] = pack16<F16>(f(i, j, r, acc[i][j][r]), f(i, j, r + 1, acc[i][j][r + 1]));
         }
-        const uint32_t send = t & 2 ? q[0] : q[1];
-        const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)send, 0x4e, 0xf, 0xf, true);  // lane ^ 2
+        quad_transpose16(w[0], w[1]);
         u32x2_t v;
-        v[0] = t & 2 ? got : q[0];
-        v[1] = t & 2 ? q[1] : got;
+        v[0] = w[0];
+        v[1] = w[1];
         if (at < rows && col + 32 * j < cols) *reinterpret_cast<u32x2_t*>(p + 64 * j) = v;
       }
       __builtin_amdgcn_sched_barrier(0);
