@@ -177,16 +177,17 @@ struct Problem {
   }
 
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const mm16::Tile& tl, int i, int wm, int wn,
+  __device__ __forceinline__ bool epilogue(const mm16::Tile& tl, int i, int wm, int wn,
                                            float16_t (&acc)[NB][WN], int lane) const {
     int e, beg, n, mt, nt;
     find(i, e, beg, n, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN;
     const int64_t row0 = MODE == DW ? (int64_t)e * g.n + m0 : beg + m0;
+    const int cols = (MODE == FORWARD ? g.n : g.k) - n0;
     char* out = g.out + row0 * g.ld_out + 2 * (int64_t)n0;
-    mm16::store16<NB, WN, F16>([&](int r) { return out + r * (int64_t)g.ld_out; }, tl.rows,
-                               (MODE == FORWARD ? g.n : g.k) - n0, wm, wn, acc, lane,
+    mm16::store16<NB, WN, F16>([&](int r) { return out + r * (int64_t)g.ld_out; }, tl.rows, cols, wm, wn, acc, lane,
                                [](int, int, int, float v) { return v; });
+    return tl.rows >= mm16::BM && cols >= mm16::BN;
   }
 };
 

@@ -207,7 +207,7 @@ struct LogitProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ bool epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
                                            int lane) const {
     const int t = tile_number(x);
     int mt, nt;
@@ -232,7 +232,7 @@ struct LogitProblem {
         const float p = __builtin_amdgcn_exp2f((z - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
         return n0 + wn + 32 * j + (lane & 31) < count ? up[j] * p : 0.0f;
       });
-      return;
+      return tl.rows >= mm16::BM && (count + 7) / 8 * 8 - n0 >= mm16::BN;
     }
     const int row = wm + 4 * (lane >> 5);  // this lane's rows: row + 32 i + 8 (r / 4) + r % 4
     float m[WN], s[WN], hit[WN];
@@ -298,6 +298,7 @@ struct LogitProblem {
         if (at[j] >= 0 && at[j] < 32 * NB && !(at[j] & 4)) g.z_target[c] = hit[j];
       }
     }
+    return false;
   }
 };
 
@@ -349,7 +350,7 @@ struct DhProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ bool epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
                                            int lane) const {
     const int t = tile_number(x);
     int mt, nt;
@@ -372,6 +373,7 @@ struct DhProblem {
         mm16::each(tl.rows, g.k - n0, wm, wn, acc, lane,
                    [&](int r, int c, float v) { out[(uint32_t)r * ld + (uint32_t)c] = v; });
     }
+    return tl.rows >= mm16::BM && g.k - n0 >= mm16::BN;
   }
 };
 
@@ -431,7 +433,7 @@ struct DwProblem {
     return r;
   }
   template <int NB, int WN>
-  __device__ __forceinline__ void epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
+  __device__ __forceinline__ bool epilogue(const Tile& tl, int x, int wm, int wn, float16_t (&acc)[NB][WN],
                                            int lane) const {
     const int t = tile_number(x);
     int mt, nt;
@@ -441,6 +443,7 @@ struct DwProblem {
     const float alpha = *g.alpha;
     mm16::store16<NB, WN, false>([&](int r) { return out + r * (int64_t)g.k * 2; }, tl.rows, g.k - n0, wm, wn, acc, lane,
                                  [&](int, int, int, float v) { return alpha * v; });
+    return tl.rows >= mm16::BM && g.k - n0 >= mm16::BN;
   }
 };
 

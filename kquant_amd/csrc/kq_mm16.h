@@ -303,6 +303,11 @@ struct Core {
   Side<AA> sa;
   Side<BA> sb;
   int ca, cb;  // slots of the slabs in use
+  // Every wave has issued STORES stores or more since the loads of the next step's slabs.  They are waited for in
+  // the order of issue, at most 63 are counted, and LOADS loads of a later slab stand between: with 63 outstanding
+  // the slabs have landed, and the stores need not have.
+  bool stored;
+  static constexpr int STORES = 63 - LOADS;
 
   __device__ __forceinline__ Core(const P& prob, unsigned char* l) : p(prob) {
     lane = threadIdx.x & 63;
@@ -383,7 +388,9 @@ struct Core {
         }
         if (kk == 0) {
           __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): no read of the current slabs is in flight
-          dma::wait_and_barrier<LOADS>();      // the next ones have landed, the current ones are free
+          // the next slabs have landed, the current ones are free
+          if (s == 0 && stored) dma::wait_and_barrier<63>();
+          else dma::wait_and_barrier<LOADS>();
           __builtin_amdgcn_sched_barrier(0);
         }
         if (kk == 1) next_b();
@@ -392,7 +399,7 @@ struct Core {
       ca = after(ca);
       cb = after(cb);
     }
-    p.template epilogue<NB, WN>(tl, it, wm, wn, acc, l);
+    stored = p.template epilogue<NB, WN>(tl, it, wm, wn, acc, l) && NB * WN == 16;
     // an epilogue that ends in a lane's branch must not be the tile loop's last statement: the loop would be taken
     // for one of divergent exit, and its scalars (the loads' resources) would be kept in vector registers
     __builtin_amdgcn_sched_barrier(0);
@@ -404,6 +411,7 @@ struct Core {
     sa.i = sb.i = 0;
     ca = 0;
     cb = 1;
+    stored = false;
     set_a();
     set_b();
 #pragma unroll
