@@ -40,7 +40,7 @@ template <int MODE, bool F16>
 struct Problem {
   Args g;
   int mtiles, ntiles, count;
-  // lane l of entry q: this worker's tile 64 q + l (forward, dx)
+  // lane l of entry q: this worker's tile 64 q + l
   int group_nt[TABLE], mt_of[TABLE], beg_of[TABLE], n_of[TABLE];
 
   __device__ __forceinline__ void range(int e, int& beg, int& n) const {
@@ -52,6 +52,11 @@ struct Problem {
   }
   __device__ __forceinline__ int tiles() const { return count; }
 
+  // Tiles of a group of n rows.
+  __device__ __forceinline__ int tiles_of(int n) const {
+    return (MODE == DW ? mtiles : (n + mm16::BM - 1) / mm16::BM) * ntiles;
+  }
+
   // Numbers the tiles; every thread of the workgroup calls it, before the slabs
   // use LDS.  The groups' tiles are summed in LDS, then every lane looks one of
   // the worker's tiles up, so the K loops find theirs in a register.
@@ -59,10 +64,6 @@ struct Problem {
     const int cols = MODE == FORWARD ? g.n : g.k;
     ntiles = (cols + mm16::BN - 1) / mm16::BN;
     mtiles = (g.n + mm16::BM - 1) / mm16::BM;
-    if (MODE == DW) {
-      count = mm16::worker_tiles(g.groups * mtiles * ntiles);
-      return;
-    }
     int* first = reinterpret_cast<int*>(lds);  // [groups + 1]
     int* part = first + MAX_GROUPS + 1;
     const int t = threadIdx.x, per = (g.groups + mm16::THREADS - 1) / mm16::THREADS;
@@ -71,7 +72,7 @@ struct Problem {
     for (int e = e0; e < e1; ++e) {
       int beg, n;
       range(e, beg, n);
-      sum += (n + mm16::BM - 1) / mm16::BM * ntiles;
+      sum += tiles_of(n);
     }
     int upto = sum;
     for (int d = 1; d < 64; d <<= 1) {
@@ -89,7 +90,7 @@ struct Problem {
       int beg, n;
       range(e, beg, n);
       first[e] = at;
-      at += (n + mm16::BM - 1) / mm16::BM * ntiles;
+      at += tiles_of(n);
     }
     if (t == 0) first[g.groups] = all;
     __syncthreads();
@@ -125,19 +126,12 @@ struct Problem {
 
   // Group, first row and row count of it, and position of this worker's tile i.
   __device__ __forceinline__ void find(int i, int& e, int& beg, int& n, int& mt, int& nt) const {
-    if (MODE == DW) {
-      const int t = mm16::worker_number() + i * (int)gridDim.x, per = mtiles * ntiles;
-      e = t / per;
-      mm16::tile_mn(t - e * per, mtiles, ntiles, mt, nt);
-      range(e, beg, n);
-    } else {
-      const int en = entry(group_nt, i);
-      e = en >> 16;
-      nt = en & 0xffff;
-      mt = entry(mt_of, i);
-      beg = entry(beg_of, i);
-      n = entry(n_of, i);
-    }
+    const int en = entry(group_nt, i);
+    e = en >> 16;
+    nt = en & 0xffff;
+    mt = entry(mt_of, i);
+    beg = entry(beg_of, i);
+    n = entry(n_of, i);
   }
 
   __device__ __forceinline__ mm16::Tile tile(int i) const {
@@ -185,7 +179,7 @@ struct Problem {
     const int64_t row0 = MODE == DW ? (int64_t)e * g.n + m0 : beg + m0;
     const int cols = (MODE == FORWARD ? g.n : g.k) - n0;
     char* out = g.out + row0 * g.ld_out + 2 * (int64_t)n0;
-    mm16::store16<NB, WN, F16>([&](int r) { return out + r * (int64_t)g.ld_out; }, tl.rows, cols, wm, wn, acc, lane,
+    mm16::store16<NB, WN, F16>(out, g.ld_out, tl.rows, cols, wm, wn, acc, lane,
                                [](int, int, int, float v) { return v; });
     return tl.rows >= mm16::BM && cols >= mm16::BN;
   }
@@ -219,11 +213,11 @@ static hipError_t launch(int dtype, const Args& g, hipStream_t st) {
   if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   if (e != hipSuccess) return e;
   int64_t grid = cus >= 8 ? cus / 8 * 8 : 8;
-  if (MODE != DW) {  // a worker's table holds 256 tiles: more workers where there may be more
-    const int64_t most = (g.rows / mm16::BM + (g.rows < g.groups ? g.rows : g.groups)) *
-                         (((MODE == FORWARD ? g.n : g.k) + mm16::BN - 1) / mm16::BN);
-    grid *= (most + grid * 64 * TABLE - 1) / (grid * 64 * TABLE);
-  }
+  // a worker's table holds 256 tiles: more workers where there may be more
+  const int64_t row_tiles = MODE == DW ? (int64_t)g.groups * ((g.n + mm16::BM - 1) / mm16::BM)
+                                       : g.rows / mm16::BM + (g.rows < g.groups ? g.rows : g.groups);
+  const int64_t most = row_tiles * (((MODE == FORWARD ? g.n : g.k) + mm16::BN - 1) / mm16::BN);
+  grid *= most > 0 ? (most + grid * 64 * TABLE - 1) / (grid * 64 * TABLE) : 1;
   if (dtype == KQ_DT_F16) grouped_kernel<MODE, true><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
   else grouped_kernel<MODE, false><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
   return hipGetLastError();

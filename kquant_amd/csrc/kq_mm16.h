@@ -181,19 +181,132 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return F16 ? f32x2_to_f16x2_bits(lo, hi) : f32x2_to_bf16x2_bits(lo, hi);
 }
 
+// The value of lane ^ 4.
+__device__ __forceinline__ uint32_t other_quad(uint32_t v) {
+  const int up = __builtin_amdgcn_update_dpp(0, (int)v, 0x104, 0xf, 0x5, true);     // even quads: lane + 4
+  return (uint32_t)__builtin_amdgcn_update_dpp(up, (int)v, 0x114, 0xf, 0xa, true);  // odd quads: lane - 4
+}
+
+// Four rows (elements 4 g .. 4 g + 3 as f(i, j, r, value)) of the columns of
+// WN blocks, exchanged over the lane's quad for four columns of one row, in 16
+// bits.  One wave runs on a SIMD, so an instruction that waits for the one
+// before it costs the wave its latency: each step of the exchange is taken for
+// all blocks before the next.
+template <int NB, int WN, bool F16, class F>
+__device__ __forceinline__ void quad_rows(const float16_t (&acc)[NB][WN], int i, int g, u32x2_t (&v)[WN], F&& f) {
+  const int t = (int)threadIdx.x & 3;
+  const uint32_t sel = t & 1 ? 0x03020706u : 0x05040100u;  // as quad_transpose16
+  uint32_t w0[WN], w1[WN], p0[WN], p1[WN], got[WN];
+#pragma unroll
+  for (int j = 0; j < WN; ++j) {
+    const int r = 4 * g;
+    w0[j] = pack16<F16>(f(i, j, r, acc[i][j][r]), f(i, j, r + 1, acc[i][j][r + 1]));
+    w1[j] = pack16<F16>(f(i, j, r + 2, acc[i][j][r + 2]), f(i, j, r + 3, acc[i][j][r + 3]));
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) {
+    p0[j] = (uint32_t)__builtin_amdgcn_mov_dpp((int)w0[j], 0xb1, 0xf, 0xf, true);  // lane ^ 1
+    p1[j] = (uint32_t)__builtin_amdgcn_mov_dpp((int)w1[j], 0xb1, 0xf, 0xf, true);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) {
+    w0[j] = __builtin_amdgcn_perm(p0[j], w0[j], sel);
+    w1[j] = __builtin_amdgcn_perm(p1[j], w1[j], sel);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) got[j] = t & 2 ? w0[j] : w1[j];
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) got[j] = (uint32_t)__builtin_amdgcn_mov_dpp((int)got[j], 0x4e, 0xf, 0xf, true);  // lane ^ 2
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN; ++j) {
+    v[j][0] = t & 2 ? got[j] : w0[j];
+    v[j][1] = t & 2 ? w1[j] : got[j];
+  }
+}
+
 // Stores a wave's blocks in 16 bits: rows below `rows`, columns below `cols` (a
 // multiple of 4) of the tile, f(i, j, r, v) the value stored for element r of
-// block (i, j), v the accumulated one, and address(row) the 8-byte aligned
-// address of a row's column 0 (asked for rows below `rows` only).  A lane holds four rows of one column and
-// exchanges them with its quad for four columns of one row, in 10 instructions
-// of its registers, so it stores 8 bytes: a store instruction takes as long for
-// 2 bytes a lane.
-template <int NB, int WN, bool F16, class At, class F>
-__device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm, int wn, float16_t (&acc)[NB][WN],
-                                        int lane, F&& f) {
-  const int t = lane & 3;
-  int row = wm + 4 * (lane >> 5) + t, col = wn + (lane & 28);
+// block (i, j), v the accumulated one, to base + row ld (16-byte aligned rows).
+// A store instruction takes the CU's memory path some 8 cycles for each line it
+// touches, so it should fill them: a lane's four rows of one column are
+// exchanged over its quad for four columns of one row (8 bytes), and in whole
+// tiles, which need no masks, over two quads for 16 bytes, of which 8 lanes
+// make a 128-byte line.  Results are larger than an XCD's L2 and read from
+// another one: nontemporal.  48 weight gradients of 7168 x 2048, 64 rows each:
+// 461 us with 8 bytes a lane, 402 nontemporal, 290 with 16 bytes (1.41 GB).
+template <int NB, int WN, bool F16, class F>
+__device__ __forceinline__ void store16(char* base, uint32_t ld, int rows, int cols, int wm, int wn,
+                                        float16_t (&acc)[NB][WN], int lane, F&& f) {
+  int row = wm + 4 * (lane >> 5) + (lane & 3), col = wn + (lane & 28);
   asm volatile("" : "+v"(row), "+v"(col));  // the elements' offsets are not kept (and spilled) from tile to tile
+  if constexpr (NB * WN == 16) if (rows >= BM && cols >= BN) {
+    // the odd quad of two takes the second of two blocks, from 4 columns to the left
+    const bool odd = lane & 4;
+    uint32_t off = (uint32_t)row * ld + 2u * (uint32_t)col + (odd ? 56u : 0u);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      in_place(acc, i);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        u32x2_t v[WN];
+        quad_rows<NB, WN, F16>(acc, i, g, v, f);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t x0[WN / 2], x1[WN / 2];
+#pragma unroll
+        for (int j = 0; j < WN; j += 2) {
+          x0[j / 2] = odd ? v[j][0] : v[j + 1][0];
+          x1[j / 2] = odd ? v[j][1] : v[j + 1][1];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < WN / 2; ++j) {
+          x0[j] = other_quad(x0[j]);
+          x1[j] = other_quad(x1[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < WN; j += 2) {
+          u32x4_t q;
+          q[0] = odd ? x0[j / 2] : v[j][0];
+          q[1] = odd ? x1[j / 2] : v[j][1];
+          q[2] = odd ? v[j + 1][0] : x0[j / 2];
+          q[3] = odd ? v[j + 1][1] : x1[j / 2];
+          __builtin_nontemporal_store(q, reinterpret_cast<u32x4_t*>(base + off + 64 * j));
+        }
+        off += 8 * ld;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    in_place(acc, i);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int at = row + 32 * i + 8 * g;
+      char* p = base + (uint32_t)at * ld + 2 * (uint32_t)col;
+      u32x2_t v[WN];
+      quad_rows<NB, WN, F16>(acc, i, g, v, f);
+#pragma unroll
+      for (int j = 0; j < WN; ++j)
+        if (at < rows && col + 32 * j < cols) __builtin_nontemporal_store(v[j], reinterpret_cast<u32x2_t*>(p + 64 * j));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// The same with rows of their own: address(row) the address of a row's column 0
+// (asked for rows below `rows` only).
+template <int NB, int WN, bool F16, class At, class F>
+__device__ __forceinline__ void store16_rows(At&& address, int rows, int cols, int wm, int wn, float16_t (&acc)[NB][WN],
+                                             int lane, F&& f) {
+  int row = wm + 4 * (lane >> 5) + (lane & 3), col = wn + (lane & 28);
+  asm volatile("" : "+v"(row), "+v"(col));
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     in_place(acc, i);
@@ -201,20 +314,11 @@ __device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm
     for (int g = 0; g < 4; ++g) {
       const int at = row + 32 * i + 8 * g;
       char* p = address(min(at, rows - 1)) + 2 * (int64_t)col;
+      u32x2_t v[WN];
+      quad_rows<NB, WN, F16>(acc, i, g, v, f);
 #pragma unroll
-      for (int j = 0; j < WN; ++j) {
-        uint32_t w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = 4 * g + 2 * h;
-          w[h] = pack16<F16>(f(i, j, r, acc[i][j][r]), f(i, j, r + 1, acc[i][j][r + 1]));
-        }
-        quad_transpose16(w[0], w[1]);
-        u32x2_t v;
-        v[0] = w[0];
-        v[1] = w[1];
-        if (at < rows && col + 32 * j < cols) *reinterpret_cast<u32x2_t*>(p + 64 * j) = v;
-      }
+      for (int j = 0; j < WN; ++j)
+        if (at < rows && col + 32 * j < cols) __builtin_nontemporal_store(v[j], reinterpret_cast<u32x2_t*>(p + 64 * j));
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -303,11 +407,11 @@ struct Core {
   Side<AA> sa;
   Side<BA> sb;
   int ca, cb;  // slots of the slabs in use
-  // Every wave has issued STORES stores or more since the loads of the next step's slabs.  They are waited for in
-  // the order of issue, at most 63 are counted, and LOADS loads of a later slab stand between: with 63 outstanding
-  // the slabs have landed, and the stores need not have.
+  // Every wave has issued STORES stores or more since the loads of the next step's slabs.  All are waited for in the
+  // order of issue, and LOADS loads of a later slab stand between: with STORES + LOADS outstanding the slabs have
+  // landed, and the stores need not have.
   bool stored;
-  static constexpr int STORES = 63 - LOADS;
+  static constexpr int STORES = 32;
 
   __device__ __forceinline__ Core(const P& prob, unsigned char* l) : p(prob) {
     lane = threadIdx.x & 63;
@@ -342,12 +446,6 @@ struct Core {
     fb.set(wn, l);
     u32x4_t a[4][NB], b[4][WN];
     float16_t acc[NB][WN];
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int j = 0; j < WN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     // fragment f of k16 block kk: 0..NB-1 of A, then B
     auto read_one = [&](uint32_t as, uint32_t bs, int kk, int f) {
       if (f < NB) a[kk][f] = fa.read(as, kk, f);
@@ -359,6 +457,13 @@ struct Core {
     for (int kk = 0; kk < 3; ++kk)
 #pragma unroll
       for (int f = 0; f < NB + WN; ++f) read_one(slot(ca), slot(cb), kk, f);
+    __builtin_amdgcn_sched_barrier(0);  // the accumulators are cleared while these are on their way
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < WN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     constexpr int NM = NB * WN;  // MFMAs of a k16 block
     for (int s = 0; s < steps; ++s) {
       const uint32_t acur = slot(ca), bcur = slot(cb), anxt = slot(after(ca)), bnxt = slot(after(cb));
@@ -389,7 +494,7 @@ struct Core {
         if (kk == 0) {
           __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): no read of the current slabs is in flight
           // the next slabs have landed, the current ones are free
-          if (s == 0 && stored) dma::wait_and_barrier<63>();
+          if (s == 0 && stored) dma::wait_and_barrier<LOADS + STORES>();
           else dma::wait_and_barrier<LOADS>();
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -432,17 +537,23 @@ struct Core {
       tl.kc = __builtin_amdgcn_readfirstlane(tl.kc);
       tl.rows = __builtin_amdgcn_readfirstlane(tl.rows);
       tl.cols = __builtin_amdgcn_readfirstlane(tl.cols);
-      if (NARROW == SMALL_ROWS && tl.rows <= 128) {
-        if (tl.rows <= 32) item<1, 2>(tl, i, 0, 64 * lw);
-        else if (tl.rows <= 64) item<2, 2>(tl, i, 0, 64 * lw);
-        else item<4, 2>(tl, i, 0, 64 * lw);
-      } else if (NARROW == SMALL_COLS && tl.cols <= 128) {
-        if (tl.cols <= 32) item<2, 1>(tl, i, 64 * lw, 0);
-        else if (tl.cols <= 64) item<2, 2>(tl, i, 64 * lw, 0);
-        else item<2, 4>(tl, i, 64 * lw, 0);
-      } else {
-        item<4, 4>(tl, i, (lw >> 1) * 128, (lw & 1) * 128);
+      if constexpr (NARROW == SMALL_ROWS) {
+        if (tl.rows <= 128) {
+          if (tl.rows <= 32) item<1, 2>(tl, i, 0, 64 * lw);
+          else if (tl.rows <= 64) item<2, 2>(tl, i, 0, 64 * lw);
+          else item<4, 2>(tl, i, 0, 64 * lw);
+          continue;
+        }
       }
+      if constexpr (NARROW == SMALL_COLS) {
+        if (tl.cols <= 128) {
+          if (tl.cols <= 32) item<2, 1>(tl, i, 64 * lw, 0);
+          else if (tl.cols <= 64) item<2, 2>(tl, i, 64 * lw, 0);
+          else item<2, 4>(tl, i, 64 * lw, 0);
+          continue;
+        }
+      }
+      item<4, 4>(tl, i, (lw >> 1) * 128, (lw & 1) * 128);
     }
     __builtin_amdgcn_s_waitcnt(dma::waitcnt_vm(0));  // no load may land after the workgroup ends
   }
