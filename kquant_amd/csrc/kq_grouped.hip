@@ -179,7 +179,7 @@ struct Problem {
     const int64_t row0 = MODE == DW ? (int64_t)e * g.n + m0 : beg + m0;
     const int cols = (MODE == FORWARD ? g.n : g.k) - n0;
     char* out = g.out + row0 * g.ld_out + 2 * (int64_t)n0;
-    mm16::store16<NB, WN, F16>(out, g.ld_out, tl.rows, cols, wm, wn, acc, lane,
+    mm16::store16<NB, WN, F16>([&](int r) { return out + (uint32_t)r * g.ld_out; }, tl.rows, cols, wm, wn, acc, lane,
                                [](int, int, int, float v) { return v; });
     return tl.rows >= mm16::BM && cols >= mm16::BN;
   }
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void grouped_kernel(Args g) {
   p.g = g;
   p.setup();
   if (MODE != DW) zero_rows(g, MODE == FORWARD ? g.n : g.k);
-  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE == DW ? mm16::WHOLE : mm16::SMALL_ROWS, Problem<MODE, F16>> core(p, lds);
+  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE == DW ? mm16::WHOLE : mm16::SMALL_ROWS, true, Problem<MODE, F16>> core(p, lds);
   core.run();
 }
 

@@ -226,7 +226,8 @@ struct LogitProblem {
       }
       char* out = g.dt + ((int64_t)mt * mm16::BM * g.ldg + n0) * 2;
       const int row = wm + 4 * (lane >> 5);
-      mm16::store16<NB, WN, false>(out, (uint32_t)g.ldg * 2u, tl.rows, (count + 7) / 8 * 8 - n0, wm, wn, acc, lane, [&](int i, int j, int r, float z) {
+      mm16::store16<NB, WN, false>([&](int r) { return out + (uint32_t)r * ((uint32_t)g.ldg * 2u); }, tl.rows,
+                                   (count + 7) / 8 * 8 - n0, wm, wn, acc, lane, [&](int i, int j, int r, float z) {
         const int at = row + 32 * i + 8 * (r >> 2) + (r & 3);
         const float p = __builtin_amdgcn_exp2f((z - lse[j]) * LOG2E) - (at == tgt[j] ? 1.0f : 0.0f);
         return n0 + wn + 32 * j + (lane & 31) < count ? up[j] * p : 0.0f;
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void logit_kernel(LogitArgs g) {
   LogitProblem<GRAD> p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (p.count + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, false, false, mm16::SMALL_COLS, LogitProblem<GRAD>> core(p, lds);
+  mm16::Core<false, false, false, mm16::SMALL_COLS, false, LogitProblem<GRAD>> core(p, lds);
   core.run();
 }
 
@@ -360,8 +361,8 @@ struct DhProblem {
       const int* map = g.rows_of + m0;
       char* out = g.dh + 2 * (int64_t)n0;
       const float alpha = *g.alpha;
-      mm16::store16_rows<NB, WN, false>([&](int r) { return out + map[r] * g.lddh; }, tl.rows, g.k - n0, wm, wn, acc, lane,
-                                        [&](int, int, int, float v) { return alpha * v; });
+      mm16::store16<NB, WN, false>([&](int r) { return out + map[r] * g.lddh; }, tl.rows, g.k - n0, wm, wn, acc, lane,
+                                   [&](int, int, int, float v) { return alpha * v; });
     } else {
       float* out = g.planes + ((int64_t)sl * g.tokens + m0) * g.k + n0;
       const uint32_t ld = (uint32_t)g.k;
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
   DhProblem p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (p.count + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
-  mm16::Core<true, true, false, mm16::SMALL_ROWS, DhProblem> core(p, lds);
+  mm16::Core<true, true, false, mm16::SMALL_ROWS, true, DhProblem> core(p, lds);
   core.run();
 }
 
@@ -440,7 +441,8 @@ struct DwProblem {
     const int n0 = nt * mm16::BN;
     char* out = g.dw + ((int64_t)mt * mm16::BM * g.k + n0) * 2;
     const float alpha = *g.alpha;
-    mm16::store16<NB, WN, false>(out, (uint32_t)g.k * 2u, tl.rows, g.k - n0, wm, wn, acc, lane,
+    mm16::store16<NB, WN, false>([&](int r) { return out + (uint32_t)r * ((uint32_t)g.k * 2u); }, tl.rows, g.k - n0, wm, wn,
+                                 acc, lane,
                                  [&](int, int, int, float v) { return alpha * v; });
     return tl.rows >= mm16::BM && g.k - n0 >= mm16::BN;
   }
@@ -450,7 +452,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dw_kernel(DwArgs g) {
   DwProblem p{g, (__builtin_amdgcn_readfirstlane(*g.count) + 7) / 8 * 8, 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, true, false, mm16::WHOLE, DwProblem> core(p, lds);
+  mm16::Core<false, true, false, mm16::WHOLE, false, DwProblem> core(p, lds);
   core.run();
 }
 

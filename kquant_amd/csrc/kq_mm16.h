@@ -15,7 +15,7 @@
 // fixed place between two MFMAs (sched_barrier pins it):
 //  * operands go HBM -> LDS by 16-byte direct loads, a step's share of one
 //    operand a slab of 32 KiB, and all of LDS is five slabs: A and B of the step
-//    in use and of the next one, and A of the step after.  A slab is whole
+//    in use and of the next one, and one operand (the leading one) of the step after.  A slab is whole
 //    128-byte lines of rows (contraction-major) or 512-byte runs of 64
 //    contraction rows (the other form), XOR-swizzled so that the lanes of a read
 //    fall on distinct banks.
@@ -24,8 +24,8 @@
 //    block 0 and of the next one after it.  Operands across the contraction
 //    are read transposed (ds_read_b64_tr_b16).
 //  * one barrier a step, after block 0: every wave then holds all of the
-//    current slabs in registers, so both are free.  B of the step after next is
-//    loaded in block 1, A of the one after that in blocks 2 and 3: a direct
+//    current slabs in registers, so both are free.  The following operand of the step
+//    after next is loaded in block 1, the leading one of the step after that in blocks 2 and 3: a direct
 //    load takes 16 cycles of the CU's address unit, so 64 of them in one block
 //    of 512 cycles held its MFMAs up (two stages of both operands, all loads in
 //    block 1: 3325 cycles a step at 4096 x 12288 x 7168).
@@ -42,6 +42,8 @@
 // tiles an XCD runs together share operand rows in its L2; the loads run on
 // across tile boundaries.
 #pragma once
+
+#include <type_traits>
 
 #include "kq_common.h"
 #include "kq_dma.h"
@@ -229,99 +231,83 @@ __device__ __forceinline__ void quad_rows(const float16_t (&acc)[NB][WN], int i,
   }
 }
 
+// The same exchanged over two quads, for pairs of blocks: eight columns of one
+// row, of the first block in the even quad and of the second in the odd one.
+template <int NB, int WN, bool F16, class F>
+__device__ __forceinline__ void eight_columns(const float16_t (&acc)[NB][WN], int i, int g, u32x4_t (&q)[WN / 2], F&& f) {
+  const bool odd = threadIdx.x & 4;
+  u32x2_t v[WN];
+  quad_rows<NB, WN, F16>(acc, i, g, v, f);
+  __builtin_amdgcn_sched_barrier(0);
+  uint32_t x0[WN / 2], x1[WN / 2];
+#pragma unroll
+  for (int j = 0; j < WN; j += 2) {
+    x0[j / 2] = odd ? v[j][0] : v[j + 1][0];
+    x1[j / 2] = odd ? v[j][1] : v[j + 1][1];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN / 2; ++j) {
+    x0[j] = other_quad(x0[j]);
+    x1[j] = other_quad(x1[j]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < WN; j += 2) {
+    q[j / 2][0] = odd ? x0[j / 2] : v[j][0];
+    q[j / 2][1] = odd ? x1[j / 2] : v[j][1];
+    q[j / 2][2] = odd ? v[j + 1][0] : x0[j / 2];
+    q[j / 2][3] = odd ? v[j + 1][1] : x1[j / 2];
+  }
+}
+
 // Stores a wave's blocks in 16 bits: rows below `rows`, columns below `cols` (a
-// multiple of 4) of the tile, f(i, j, r, v) the value stored for element r of
-// block (i, j), v the accumulated one, to base + row ld (16-byte aligned rows).
+// multiple of 8) of the tile, f(i, j, r, v) the value stored for element r of
+// block (i, j), v the accumulated one; address(row) is the 16-byte aligned
+// address of a row's column 0 (asked for rows below `rows` only).
 // A store instruction takes the CU's memory path some 8 cycles for each line it
 // touches, so it should fill them: a lane's four rows of one column are
-// exchanged over its quad for four columns of one row (8 bytes), and in whole
-// tiles, which need no masks, over two quads for 16 bytes, of which 8 lanes
-// make a 128-byte line.  Results are larger than an XCD's L2 and read from
-// another one: nontemporal.  48 weight gradients of 7168 x 2048, 64 rows each:
-// 461 us with 8 bytes a lane, 402 nontemporal, 290 with 16 bytes (1.41 GB).
-template <int NB, int WN, bool F16, class F>
-__device__ __forceinline__ void store16(char* base, uint32_t ld, int rows, int cols, int wm, int wn,
-                                        float16_t (&acc)[NB][WN], int lane, F&& f) {
+// exchanged over two quads for eight columns of one row, of which 8 lanes make
+// a 128-byte line.  Results are larger than an XCD's L2 and read from another
+// one: nontemporal.  48 weight gradients of 7168 x 2048, 64 rows each: 461 us
+// with 8 bytes a lane, 402 nontemporal, 290 with 16 bytes (1.41 GB).
+template <int NB, int WN, bool F16, class At, class F>
+__device__ __forceinline__ void store16(At&& address, int rows, int cols, int wm, int wn, float16_t (&acc)[NB][WN],
+                                        int lane, F&& f) {
   int row = wm + 4 * (lane >> 5) + (lane & 3), col = wn + (lane & 28);
+  if (WN > 1 && (lane & 4)) col += 28;  // the second block, from 4 columns to the left
   asm volatile("" : "+v"(row), "+v"(col));  // the elements' offsets are not kept (and spilled) from tile to tile
-  if constexpr (NB * WN == 16) if (rows >= BM && cols >= BN) {
-    // the odd quad of two takes the second of two blocks, from 4 columns to the left
-    const bool odd = lane & 4;
-    uint32_t off = (uint32_t)row * ld + 2u * (uint32_t)col + (odd ? 56u : 0u);
+  auto block_rows = [&](auto whole) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       in_place(acc, i);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        u32x2_t v[WN];
-        quad_rows<NB, WN, F16>(acc, i, g, v, f);
-        __builtin_amdgcn_sched_barrier(0);
-        uint32_t x0[WN / 2], x1[WN / 2];
+        const int at = row + 32 * i + 8 * g;
+        char* p = address(whole.value ? at : min(at, rows - 1)) + 2 * (int64_t)col;
+        if constexpr (WN > 1) {
+          u32x4_t q[WN / 2];
+          eight_columns<NB, WN, F16>(acc, i, g, q, f);
 #pragma unroll
-        for (int j = 0; j < WN; j += 2) {
-          x0[j / 2] = odd ? v[j][0] : v[j + 1][0];
-          x1[j / 2] = odd ? v[j][1] : v[j + 1][1];
+          for (int j = 0; j < WN / 2; ++j)
+            if (whole.value || (at < rows && col + 64 * j < cols))
+              __builtin_nontemporal_store(q[j], reinterpret_cast<u32x4_t*>(p + 128 * j));
+        } else {
+          u32x2_t v[WN];
+          quad_rows<NB, WN, F16>(acc, i, g, v, f);
+          if (at < rows && col < cols) __builtin_nontemporal_store(v[0], reinterpret_cast<u32x2_t*>(p));
         }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < WN / 2; ++j) {
-          x0[j] = other_quad(x0[j]);
-          x1[j] = other_quad(x1[j]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < WN; j += 2) {
-          u32x4_t q;
-          q[0] = odd ? x0[j / 2] : v[j][0];
-          q[1] = odd ? x1[j / 2] : v[j][1];
-          q[2] = odd ? v[j + 1][0] : x0[j / 2];
-          q[3] = odd ? v[j + 1][1] : x1[j / 2];
-          __builtin_nontemporal_store(q, reinterpret_cast<u32x4_t*>(base + off + 64 * j));
-        }
-        off += 8 * ld;
+        if (!whole.value) __builtin_amdgcn_sched_barrier(0);
       }
     }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    in_place(acc, i);
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int at = row + 32 * i + 8 * g;
-      char* p = base + (uint32_t)at * ld + 2 * (uint32_t)col;
-      u32x2_t v[WN];
-      quad_rows<NB, WN, F16>(acc, i, g, v, f);
-#pragma unroll
-      for (int j = 0; j < WN; ++j)
-        if (at < rows && col + 32 * j < cols) __builtin_nontemporal_store(v[j], reinterpret_cast<u32x2_t*>(p + 64 * j));
-      __builtin_amdgcn_sched_barrier(0);
+  };
+  if constexpr (NB * WN == 16) {
+    if (rows >= BM && cols >= BN) {  // without masks and their branches
+      block_rows(std::true_type{});
+      return;
     }
   }
-}
-
-// The same with rows of their own: address(row) the address of a row's column 0
-// (asked for rows below `rows` only).
-template <int NB, int WN, bool F16, class At, class F>
-__device__ __forceinline__ void store16_rows(At&& address, int rows, int cols, int wm, int wn, float16_t (&acc)[NB][WN],
-                                             int lane, F&& f) {
-  int row = wm + 4 * (lane >> 5) + (lane & 3), col = wn + (lane & 28);
-  asm volatile("" : "+v"(row), "+v"(col));
-#pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    in_place(acc, i);
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int at = row + 32 * i + 8 * g;
-      char* p = address(min(at, rows - 1)) + 2 * (int64_t)col;
-      u32x2_t v[WN];
-      quad_rows<NB, WN, F16>(acc, i, g, v, f);
-#pragma unroll
-      for (int j = 0; j < WN; ++j)
-        if (at < rows && col + 32 * j < cols) __builtin_nontemporal_store(v[j], reinterpret_cast<u32x2_t*>(p + 64 * j));
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
+  block_rows(std::false_type{});
 }
 
 // One operand's loads, slab after slab, across this worker's tiles.  The
@@ -379,6 +365,8 @@ struct Side {
   __device__ __forceinline__ void issue(int u, uint32_t slot, int lw) const {
     dma::load_to_lds16(r, at + (uint32_t)u * step, slot + (uint32_t)((4 * u + lw) * 1024));
   }
+  // loads that hold a valid row (contraction-major; the others write zeros that only rows past the tile read)
+  __device__ __forceinline__ int needed() const { return ACROSS ? LOADS : (int)(rows + 31) / 32; }
   // the next slab of this tile; false at its end
   __device__ __forceinline__ bool next() {
     k += BK;
@@ -399,14 +387,19 @@ enum { WHOLE = 0, SMALL_ROWS = 1, SMALL_COLS = 2 };  // which tiles may be narro
 //   epilogue<NB, WN>(const Tile&, int i, int wm, int wn, float16_t (&acc)[NB][WN], int lane)
 // with element r of acc[a][b] at row wm + 32 a + 8 (r / 4) + 4 (lane / 32) + r % 4,
 // column wn + 32 b + lane % 32 of the tile.
-template <bool AA, bool BA, bool F16, int NARROW, class P>
+//
+// LEAD_B: B's loads run a step further ahead than A's, not A's than B's: for
+// the operand that comes from memory rather than from a cache.  (Narrow tiles'
+// steps are shorter than memory's latency: 333 rows in 12 groups, 1416 x 1032,
+// forward LEAD_US.)
+template <bool AA, bool BA, bool F16, int NARROW, bool LEAD_B, class P>
 struct Core {
   const P& p;
   uint32_t lds0;
   int lane, lw, tiles;
   Side<AA> sa;
   Side<BA> sb;
-  int ca, cb;  // slots of the slabs in use
+  int cl, cf;  // slots of the slabs in use: the leading operand's and the other's
   // Every wave has issued STORES stores or more since the loads of the next step's slabs.  All are waited for in the
   // order of issue, and LOADS loads of a later slab stand between: with STORES + LOADS outstanding the slabs have
   // landed, and the stores need not have.
@@ -435,6 +428,23 @@ struct Core {
     }
   }
 
+  __device__ __forceinline__ void lead_issue(int u, uint32_t to) {
+    if (LEAD_B) sb.issue(u, to, lw);
+    else sa.issue(u, to, lw);
+  }
+  __device__ __forceinline__ void lead_next() {
+    if (LEAD_B) next_b();
+    else next_a();
+  }
+  __device__ __forceinline__ void follow_issue(int u, uint32_t to) {
+    if (LEAD_B) sa.issue(u, to, lw);
+    else sb.issue(u, to, lw);
+  }
+  __device__ __forceinline__ void follow_next() {
+    if (LEAD_B) next_a();
+    else next_b();
+  }
+
   // Wave tile of NB x WN blocks at (wm, wn): this item's steps, then its epilogue.
   template <int NB, int WN>
   __device__ __forceinline__ void item(const Tile& tl, int it, int wm, int wn) {
@@ -447,16 +457,16 @@ struct Core {
     u32x4_t a[4][NB], b[4][WN];
     float16_t acc[NB][WN];
     // fragment f of k16 block kk: 0..NB-1 of A, then B
-    auto read_one = [&](uint32_t as, uint32_t bs, int kk, int f) {
-      if (f < NB) a[kk][f] = fa.read(as, kk, f);
-      else b[kk][f - NB] = fb.read(bs, kk, f - NB);
+    auto read_one = [&](uint32_t lead, uint32_t follow, int kk, int f) {
+      if (f < NB) a[kk][f] = fa.read(LEAD_B ? follow : lead, kk, f);
+      else b[kk][f - NB] = fb.read(LEAD_B ? lead : follow, kk, f - NB);
     };
     const int steps = steps_of(tl.kc);
     // this item's first slabs have landed: in run() or at the last barrier of the item before
 #pragma unroll
     for (int kk = 0; kk < 3; ++kk)
 #pragma unroll
-      for (int f = 0; f < NB + WN; ++f) read_one(slot(ca), slot(cb), kk, f);
+      for (int f = 0; f < NB + WN; ++f) read_one(slot(cl), slot(cf), kk, f);
     __builtin_amdgcn_sched_barrier(0);  // the accumulators are cleared while these are on their way
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -466,7 +476,10 @@ struct Core {
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     constexpr int NM = NB * WN;  // MFMAs of a k16 block
     for (int s = 0; s < steps; ++s) {
-      const uint32_t acur = slot(ca), bcur = slot(cb), anxt = slot(after(ca)), bnxt = slot(after(cb));
+      // Narrow tiles: loads of the following operand's rows that are there.  The barrier below counts the leading
+      // operand's alone, which are younger.
+      const int few = LEAD_B ? sa.needed() : sb.needed();
+      const uint32_t lcur = slot(cl), fcur = slot(cf), lnxt = slot(after(cl)), fnxt = slot(after(cf));
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
@@ -479,15 +492,16 @@ struct Core {
 #pragma unroll
           for (int f = 0; f < NB + WN; ++f)
             if (f * rn / (NB + WN) == m)
-              read_one(kk == 0 ? acur : anxt, kk == 0 ? bcur : bnxt, (kk + 3) & 3, f);
-          if (kk == 1) {  // B of the step after next, into A's slot
+              read_one(kk == 0 ? lcur : lnxt, kk == 0 ? fcur : fnxt, (kk + 3) & 3, f);
+          if (kk == 1) {  // the following operand of the step after next, into the leading one's slot
 #pragma unroll
-            for (int u = m * LOADS / NM; u < (m + 1) * LOADS / NM; ++u) sb.issue(u, acur, lw);
+            for (int u = m * LOADS / NM; u < (m + 1) * LOADS / NM; ++u)
+              if (NM == 16 || u < few) follow_issue(u, lcur);
           }
-          if (kk >= 2) {  // A of the step after that, into B's slot
+          if (kk >= 2) {  // the leading operand of the step after that, into the other's slot
 #pragma unroll
             for (int u = ((kk - 2) * NM + m) * LOADS / (2 * NM); u < ((kk - 2) * NM + m + 1) * LOADS / (2 * NM); ++u)
-              sa.issue(u, bcur, lw);
+              lead_issue(u, fcur);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -498,11 +512,11 @@ struct Core {
           else dma::wait_and_barrier<LOADS>();
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (kk == 1) next_b();
-        if (kk == 3) next_a();
+        if (kk == 1) follow_next();
+        if (kk == 3) lead_next();
       }
-      ca = after(ca);
-      cb = after(cb);
+      cl = after(cl);
+      cf = after(cf);
     }
     stored = p.template epilogue<NB, WN>(tl, it, wm, wn, acc, l) && NB * WN == 16;
     // an epilogue that ends in a lane's branch must not be the tile loop's last statement: the loop would be taken
@@ -514,22 +528,20 @@ struct Core {
     tiles = __builtin_amdgcn_readfirstlane(p.tiles());
     if (tiles <= 0) return;
     sa.i = sb.i = 0;
-    ca = 0;
-    cb = 1;
+    cl = 0;
+    cf = 1;
     stored = false;
     set_a();
     set_b();
 #pragma unroll
-    for (int q = 0; q < SLOTS; ++q) {  // A, B, A, B, A
-      if (q & 1) {
+    for (int q = 0; q < SLOTS; ++q) {  // leading, following, leading, following, leading
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) sb.issue(u, slot(q), lw);
-        next_b();
-      } else {
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) sa.issue(u, slot(q), lw);
-        next_a();
+      for (int u = 0; u < LOADS; ++u) {
+        if (q & 1) follow_issue(u, slot(q));
+        else lead_issue(u, slot(q));
       }
+      if (q & 1) follow_next();
+      else lead_next();
     }
     dma::wait_and_barrier<(SLOTS - 2) * LOADS>();
     for (int i = 0; i < tiles; ++i) {
