@@ -329,8 +329,8 @@ int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x,
  * over the counted tokens (NaN if none).
  * h bf16 [tokens, k] (row stride ldh elements, ldh % 8 == 0).  w_fmt: the head
  * as KQ_FMT_BF16 [vocab, k] (k % 8 == 0, w_scale NULL), or MXFP8 / MXFP4 rows
- * with E8M0 scales [vocab, k/32] (k % 64 == 0).  target: device int64.
- * tokens <= 2^20, vocab <= 2^24, k <= 2^16.  workspace: 256-byte aligned,
+ * with E8M0 scales [vocab, k/32] (k % 64 == 0).  target: device int64.  h, w
+ * and the gradients are 16-byte aligned, target 8, w_scale 4.  tokens <= 2^20, vocab <= 2^24, k <= 2^16.  workspace: 256-byte aligned,
  * uninitialised; it holds the counted rows and 32 bytes per token and 256
  * vocabulary rows, of an MX head an expanded piece (the size functions plan
  * for the current device).  Deterministic. */

@@ -262,6 +262,30 @@ def to_gpu(tensors: Iterable[torch.Tensor | None]) -> tuple[list, torch.device, 
     return moved, gpu, host
 
 
+_LEAF_STREAM = "kquant_amd.stream"
+
+
+def hold_leaves(*tensors: torch.Tensor) -> list:
+    """The gradient accumulators of leaves, to be held over the call that differentiates them.
+
+    A leaf's accumulator belongs to the stream on which its first living graph
+    was built.  A backward pass captured on another stream would pull that
+    stream into the capture, which ends the process: it is refused here.
+    """
+
+    held = []
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad and t.is_leaf:
+                node = torch.autograd.graph.get_gradient_edge(t).node
+                here = torch.cuda.current_stream(t.device).cuda_stream
+                if node.metadata.setdefault(_LEAF_STREAM, here) != here and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("an autograd graph of these leaves that was built on another stream still lives: "
+                                       "drop it (its results) before capturing their forward and backward pass")
+                held.append(node)
+    return held
+
+
 def aligned(t: torch.Tensor, align: int = 16) -> torch.Tensor:
     """Contiguous tensor whose data pointer is ``align``-byte aligned."""
 

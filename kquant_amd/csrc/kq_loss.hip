@@ -90,7 +90,8 @@ __global__ __launch_bounds__(1024) void alpha_kernel(const float* __restrict__ g
                                                      float* __restrict__ alpha) {
   __shared__ float wave_max[16];
   if (reduction != NONE) {
-    if (threadIdx.x == 0) *alpha = reduction == SUM ? grad[0] : *count > 0 ? grad[0] / (float)*count : 0.0f;
+    const int n = *count;  // none: gradients of zero whatever the upstream one is
+    if (threadIdx.x == 0) *alpha = n == 0 ? 0.0f : reduction == SUM ? grad[0] : grad[0] / (float)n;
     return;
   }
   float m = 0.0f;  // the largest finite one: another leaves u infinite or NaN, as it should
@@ -558,8 +559,8 @@ static int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backward, int cus) {
   Plan p{};
   const bool mx = w_fmt != KQ_FMT_BF16;
-  // A block-scaled head at few tokens is read as it is, once (5 tokens, V = 129280, K = 7168 E4M3: FEW_US; expanded
-  // to bf16 and multiplied in tiles 835 us).  A bf16 head's tiles stream it at the chip's rate at any count.
+  // A block-scaled head at few tokens is read as it is, once (5 tokens, V = 129280, K = 7168 E4M3: 276 us; expanded
+  // to bf16 and multiplied in tiles 760 us).  A bf16 head's tiles stream it at the chip's rate at any count.
   p.few = mx && !backward && tokens >= 1 && tokens <= 64;
   if (p.few) {
     p.o_z = 0;
@@ -636,8 +637,8 @@ static int check(const char* fn, int w_fmt, const void* h, int64_t ldh, int64_t 
   if (tokens > 1 << 20 || vocab > 1 << 24 || k > 1 << 16)
     return kq_fail(KQ_ERR_LIMIT, "%s: at most 2^20 tokens, 2^24 vocabulary rows and k = 2^16", fn);
   if (mx && !w_scale) return kq_fail(KQ_ERR_INVALID, "%s: a block-scaled head needs its scales", fn);
-  if (kq_misaligned(h, 16) || kq_misaligned(w, 16) || kq_misaligned(target, 8) || kq_misaligned(w_scale, 2))
-    return kq_fail(KQ_ERR_INVALID, "%s: h and w must be 16-byte aligned", fn);
+  if (kq_misaligned(h, 16) || kq_misaligned(w, 16) || kq_misaligned(target, 8) || kq_misaligned(w_scale, 4))
+    return kq_fail(KQ_ERR_INVALID, "%s: h and w must be 16-byte aligned, target 8, scales 4", fn);
   return KQ_OK;
 }
 

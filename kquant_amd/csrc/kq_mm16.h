@@ -390,8 +390,8 @@ enum { WHOLE = 0, SMALL_ROWS = 1, SMALL_COLS = 2 };  // which tiles may be narro
 //
 // LEAD_B: B's loads run a step further ahead than A's, not A's than B's: for
 // the operand that comes from memory rather than from a cache.  (Narrow tiles'
-// steps are shorter than memory's latency: 333 rows in 12 groups, 1416 x 1032,
-// forward LEAD_US.)
+// steps are shorter than memory's latency: 64 rows in 48 groups, 4096 x 7168,
+// forward 443 us with A's ahead, 404 with B's.)
 template <bool AA, bool BA, bool F16, int NARROW, bool LEAD_B, class P>
 struct Core {
   const P& p;

@@ -77,7 +77,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     Offsets outside [0, rows] are taken as the nearest of the two.
 
     Differentiable once, in x and weight; an empty group's weight gradient is
-    zero.  Results do not change from call to call (no atomics).
+    zero.  Results do not change from call to call (no atomics).  Captured into
+    a graph, forward and backward go into one capture, made while no eager graph
+    of the same leaves lives.
     """
 
     if x.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != x.dtype:
@@ -101,6 +103,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     if host is not None:
         gpu = N.require_gpu()
         x, weight, offsets = x.to(gpu), weight.to(gpu), offsets.to(gpu)
+    held = N.hold_leaves(x, weight) if host is None else None
     offsets = N.aligned(offsets.to(torch.int64), 8)
     y = _GroupedLinear.apply(x, weight, offsets)
+    del held
     return y if host is None else y.to(host)

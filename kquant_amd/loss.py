@@ -84,7 +84,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     Differentiable once, in hidden and in a bf16 weight; a block-scaled head is
     frozen.  The logits and all sums are fp32; the gradients are bf16, their
     softmax terms rounded to bf16 as operands of the gradients' products.
-    Results do not change from call to call (no atomics).
+    Results do not change from call to call (no atomics).  Captured into a graph,
+    forward and backward go into one capture, made while no eager graph of the
+    same leaves lives.
     """
 
     if reduction not in _REDUCTIONS:
@@ -120,6 +122,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     if any(t.device != hidden.device for t in tensors):
         raise ValueError("hidden, weight, target and scale must be on one device")
     host = None if hidden.is_cuda else hidden.device
+    held = N.hold_leaves(hidden, weight) if host is None else None
     h, t = hidden.reshape(-1, k), target.reshape(-1)
     if host is not None:
         gpu = N.require_gpu()
@@ -129,6 +132,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         weight, scale = weight.view(torch.uint8), N.aligned(scale)
     weight, t = N.aligned(weight), N.aligned(t, 8)
     loss = _LinearCrossEntropy.apply(h, weight, scale, t, fmt, int(ignore_index), _REDUCTIONS[reduction])
+    del held
     if reduction == "none":
         loss = loss.reshape(target.shape)
     return loss if host is None else loss.to(host)

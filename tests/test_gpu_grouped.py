@@ -239,3 +239,83 @@ def test_large_offsets(gpu):
     y = grouped_linear(x, w, torch.tensor(starts, device=gpu))
     close(y, x, w[-1], k)
     assert grouped.MAX_GROUPS >= groups
+
+
+def test_more_tiles_than_a_table_holds(gpu):
+    """More than 256 output tiles for each compute unit, in all three products."""
+    groups, n, k = 4096, 1032, 1032
+    rows = 3 * groups
+    g = torch.Generator(device=gpu).manual_seed(1)
+    sizes = torch.randint(0, 6, (groups,), generator=g, device=gpu)
+    sizes[0], sizes[-1] = 2, 1
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64, device=gpu), sizes.cumsum(0)]).clamp(max=rows)
+    starts = offsets.tolist()
+    x = torch.randn(rows, k, generator=g, device=gpu).to(torch.bfloat16)
+    dy = torch.randn(rows, n, generator=g, device=gpu).to(torch.bfloat16)
+    w = torch.randn(groups, n, k, dtype=torch.bfloat16, generator=g, device=gpu).requires_grad_()
+    (dw,) = torch.autograd.grad(grouped_linear(x, w, offsets), w, dy)
+    for e in [0, 1, 2, 777, 2047, 2048, 3333, groups - 2, groups - 1]:
+        a, b = starts[e], starts[e + 1]
+        close(dw[e], dy[a:b].T, x[a:b].T, b - a)
+    empty = (offsets[1:] == offsets[:-1]).nonzero()[:, 0]
+    assert empty.numel() > 0 and not dw[empty].any()
+    del w, dw
+    n, k = 6152, 64  # 25 column tiles of a row tile for each group
+    w = torch.randn(groups, n, k, dtype=torch.bfloat16, generator=g, device=gpu)
+    x = torch.randn(rows, k, generator=g, device=gpu).to(torch.bfloat16).requires_grad_()
+    dy = torch.randn(rows, n, generator=g, device=gpu).to(torch.bfloat16)
+    y = grouped_linear(x, w, offsets)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for e in [0, 1, 2, 777, 2047, 2048, 3333, groups - 2, groups - 1]:
+        a, b = starts[e], starts[e + 1]
+        close(y[a:b].detach(), x[a:b].detach(), w[e], k)
+        close(dx[a:b], dy[a:b], w[e].T, n)
+
+
+def test_differentiable_once(gpu):
+    x, w, dy = operands(20, 2, 16, 24, torch.bfloat16, gpu)
+    x.requires_grad_()
+    (dx,) = torch.autograd.grad(grouped_linear(x, w, torch.tensor([0, 5, 20], device=gpu)), x, dy.requires_grad_(),
+                                create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.float().sum().backward()
+
+
+def test_views_of_weights_and_gradients(gpu):
+    """Transposed and sliced weights, an expanded upstream gradient."""
+    x, w, _ = operands(70, 3, 40, 48, torch.bfloat16, gpu)
+    offsets = torch.tensor([0, 30, 30, 65], device=gpu)
+    leaf = w.transpose(1, 2).contiguous().requires_grad_()  # [groups, K, N]
+    y = grouped_linear(x, leaf.transpose(1, 2), offsets)
+    up = torch.ones(1, 1, dtype=torch.bfloat16, device=gpu).expand_as(y)
+    (dleaf,) = torch.autograd.grad(y, leaf, up)
+    want = _all(x, w, up.contiguous(), offsets)
+    assert torch.equal(y.detach(), want[0]) and torch.equal(dleaf, want[2].transpose(1, 2))
+    wide = torch.randn(5, 40, 48, device=gpu).to(torch.bfloat16).requires_grad_()
+    (dwide,) = torch.autograd.grad(grouped_linear(x, wide[1:4], offsets), wide, up)
+    assert not dwide[0].any() and not dwide[4].any() and torch.equal(dwide[1:4], want[2])
+
+
+def test_capture_beside_a_living_graph(gpu):
+    """Refused before anything of it is captured; once that graph is gone, it goes through."""
+    x, w, dy = operands(64, 3, 64, 64, torch.bfloat16, gpu)
+    offsets = torch.tensor([0, 9, 40, 64], device=gpu)
+    want = _all(x, w, dy, offsets)
+    sx, sw, flag = x.clone().requires_grad_(), w.clone().requires_grad_(), torch.ones(4, device=gpu)
+    eager = grouped_linear(sx, sw, offsets)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        flag.zero_()
+        with pytest.raises(RuntimeError, match="still lives"):
+            grouped_linear(sx, sw, offsets)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = grouped_linear(sx, sw, offsets)
+        dx, dw = torch.autograd.grad(y, (sx, sw), dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((y, dx, dw), want):
+            assert torch.equal(a.detach(), b)

@@ -168,3 +168,28 @@ def test_captured(gpu, m):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, f(x, q, s, bias=bias, activation="gelu", residual=residual))
+
+
+@pytest.mark.parametrize("shift,pad", [(0, 0), (0, 1), (0, 2), (0, 4), (1, 0), (2, 0), (4, 8)])
+@pytest.mark.parametrize("m,n,k", [(1, 264, 256), (100, 520, 2048), (300, 776, 192), (4100, 4100, 256)])
+def test_any_alignment_of_results_and_residuals(gpu, m, n, k, shift, pad):
+    """Results and residuals at any element, with any row stride; what lies between the rows stays."""
+    x, w, bias, residual = inputs(m, n, k, torch.bfloat16, gpu)
+    q, s, _, f = quantized(w, "mxfp8")
+    want = f(x, q, s, bias=bias, activation="relu", residual=residual)
+    ld = n + pad
+    need = int(N.library().kq_mx_linear_workspace_size(m, n, k))
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=gpu)
+    for which in ("c", "r"):
+        ldc, ldr = (ld, n) if which == "c" else (n, ld)
+        out = torch.full((m * ldc + 16,), 7.0, dtype=torch.bfloat16, device=gpu)
+        res = torch.full((m * ldr + 16,), 7.0, dtype=torch.bfloat16, device=gpu)
+        c0, r0 = (shift, 0) if which == "c" else (0, shift)
+        res[r0:r0 + m * ldr].view(m, ldr)[:, :n] = residual
+        N.call("kq_mx_linear_epilogue", N.FMT_MXFP8_E4M3, N.DT_BF16, N.ptr(x), k, N.ptr(q), N.ptr(s), m, n, k, 1,
+               N.ptr(bias), N.DT_F32, N.ptr(res[r0:]), ldr, N.DT_BF16, N.ptr(out[c0:]), ldc, N.ptr(ws), need,
+               N.stream(gpu))
+        torch.cuda.synchronize()
+        body = out[c0:c0 + m * ldc].view(m, ldc)
+        assert torch.equal(body[:, :n], want)
+        assert (body[:, n:] == 7).all() and (out[:c0] == 7).all() and (out[c0 + m * ldc:] == 7).all()

@@ -322,3 +322,100 @@ def test_cpu_tensors(gpu):
     assert loss.device.type == "cpu" and torch.equal(loss.detach(), want.detach().cpu())
     for a, b in zip(grads, torch.autograd.grad(want, (gx, gy))):
         assert torch.equal(a, b.cpu())
+
+
+@pytest.mark.parametrize("tokens,k", [(3, 128), (3, 192), (40, 256), (70, 128)])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_block_scaled_ignored_captured_and_offset(gpu, fmt, tokens, k):
+    """A block-scaled head: NaN in ignored rows, a target outside, scales that begin at odd bytes, and replays."""
+    h, w, target = inputs(tokens, 333, k, gpu, ignored=0.3)
+    target[0], target[1], target[2] = 332, -100, 333
+    q, s = (mxfp8.mxfp8_quantize if fmt == "mxfp8" else mxfp4.mxfp4_quantize)(w)
+    odd = torch.zeros(s.numel() + 1, dtype=torch.uint8, device=gpu)
+    odd[1:] = s.reshape(-1)
+    odd = odd[1:].reshape(s.shape)
+    bad = h.clone()
+    bad[target == -100] = float("nan")
+    want = linear_cross_entropy(h, q, target, s, reduction="none")
+    got = linear_cross_entropy(bad, q, target, odd, reduction="none")
+    inside = target != 333
+    assert got[2].isnan() and torch.equal(got[inside], want[inside]) and not got[target == -100].any()
+    still, st = bad.clone(), target.clone()
+    linear_cross_entropy(still, q, st, s, reduction="none")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = linear_cross_entropy(still, q, st, s, reduction="none")
+    for seed in range(3):
+        nh, _, nt = inputs(tokens, 333, k, gpu, seed=seed, ignored=0.3)
+        still.copy_(nh)
+        st.copy_(nt)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, linear_cross_entropy(nh, q, nt, s, reduction="none"))
+
+
+@pytest.mark.parametrize("head", ["bf16", "mxfp8", "mxfp4"])
+def test_head_past_2_gib(gpu, head):
+    tokens, vocab, k = 6, 70_000, 32_768
+    if head == "mxfp4":
+        vocab = 140_000
+    g = torch.Generator(device=gpu).manual_seed(0)
+    h = torch.randn(tokens, k, generator=g, device=gpu).to(torch.bfloat16)
+    q, s, z, err = [], [], [], []
+    for r in range(0, vocab, 10_000):
+        w = (torch.randn(10_000, k, generator=g, device=gpu) * (3 / math.sqrt(k))).to(torch.bfloat16)
+        if head != "bf16":
+            a, b = (mxfp8.mxfp8_quantize if head == "mxfp8" else mxfp4.mxfp4_quantize)(w)
+            w = (mxfp8.mxfp8_dequantize if head == "mxfp8" else mxfp4_io.dequant)(a, b)
+            q.append(a.view(torch.uint8))
+            s.append(b)
+        else:
+            q.append(w)
+        z.append(h.double() @ w.double().T)
+        err.append((h.double().abs() @ w.double().abs().T).amax(1))
+    q, s = torch.cat(q), torch.cat(s) if s else None
+    z, err = torch.cat(z, 1), k * U24 * torch.stack(err).amax(0)
+    assert q.numel() * q.element_size() > 1 << 31
+    target = torch.tensor([0, vocab - 1, 65_535, 65_536, vocab - 300, -100], device=gpu)
+    lse = torch.logsumexp(z, 1)
+    want = lse - z.gather(1, target.clamp(min=0)[:, None])[:, 0]
+    want[-1] = 0
+    tol = 2 * err + U24 * (8 * 31 + 400) + U24 * 4 * (lse.abs() + z.abs().amax(1) + want.abs())
+    near(linear_cross_entropy(h, q, target, s, reduction="none"), want, tol)
+
+
+def test_infinite_upstream_of_no_token(gpu):
+    h, w, target = inputs(5, 40, 64, gpu)
+    h.requires_grad_()
+    w.requires_grad_()
+    for reduction in ("sum", "mean"):
+        loss = linear_cross_entropy(h, w, torch.full_like(target, -100), reduction=reduction)
+        dh, dw = torch.autograd.grad(loss, (h, w), torch.full_like(loss, float("inf")))
+        assert not dh.any() and not dw.any()
+
+
+def test_differentiable_once(gpu):
+    h, w, target = inputs(5, 40, 64, gpu)
+    target[0] = 1
+    h.requires_grad_()
+    up = torch.ones((), device=gpu, requires_grad=True)
+    (dh,) = torch.autograd.grad(linear_cross_entropy(h, w, target), h, up, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dh.float().sum().backward()
+
+
+def test_capture_beside_a_living_graph(gpu):
+    h, w, target = inputs(30, 100, 64, gpu)
+    target[0] = 1
+    x, y, flag = h.clone().requires_grad_(), w.clone().requires_grad_(), torch.ones(4, device=gpu)
+    eager = linear_cross_entropy(x, y, target)
+    want = torch.autograd.grad(eager, (x, y), retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        flag.zero_()
+        with pytest.raises(RuntimeError, match="still lives"):
+            linear_cross_entropy(x, y, target)
+    for a, b in zip(want, torch.autograd.grad(eager, (x, y))):
+        assert torch.equal(a, b)

@@ -143,3 +143,32 @@ def test_linear_epilogue_c_entry():
         args = list(ok)
         args[at] = value
         assert lib.kq_mx_linear_epilogue(*args) == N.KQ_ERR_INVALID and text in lib.kq_last_error(), (at, lib.kq_last_error())
+
+
+def test_loss_scale_alignment():
+    lib = N.library()
+    p = ctypes.c_void_p(256)
+    for fmt in (N.FMT_MXFP8_E4M3, N.FMT_MXFP4_E2M1):
+        args = [fmt, p, 128, 10, p, ctypes.c_void_p(258), 99, 128, p, -100, p, p, p, p, 1 << 30, None]
+        assert lib.kq_linear_cross_entropy(*args) == N.KQ_ERR_INVALID and b"scales 4" in lib.kq_last_error()
+
+
+def test_capture_beside_a_living_graph(monkeypatch):
+    """A leaf whose accumulator belongs to another stream is refused in a capture, and only there."""
+    leaf = torch.zeros(3, requires_grad=True)
+    state = {"stream": 7, "capturing": False}
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": state["stream"]}))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    held = N.hold_leaves(leaf, torch.zeros(3), leaf * 2)
+    assert len(held) == 1
+    eager = leaf * 2
+    del held
+    state["stream"] = 8
+    assert len(N.hold_leaves(leaf)) == 1
+    state["capturing"] = True
+    with pytest.raises(RuntimeError, match="still lives"):
+        N.hold_leaves(leaf)
+    with torch.no_grad():
+        assert N.hold_leaves(leaf) == []
+    del eager
+    assert len(N.hold_leaves(leaf)) == 1
