@@ -265,25 +265,35 @@ def to_gpu(tensors: Iterable[torch.Tensor | None]) -> tuple[list, torch.device, 
 _LEAF_STREAM = "kquant_amd.stream"
 
 
-def hold_leaves(*tensors: torch.Tensor) -> list:
-    """The gradient accumulators of leaves, to be held over the call that differentiates them.
+def check_capture(*leaves: torch.Tensor) -> None:
+    """Refuses a capture that would end the process.
 
-    A leaf's accumulator belongs to the stream on which its first living graph
-    was built.  A backward pass captured on another stream would pull that
-    stream into the capture, which ends the process: it is refused here.
+    A leaf's gradient accumulator belongs to the stream on which its first
+    living graph was built (``note_leaves``); a backward pass captured on
+    another stream would pull that stream into the capture.
     """
 
-    held = []
-    if torch.is_grad_enabled():
-        for t in tensors:
+    if torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled():
+        for t in leaves:
             if t.requires_grad and t.is_leaf:
                 node = torch.autograd.graph.get_gradient_edge(t).node
-                here = torch.cuda.current_stream(t.device).cuda_stream
-                if node.metadata.setdefault(_LEAF_STREAM, here) != here and torch.cuda.is_current_stream_capturing():
+                here = stream_handle(t.device)
+                if node.metadata.get(_LEAF_STREAM, here) != here:
                     raise RuntimeError("an autograd graph of these leaves that was built on another stream still lives: "
                                        "drop it (its results) before capturing their forward and backward pass")
-                held.append(node)
-    return held
+
+
+def note_leaves(result: torch.Tensor) -> None:
+    """Writes this stream into the accumulators of the leaves that ``result``
+    was computed from, directly or by one view or copy."""
+
+    if result.grad_fn is not None:
+        here = stream_handle(result.device)
+        for node, _ in result.grad_fn.next_functions:
+            if node is not None and not hasattr(node, "variable"):
+                node = next((n for n, _ in node.next_functions if n is not None), None)
+            if node is not None:
+                node.metadata.setdefault(_LEAF_STREAM, here)
 
 
 def aligned(t: torch.Tensor, align: int = 16) -> torch.Tensor:

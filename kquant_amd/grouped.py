@@ -103,8 +103,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     if host is not None:
         gpu = N.require_gpu()
         x, weight, offsets = x.to(gpu), weight.to(gpu), offsets.to(gpu)
-    held = N.hold_leaves(x, weight) if host is None else None
-    offsets = N.aligned(offsets.to(torch.int64), 8)
+    else:
+        N.check_capture(x, weight)
+    offsets = N.aligned(offsets if offsets.dtype == torch.int64 else offsets.to(torch.int64), 8)
     y = _GroupedLinear.apply(x, weight, offsets)
-    del held
+    N.note_leaves(y)
     return y if host is None else y.to(host)

@@ -122,8 +122,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     if any(t.device != hidden.device for t in tensors):
         raise ValueError("hidden, weight, target and scale must be on one device")
     host = None if hidden.is_cuda else hidden.device
-    held = N.hold_leaves(hidden, weight) if host is None else None
-    h, t = hidden.reshape(-1, k), target.reshape(-1)
+    if host is None:
+        N.check_capture(hidden, weight)
+    h, t = hidden if hidden.ndim == 2 else hidden.reshape(-1, k), target.reshape(-1)
     if host is not None:
         gpu = N.require_gpu()
         h, weight, t = h.to(gpu), weight.to(gpu), t.to(gpu)
@@ -132,7 +133,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         weight, scale = weight.view(torch.uint8), N.aligned(scale)
     weight, t = N.aligned(weight), N.aligned(t, 8)
     loss = _LinearCrossEntropy.apply(h, weight, scale, t, fmt, int(ignore_index), _REDUCTIONS[reduction])
-    del held
+    N.note_leaves(loss)
     if reduction == "none":
         loss = loss.reshape(target.shape)
     return loss if host is None else loss.to(host)

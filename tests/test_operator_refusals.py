@@ -155,20 +155,23 @@ def test_loss_scale_alignment():
 
 def test_capture_beside_a_living_graph(monkeypatch):
     """A leaf whose accumulator belongs to another stream is refused in a capture, and only there."""
-    leaf = torch.zeros(3, requires_grad=True)
+    leaf, other = torch.zeros(3, requires_grad=True), torch.zeros(2, 3, requires_grad=True)
     state = {"stream": 7, "capturing": False}
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": state["stream"]}))
+    monkeypatch.setattr(N, "stream_handle", lambda device: state["stream"])
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
-    held = N.hold_leaves(leaf, torch.zeros(3), leaf * 2)
-    assert len(held) == 1
-    eager = leaf * 2
-    del held
+    N.note_leaves(torch.zeros(3))
+    kept = leaf * 1.0, other.reshape(6) * 1.0  # a leaf, and one behind a view
+    for t in kept:
+        N.note_leaves(t)
+    N.check_capture(leaf, other)
     state["stream"] = 8
-    assert len(N.hold_leaves(leaf)) == 1
+    N.check_capture(leaf, other)
     state["capturing"] = True
-    with pytest.raises(RuntimeError, match="still lives"):
-        N.hold_leaves(leaf)
-    with torch.no_grad():
-        assert N.hold_leaves(leaf) == []
-    del eager
-    assert len(N.hold_leaves(leaf)) == 1
+    for t in (leaf, other):
+        with pytest.raises(RuntimeError, match="still lives"):
+            N.check_capture(torch.zeros(3), t)
+        with torch.no_grad():
+            N.check_capture(t)
+    N.check_capture(leaf * 2, torch.zeros(3))
+    del kept, t
+    N.check_capture(leaf, other)
