@@ -6,11 +6,18 @@
 // its weights alone; here a workgroup owns 16 R weight rows and every wave a
 // contiguous run of 128-k windows of them, so N / (16 R) workgroups of
 // independent waves keep the loads of the whole chip in flight.
-//  * lane (r, g) of a wave (r = lane % 16, g = lane / 16) loads its weight row
-//    with 16-byte loads: E4M3 windows as chunks 64 h + 16 g (h = 0, 1), E2M1
-//    windows as the one chunk 32 g.  The 16x16x32 MFMA sums over any
+//  * lane (r, g) of a wave (r = lane % 16, g = lane / 16) multiplies weight row
+//    r: of E4M3 windows the 16-byte chunks 64 h + 16 g (h = 0, 1), of E2M1
+//    windows the one chunk 32 g.  The 16x16x32 MFMA sums over any
 //    assignment of k to (lane group, element), so the activations are read
 //    with the same one and nothing is permuted.
+//  * an E4M3 window of 16 rows is 16 lines of 128 bytes.  A load of 64 of each
+//    line's bytes asks memory for them twice (5.1 TB/s with nontemporal loads, 6.3
+//    without, where 6.9 are had by whole lines), so 8 lanes load a line and the
+//    chunks are exchanged through 2 KiB of the wave's own LDS (N = 129280,
+//    K = 7168, 5 rows: 271 -> 186 us; 163 with two blocks of weight rows).
+//    Windows that are no whole lines (E2M1; K % 128 == 64) are loaded by the
+//    lanes that multiply them, through the caches.
 //  * weights are expanded to bf16 in registers (exact); activations come
 //    straight from memory (each wave has its own k, so LDS would hold
 //    nothing twice): bf16 rows, fp32 rows split exactly into three bf16 terms
@@ -60,6 +67,8 @@ __device__ __forceinline__ u32x4_t load16_nt(const void* p) {
 // flight; HALF: K % 128 == 64 (2-byte aligned scale rows, a half window at
 // the end); TAIL: what becomes of the sums.
 enum { TAIL_STORE = 0, TAIL_EPILOGUE = 1, TAIL_LOSS = 2 };
+// LDS bytes of a wave: its partial tile, and the exchange of a window's lines.
+constexpr int wave_lds(int mb, int r) { return (mb < 2 ? 2 : mb) * r * 1024; }
 template <int FMT, int AT, int OUT, int MB, int R, int P, bool HALF, int TAIL>
 __global__ __launch_bounds__(512) void mx_skinny_kernel(
     const void* __restrict__ a, const uint8_t* __restrict__ a_scale, int64_t lda, const uint8_t* __restrict__ wq,
@@ -67,6 +76,8 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
     LossTail loss) {
   static_assert(AT != A_MXFP8 || (FMT == 0 && !HALF), "MXFP8 rows take E4M3 weights and whole windows");
   using Win = Window<FMT, AT, MB, R>;
+  // (two blocks of fp32 rows leave no registers for the exchange: N = 12288, 32 rows 70 us with it, 63 without)
+  constexpr bool LINES = FMT == 0 && !HALF && !(AT == A_F32 && MB > 1);
   extern __shared__ __attribute__((aligned(16))) float skinny_red[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -81,14 +92,20 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
   const int w_begin = (int)((int64_t)wave * nwin / waves), w_end = (int)((int64_t)(wave + 1) * nwin / waves);
   const int64_t kw = FMT == 0 ? K : K / 2, ks = K / 32;
 
-  const uint8_t* wrow[R];
+  const uint8_t* wrow[R][LINES ? 2 : 1];  // this lane's row; LINES: the two rows whose lines it loads 16 bytes of
   const uint8_t* srow[R];
   const uint8_t* arow[MB];
   const uint8_t* asrow[MB];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int64_t n = min(n0 + 16 * j + r, N - 1);
-    wrow[j] = wq + n * kw + 16 * g;
+    if constexpr (LINES) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        wrow[j][q] = wq + min(n0 + 16 * j + 8 * q + (lane >> 3), N - 1) * kw + 16 * (lane & 7);
+    } else {
+      wrow[j][0] = wq + n * kw + 16 * g;
+    }
     srow[j] = ws + n * ks;
   }
 #pragma unroll
@@ -106,12 +123,15 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
     const bool cut = half && (FMT == 0 || g >= 2);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      if (FMT == 0) {
-        v.w[j][0] = load16_nt(wrow[j] + k0);
-        v.w[j][Win::WC - 1] = load16_nt(wrow[j] + k0 + (cut ? 0 : 64));
+      if constexpr (LINES) {
+        v.w[j][0] = load16_nt(wrow[j][0] + k0);
+        v.w[j][1] = load16_nt(wrow[j][1] + k0);
+      } else if (FMT == 0) {
+        v.w[j][0] = load16(wrow[j][0] + k0);
+        v.w[j][Win::WC - 1] = load16(wrow[j][0] + k0 + (cut ? 0 : 64));
         if (cut) v.w[j][Win::WC - 1] = u32x4_t{0u, 0u, 0u, 0u};
       } else {
-        v.w[j][0] = load16_nt(wrow[j] + k0 / 2 - (cut ? 32 : 0));
+        v.w[j][0] = load16(wrow[j][0] + k0 / 2 - (cut ? 32 : 0));
         if (cut) v.w[j][0] = u32x4_t{0u, 0u, 0u, 0u};
       }
       if (HALF) {
@@ -144,6 +164,26 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
     }
   };
 
+  // LINES: the lines of a window for the chunks of this lane's row, by way of LDS (rows of 128 bytes, the chunks of
+  // row x at c ^ x % 8, so that 8 rows' chunks fall on distinct banks).  One wave's accesses to LDS stay in order.
+  unsigned char* const lines = reinterpret_cast<unsigned char*>(skinny_red) + wave * wave_lds(MB, R);
+  auto exchange = [&](Win& v) {
+    if constexpr (LINES) {
+      const int to = (lane >> 3) * 128 + 16 * ((lane & 7) ^ (lane >> 3));
+      const int from = r * 128 + 16 * (g ^ (r & 7));  // and the chunk 64 bytes on, at from ^ 64
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) *reinterpret_cast<u32x4_t*>(lines + j * 2048 + q * 1024 + to) = v.w[j][q];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) v.w[j][q] = *reinterpret_cast<const u32x4_t*>(lines + j * 2048 + (from ^ 64 * q));
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+
   f32x4_t acc[MB][R];
 #pragma unroll
   for (int i = 0; i < MB; ++i)
@@ -162,13 +202,14 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
   };
   bool left = false;
 
-  auto compute = [&](const Win& v) {
+  auto compute = [&](Win v) {
     if constexpr (AT == A_MXFP8) {
       if (odd_scales(v)) {
         left = true;
         return;
       }
     }
+    exchange(v);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         bf16x8_t fa[MB][AT == A_F32 ? 3 : 1];
@@ -241,6 +282,7 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
       Win v;
       load(w, v);
       if (!odd_scales(v)) continue;
+      exchange(v);
 #pragma nounroll
       for (int blk = 0; blk < 4; ++blk) {
         const bool mine = (g >> 1) == (blk & 1);
@@ -273,12 +315,12 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
   }
 
   // D (16x16): lane holds column lane % 16, rows 4 (lane / 16) + j
-  constexpr int TILE = MB * R * 256;
+  constexpr int TILE = MB * R * 256, STRIDE = wave_lds(MB, R) / 4;
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < R; ++j)
-      *reinterpret_cast<f32x4_t*>(skinny_red + wave * TILE + (i * R + j) * 256 + lane * 4) = acc[i][j];
+      *reinterpret_cast<f32x4_t*>(skinny_red + wave * STRIDE + (i * R + j) * 256 + lane * 4) = acc[i][j];
   __syncthreads();
   for (int e = (int)threadIdx.x; e < TILE; e += (int)blockDim.x) {
     const int n = e % (16 * R), m = e / (16 * R);
@@ -286,7 +328,7 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
     if (TAIL != TAIL_LOSS && !in) continue;
     const int at = ((m >> 4) * R + (n >> 4)) * 256 + (16 * ((m & 15) >> 2) + (n & 15)) * 4 + (m & 3);
     float sum = skinny_red[at];
-    for (int w = 1; w < waves; ++w) sum += skinny_red[w * TILE + at];
+    for (int w = 1; w < waves; ++w) sum += skinny_red[w * STRIDE + at];
     if constexpr (TAIL == TAIL_LOSS) {
       // logits of 16 columns of one row in 16 lanes (whole waves run: TILE is a multiple of 64)
       if (in && loss.target[m0 + m] == n0 + n) loss.z_target[m0 + m] = sum;

@@ -30,7 +30,7 @@ template <int FMT, int AT, int OUT, int MB, int R, int P, bool HALF, class To>
 static hipError_t launch(const SkinnyArgs& s, const To& to, hipStream_t st) {
   const int nwin = (s.k + WIN - 1) / WIN;
   const int waves = nwin < 8 ? nwin : 8;
-  const size_t lds = (size_t)waves * MB * R * 1024;
+  const size_t lds = (size_t)waves * wave_lds(MB, R);
   auto kern = to.template kernel<FMT, AT, OUT, MB, R, P, HALF>(s);
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -44,7 +44,10 @@ static hipError_t launch(const SkinnyArgs& s, const To& to, hipStream_t st) {
 
 // Row blocks per workgroup.  One block of 16 weight rows (R = 1) puts the
 // most workgroups on the chip, which is what a decode row needs (N = 12288,
-// K = 7168 E4M3, one row, cold: 24 us; R = 2 / 4: 27 / 30); with 17 rows and
+// K = 7168 E4M3, one row, cold: 19.9 us; R = 2 / 4: 21.3 / 21.8).  Two share
+// the activations' reads, which pays from three workgroups a CU on (N = 24576,
+// 1 / 5 / 16 rows: 35 / 38 / 59 us with one, 32 / 34 / 46 with two; E2M1, with
+// one window in flight, 33 / 40 / 66 and 30 / 33 / 44); with 17 rows and
 // more the activations outweigh the weights unless four blocks share a read
 // of them (32 rows: 42.6 us against 52; 64 rows: 57 against 95), which pays
 // while N / 64 workgroups still cover half the CUs.  Half windows keep R = 1
@@ -54,7 +57,11 @@ static hipError_t launch(const SkinnyArgs& s, const To& to, hipStream_t st) {
 template <int FMT, int AT, int OUT, bool HALF, class To>
 static hipError_t launch_rows(const SkinnyArgs& s, const To& to, hipStream_t st) {
   const bool wide = s.n >= 64 * 128;
-  if (s.m <= 16) return launch<FMT, AT, OUT, 1, 1, 2, HALF>(s, to, st);
+  if (s.m <= 16) {
+    if constexpr (!HALF && AT != A_F32)
+      if (s.n >= 32 * 768) return launch<FMT, AT, OUT, 1, 2, FMT == 0 ? 2 : 1, false>(s, to, st);
+    return launch<FMT, AT, OUT, 1, 1, 2, HALF>(s, to, st);
+  }
   if constexpr (AT == A_F32) {
     if (wide && !HALF) return launch<FMT, AT, OUT, 2, 4, 2, false>(s, to, st);
     return launch<FMT, AT, OUT, 2, 1, 2, HALF>(s, to, st);
