@@ -28,6 +28,7 @@ struct Args {
   int groups, n, k;
 };
 
+constexpr int64_t LAST_LEVEL_CACHE = 256ll << 20;
 constexpr int TABLE = 4;  // 64 tiles of a worker each
 
 __shared__ __attribute__((aligned(16))) unsigned char lds[mm16::LDS_BYTES];
@@ -36,7 +37,8 @@ __shared__ __attribute__((aligned(16))) unsigned char lds[mm16::LDS_BYTES];
 // them reads or writes outside.
 __device__ __forceinline__ int64_t clamped(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-template <int MODE, bool F16>
+// STREAM: the weights are more than the last-level cache holds.
+template <int MODE, bool F16, bool STREAM>
 struct Problem {
   Args g;
   int mtiles, ntiles, count;
@@ -96,9 +98,15 @@ struct Problem {
     __syncthreads();
     all = __builtin_amdgcn_readfirstlane(all);
     count = mm16::worker_tiles(all);
+    // The XCDs go through the rounds that all of them take part in from an eighth of the way apart: tiles of large
+    // groups, bound by their MFMAs, run beside tiles of small ones, bound by the weights' bytes (8192 rows in 48
+    // groups, 7168 x 2048, Zipf: 388 us in one order, 362 so).
+    const int whole = all / (int)gridDim.x, from = (int)(blockIdx.x % 8) * whole / 8;
 #pragma unroll
     for (int q = 0; q < TABLE; ++q) {
-      const int tile = mm16::worker_number() + (64 * q + (t & 63)) * (int)gridDim.x;
+      int x = 64 * q + (t & 63);
+      if (MODE != DW && x < whole) x = x + from < whole ? x + from : x + from - whole;
+      const int tile = mm16::worker_number() + x * (int)gridDim.x;
       group_nt[q] = mt_of[q] = beg_of[q] = n_of[q] = 0;
       if (tile < all) {
         int lo = 0, hi = g.groups;  // first[lo] <= tile < first[hi]
@@ -166,6 +174,7 @@ struct Problem {
         r.b.rows = 0;
         r.b.width = 2u * (uint32_t)(g.k - n0);
       }
+      r.once = STREAM && n <= 128;
     }
     return r;
   }
@@ -196,13 +205,14 @@ __device__ __forceinline__ void zero_rows(const Args& g, int cols) {
   }
 }
 
-template <int MODE, bool F16>
+template <int MODE, bool F16, bool STREAM>
 __global__ __launch_bounds__(mm16::THREADS, 1) void grouped_kernel(Args g) {
-  Problem<MODE, F16> p;
+  Problem<MODE, F16, STREAM> p;
   p.g = g;
   p.setup();
   if (MODE != DW) zero_rows(g, MODE == FORWARD ? g.n : g.k);
-  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE == DW ? mm16::WHOLE : mm16::SMALL_ROWS, true, Problem<MODE, F16>> core(p, lds);
+  mm16::Core<MODE == DW, MODE != FORWARD, F16, MODE == DW ? mm16::WHOLE : mm16::SMALL_ROWS, true,
+             STREAM, Problem<MODE, F16, STREAM>> core(p, lds);
   core.run();
 }
 
@@ -218,8 +228,14 @@ static hipError_t launch(int dtype, const Args& g, hipStream_t st) {
                                        : g.rows / mm16::BM + (g.rows < g.groups ? g.rows : g.groups);
   const int64_t most = row_tiles * (((MODE == FORWARD ? g.n : g.k) + mm16::BN - 1) / mm16::BN);
   grid *= most > 0 ? (most + grid * 64 * TABLE - 1) / (grid * 64 * TABLE) : 1;
-  if (dtype == KQ_DT_F16) grouped_kernel<MODE, true><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
-  else grouped_kernel<MODE, false><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
+  const bool stream = (int64_t)g.groups * g.n * g.k * 2 > LAST_LEVEL_CACHE;
+  auto run = [&](auto streamed) {
+    constexpr bool S = MODE != DW && streamed.value;
+    if (dtype == KQ_DT_F16) grouped_kernel<MODE, true, S><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
+    else grouped_kernel<MODE, false, S><<<(unsigned)grid, mm16::THREADS, 0, st>>>(g);
+  };
+  if (stream) run(std::true_type{});
+  else run(std::false_type{});
   return hipGetLastError();
 }
 

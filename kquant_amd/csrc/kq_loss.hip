@@ -308,7 +308,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void logit_kernel(LogitArgs g) {
   LogitProblem<GRAD> p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (p.count + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, false, false, mm16::SMALL_COLS, false, LogitProblem<GRAD>> core(p, lds);
+  mm16::Core<false, false, false, mm16::SMALL_COLS, false, false, LogitProblem<GRAD>> core(p, lds);
   core.run();
 }
 
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
   DhProblem p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
   p.mtiles = (p.count + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
-  mm16::Core<true, true, false, mm16::SMALL_ROWS, true, DhProblem> core(p, lds);
+  mm16::Core<true, true, false, mm16::SMALL_ROWS, true, false, DhProblem> core(p, lds);
   core.run();
 }
 
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dw_kernel(DwArgs g) {
   DwProblem p{g, (__builtin_amdgcn_readfirstlane(*g.count) + 7) / 8 * 8, 0, 0};
   p.mtiles = (g.rows + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
-  mm16::Core<false, true, false, mm16::WHOLE, false, DwProblem> core(p, lds);
+  mm16::Core<false, true, false, mm16::WHOLE, false, false, DwProblem> core(p, lds);
   core.run();
 }
 

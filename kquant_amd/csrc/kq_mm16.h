@@ -81,6 +81,7 @@ struct Tile {
   int kc;    // contraction length (0 gives zeros)
   int rows;  // rows of the tile that are stored
   int cols;  // and columns
+  bool once = false;  // b (the leading operand) is read for this row of tiles alone, from memory
 };
 
 // The same in every lane, in scalar registers.
@@ -323,6 +324,7 @@ struct Side {
   uint32_t width;     // its valid bytes of a row (across)
   uint32_t off, at, step;  // this lane's offset in a slab, in this slab, and from load to load
   int col;            // contraction-major: this lane's first contraction index in a slab
+  bool once;          // the tile's operand is read once
 
   // what the slab at k ends with: rows and columns past it read as zero
   __device__ __forceinline__ void limit() {
@@ -337,12 +339,14 @@ struct Side {
   template <class P, class Pick>
   __device__ __forceinline__ void set(const P& p, int tiles, int lw, int lane, Pick&& pick) {
     k = 0;
+    once = false;
     kc = 0;  // loads past the last tile read zeros and touch nothing
     if (i < tiles) {
       const Tile t = p.tile(i);
       Operand o = pick(t);
       make_scalar(o);
       kc = __builtin_amdgcn_readfirstlane(t.kc);
+      once = __builtin_amdgcn_readfirstlane((int)t.once) != 0;
       r = dma::make_rsrc(o.base, 0);
       ld = o.ld;
       rows = (uint32_t)o.rows;
@@ -364,6 +368,9 @@ struct Side {
   // load u (0..7) of the slab at k into LDS slot base `slot`: 1 KiB at (4 u + lw) * 1024
   __device__ __forceinline__ void issue(int u, uint32_t slot, int lw) const {
     dma::load_to_lds16(r, at + (uint32_t)u * step, slot + (uint32_t)((4 * u + lw) * 1024));
+  }
+  __device__ __forceinline__ void issue_once(int u, uint32_t slot, int lw) const {
+    dma::load_to_lds16_nt(r, at + (uint32_t)u * step, slot + (uint32_t)((4 * u + lw) * 1024));
   }
   // loads that hold a valid row (contraction-major; the others write zeros that only rows past the tile read)
   __device__ __forceinline__ int needed() const { return ACROSS ? LOADS : (int)(rows + 31) / 32; }
@@ -391,8 +398,11 @@ enum { WHOLE = 0, SMALL_ROWS = 1, SMALL_COLS = 2 };  // which tiles may be narro
 // LEAD_B: B's loads run a step further ahead than A's, not A's than B's: for
 // the operand that comes from memory rather than from a cache.  (Narrow tiles'
 // steps are shorter than memory's latency: 64 rows in 48 groups, 4096 x 7168,
-// forward 443 us with A's ahead, 404 with B's.)
-template <bool AA, bool BA, bool F16, int NARROW, bool LEAD_B, class P>
+// forward 443 us with A's ahead, 404 with B's.)  ONCE: narrow tiles load a B that
+// is read for them alone nontemporally: 384 -> 349 us.
+// Not B that others read too or that may still be in a cache: 12 groups of
+// 1416 x 1032 again and again, 21 us a call and 29 so.
+template <bool AA, bool BA, bool F16, int NARROW, bool LEAD_B, bool ONCE, class P>
 struct Core {
   const P& p;
   uint32_t lds0;
@@ -501,7 +511,8 @@ struct Core {
           if (kk >= 2) {  // the leading operand of the step after that, into the other's slot
 #pragma unroll
             for (int u = ((kk - 2) * NM + m) * LOADS / (2 * NM); u < ((kk - 2) * NM + m + 1) * LOADS / (2 * NM); ++u)
-              lead_issue(u, fcur);
+              if (ONCE && NM != 16 && sb.once) sb.issue_once(u, fcur, lw);
+              else lead_issue(u, fcur);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
