@@ -65,19 +65,30 @@ __device__ __forceinline__ float epi_activate_any(const Epilogue& e, float x) {
                                : epi_activate<EPI_CLAMP>(e, x);
 }
 
-__device__ __forceinline__ float epi_bias(const Epilogue& e, int64_t n) {
-  if (!e.bias) return 0.0f;
-  return e.bias_f32 ? static_cast<const float*>(e.bias)[n]
-                    : bf16_bits_to_f32(static_cast<const uint16_t*>(e.bias)[n]);
+// Bits as loaded (0 where there is none) and their value, apart, so that a load can be on its way for long.
+__device__ __forceinline__ uint32_t epi_bias_bits(const Epilogue& e, int64_t n) {
+  if (!e.bias) return 0u;
+  return e.bias_f32 ? static_cast<const uint32_t*>(e.bias)[n] : static_cast<const uint16_t*>(e.bias)[n];
 }
+__device__ __forceinline__ float epi_bias_value(const Epilogue& e, uint32_t bits) {
+  return __uint_as_float(e.bias_f32 ? bits : bits << 16);
+}
+__device__ __forceinline__ float epi_bias(const Epilogue& e, int64_t n) { return epi_bias_value(e, epi_bias_bits(e, n)); }
 
 // OUT: KQ_DT_BF16 or KQ_DT_F32, the output's and so the residual's type.
 template <int OUT>
-__device__ __forceinline__ float epi_residual(const Epilogue& e, int64_t m, int64_t n) {
-  if (!e.residual) return 0.0f;
+__device__ __forceinline__ uint32_t epi_residual_bits(const Epilogue& e, int64_t m, int64_t n) {
+  if (!e.residual) return 0u;
   const int64_t at = m * e.ldr + n;
-  return OUT == KQ_DT_F32 ? static_cast<const float*>(e.residual)[at]
-                          : bf16_bits_to_f32(static_cast<const uint16_t*>(e.residual)[at]);
+  return OUT == KQ_DT_F32 ? static_cast<const uint32_t*>(e.residual)[at] : static_cast<const uint16_t*>(e.residual)[at];
+}
+template <int OUT>
+__device__ __forceinline__ float epi_residual_value(uint32_t bits) {
+  return __uint_as_float(OUT == KQ_DT_F32 ? bits : bits << 16);
+}
+template <int OUT>
+__device__ __forceinline__ float epi_residual(const Epilogue& e, int64_t m, int64_t n) {
+  return epi_residual_value<OUT>(epi_residual_bits<OUT>(e, m, n));
 }
 
 // The value at (m, n) of the matrix from its accumulated product.

@@ -559,7 +559,7 @@ static int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backward, int cus) {
   Plan p{};
   const bool mx = w_fmt != KQ_FMT_BF16;
-  // A block-scaled head at few tokens is read as it is, once (5 tokens, V = 129280, K = 7168 E4M3: 276 us; expanded
+  // A block-scaled head at few tokens is read as it is, once (5 tokens, V = 129280, K = 7168 E4M3: 172 us; expanded
   // to bf16 and multiplied in tiles 760 us).  A bf16 head's tiles stream it at the chip's rate at any count.
   p.few = mx && !backward && tokens >= 1 && tokens <= 64;
   if (p.few) {

@@ -255,10 +255,22 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
       }
   };
 
+  // What the epilogue reads for this thread's first sum is on its way during the K loop (one row, N = 12288, K = 7168
+  // with bias, SiLU and residual: 22.2 us without, 20.0 so; 18.3 without an epilogue).
+  uint32_t bias_bits = 0, residual_bits = 0;
+  auto load_tail = [&]() {
+    const int n = n0 + (int)threadIdx.x % (16 * R), m = m0 + (int)threadIdx.x / (16 * R);
+    if ((int)threadIdx.x < MB * R * 256 && m < M && n < N) {
+      bias_bits = epi_bias_bits(epi, n);
+      residual_bits = epi_residual_bits<OUT>(epi, m, n);
+    }
+  };
+
   if (w_begin < w_end) {
     Win v[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) load(min(w_begin + p, w_end - 1), v[p]);
+    if constexpr (TAIL == TAIL_EPILOGUE) load_tail();
     int w = w_begin;
     for (; w + P <= w_end; w += P) {
 #pragma unroll
@@ -346,7 +358,13 @@ __global__ __launch_bounds__(512) void mx_skinny_kernel(
         loss.part[(int64_t)(m0 + m) * loss.parts + (n0 + n) / 16] = v;
       }
     } else {
-      if (TAIL == TAIL_EPILOGUE) sum = epi_apply<OUT>(epi, sum, m0 + m, n0 + n);
+      if (TAIL == TAIL_EPILOGUE) {
+        if (e != (int)threadIdx.x || w_begin >= w_end) {
+          bias_bits = epi_bias_bits(epi, n0 + n);
+          residual_bits = epi_residual_bits<OUT>(epi, m0 + m, n0 + n);
+        }
+        sum = epi_activate_any(epi, sum + epi_bias_value(epi, bias_bits)) + epi_residual_value<OUT>(residual_bits);
+      }
       if (OUT == 2) static_cast<float*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = sum;
       else static_cast<__bf16*>(c)[(int64_t)(m0 + m) * ldc + n0 + n] = (__bf16)sum;
     }
