@@ -128,7 +128,8 @@ def mxfp8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor
     ``bias`` [N] (bf16 or fp32), ``activation`` ("relu", "silu", "gelu", its
     tanh form "gelu_tanh", or None) and ``residual`` (of the result's shape and
     type) are applied in the kernel's epilogue on the fp32 sums, which are then
-    rounded once: ``activation(source @ W.T + bias) + residual``.
+    rounded once: ``activation(source @ W.T + bias) + residual``.  The result
+    carries no gradient.
     """
     if weight.dtype not in (torch.float8_e4m3fn, torch.uint8):
         raise TypeError(f"MXFP8 weight must be float8_e4m3fn, got {weight.dtype}")
