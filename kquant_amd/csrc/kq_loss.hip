@@ -459,7 +459,9 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dw_kernel(DwArgs g) {
 
 // lse and loss of every token from its partial maxima and sums (nparts rows of
 // `tokens`), 16 tokens a workgroup; 0 for the ignored ones, NaN where the
-// target is outside the vocabulary.
+// target is outside the vocabulary.  Few workgroups of long columns: what bounds
+// it is latency, so eight loads are out at a time and the columns meet in a tree
+// (777 tokens, 2020 parts: 24 us one after the other, 14 so).
 __global__ __launch_bounds__(1024) void combine_kernel(const float2_t* __restrict__ part, int nparts, int tokens,
                                                        const int* __restrict__ place, const int* __restrict__ target_c,
                                                        const float* __restrict__ z_target, float* __restrict__ losses,
@@ -469,15 +471,28 @@ __global__ __launch_bounds__(1024) void combine_kernel(const float2_t* __restric
   const int at = t < tokens ? place[t] : -1;
   float m = -__builtin_inff(), s = 0.0f;
   if (at >= 0)
-    for (int p = y; p < nparts; p += 64) {
-      const float2_t v = part[(int64_t)p * tokens + at];
-      join(m, s, v[0], v[1]);
+    for (int p = y; p < nparts; p += 64 * 8) {
+      float2_t v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {  // past the end: the last one again, not joined
+        const int row = p + 64 * q < nparts ? p + 64 * q : nparts - 1;
+        v[q] = part[(int64_t)row * tokens + at];
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (p + 64 * q < nparts) join(m, s, v[q][0], v[q][1]);
     }
   ms[y][x] = m;
   ss[y][x] = s;
-  __syncthreads();
+  for (int w = 32; w > 0; w >>= 1) {
+    __syncthreads();
+    if (y < w) {
+      join(m, s, ms[y + w][x], ss[y + w][x]);
+      ms[y][x] = m;
+      ss[y][x] = s;
+    }
+  }
   if (y != 0 || t >= tokens) return;
-  for (int q = 1; q < 64; ++q) join(m, s, ms[q][x], ss[q][x]);
   const float l = m + LN2 * __builtin_amdgcn_logf(s);
   lse[t] = at < 0 ? 0.0f : l;
   losses[t] = at < 0 ? 0.0f : target_c[at] < 0 ? __builtin_nanf("") : l - z_target[at];
