@@ -43,10 +43,29 @@ constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
 
 __shared__ __attribute__((aligned(16))) unsigned char lds[mm16::LDS_BYTES];
 
-// Counted tokens in order: rows[i] the i-th one's row, place[t] its i or -1.
+// dh's contraction over the vocabulary runs in slices until its tiles fill the workers; a slice's plane is written
+// and read once (5 TB/s), a 64-row step of a tile takes 1.3 us.
+constexpr int MAX_SLICES = 16;
+__host__ __device__ inline bool slices_allowed(int64_t s, int64_t steps) { return s == 1 || s * 4 <= steps; }
+__host__ __device__ inline float slices_us(int64_t s, int64_t counted, int64_t k, int64_t steps, int workers, bool planes) {
+  const int64_t tiles = ((counted + 255) / 256) * ((k + 255) / 256);
+  return (float)((tiles * s + workers - 1) / workers) * (float)((steps + s - 1) / s) * 1.3f +
+         (s > 1 || planes ? 5.0f + (float)(s * counted * k * 8) / 5e6f : 0.0f);
+}
+
+// What the device chooses the slices from: the planes there is room for (0: dh is stored at once), a piece's
+// steps of 64 vocabulary rows, K, and the workers.
+struct Slicing {
+  int64_t room;  // rows of planes
+  int steps, k, workers;
+};
+
+// Counted tokens in order: rows[i] the i-th one's row, place[t] its i or -1.  count[0]: their number, count[1]:
+// dh's slices for it (2048 tokens of which 1434 count, V = 50257, K = 2048: dh 292 us with the slices of all
+// tokens, 245 so).
 __global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict__ target, int64_t ignore_index,
                                                        int tokens, int* __restrict__ rows, int* __restrict__ place,
-                                                       int* __restrict__ count) {
+                                                       int* __restrict__ count, Slicing dh) {
   __shared__ int wave_sum[16];
   constexpr int PER = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -81,7 +100,19 @@ __global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict
     base += all;
     __syncthreads();
   }
-  if (tid == 0) *count = base;
+  if (tid < 64) {  // lane s - 1: s slices
+    const int s = tid + 1;
+    float us = __builtin_inff();
+    if (dh.workers > 0 && s <= MAX_SLICES && (int64_t)s * base <= dh.room && slices_allowed(s, dh.steps))
+      us = slices_us(s, base, dh.k, dh.steps, dh.workers, true);
+    float least = us;
+    for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
+    const uint64_t best = __ballot(us == least && us < __builtin_inff());
+    if (tid == 0) {
+      count[0] = base;
+      count[1] = best ? __builtin_ctzll(best) + 1 : 1;
+    }
+  }
 }
 
 // alpha of the upstream gradients (see above); 1 where they are all zero.
@@ -314,14 +345,14 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void logit_kernel(LogitArgs g) {
 
 // dh: d (its transpose, read across) x the piece's rows (read across), the
 // vocabulary cut into slices.  One slice of one piece stores dh itself, at the
-// tokens' own rows; else slices add up in fp32 planes [slice][token][k].
+// tokens' own rows; else slices add up in fp32 planes [slice][counted token][k].
 struct DhArgs {
   const char* dt;
   int ldg;
   const char* w;
   const int* count;
   const int* rows_of;
-  int rows, k, slices, tokens;
+  int rows, k;
   const float* alpha;
   char* dh;  // or null
   int64_t lddh;  // bytes
@@ -331,17 +362,17 @@ struct DhArgs {
 
 struct DhProblem {
   DhArgs g;
-  int count, mtiles, ntiles;
+  int count, slices, mtiles, ntiles;
 
-  __device__ __forceinline__ int tiles() const { return mm16::worker_tiles(mtiles * ntiles * g.slices); }
+  __device__ __forceinline__ int tiles() const { return mm16::worker_tiles(mtiles * ntiles * slices); }
   __device__ __forceinline__ Tile tile(int x) const {
     const int t = tile_number(x);
     int mt, nt;
     const int per = mtiles * ntiles, sl = t / per;
     mm16::tile_mn(t - sl * per, mtiles, ntiles, mt, nt);
     const int m0 = mt * mm16::BM, n0 = nt * mm16::BN, steps = (g.rows + mm16::BK - 1) / mm16::BK;
-    const int v0 = sl * steps / g.slices * mm16::BK;  // slices <= 16, steps <= 2^18
-    const int v1 = min((sl + 1) * steps / g.slices * mm16::BK, g.rows);
+    const int v0 = sl * steps / slices * mm16::BK;  // slices <= 16, steps <= 2^18
+    const int v1 = min((sl + 1) * steps / slices * mm16::BK, g.rows);
     Tile r;
     r.cols = mm16::BN;
     r.kc = v1 - v0;
@@ -365,7 +396,7 @@ struct DhProblem {
       mm16::store16<NB, WN, false>([&](int r) { return out + map[r] * g.lddh; }, tl.rows, g.k - n0, wm, wn, acc, lane,
                                    [&](int, int, int, float v) { return alpha * v; });
     } else {
-      float* out = g.planes + ((int64_t)sl * g.tokens + m0) * g.k + n0;
+      float* out = g.planes + ((int64_t)sl * count + m0) * g.k + n0;
       const uint32_t ld = (uint32_t)g.k;
       if (g.add)
         mm16::each(tl.rows, g.k - n0, wm, wn, acc, lane,
@@ -379,7 +410,7 @@ struct DhProblem {
 };
 
 __global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
-  DhProblem p{g, __builtin_amdgcn_readfirstlane(*g.count), 0, 0};
+  DhProblem p{g, __builtin_amdgcn_readfirstlane(g.count[0]), __builtin_amdgcn_readfirstlane(g.count[1]), 0, 0};
   p.mtiles = (p.count + mm16::BM - 1) / mm16::BM;
   p.ntiles = (g.k + mm16::BN - 1) / mm16::BN;
   mm16::Core<true, true, false, mm16::SMALL_ROWS, true, false, DhProblem> core(p, lds);
@@ -387,17 +418,18 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dh_kernel(DhArgs g) {
 }
 
 // dh at the tokens' own rows = the sum of the planes, in slice order.
-__global__ __launch_bounds__(256) void dh_sum_kernel(const float* __restrict__ planes, int slices, int tokens, int k,
+__global__ __launch_bounds__(256) void dh_sum_kernel(const float* __restrict__ planes, const int* __restrict__ count, int k,
                                                      const int* __restrict__ place,
                                                      const float* __restrict__ alpha_at, char* __restrict__ dh,
                                                      int64_t lddh) {
   const int t = blockIdx.x, at = place[t];
   if (at < 0) return;
   const float alpha = *alpha_at;
+  const int counted = count[0], slices = count[1];
   for (int c = (int)threadIdx.x * 4; c < k; c += 1024) {
     const float* p = planes + (int64_t)at * k + c;
     float4_t v = *reinterpret_cast<const float4_t*>(p);
-    for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const float4_t*>(p + (int64_t)s * tokens * k);
+    for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const float4_t*>(p + (int64_t)s * counted * k);
     uint32_t* o = reinterpret_cast<uint32_t*>(dh + t * lddh + 2 * (int64_t)c);
     o[0] = f32x2_to_bf16x2_bits(alpha * v[0], alpha * v[1]);
     o[1] = f32x2_to_bf16x2_bits(alpha * v[2], alpha * v[3]);
@@ -592,15 +624,13 @@ static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backw
   p.pieces = most >= vocab ? 1 : (vocab + most - 1) / most;
   p.piece = p.pieces == 1 ? vocab : up((vocab + p.pieces - 1) / p.pieces, 256);
   p.pieces = (vocab + p.piece - 1) / p.piece;
-  // dh: slices of the vocabulary until its tiles fill the CUs; a slice's plane is written and read once (5 TB/s),
-  // a 64-row step of a tile takes 1.3 us
+  // dh: the planes that all tokens would take; fewer counted ones may be cut finer in the same room
   p.slices = 1;
   if (backward) {
-    const int64_t tiles = ((tokens + 255) / 256) * ((k + 255) / 256), steps = (p.piece + 63) / 64;
-    double best = 1e30;
-    for (int64_t s = 1; s <= 16 && (s == 1 || s * 4 <= steps); ++s) {
-      const double t = (double)((tiles * s + cus - 1) / cus) * (double)((steps + s - 1) / s) * 1.3 +
-                       (s > 1 || p.pieces > 1 ? 5.0 + (double)(s * tokens * k * 8) / 5e6 : 0.0);
+    const int64_t steps = (p.piece + 63) / 64;
+    float best = 1e30f;
+    for (int64_t s = 1; s <= MAX_SLICES && slices_allowed(s, steps); ++s) {
+      const float t = slices_us(s, tokens, k, steps, cus, p.pieces > 1);
       if (t < best) {
         best = t;
         p.slices = (int)s;
@@ -615,7 +645,7 @@ static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backw
   };
   p.o_rows = take(tokens * 4);
   p.o_place = take(tokens * 4);
-  p.o_count = take(4);
+  p.o_count = take(8);
   p.o_target = take(tokens * 4);
   p.o_hc = take(up(tokens, 8) * k * 2);
   if (mx) p.o_w = take(p.piece * k * 2);
@@ -715,7 +745,7 @@ extern "C" int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, in
   }
   int* count = (int*)(ws + p.o_count);
   loss::compact_kernel<<<1, 1024, 0, st>>>(target, ignore_index, (int)tokens, (int*)(ws + p.o_rows),
-                                           (int*)(ws + p.o_place), count);
+                                           (int*)(ws + p.o_place), count, loss::Slicing{});
   if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   if (tokens > 0) {
     loss::Gather g{};
@@ -773,8 +803,10 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
     return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes, 256-byte aligned", fn, (long long)p.bytes);
   char* ws = (char*)workspace;
   int* count = (int*)(ws + p.o_count);
-  loss::compact_kernel<<<1, 1024, 0, st>>>(target, ignore_index, (int)tokens, (int*)(ws + p.o_rows),
-                                           (int*)(ws + p.o_place), count);
+  const bool planes = p.slices > 1 || p.pieces > 1;
+  loss::compact_kernel<<<1, 1024, 0, st>>>(
+      target, ignore_index, (int)tokens, (int*)(ws + p.o_rows), (int*)(ws + p.o_place), count,
+      loss::Slicing{planes ? p.slices * tokens : 0, (int)((p.piece + 63) / 64), (int)k, (int)loss::persistent_grid(cus)});
   if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   if (tokens == 0 && !dw) return KQ_OK;
   loss::Gather g{};
@@ -812,7 +844,6 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
   a.u_c = g.u_c;
   a.dt = ws + p.o_dt;
   a.ldg = (int)p.ldg;
-  const bool planes = p.slices > 1 || p.pieces > 1;
   for (int64_t first = 0; first < vocab; first += p.piece) {
     a.first = (int)first;
     a.rows = (int)(vocab - first < p.piece ? vocab - first : p.piece);
@@ -820,7 +851,7 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
     loss::logit_kernel<true><<<grid, mm16::THREADS, 0, st>>>(a);
     if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
     if (dh) {
-      const loss::DhArgs d{a.dt, (int)p.ldg, a.w, count, (int*)(ws + p.o_rows), a.rows, (int)k, p.slices, (int)tokens,
+      const loss::DhArgs d{a.dt, (int)p.ldg, a.w, count, (int*)(ws + p.o_rows), a.rows, (int)k,
                            alpha, planes ? nullptr : (char*)dh, 2 * lddh, (float*)(ws + p.o_planes), first > 0};
       loss::dh_kernel<<<grid, mm16::THREADS, 0, st>>>(d);
       if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
@@ -832,7 +863,7 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
     }
   }
   if (dh && planes && tokens > 0) {
-    loss::dh_sum_kernel<<<(unsigned)tokens, 256, 0, st>>>((const float*)(ws + p.o_planes), p.slices, (int)tokens, (int)k,
+    loss::dh_sum_kernel<<<(unsigned)tokens, 256, 0, st>>>((const float*)(ws + p.o_planes), count, (int)k,
                                                          g.place, alpha, (char*)dh, 2 * lddh);
     if (int rc = kq_check_launch(hipGetLastError(), fn)) return rc;
   }

@@ -419,3 +419,23 @@ def test_capture_beside_a_living_graph(gpu):
             linear_cross_entropy(x, y, target)
     for a, b in zip(want, torch.autograd.grad(eager, (x, y))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("ignored", [0.0, 0.5, 0.9, 0.999])
+def test_slices_follow_the_counted_tokens(gpu, ignored):
+    """The hidden gradient's contraction, cut into the more slices the fewer tokens count; one captured graph for all."""
+    h, w, target = inputs(1500, 6000, 136, gpu, ignored=ignored)
+    target[700] = 5999
+    want = check(h, w, target)
+    sh, sw, st = h.clone().requires_grad_(), w.clone().requires_grad_(), torch.randint(0, 6000, (1500,), device=gpu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = linear_cross_entropy(sh, sw, st)
+        grads = torch.autograd.grad(loss, (sh, sw))
+    st.copy_(target)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((loss.detach(), *grads), want):
+            assert torch.equal(a, b)
