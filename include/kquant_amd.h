@@ -326,7 +326,7 @@ int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x,
  *   lse[t] = log sum_v exp z[t][v],  losses[t] = lse[t] - z[t][target[t]],
  * both fp32 [tokens] and 0 where target[t] == ignore_index; a target outside
  * [0, vocab) gives a NaN loss.  sums: fp32 [2], the losses' sum and their mean
- * over the counted tokens (NaN if none).
+ * over the counted tokens (NaN if none), or NULL.
  * h bf16 [tokens, k] (row stride ldh elements, ldh % 8 == 0).  w_fmt: the head
  * as KQ_FMT_BF16 [vocab, k] (k % 8 == 0, w_scale NULL), or MXFP8 / MXFP4 rows
  * with E8M0 scales [vocab, k/32] (k % 64 == 0).  target: device int64.  h, w

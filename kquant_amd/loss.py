@@ -35,7 +35,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             hidden = _rows(hidden)
             losses = torch.empty(tokens, dtype=torch.float32, device=hidden.device)
             lse = torch.empty_like(losses)
-            sums = torch.empty(2, dtype=torch.float32, device=hidden.device)
+            sums = None if reduction == N.LOSS_NONE else torch.empty(2, dtype=torch.float32, device=hidden.device)
             ws = _workspace(fmt, tokens, vocab, k, 0, hidden.device)
             N.call("kq_linear_cross_entropy", fmt, N.ptr(hidden), hidden.stride(0), tokens, N.ptr(weight), N.ptr(scale),
                    vocab, k, N.ptr(target), ignore_index, N.ptr(losses), N.ptr(lse), N.ptr(sums), N.ptr(ws), ws.numel(),
