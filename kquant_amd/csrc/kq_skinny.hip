@@ -49,10 +49,12 @@ static hipError_t launch(const SkinnyArgs& s, const To& to, hipStream_t st) {
 // 1 / 5 / 16 rows: 35 / 38 / 59 us with one, 32 / 34 / 46 with two; E2M1, with
 // one window in flight, 33 / 40 / 66 and 30 / 33 / 44); with 17 rows and
 // more the activations outweigh the weights unless four blocks share a read
-// of them (32 rows: 42.6 us against 52; 64 rows: 57 against 95), which pays
-// while N / 64 workgroups still cover half the CUs.  Half windows keep R = 1
-// past 16 rows: fp32 rows, N = 12288, K = 2112, 17 / 32 rows 44 / 58 us with E4M3 weights
-// (171 / 172 in whole tiles), 53 at 17 with E2M1 (16 registers spill; 160), and
+// of them (N = 12288, E4M3, 32 rows: 33.7 us against 49.5), which pays
+// while N / 64 workgroups still cover half the CUs; four row blocks beside them
+// leave E4M3's windows registers for one in flight (the head loss at N = 129280, 33 /
+// 64 rows: 341 / 411 us with one, 625 / 664 with two).  Half windows keep R = 1
+// past 16 rows: fp32 rows, N = 12288, K = 2112, 17 / 32 rows 38 / 52 us with E4M3 weights
+// (171 / 172 in whole tiles), 49 at 17 with E2M1 (16 registers spill; 160), and
 // the tiles' split, 46, at 32.
 template <int FMT, int AT, int OUT, bool HALF, class To>
 static hipError_t launch_rows(const SkinnyArgs& s, const To& to, hipStream_t st) {
@@ -71,7 +73,7 @@ static hipError_t launch_rows(const SkinnyArgs& s, const To& to, hipStream_t st)
       return launch<FMT, AT, OUT, 2, 1, 2, HALF>(s, to, st);
     }
     if constexpr (AT == A_BF16)  // (expanding MXFP8 rows too takes more registers than there are)
-      if (wide && !HALF) return launch<FMT, AT, OUT, 4, 4, 2, false>(s, to, st);
+      if (wide && !HALF) return launch<FMT, AT, OUT, 4, 4, FMT == 0 ? 1 : 2, false>(s, to, st);
     return launch<FMT, AT, OUT, 4, 1, 2, HALF>(s, to, st);
   }
 }

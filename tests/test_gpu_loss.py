@@ -439,3 +439,15 @@ def test_slices_follow_the_counted_tokens(gpu, ignored):
         torch.cuda.synchronize()
         for a, b in zip((loss.detach(), *grads), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("tokens,vocab,k", [(5, 24601, 256), (16, 24601, 1152), (20, 8209, 256), (33, 8209, 384), (64, 8209, 256),
+                                            (64, 8209, 192)])
+def test_wide_block_scaled_heads_few_tokens(gpu, fmt, tokens, vocab, k):
+    """Each cut of the one-pass kernel that wide heads take, with odd vocabularies."""
+    h, w, target = inputs(tokens, vocab, k, gpu, ignored=0.2)
+    target[0] = vocab - 1
+    q, s = (mxfp8.mxfp8_quantize if fmt == "mxfp8" else mxfp4.mxfp4_quantize)(w)
+    values = (mxfp8.mxfp8_dequantize if fmt == "mxfp8" else mxfp4_io.dequant)(q, s).double()
+    check(h, q, target, values, s, reduction="none")
