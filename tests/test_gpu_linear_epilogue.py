@@ -193,3 +193,14 @@ def test_any_alignment_of_results_and_residuals(gpu, m, n, k, shift, pad):
         body = out[c0:c0 + m * ldc].view(m, ldc)
         assert torch.equal(body[:, :n], want)
         assert (body[:, n:] == 7).all() and (out[:c0] == 7).all() and (out[c0 + m * ldc:] == 7).all()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("m,n,k", [(1, 24601, 128), (16, 24601, 256), (17, 8209, 256), (32, 8209, 128), (40, 8209, 256),
+                                   (64, 8209, 192)])
+def test_wide_outputs_of_few_rows(gpu, fmt, dtype, m, n, k):
+    """Several blocks of weight rows a workgroup, so that a thread has more than one sum."""
+    x, w, bias, residual = inputs(m, n, k, dtype, gpu)
+    q, s, values, f = quantized(w, fmt)
+    check(f(x, q, s, bias=bias, activation="silu", residual=residual), x, values, bias, "silu", residual, dtype)
