@@ -28,7 +28,7 @@
 // exponentials, their sums and dh's planes; d is rounded to bf16 to be an
 // operand (half a step, 2^-8 relative, of each term of sums that are themselves
 // rounded to bf16).  Heads in MXFP8 / MXFP4 are expanded piece by piece to bf16,
-// which holds their values exactly.
+// which holds their values exactly (but for those below bf16's subnormals, 2^-133).
 #include "kq_internal.h"
 #include "kq_mm16.h"
 
