@@ -44,7 +44,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.args = fmt, ignore_index, reduction
         if reduction == N.LOSS_NONE:
             return losses
-        return sums[1] if reduction == N.LOSS_MEAN else sums[0]
+        # a tensor of its own over sums' memory: a view made in here could not be changed in place (loss /= steps)
+        at = 1 if reduction == N.LOSS_MEAN else 0
+        return sums.new_empty(0).set_(sums.untyped_storage(), at, (), ())
 
     @staticmethod
     @once_differentiable

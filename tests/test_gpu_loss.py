@@ -451,3 +451,18 @@ def test_wide_block_scaled_heads_few_tokens(gpu, fmt, tokens, vocab, k):
     q, s = (mxfp8.mxfp8_quantize if fmt == "mxfp8" else mxfp4.mxfp4_quantize)(w)
     values = (mxfp8.mxfp8_dequantize if fmt == "mxfp8" else mxfp4_io.dequant)(q, s).double()
     check(h, q, target, values, s, reduction="none")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_changed_in_place(gpu, reduction):
+    """loss /= steps and loss += another one, as with F.cross_entropy's result."""
+    h, w, target = inputs(80, 300, 64, gpu)
+    x, y = h.clone().requires_grad_(), w.clone().requires_grad_()
+    want = linear_cross_entropy(x, y, target, reduction=reduction)
+    grads = torch.autograd.grad(want, (x, y), torch.full_like(want, 0.25))
+    loss = linear_cross_entropy(x, y, target, reduction=reduction)
+    loss /= 4
+    assert torch.equal(loss.detach(), want.detach() / 4)
+    loss += 1.0
+    for a, b in zip(torch.autograd.grad(loss.sum(), (x, y)), grads):
+        assert torch.equal(a, b)

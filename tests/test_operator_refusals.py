@@ -3,12 +3,14 @@ epilogues refuse, before anything reaches a GPU."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import pytest
 import torch
 
 from kquant_amd import _native as N
+from kquant_amd import loss as loss_module
 from kquant_amd.grouped import grouped_linear
 from kquant_amd.linear import mxfp4_linear, mxfp8_linear
 from kquant_amd.loss import linear_cross_entropy
@@ -175,3 +177,30 @@ def test_capture_beside_a_living_graph(monkeypatch):
     N.check_capture(leaf * 2, torch.zeros(3))
     del kept, t
     N.check_capture(leaf, other)
+
+
+@pytest.mark.parametrize("reduction,value", [(N.LOSS_MEAN, 5.0), (N.LOSS_SUM, 3.0)])
+def test_reduced_loss_is_no_view(monkeypatch, reduction, value):
+    """The scalar may be changed in place (loss /= steps), as a loss accumulated over batches is; the kernels are stood in for."""
+    sums = torch.tensor([3.0, 5.0])
+
+    def call(name, *args):
+        if name == "kq_linear_cross_entropy":
+            ctypes.memmove(args[12], sums.data_ptr(), 8)
+        else:
+            up, dh = ctypes.cast(args[11], ctypes.POINTER(ctypes.c_float)), args[13]
+            seen.append(up[0])
+            ctypes.memset(dh, 0, 4 * 64 * 2)
+
+    seen = []
+    monkeypatch.setattr(N, "call", call)
+    monkeypatch.setattr(N, "stream", lambda device: None)
+    monkeypatch.setattr(N, "on_device", lambda device: contextlib.nullcontext())
+    h = bf16(4, 64).requires_grad_()
+    loss = loss_module._LinearCrossEntropy.apply(h, bf16(9, 64), None, torch.zeros(4, dtype=torch.int64), N.FMT_BF16, -100,
+                                                 reduction)
+    assert loss.shape == () and loss.item() == value and not loss._is_view()
+    loss /= 4
+    loss += 1
+    loss.backward()
+    assert loss.item() == value / 4 + 1 and seen == [0.25] and h.grad.shape == (4, 64)
