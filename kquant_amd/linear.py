@@ -29,7 +29,7 @@ import torch
 from . import _native as N
 
 
-def _check_epilogue(bias, activation, residual, lead, n: int, f32: bool, out_dtype: torch.dtype) -> None:
+def _check_epilogue(source, bias, activation, residual, lead, n: int, f32: bool, out_dtype: torch.dtype) -> None:
     if activation not in N.LIN_ACTIVATIONS:
         raise ValueError(f"activation must be None, relu, silu, gelu or gelu_tanh, got {activation!r}")
     if f32 and out_dtype != torch.float32:
@@ -44,6 +44,9 @@ def _check_epilogue(bias, activation, residual, lead, n: int, f32: bool, out_dty
             raise TypeError(f"residual must have the result's type {out_dtype}, got {residual.dtype}")
         if tuple(residual.shape) != (*lead, n):
             raise ValueError(f"residual shape {tuple(residual.shape)} != {(*lead, n)}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (source, bias, residual)):
+        raise RuntimeError("a linear with bias, activation or residual carries no gradient: detach its inputs or call it "
+                           "under torch.no_grad()")
 
 
 def _linear(fmt: int, source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
@@ -73,7 +76,7 @@ def _linear(fmt: int, source: torch.Tensor, weight: torch.Tensor, scale: torch.T
         a = a.to(torch.bfloat16)
     epilogue = bias is not None or activation is not None or residual is not None
     if epilogue:
-        _check_epilogue(bias, activation, residual, lead, n, exact_f32, out_dtype)
+        _check_epilogue(source, bias, activation, residual, lead, n, exact_f32, out_dtype)
         residual = None if residual is None else residual.reshape(-1, n)
     (a, w, s, bias, residual), gpu, host = N.to_gpu([a, weight.view(torch.uint8), scale, bias, residual])
     a, w, s = N.aligned(a), N.aligned(w), N.aligned(s)
@@ -129,7 +132,9 @@ def mxfp8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor
     tanh form "gelu_tanh", or None) and ``residual`` (of the result's shape and
     type) are applied in the kernel's epilogue on the fp32 sums, which are then
     rounded once: ``activation(source @ W.T + bias) + residual``.  The result
-    carries no gradient.
+    carries no gradient: with any of the three, a source, bias or residual that
+    requires one is refused while autograd records (a skip connection inside
+    the call would leave the graph unseen).
     """
     if weight.dtype not in (torch.float8_e4m3fn, torch.uint8):
         raise TypeError(f"MXFP8 weight must be float8_e4m3fn, got {weight.dtype}")

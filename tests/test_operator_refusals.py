@@ -204,3 +204,28 @@ def test_reduced_loss_is_no_view(monkeypatch, reduction, value):
     loss += 1
     loss.backward()
     assert loss.item() == value / 4 + 1 and seen == [0.25] and h.grad.shape == (4, 64)
+
+
+@pytest.mark.parametrize("which", ["source", "bias", "residual", "skip"])
+def test_linear_epilogue_drops_no_gradient(monkeypatch, which):
+    """Inputs that require a gradient are refused while autograd records, and only then."""
+    reached = RuntimeError("reached the GPU")
+
+    def to_gpu(tensors):
+        raise reached
+
+    monkeypatch.setattr(N, "to_gpu", to_gpu)
+    source, bias, residual = bf16(4, 64), torch.zeros(64), bf16(4, 64)
+    if which == "skip":
+        residual = source
+    {"source": source, "bias": bias, "residual": residual, "skip": source}[which].requires_grad_()
+    for f, q in ((mxfp8_linear, torch.zeros(64, 64, dtype=torch.uint8)), (mxfp4_linear, torch.zeros(64, 32, dtype=torch.uint8))):
+        scale = torch.zeros(64, 2, dtype=torch.uint8)
+        with pytest.raises(RuntimeError, match="carries no gradient"):
+            f(source, q, scale, bias=bias, activation="silu", residual=residual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="reached the GPU"):
+            f(source, q, scale, bias=bias, activation="silu", residual=residual)
+        with pytest.raises(RuntimeError, match="reached the GPU"):
+            f(source.detach(), q, scale, bias=bias.detach(), residual=residual.detach())
+        with pytest.raises(RuntimeError, match="reached the GPU"):
+            f(source, q, scale)  # the linear without an epilogue takes any source, as it always has
