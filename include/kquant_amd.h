@@ -330,10 +330,12 @@ int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x,
  * h bf16 [tokens, k] (row stride ldh elements, ldh % 8 == 0).  w_fmt: the head
  * as KQ_FMT_BF16 [vocab, k] (k % 8 == 0, w_scale NULL), or MXFP8 / MXFP4 rows
  * with E8M0 scales [vocab, k/32] (k % 64 == 0).  target: device int64.  h, w
- * and the gradients are 16-byte aligned, target 8, w_scale 4.  tokens <= 2^20, vocab <= 2^24, k <= 2^16.  workspace: 256-byte aligned,
- * uninitialised; it holds the counted rows and 32 bytes per token and 256
- * vocabulary rows, of an MX head an expanded piece (the size functions plan
- * for the current device).  Deterministic. */
+ * and the gradients are 16-byte aligned, target 8, w_scale 4.  tokens <= 2^20, vocab <= 2^24, k <= 2^16.
+ * workspace: 256-byte aligned, uninitialised (the size function plans for the
+ * current device).  Forward it holds the counted rows, 32 bytes per token and
+ * 256 vocabulary rows, and of an MX head a piece of it in bf16 (at most 1 GiB);
+ * up to 64 tokens of an MX head take 128 bytes per token and 256 vocabulary
+ * rows instead, and nothing else of that size.  Deterministic. */
 int64_t kq_linear_cross_entropy_workspace_size(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, int backward);
 int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
                             const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target,
@@ -348,7 +350,10 @@ int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, int64_t token
  * kq_linear_cross_entropy's.  d is formed in fp32 piece by piece of the
  * vocabulary (at most 1 GiB of it at once) and rounded to bf16 as an operand.
  * Ignored tokens' rows of h reach nothing; their dh is zero.  Deterministic.
- * workspace: kq_linear_cross_entropy_workspace_size(..., backward = 1). */
+ * workspace: kq_linear_cross_entropy_workspace_size(..., backward = 1): the
+ * counted rows, a piece of d and of an MX head (at most 1 GiB each), and, where
+ * there are several pieces or dh's sums are cut into slices, up to 16 fp32
+ * planes [tokens, k] of dh (also where only dw is asked for). */
 int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_t ldh, int64_t tokens, const void* w,
                                      const uint8_t* w_scale, int64_t vocab, int64_t k, const int64_t* target,
                                      int64_t ignore_index, const float* lse, const float* grad, int reduction,

@@ -622,7 +622,7 @@ static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backw
   int64_t most = vocab;
   if (mx) most = PIECE_BYTES / (2 * k);
   if (backward && PIECE_BYTES / (2 * p.ldg) < most) most = PIECE_BYTES / (2 * p.ldg);
-  if (most < 1024) most = 1024;
+  if (most < 256) most = 256;  // (2^20 tokens leave 512, K = 2^16 8192)
   most = most / 256 * 256;
   p.pieces = most >= vocab ? 1 : (vocab + most - 1) / most;
   p.piece = p.pieces == 1 ? vocab : up((vocab + p.pieces - 1) / p.pieces, 256);

@@ -466,3 +466,18 @@ def test_changed_in_place(gpu, reduction):
     loss += 1.0
     for a, b in zip(torch.autograd.grad(loss.sum(), (x, y)), grads):
         assert torch.equal(a, b)
+
+
+def test_pieces_of_many_tokens(gpu):
+    """More tokens than a piece of 1024 vocabulary rows has room for: pieces of 768 rows."""
+    tokens, vocab, k = (1 << 19) + 9, 1300, 64
+    h, w, target = inputs(tokens, vocab, k, gpu, ignored=0.1)
+    target[-3:] = torch.tensor([767, 768, vocab - 1], device=gpu)
+    x, y = h.clone().requires_grad_(), w.clone().requires_grad_()
+    dh, dw = torch.autograd.grad(linear_cross_entropy(x, y, target, reduction="sum"), (x, y))
+    some = torch.cat([torch.arange(0, tokens, 5003, device=gpu), torch.arange(tokens - 9, tokens, device=gpu)])
+    losses, tol, d, dtol = formula(h[some], w, target[some])
+    near(linear_cross_entropy(h, w, target, reduction="none")[some], losses, tol)
+    check_sum(dh[some], d, dtol, w)
+    _, _, d, dtol = formula(h, w, target)
+    check_sum(dw, d.T, dtol.T, torch.where((target != -100)[:, None], h, torch.zeros_like(h)))

@@ -229,3 +229,12 @@ def test_linear_epilogue_drops_no_gradient(monkeypatch, which):
             f(source.detach(), q, scale, bias=bias.detach(), residual=residual.detach())
         with pytest.raises(RuntimeError, match="reached the GPU"):
             f(source, q, scale)  # the linear without an epilogue takes any source, as it always has
+
+
+@pytest.mark.parametrize("tokens", [1 << 19, (1 << 19) + 8, 600_001, 1 << 20])
+def test_loss_workspace_of_many_tokens(tokens):
+    """At most 1 GiB of softmax gradients at once up to the most tokens; K = 8, so that little else counts: the rows
+    (16 bytes), dh's planes (32 each, two at most of so few steps), 24 bytes a token."""
+    size = N.library().kq_linear_cross_entropy_workspace_size
+    for vocab in (131072, 1 << 24):
+        assert size(N.FMT_BF16, tokens, vocab, 8, 1) <= (1 << 30) + tokens * (16 + 64 + 24) + 4096
