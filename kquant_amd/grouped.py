@@ -20,12 +20,15 @@ from torch.autograd.function import once_differentiable
 from . import _native as N
 
 MAX_GROUPS = 4096
+MAX_STRIDE = 1 << 22  # elements from row to row
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
+def _rows(t: torch.Tensor, most: int | None = None) -> torch.Tensor:
     """``t`` [rows, columns] with unit column stride, a row stride that is a
-    multiple of 8 and 16-byte aligned rows (copied where it is not)."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+    multiple of 8 and no more than ``most``, and 16-byte aligned rows (copied
+    where it is not)."""
+    near = most is None or t.stride(0) <= most
+    if near and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -42,7 +45,7 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
         with N.on_device(x.device):
-            x, weight = _rows(x), N.aligned(weight)
+            x, weight = _rows(x, MAX_STRIDE), N.aligned(weight)
             ctx.save_for_backward(x, weight, offsets)
             return _forward(x, weight, offsets)
 
@@ -54,7 +57,7 @@ class _GroupedLinear(torch.autograd.Function):
         code = N.DTYPE_CODES[x.dtype]
         dx = dw = None
         with N.on_device(x.device):
-            dy = _rows(dy)
+            dy = _rows(dy, MAX_STRIDE)
             if ctx.needs_input_grad[0]:
                 dx = torch.empty(rows, k, dtype=x.dtype, device=x.device)
                 N.call("kq_grouped_linear_dx", code, N.ptr(dy), dy.stride(0), rows, N.ptr(offsets), groups,
@@ -74,7 +77,11 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     decreasing, on x's device) may leave groups empty and rows in front of the
     first or behind the last group: those rows of y and of x's gradient are
     zero.  Products accumulate in fp32 and are rounded once, to x's type.
-    Offsets outside [0, rows] are taken as the nearest of the two.
+    Offsets outside [0, rows] are taken as the nearest of the two.  x and y's
+    gradient may have any strides (copied unless rows are contiguous, 16-byte
+    aligned and at most 2^22 elements apart, a multiple of 8); a weight whose
+    matrices are not contiguous, a transposed one among them, is copied whole in
+    every call.
 
     Differentiable once, in x and weight; an empty group's weight gradient is
     zero.  Results do not change from call to call (no atomics).  Captured into

@@ -83,6 +83,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     and gradient are 0 whatever their row holds.  Another target outside [0, V)
     gives a NaN loss.
 
+    hidden may have any strides (copied unless its rows are contiguous, 16-byte
+    aligned and a multiple of 8 elements apart); a head that is not contiguous,
+    such as the transpose of one stored [K, V], is copied whole in every call.
+
     Differentiable once, in hidden and in a bf16 weight; a block-scaled head is
     frozen.  The logits and all sums are fp32; the gradients are bf16, their
     softmax terms rounded to bf16 as operands of the gradients' products.

@@ -319,3 +319,17 @@ def test_capture_beside_a_living_graph(gpu):
         torch.cuda.synchronize()
         for a, b in zip((y, dx, dw), want):
             assert torch.equal(a.detach(), b)
+
+
+def test_rows_far_apart(gpu):
+    """Every so many rows of a long buffer, past the row stride that the kernels take, forward and backward."""
+    x, w, dy = operands(5, 2, 40, 64, torch.bfloat16, gpu)
+    starts = [0, 2, 5]
+    want = check(x, w, dy, starts)
+    stride = grouped.MAX_STRIDE + 64
+    far = torch.zeros(4 * stride + 64, dtype=torch.bfloat16, device=gpu)
+    fx, fdy = far.as_strided((5, 64), (stride, 1)), far.clone().as_strided((5, 40), (stride, 1))
+    fx.copy_(x)
+    fdy.copy_(dy)
+    for a, b in zip(_all(fx, w, fdy, torch.tensor(starts, device=gpu)), want):
+        assert torch.equal(a, b)

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from kquant_amd import _native as N
+from kquant_amd import grouped
 from kquant_amd import loss as loss_module
 from kquant_amd.grouped import grouped_linear
 from kquant_amd.linear import mxfp4_linear, mxfp8_linear
@@ -238,3 +239,16 @@ def test_loss_workspace_of_many_tokens(tokens):
     size = N.library().kq_linear_cross_entropy_workspace_size
     for vocab in (131072, 1 << 24):
         assert size(N.FMT_BF16, tokens, vocab, 8, 1) <= (1 << 30) + tokens * (16 + 64 + 24) + 4096
+
+
+def test_grouped_rows_far_apart(monkeypatch):
+    """Rows further apart than the kernels' strides reach are copied, not refused."""
+    strides = []
+    monkeypatch.setattr(N, "call", lambda name, *args: strides.append(args[2]))
+    monkeypatch.setattr(N, "stream", lambda device: None)
+    monkeypatch.setattr(N, "on_device", lambda device: contextlib.nullcontext())
+    w, offsets = bf16(1, 8, 16), torch.tensor([0, 2])
+    for stride in (16, grouped.MAX_STRIDE, grouped.MAX_STRIDE + 8):
+        x = torch.empty(stride + 16, dtype=BF16).as_strided((2, 16), (stride, 1))
+        grouped._GroupedLinear.apply(x, w, offsets)
+    assert strides == [16, grouped.MAX_STRIDE, 16]
