@@ -70,33 +70,38 @@ struct Problem {
     int* part = first + MAX_GROUPS + 1;
     const int t = threadIdx.x, per = (g.groups + mm16::THREADS - 1) / mm16::THREADS;
     const int e0 = min(t * per, g.groups), e1 = min(e0 + per, g.groups);
-    int sum = 0;
+    // Offsets that decrease make groups overlap, and their tiles more than the tables hold: the sums stop at what those
+    // do, so that none overflows and each tile found is one of its group's.
+    const uint32_t most = 64u * TABLE * gridDim.x;  // at most 2^30 and a round
+    auto add = [&](uint32_t a, uint32_t b) { return min(a + b, most); };
+    uint32_t sum = 0;
     for (int e = e0; e < e1; ++e) {
       int beg, n;
       range(e, beg, n);
-      sum += tiles_of(n);
+      sum = add(sum, (uint32_t)tiles_of(n));
     }
-    int upto = sum;
+    uint32_t upto = sum;
     for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(upto, d);
-      if ((t & 63) >= d) upto += v;
+      const uint32_t v = __shfl_up(upto, d);
+      if ((t & 63) >= d) upto = add(upto, v);
     }
-    if ((t & 63) == 63) part[t >> 6] = upto;
+    if ((t & 63) == 63) part[t >> 6] = (int)upto;
+    upto = __shfl_up(upto, 1);  // of the threads before
     __syncthreads();
-    int all = 0, at = upto - sum;
+    uint32_t total = 0, at = (t & 63) ? upto : 0u;
     for (int w = 0; w < mm16::THREADS / 64; ++w) {
-      at += w < t >> 6 ? part[w] : 0;
-      all += part[w];
+      at = add(at, w < t >> 6 ? (uint32_t)part[w] : 0u);
+      total = add(total, (uint32_t)part[w]);
     }
     for (int e = e0; e < e1; ++e) {
       int beg, n;
       range(e, beg, n);
-      first[e] = at;
-      at += tiles_of(n);
+      first[e] = (int)at;
+      at = add(at, (uint32_t)tiles_of(n));
     }
-    if (t == 0) first[g.groups] = all;
+    if (t == 0) first[g.groups] = (int)total;
     __syncthreads();
-    all = __builtin_amdgcn_readfirstlane(all);
+    const int all = __builtin_amdgcn_readfirstlane((int)total);
     count = mm16::worker_tiles(all);
     // The XCDs go through the rounds that all of them take part in from an eighth of the way apart: tiles of large
     // groups, bound by their MFMAs, run beside tiles of small ones, bound by the weights' bytes (8192 rows in 48
@@ -115,10 +120,10 @@ struct Problem {
           if (first[mid] <= tile) lo = mid;
           else hi = mid;
         }
-        int nt;
-        mm16::tile_mn(tile - first[lo], (first[lo + 1] - first[lo]) / ntiles, ntiles, mt_of[q], nt);
-        group_nt[q] = lo << 16 | nt;
         range(lo, beg_of[q], n_of[q]);
+        int nt;
+        mm16::tile_mn(tile - first[lo], tiles_of(n_of[q]) / ntiles, ntiles, mt_of[q], nt);
+        group_nt[q] = lo << 16 | nt;
       }
     }
     __syncthreads();  // the slabs' loads overwrite the sums

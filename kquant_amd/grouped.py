@@ -77,7 +77,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     decreasing, on x's device) may leave groups empty and rows in front of the
     first or behind the last group: those rows of y and of x's gradient are
     zero.  Products accumulate in fp32 and are rounded once, to x's type.
-    Offsets outside [0, rows] are taken as the nearest of the two.  x and y's
+    Offsets outside [0, rows] are taken as the nearest of the two; where they
+    decrease, results are undefined, but nothing outside them is touched.  x and y's
     gradient may have any strides (copied unless rows are contiguous, 16-byte
     aligned and at most 2^22 elements apart, a multiple of 8); a weight whose
     matrices are not contiguous, a transposed one among them, is copied whole in

@@ -333,3 +333,24 @@ def test_rows_far_apart(gpu):
     fdy.copy_(dy)
     for a, b in zip(_all(fx, w, fdy, torch.tensor(starts, device=gpu)), want):
         assert torch.equal(a, b)
+
+
+def test_overlapping_groups_of_many_tiles(gpu):
+    """Decreasing offsets: 2048 groups of all rows, 2^32 tiles and more by their sizes alone.  All weights are the same,
+    so that each row's result is known whichever group wrote it last."""
+    rows, groups, n, k = (1 << 29) + (1 << 20), 4096, 8, 8
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=gpu)
+    at = [0, 1, 255, 256, 1 << 20, rows // 2, rows - 257, rows - 1]
+    for r in at:
+        x[r] = torch.randn(k, device=gpu).to(torch.bfloat16)
+    w = torch.randn(1, n, k, device=gpu).to(torch.bfloat16).expand(groups, n, k).contiguous()
+    offsets = torch.zeros(groups + 1, dtype=torch.int64, device=gpu)
+    offsets[1::2] = rows
+    offsets[-1] = rows
+    with torch.no_grad():
+        y = grouped_linear(x, w, offsets)
+    close(torch.stack([y[r] for r in at]), torch.stack([x[r] for r in at]), w[0], k)
+    for r in at:
+        y[r] = 0
+    for r in range(0, rows, 1 << 26):
+        assert not y[r:r + (1 << 26)].any()
