@@ -270,11 +270,14 @@ def check_capture(*leaves: torch.Tensor) -> None:
 
     A leaf's gradient accumulator belongs to the stream on which its first
     living graph was built (``note_leaves``); a backward pass captured on
-    another stream would pull that stream into the capture.
+    another stream would pull that stream into the capture.  A view stands for
+    the leaf that it was taken from.
     """
 
     if torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled():
         for t in leaves:
+            if t.requires_grad and t._base is not None:
+                t = t._base
             if t.requires_grad and t.is_leaf:
                 node = torch.autograd.graph.get_gradient_edge(t).node
                 here = stream_handle(t.device)
@@ -285,12 +288,14 @@ def check_capture(*leaves: torch.Tensor) -> None:
 
 def note_leaves(result: torch.Tensor) -> None:
     """Writes this stream into the accumulators of the leaves that ``result``
-    was computed from, directly or by one view or copy."""
+    was computed from, directly or by up to four views or copies."""
 
     if result.grad_fn is not None:
         here = stream_handle(result.device)
         for node, _ in result.grad_fn.next_functions:
-            if node is not None and not hasattr(node, "variable"):
+            for _ in range(4):
+                if node is None or hasattr(node, "variable"):
+                    break
                 node = next((n for n, _ in node.next_functions if n is not None), None)
             if node is not None:
                 node.metadata.setdefault(_LEAF_STREAM, here)

@@ -354,3 +354,27 @@ def test_overlapping_groups_of_many_tiles(gpu):
         y[r] = 0
     for r in range(0, rows, 1 << 26):
         assert not y[r:r + (1 << 26)].any()
+
+
+def test_capture_of_views_beside_a_living_graph(gpu):
+    """Weights kept as [groups N, K]: refused while an eager graph lives, captured once it is gone."""
+    x, w, dy = operands(64, 3, 64, 64, torch.bfloat16, gpu)
+    offsets = torch.tensor([0, 9, 40, 64], device=gpu)
+    want = _all(x, w, dy, offsets)
+    leaf, flag = w.reshape(192, 64).clone().requires_grad_(), torch.ones(4, device=gpu)
+    eager = grouped_linear(x, leaf.view(3, 64, 64), offsets)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        flag.zero_()
+        with pytest.raises(RuntimeError, match="still lives"):
+            grouped_linear(x, leaf.view(3, 64, 64), offsets)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = grouped_linear(x, leaf.view(3, 64, 64), offsets)
+        (dw,) = torch.autograd.grad(y, leaf, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.detach(), want[0]) and torch.equal(dw.view(3, 64, 64), want[2])

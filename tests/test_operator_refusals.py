@@ -252,3 +252,22 @@ def test_grouped_rows_far_apart(monkeypatch):
         x = torch.empty(stride + 16, dtype=BF16).as_strided((2, 16), (stride, 1))
         grouped._GroupedLinear.apply(x, w, offsets)
     assert strides == [16, grouped.MAX_STRIDE, 16]
+
+
+def test_capture_of_views_beside_a_living_graph(monkeypatch):
+    """Leaves behind several views, in the graph that lives and in the capture."""
+    state = {"stream": 7, "capturing": False}
+    monkeypatch.setattr(N, "stream_handle", lambda device: state["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    direct, viewed = torch.zeros(6, 4, requires_grad=True), torch.zeros(6, 4, requires_grad=True)
+    kept = direct * 1.0, viewed.view(2, 3, 4).transpose(1, 2).contiguous() * 1.0
+    for t in kept:
+        N.note_leaves(t)
+    state.update(stream=8, capturing=True)
+    for leaf in (direct, viewed):
+        for t in (leaf, leaf.view(2, 3, 4), leaf.view(2, 3, 4).transpose(1, 2), leaf[1:3]):
+            with pytest.raises(RuntimeError, match="still lives"):
+                N.check_capture(torch.zeros(3), t)
+        N.check_capture(leaf.detach().view(2, 12), torch.zeros(3))
+    del kept, t
+    N.check_capture(direct.view(2, 12), viewed[1:])
