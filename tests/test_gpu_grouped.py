@@ -11,6 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kquant_amd import _native as N
 from kquant_amd import grouped
 from kquant_amd.grouped import grouped_linear
 
@@ -378,3 +379,24 @@ def test_capture_of_views_beside_a_living_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y.detach(), want[0]) and torch.equal(dw.view(3, 64, 64), want[2])
+
+
+@pytest.mark.parametrize("offsets", [[50, 20, 0, 10], [-(2 ** 62), 2 ** 62, -3, 7], [0, 50, 0, 50], [60, 70, 80, 90],
+                                     [-9, -8, -7, -6], [0, 20, 30, 50]], ids=str)
+def test_nothing_outside_the_results_is_written(gpu, offsets):
+    """Offsets of any values: what lies before, behind and between the rows of each result stays."""
+    rows, groups, n, k = 50, 3, 40, 72
+    x, w, dy = operands(rows, groups, n, k, torch.bfloat16, gpu)
+    at = torch.tensor(offsets, dtype=torch.int64, device=gpu)
+    st, code = N.stream(gpu), N.DT_BF16
+    ldy, ldx, edge = n + 16, k + 24, 300
+    for width, ld, name in ((n, ldy, "kq_grouped_linear"), (k, ldx, "kq_grouped_linear_dx")):
+        out = torch.full((rows + 2 * edge, ld), 7.0, dtype=torch.bfloat16, device=gpu)
+        source = x if name == "kq_grouped_linear" else dy
+        N.call(name, code, N.ptr(source), source.stride(0), rows, N.ptr(at), groups, N.ptr(w), n, k, N.ptr(out[edge:]), ld, st)
+        torch.cuda.synchronize()
+        assert (out[:edge] == 7).all() and (out[-edge:] == 7).all() and (out[:, width:] == 7).all(), name
+    out = torch.full((groups + 2, n, k), 7.0, dtype=torch.bfloat16, device=gpu)
+    N.call("kq_grouped_linear_dw", code, N.ptr(dy), n, N.ptr(x), k, rows, N.ptr(at), groups, n, k, N.ptr(out[1:]), st)
+    torch.cuda.synchronize()
+    assert (out[0] == 7).all() and (out[-1] == 7).all()

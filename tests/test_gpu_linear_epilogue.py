@@ -204,3 +204,23 @@ def test_wide_outputs_of_few_rows(gpu, fmt, dtype, m, n, k):
     x, w, bias, residual = inputs(m, n, k, dtype, gpu)
     q, s, values, f = quantized(w, fmt)
     check(f(x, q, s, bias=bias, activation="silu", residual=residual), x, values, bias, "silu", residual, dtype)
+
+
+# the one-pass kernel, the K split, register-staged and whole direct-load tiles
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("shape", [(1, 264, 256), (20, 264, 192), (100, 520, 2048), (300, 777, 192), (1030, 4100, 128)], ids=str)
+@pytest.mark.parametrize("kind", KINDS)
+def test_paths_of_f32_rows(gpu, fmt, shape, kind):
+    m, n, k = shape
+    x, w, bias, residual = inputs(m, n, k, torch.float32, gpu)
+    q, s, values, f = quantized(w, fmt)
+    check(f(x, q, s, bias=bias, activation=kind, residual=residual), x, values, bias, kind, residual, torch.float32)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_f32_results_of_bf16_rows(gpu, kind):
+    for m, n, k in ((5, 264, 256), (100, 520, 2048), (300, 777, 192), (1030, 4100, 128)):
+        x, w, bias, residual = inputs(m, n, k, torch.bfloat16, gpu)
+        q, s, values, f = quantized(w, "mxfp4")
+        check(f(x, q, s, bias=bias, activation=kind, residual=residual.float(), out_dtype=torch.float32), x, values, bias, kind,
+              residual.float(), torch.float32)

@@ -17,6 +17,7 @@ import math
 import pytest
 import torch
 
+from kquant_amd import _native as N
 from kquant_amd import mxfp4, mxfp8
 from kquant_amd.io import mxfp4 as mxfp4_io
 from kquant_amd.loss import linear_cross_entropy
@@ -481,3 +482,103 @@ def test_pieces_of_many_tokens(gpu):
     check_sum(dh[some], d, dtol, w)
     _, _, d, dtol = formula(h, w, target)
     check_sum(dw, d.T, dtol.T, torch.where((target != -100)[:, None], h, torch.zeros_like(h)))
+
+
+def exact_inputs(tokens, vocab, k, fmt, gpu):
+    """Block-scaled heads and states whose logits are exact in fp32 in any order of the sums: multiples of 2^-9 below 2^7."""
+    g = torch.Generator(device=gpu).manual_seed(tokens)
+    h = torch.randint(-1, 2, (tokens, k), generator=g, device=gpu).to(torch.bfloat16)
+    steps = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, -0.5, -1.0, -1.5, -2.0, -3.0], device=gpu)
+    w = steps[torch.randint(0, 11, (vocab, k), generator=g, device=gpu)]
+    w[:, :64] = w[:, :64].abs()  # sums over the vocabulary that do not cancel
+    scale = torch.full((vocab, k // 32), 127 - 8, dtype=torch.uint8, device=gpu)
+    if fmt == "mxfp8":
+        q = w.to(torch.float8_e4m3fn)
+    else:
+        grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0], device=gpu)
+        code = torch.bucketize(w.abs(), grid).to(torch.uint8) | ((w < 0).to(torch.uint8) << 3)
+        q = code[:, 0::2] | (code[:, 1::2] << 4)
+    values = w.double() / 256
+    target = torch.randint(0, vocab, (tokens,), generator=g, device=gpu)
+    target[::5] = -100
+    return h, q, scale, values, target
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_pieces_of_block_scaled_heads(gpu, fmt):
+    """A head expanded in two pieces of 8704 and 8296 rows, forward and backward, targets on both sides of the seam.
+
+    The logits are exact, so that a loss is within what the exponentials and the roundings add (see above, E = 0)."""
+    tokens, vocab, k = 70, 17_000, 32_768
+    h, q, scale, values, target = exact_inputs(tokens, vocab, k, fmt, gpu)
+    target[1:5] = torch.tensor([8703, 8704, vocab - 1, 0], device=gpu)
+    size = N.library().kq_linear_cross_entropy_workspace_size
+    head = N.FMT_MXFP8_E4M3 if fmt == "mxfp8" else N.FMT_MXFP4_E2M1
+    assert size(head, tokens, vocab, k, 0) < vocab * k * 2  # not all of it at once
+    counted = target != -100
+    z = h.double() @ values.T
+    assert z.abs().max() < 128
+    lse = torch.logsumexp(z, 1)
+    losses = (lse - z.gather(1, target.clamp(min=0)[:, None])[:, 0]) * counted
+    rel = U24 * (8 * 31 + 400)
+    tol = rel + U24 * 4 * (lse.abs() + z.abs().amax(1) + losses.abs())
+    x = h.clone().requires_grad_()
+    got = linear_cross_entropy(x, q, target, scale, reduction="none")
+    near(got.detach(), losses, tol)
+    (dh,) = torch.autograd.grad(got.sum(), x)
+    d = torch.exp(z - lse[:, None])
+    dtol = d * (tol + rel)[:, None] + 4 * U24
+    d.scatter_add_(1, target.clamp(min=0)[:, None], -torch.ones(tokens, 1, dtype=torch.float64, device=gpu))
+    check_sum(dh, d * counted[:, None], dtol * counted[:, None], values)
+    assert (dh[counted].abs().amax(1) > 0).all() and not dh[~counted].any()
+
+
+@pytest.mark.parametrize("head", ["bf16", "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("batch", [1, 4, 5])
+def test_row_strides_of_states(gpu, head, batch):
+    """States that stay a slice of a wider buffer (20, 80 and 100 rows, 104 apart), NaN beside them."""
+    k, vocab = 64, 321
+    h, w, target = inputs(20 * batch, vocab, k, gpu)
+    if head == "bf16":
+        q, s = w, None
+    else:
+        q, s = (mxfp8.mxfp8_quantize if head == "mxfp8" else mxfp4.mxfp4_quantize)(w)
+    wide = torch.full((batch, 20, 104), float("nan"), dtype=torch.bfloat16, device=gpu)
+    wide[..., 8:72] = h.reshape(batch, 20, k)
+    view = wide[..., 8:72]
+    assert view.reshape(-1, k).data_ptr() == view.data_ptr()
+    x, y = view.detach().requires_grad_(), h.clone().requires_grad_()
+    got = linear_cross_entropy(x, q, target.reshape(batch, 20), s, reduction="sum")
+    want = linear_cross_entropy(y, q, target, s, reduction="sum")
+    assert torch.equal(got.detach(), want.detach())
+    (dx,), (dy,) = torch.autograd.grad(got, x), torch.autograd.grad(want, y)
+    assert torch.equal(dx.reshape(-1, k), dy) and torch.isfinite(dy).all()
+
+
+@pytest.mark.parametrize("tokens,vocab", [(70, 300), (300, 20_000)])
+def test_row_strides_of_gradients(gpu, tokens, vocab):
+    """The C entry point with rows of h and dh further apart than K: stored at once, and as a sum of slices; what lies
+    between the rows and around them stays."""
+    k, ldh, lddh = 136, 152, 168
+    h, w, target = inputs(tokens, vocab, k, gpu)
+    y = h.clone().requires_grad_()
+    loss = linear_cross_entropy(y, w, target, reduction="sum")
+    (want,) = torch.autograd.grad(loss, y)
+    wide = torch.full((tokens, ldh), float("nan"), dtype=torch.bfloat16, device=gpu)
+    wide[:, :k] = h
+    out = torch.full((tokens + 2, lddh), 7.0, dtype=torch.bfloat16, device=gpu)
+    losses, lse = (torch.empty(tokens, device=gpu) for _ in range(2))
+    for backward in (0, 1):
+        need = int(N.library().kq_linear_cross_entropy_workspace_size(N.FMT_BF16, tokens, vocab, k, backward))
+        ws = torch.empty(need, dtype=torch.uint8, device=gpu)
+        if backward:
+            N.call("kq_linear_cross_entropy_backward", N.FMT_BF16, N.ptr(wide), ldh, tokens, N.ptr(w), None, vocab, k,
+                   N.ptr(target), -100, N.ptr(lse), N.ptr(torch.ones(1, device=gpu)), N.LOSS_SUM, N.ptr(out[1:]), lddh, None,
+                   N.ptr(ws), need, N.stream(gpu))
+        else:
+            N.call("kq_linear_cross_entropy", N.FMT_BF16, N.ptr(wide), ldh, tokens, N.ptr(w), None, vocab, k, N.ptr(target),
+                   -100, N.ptr(losses), N.ptr(lse), None, N.ptr(ws), need, N.stream(gpu))
+        torch.cuda.synchronize()
+    assert torch.equal(losses, linear_cross_entropy(h, w, target, reduction="none"))
+    assert torch.equal(out[1:-1, :k], want)
+    assert (out[:, k:] == 7).all() and (out[0] == 7).all() and (out[-1] == 7).all()
