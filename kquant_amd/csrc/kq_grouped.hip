@@ -120,10 +120,11 @@ struct Problem {
           if (first[mid] <= tile) lo = mid;
           else hi = mid;
         }
-        range(lo, beg_of[q], n_of[q]);
+        // (rounded up: the last group before the sums stop may have part of its tiles)
         int nt;
-        mm16::tile_mn(tile - first[lo], tiles_of(n_of[q]) / ntiles, ntiles, mt_of[q], nt);
+        mm16::tile_mn(tile - first[lo], (first[lo + 1] - first[lo] + ntiles - 1) / ntiles, ntiles, mt_of[q], nt);
         group_nt[q] = lo << 16 | nt;
+        range(lo, beg_of[q], n_of[q]);
       }
     }
     __syncthreads();  // the slabs' loads overwrite the sums
