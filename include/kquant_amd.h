@@ -346,7 +346,7 @@ int kq_linear_cross_entropy(int w_fmt, const void* h, int64_t ldh, int64_t token
  * else one value, the gradient of the mean or the sum.  With
  *   d[t][v] = g_t (exp(z[t][v] - lse[t]) - [v == target[t]]),
  * g_t zero for ignored tokens: dh = d w (bf16 [tokens, k], row stride lddh, or
- * NULL) and, for a bf16 head, dw = d^T h (bf16 [vocab, k], or NULL).  lse is
+ * NULL without one) and, for a bf16 head, dw = d^T h (bf16 [vocab, k], or NULL).  lse is
  * kq_linear_cross_entropy's.  d is formed in fp32 piece by piece of the
  * vocabulary (at most 1 GiB of it at once) and rounded to bf16 as an operand.
  * Ignored tokens' rows of h reach nothing; their dh is zero.  Deterministic.

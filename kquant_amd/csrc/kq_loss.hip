@@ -798,7 +798,7 @@ extern "C" int kq_linear_cross_entropy_backward(int w_fmt, const void* h, int64_
   const char* fn = "kq_linear_cross_entropy_backward";
   if (int rc = loss::check(fn, w_fmt, h, ldh, tokens, w, w_scale, vocab, k, target, reduction)) return rc;
   if (dw && w_fmt != KQ_FMT_BF16) return kq_fail(KQ_ERR_INVALID, "%s: only a bf16 head has a gradient", fn);
-  if (lddh < k || lddh % 8 || kq_misaligned(dh, 16) || kq_misaligned(dw, 16))
+  if ((dh && (lddh < k || lddh % 8)) || kq_misaligned(dh, 16) || kq_misaligned(dw, 16))
     return kq_fail(KQ_ERR_INVALID, "%s: need lddh >= k, lddh %% 8 == 0, dh and dw 16-byte aligned", fn);
   hipStream_t st = (hipStream_t)stream;
   int cus = 0;

@@ -582,3 +582,21 @@ def test_row_strides_of_gradients(gpu, tokens, vocab):
     assert torch.equal(losses, linear_cross_entropy(h, w, target, reduction="none"))
     assert torch.equal(out[1:-1, :k], want)
     assert (out[:, k:] == 7).all() and (out[0] == 7).all() and (out[-1] == 7).all()
+
+
+def test_gradient_of_the_head_alone(gpu):
+    """The C entry point with neither dh nor its row stride."""
+    tokens, vocab, k = 70, 300, 136
+    h, w, target = inputs(tokens, vocab, k, gpu)
+    y = w.clone().requires_grad_()
+    (want,) = torch.autograd.grad(linear_cross_entropy(h, y, target, reduction="sum"), y)
+    lse = torch.logsumexp(h.float() @ w.float().T, 1)
+    dw = torch.empty_like(w)
+    need = int(N.library().kq_linear_cross_entropy_workspace_size(N.FMT_BF16, tokens, vocab, k, 1))
+    ws = torch.empty(need, dtype=torch.uint8, device=gpu)
+    N.call("kq_linear_cross_entropy_backward", N.FMT_BF16, N.ptr(h), k, tokens, N.ptr(w), None, vocab, k, N.ptr(target), -100,
+           N.ptr(lse), N.ptr(torch.ones(1, device=gpu)), N.LOSS_SUM, None, 0, N.ptr(dw), N.ptr(ws), need, N.stream(gpu))
+    torch.cuda.synchronize()
+    _, _, d, dtol = formula(h, w, target)
+    for got in (dw, want):
+        check_sum(got, d.T, dtol.T, torch.where((target != -100)[:, None], h, torch.zeros_like(h)))

@@ -271,3 +271,13 @@ def test_capture_of_views_beside_a_living_graph(monkeypatch):
         N.check_capture(leaf.detach().view(2, 12), torch.zeros(3))
     del kept, t
     N.check_capture(direct.view(2, 12), viewed[1:])
+
+
+def test_no_row_stride_without_rows():
+    """A caller that asks for dw alone has no row stride of dh to give (refused here for the workspace at the latest)."""
+    lib = N.library()
+    p = ctypes.c_void_p(256)
+    back = [N.FMT_BF16, p, 64, 10, p, None, 99, 64, p, -100, p, p, N.LOSS_SUM, None, 0, p, None, 0, None]
+    assert lib.kq_linear_cross_entropy_backward(*back) != N.KQ_OK and b"lddh" not in lib.kq_last_error()
+    back[13] = p
+    assert lib.kq_linear_cross_entropy_backward(*back) == N.KQ_ERR_INVALID and b"lddh" in lib.kq_last_error()
