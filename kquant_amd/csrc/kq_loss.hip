@@ -610,7 +610,8 @@ static Plan plan(int w_fmt, int64_t tokens, int64_t vocab, int64_t k, bool backw
   Plan p{};
   const bool mx = w_fmt != KQ_FMT_BF16;
   // A block-scaled head at few tokens is read as it is, once (5 tokens, V = 129280, K = 7168 E4M3: 172 us; expanded
-  // to bf16 and multiplied in tiles 760 us).  A bf16 head's tiles stream it at the chip's rate at any count.
+  // to bf16 and multiplied in tiles 760 us).  A bf16 head's tiles stream it whatever the count (1.85 GB,
+  // 1 / 16 / 64 tokens: 323 / 332 / 334 us, 5.5 to 5.7 TB/s).
   p.few = mx && !backward && tokens >= 1 && tokens <= 64;
   if (p.few) {
     p.o_z = 0;
