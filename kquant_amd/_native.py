@@ -265,6 +265,17 @@ def to_gpu(tensors: Iterable[torch.Tensor | None]) -> tuple[list, torch.device, 
 _LEAF_STREAM = "kquant_amd.stream"
 
 
+def _accumulator(node):
+    """The gradient accumulator that an autograd node leads to by up to four
+    views or copies, or None."""
+
+    for _ in range(4):
+        if node is None or hasattr(node, "variable"):
+            break
+        node = next((n for n, _ in node.next_functions if n is not None), None)
+    return node if hasattr(node, "variable") else None
+
+
 def check_capture(*leaves: torch.Tensor) -> None:
     """Refuses a capture that would end the process.
 
@@ -276,14 +287,13 @@ def check_capture(*leaves: torch.Tensor) -> None:
 
     if torch.cuda.is_current_stream_capturing() and torch.is_grad_enabled():
         for t in leaves:
-            if t.requires_grad and t._base is not None:
-                t = t._base
-            if t.requires_grad and t.is_leaf:
-                node = torch.autograd.graph.get_gradient_edge(t).node
-                here = stream_handle(t.device)
-                if node.metadata.get(_LEAF_STREAM, here) != here:
-                    raise RuntimeError("an autograd graph of these leaves that was built on another stream still lives: "
-                                       "drop it (its results) before capturing their forward and backward pass")
+            if not t.requires_grad or not (t.is_leaf or t._is_view()):
+                continue
+            node = torch.autograd.graph.get_gradient_edge(t).node if t.is_leaf else _accumulator(t.grad_fn)
+            here = stream_handle(t.device)
+            if node is not None and node.metadata.get(_LEAF_STREAM, here) != here:
+                raise RuntimeError("an autograd graph of these leaves that was built on another stream still lives: "
+                                   "drop it (its results) before capturing their forward and backward pass")
 
 
 def note_leaves(result: torch.Tensor) -> None:
@@ -293,10 +303,7 @@ def note_leaves(result: torch.Tensor) -> None:
     if result.grad_fn is not None:
         here = stream_handle(result.device)
         for node, _ in result.grad_fn.next_functions:
-            for _ in range(4):
-                if node is None or hasattr(node, "variable"):
-                    break
-                node = next((n for n, _ in node.next_functions if n is not None), None)
+            node = _accumulator(node)
             if node is not None:
                 node.metadata.setdefault(_LEAF_STREAM, here)
 

@@ -281,3 +281,20 @@ def test_no_row_stride_without_rows():
     assert lib.kq_linear_cross_entropy_backward(*back) != N.KQ_OK and b"lddh" not in lib.kq_last_error()
     back[13] = p
     assert lib.kq_linear_cross_entropy_backward(*back) == N.KQ_ERR_INVALID and b"lddh" in lib.kq_last_error()
+
+
+def test_capture_of_a_leaf_that_is_a_view(monkeypatch):
+    """A leaf made of part of a tensor that needs no gradient is a leaf of its own."""
+    state = {"stream": 7, "capturing": False}
+    monkeypatch.setattr(N, "stream_handle", lambda device: state["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    leaf = torch.zeros(8, 4)[2:6].requires_grad_()
+    assert leaf.is_leaf and leaf._base is not None
+    kept = leaf * 1.0
+    N.note_leaves(kept)
+    state.update(stream=8, capturing=True)
+    for t in (leaf, leaf.view(2, 8)):
+        with pytest.raises(RuntimeError, match="still lives"):
+            N.check_capture(t)
+    del kept, t
+    N.check_capture(leaf)
