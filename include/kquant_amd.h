@@ -42,6 +42,8 @@ enum { KQ_LIN_NONE = 0, KQ_LIN_RELU = 1, KQ_LIN_SILU = 2, KQ_LIN_GELU = 3, KQ_LI
 enum { KQ_LOSS_NONE = 0, KQ_LOSS_MEAN = 1, KQ_LOSS_SUM = 2 };
 /* dense element types */
 enum { KQ_DT_BF16 = 0, KQ_DT_F16 = 1, KQ_DT_F32 = 2 };
+/* 8-bit integers, where an entry point says that it takes them */
+enum { KQ_DT_I8 = 4 };
 /* flags */
 enum {
   /* use the bit-level software rounding instead of the gfx950 convert
@@ -317,6 +319,41 @@ int kq_grouped_linear_dx(int dtype, const void* dy, int64_t lddy, int64_t rows, 
  * an empty group). */
 int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows,
                          const int64_t* offsets, int groups, int64_t n, int64_t k, void* dw, void* stream);
+
+/* ---------------------------------------------------------- 8-bit integers -- */
+
+/* Rows as 8-bit integers with one scale a row (no kquant counterpart):
+ *   scale[r] = max(fl(max_k |x[r][k]| / 127), 2^-126),
+ *   q[r][k] = the integer nearest to x[r][k] / scale[r], of two the even one,
+ * of the exact quotient.  A row with an infinity or a NaN: scale NaN, codes 0.
+ * dtype: KQ_DT_*; x [rows, k] (row stride ldx elements) and q (row stride ldq)
+ * at any alignment of their types (16-byte aligned rows are the fast ones). */
+int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t k, int8_t* q, int64_t ldq,
+                     float* scale, void* stream);
+
+/* c = act(a_scale[m] w_scale[n] sum_k a[m][k] w[n][k] + bias) + residual over
+ * 8-bit integers w [n, k] with an fp32 scale a row; int32 sums (exact), fp32
+ * after them, rounded once to out_dtype (KQ_DT_*).  a_dtype KQ_DT_I8: a holds
+ * codes with a_scale [m]; otherwise rows of that type, quantized as
+ * kq_int8_quantize does (a_scale is not read).  activation, bias, residual as
+ * kq_mx_linear_epilogue takes them, the residual of out_dtype (row stride ldr).
+ * k % 16 == 0, k <= 131056; w and codes 16-byte aligned, lda of codes a multiple
+ * of 16.  workspace: kq_int8_linear_workspace_size bytes (the rows' codes; 0 for
+ * codes and a few rows), 16-byte aligned, written and read by this call alone. */
+int64_t kq_int8_linear_workspace_size(int a_dtype, int64_t m, int64_t n, int64_t k);
+int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const float* a_scale, const int8_t* w, const float* w_scale,
+                   int64_t m, int64_t n, int64_t k, int activation, const void* bias, int bias_dtype,
+                   const void* residual, int64_t ldr, int out_dtype, void* c, int64_t ldc, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* y[r] = x_scale[r] w_scale[g][n] (W_g x[r]) over 8-bit integers for the rows r of
+ * group g: offsets, rows of no group and strides as kq_grouped_linear takes them,
+ * x codes [rows, k] with scales [rows], w [groups, n, k] with scales [groups, n],
+ * y of out_dtype (KQ_DT_*).  int32 sums, rounded once after the scaling.  n % 8,
+ * k % 16 == 0, ldx a multiple of 16, ldy of 8; x, w, y 16-byte aligned. */
+int kq_int8_grouped_linear(const int8_t* x, int64_t ldx, const float* x_scale, int64_t rows, const int64_t* offsets,
+                           int groups, const int8_t* w, const float* w_scale, int64_t n, int64_t k, int out_dtype,
+                           void* y, int64_t ldy, void* stream);
 
 /* --------------------------------------------------- vocabulary head loss -- */
 

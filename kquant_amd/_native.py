@@ -32,6 +32,7 @@ LOSS_SUM = 2
 DT_BF16 = 0
 DT_F16 = 1
 DT_F32 = 2
+DT_I8 = 4
 QSRT_OUT_E4M3 = 3  # kq_qsrt_decode_weight's E4M3 label-byte output (KQ_QSRT_OUT_E4M3)
 FLAG_SOFTWARE_CVT = 1
 TABLE_E8M0 = 0
@@ -130,6 +131,11 @@ SIGNATURES: dict[str, list] = {
     "kq_grouped_linear": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dx": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dw": [_INT, _VP, _I64, _VP, _I64, _I64, _VP, _INT, _I64, _I64, _VP, _VP],
+    "kq_int8_quantize": [_INT, _VP, _I64, _I64, _I64, _VP, _I64, _VP, _VP],
+    "kq_int8_linear_workspace_size": [_INT, _I64, _I64, _I64],
+    "kq_int8_linear": [_INT, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _INT, _VP, _INT, _VP, _I64, _INT, _VP, _I64, _VP,
+                       _I64, _VP],
+    "kq_int8_grouped_linear": [_VP, _I64, _VP, _I64, _VP, _INT, _VP, _VP, _I64, _I64, _INT, _VP, _I64, _VP],
     "kq_linear_cross_entropy_workspace_size": [_INT, _I64, _I64, _I64, _INT],
     "kq_linear_cross_entropy": [_INT, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _VP],
     "kq_linear_cross_entropy_backward": [_INT, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _INT, _VP,

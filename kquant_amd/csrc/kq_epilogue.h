@@ -75,7 +75,7 @@ __device__ __forceinline__ float epi_bias_value(const Epilogue& e, uint32_t bits
 }
 __device__ __forceinline__ float epi_bias(const Epilogue& e, int64_t n) { return epi_bias_value(e, epi_bias_bits(e, n)); }
 
-// OUT: KQ_DT_BF16 or KQ_DT_F32, the output's and so the residual's type.
+// OUT: the output's and so the residual's type (KQ_DT_BF16 or KQ_DT_F32; of int8 products KQ_DT_F16 too).
 template <int OUT>
 __device__ __forceinline__ uint32_t epi_residual_bits(const Epilogue& e, int64_t m, int64_t n) {
   if (!e.residual) return 0u;
@@ -84,6 +84,7 @@ __device__ __forceinline__ uint32_t epi_residual_bits(const Epilogue& e, int64_t
 }
 template <int OUT>
 __device__ __forceinline__ float epi_residual_value(uint32_t bits) {
+  if (OUT == KQ_DT_F16) return f16_bits_to_f32(bits);
   return __uint_as_float(OUT == KQ_DT_F32 ? bits : bits << 16);
 }
 template <int OUT>
@@ -95,6 +96,19 @@ __device__ __forceinline__ float epi_residual(const Epilogue& e, int64_t m, int6
 template <int OUT>
 __device__ __forceinline__ float epi_apply(const Epilogue& e, float x, int64_t m, int64_t n) {
   return epi_activate_any(e, x + epi_bias(e, n)) + epi_residual<OUT>(e, m, n);
+}
+
+// The activation's class and constants (KQ_LIN_*).
+static inline Epilogue make_epilogue(int activation) {
+  Epilogue e{};
+  e.kind = activation == KQ_LIN_GELU                                     ? EPI_ERF
+           : activation == KQ_LIN_SILU || activation == KQ_LIN_GELU_TANH ? EPI_SIGMOID
+                                                                         : EPI_CLAMP;
+  e.low = activation == KQ_LIN_RELU ? 0.0f : -__builtin_inff();
+  constexpr double C = 1.5957691216057308;  // 2 sqrt(2 / pi)
+  e.c1 = activation == KQ_LIN_GELU_TANH ? (float)C : 1.0f;
+  e.c3 = activation == KQ_LIN_GELU_TANH ? (float)(0.044715 * C) : 0.0f;
+  return e;
 }
 
 // The epilogue of the rows from m0 and the columns from n0 on.

@@ -1415,14 +1415,7 @@ extern "C" int kq_mx_linear_epilogue(int w_fmt, int a_dtype, const void* a, int6
   if (residual && ldr < n) return kq_fail(KQ_ERR_INVALID, "%s: need ldr >= n", fn);
   if (kq_misaligned(bias, bias_dtype == KQ_DT_F32 ? 4 : 2) || kq_misaligned(residual, out_dtype == KQ_DT_F32 ? 4 : 2))
     return kq_fail(KQ_ERR_INVALID, "%s: bias and residual must be aligned to their type", fn);
-  Epilogue e{};
-  e.kind = activation == KQ_LIN_GELU                                             ? EPI_ERF
-           : activation == KQ_LIN_SILU || activation == KQ_LIN_GELU_TANH ? EPI_SIGMOID
-                                                                                 : EPI_CLAMP;
-  e.low = activation == KQ_LIN_RELU ? 0.0f : -__builtin_inff();
-  constexpr double C = 1.5957691216057308;  // 2 sqrt(2 / pi)
-  e.c1 = activation == KQ_LIN_GELU_TANH ? (float)C : 1.0f;
-  e.c3 = activation == KQ_LIN_GELU_TANH ? (float)(0.044715 * C) : 0.0f;
+  Epilogue e = make_epilogue(activation);
   e.bias = bias;
   e.bias_f32 = bias_dtype == KQ_DT_F32;
   e.residual = residual;

@@ -1,5 +1,6 @@
-// Matrix products of 16-bit operands (bf16 or fp16) with fp32 accumulation,
-// the core shared by the grouped products and the head loss:
+// Matrix products of 16-bit operands (bf16 or fp16) with fp32 accumulation, and
+// of 8-bit integers with int32 accumulation, the core shared by the grouped
+// products, the head loss and the int8 linear:
 //
 //   D[m][n] = sum over c of A(m, c) B(n, c)
 //
@@ -137,9 +138,20 @@ struct Reader {
   }
 };
 
-template <bool F16>
+// What the 16-byte fragments hold.  Of 8-bit integers (I8) a pair counts as one
+// element in every index and length here, and the accumulators' registers hold
+// int32 bits: the same bytes and the same cycles for twice the products.
+enum { BF16 = 0, F16 = 1, I8 = 2 };
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x16_t __attribute__((ext_vector_type(16)));
+
+template <int KIND>
 __device__ __forceinline__ float16_t mfma(u32x4_t a, u32x4_t b, float16_t c) {
-  if (F16)
+  if (KIND == I8)
+    return __builtin_bit_cast(float16_t, __builtin_amdgcn_mfma_i32_32x32x32_i8(
+                                             __builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b),
+                                             __builtin_bit_cast(i32x16_t, c), 0, 0, 0));
+  if (KIND == F16)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
                                                   0, 0);
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
@@ -406,7 +418,7 @@ enum { WHOLE = 0, SMALL_ROWS = 1, SMALL_COLS = 2 };  // which tiles may be narro
 // is read for them alone nontemporally: 384 -> 349 us.
 // Not B that others read too or that may still be in a cache: 12 groups of
 // 1416 x 1032 again and again, 21 us a call and 29 so.
-template <bool AA, bool BA, bool F16, int NARROW, bool LEAD_B, bool ONCE, class P>
+template <bool AA, bool BA, int KIND, int NARROW, bool LEAD_B, bool ONCE, class P>
 struct Core {
   const P& p;
   uint32_t lds0;
@@ -499,7 +511,7 @@ struct Core {
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
           const int i = m / WN, j = m % WN;
-          acc[i][j] = mfma<F16>(a[kk][i], b[kk][j], acc[i][j]);
+          acc[i][j] = mfma<KIND>(a[kk][i], b[kk][j], acc[i][j]);
           // block 0 reads in its first half, so that nothing is in flight at the barrier
           constexpr int HALF = NM > 1 ? NM / 2 : 1;
           const int rn = kk == 0 ? HALF : NM;

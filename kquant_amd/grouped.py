@@ -6,7 +6,8 @@ differentiable in the rows and in the weights.  It is the product that the
 unquantized experts need (``moe.reconstruct_source`` gives their bf16
 matrices): a teacher's forward pass for calibration rows, and the training or
 recovery of experts; ``moe.grouped_expert_forward`` is the fused inference path
-over MXFP4 weights.
+over MXFP4 weights.  ``int8_grouped_linear`` is the product of experts held in
+8-bit integers.
 
 Group sizes are device data throughout: nothing is read back to the host, so
 the calls can be captured into a graph and replayed with other offsets.
@@ -18,6 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
+from .int8 import INT8_K_ALIGN, _check_source_scale, _check_weight, _pad_k, _quantize, _row_stride, _row_view
 
 MAX_GROUPS = 4096
 MAX_STRIDE = 1 << 22  # elements from row to row
@@ -116,4 +118,59 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     offsets = N.aligned(offsets if offsets.dtype == torch.int64 else offsets.to(torch.int64), 8)
     y = _GroupedLinear.apply(x, weight, offsets)
     N.note_leaves(y)
+    return y if host is None else y.to(host)
+
+
+def int8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, offsets: torch.Tensor, *,
+                        x_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``y[r] = dequant(weight[g]) @ dequant(x[r])`` over 8-bit integers for the
+    rows r in [offsets[g], offsets[g + 1]).
+
+    weight int8 [groups, N, K] with fp32 scales [groups, N] (or [groups, N, 1]);
+    x either int8 codes [rows, K] with ``x_scale`` [rows], or bf16, fp16 or fp32
+    rows, which are quantized in the call as ``int8.int8_quantize`` does.
+    Offsets, rows of no group (zeros) and undefined orders are those of
+    ``grouped_linear``.  N is a multiple of 8; a K that is no multiple of 16 is
+    padded with zeros (a copy of the weight in every call).  The sums are exact;
+    the scaled result is rounded once to ``out_dtype`` (x's type, bf16 for codes).
+    No gradient: an x that requires one is refused while autograd records.
+    """
+
+    x_scale = _check_source_scale(x, x_scale)
+    if offsets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"offsets must be int64 or int32, got {offsets.dtype}")
+    if x.ndim != 2:
+        raise ValueError("x must be [rows, K]")
+    rows, k = x.shape
+    scale = _check_weight(weight, scale, 3, k)
+    groups, n = weight.shape[:2]
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"groups={groups} must be between 1 and {MAX_GROUPS}")
+    if n == 0 or n % 8:
+        raise ValueError(f"N={n} must be a positive multiple of 8")
+    if tuple(offsets.shape) != (groups + 1,):
+        raise ValueError(f"offsets shape {tuple(offsets.shape)} != {(groups + 1,)}")
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if x.dtype == torch.int8 else x.dtype
+    if out_dtype not in N.DTYPE_CODES:
+        raise TypeError("out_dtype must be bfloat16, float16 or float32")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("int8_grouped_linear carries no gradient: detach x or call it under torch.no_grad()")
+    given = [x, weight, scale, x_scale, offsets]
+    (a, w, s, sx, offsets), gpu, host = N.to_gpu([None if t is None else t.detach() for t in given])
+    a, s = _row_view(a), N.aligned(s, 4)
+    kp = -(-k // INT8_K_ALIGN) * INT8_K_ALIGN
+    w = N.aligned(_pad_k(w, kp))
+    with N.on_device(gpu):
+        offsets = N.aligned(offsets if offsets.dtype == torch.int64 else offsets.to(torch.int64), 8)
+        if sx is None:
+            a, sx = _quantize(a, kp)
+        else:
+            sx = N.aligned(sx, 4)
+            a = _pad_k(a, kp)
+            if a.data_ptr() % 16 or _row_stride(a) % 16 or _row_stride(a) > MAX_STRIDE:
+                a = a.clone(memory_format=torch.contiguous_format)
+        y = torch.empty(rows, n, dtype=out_dtype, device=gpu)
+        N.call("kq_int8_grouped_linear", N.ptr(a), _row_stride(a), N.ptr(sx), rows, N.ptr(offsets), groups, N.ptr(w),
+               N.ptr(s), n, kp, N.DTYPE_CODES[out_dtype], N.ptr(y), n, N.stream(gpu))
     return y if host is None else y.to(host)

@@ -20,6 +20,9 @@ MXFP8 with the ``mxfp8_quantize`` rule (``block_fp8_linear.quantize_input``,
 fp8 matrix cores (``kq_mx_linear_mm``); ``mxfp8_linear_mx`` takes input rows
 that are already quantized (``kq_mx_linear_mx``).  Its oracle is
 ``_reference_from_packed`` (:146-160): dequantize both operands, fp32 product.
+
+``int8_linear`` is the linear over 8-bit integers with a scale of each token and
+each channel (``kq_int8_linear``), with the same epilogue.
 """
 
 from __future__ import annotations
@@ -27,6 +30,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
+from .int8 import INT8_K_ALIGN, _check_source_scale, _check_weight, _pad_k as _pad_codes, _quantize, _row_stride, _row_view
 
 
 def _check_epilogue(source, bias, activation, residual, lead, n: int, f32: bool, out_dtype: torch.dtype) -> None:
@@ -237,4 +241,64 @@ def mxfp8_linear_mx(source_q: torch.Tensor, source_scale: torch.Tensor, weight: 
                      device=gpu)
     N.call("kq_mx_linear_mx", N.FMT_MXFP8_E4M3, N.ptr(aq), N.ptr(as_), kp, N.FMT_MXFP8_E4M3, N.ptr(w), N.ptr(s),
            m, n, kp, N.DTYPE_CODES[out_dtype], N.ptr(out), n, N.ptr(ws), ws.numel(), N.stream(gpu))
+    return out if host is None else out.to(host)
+
+
+def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, *,
+                source_scale: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                activation: str | None = None, residual: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``activation(dequant(source) @ dequant(weight).T + bias) + residual`` over
+    8-bit integers: weight int8 [N, K] with fp32 scales [N] (or [N, 1]), source
+    either int8 codes [..., K] with ``source_scale`` [...] (``int8_quantize``,
+    once for all layers that read the rows) or bf16, fp16 or fp32 rows, which are
+    quantized in the call by the same rule.
+
+    The integer sums are exact; scaling, bias [N] (bf16 or fp32), activation
+    ("relu", "silu", "gelu", "gelu_tanh") and residual (of the result's shape and
+    type) are fp32, rounded once.  The result is bf16, fp16 or fp32: ``out_dtype``,
+    else the source's type, else (codes) bf16.  A row whose source holds an
+    infinity or a NaN is NaN.  K is at most 131056; a K that is no multiple of 16
+    is padded with zeros (a copy of the weight in every call: pad it once to skip
+    that).  Results do not change from call to call.  They carry no gradient: a
+    source, bias or residual that requires one is refused while autograd records.
+    """
+    source_scale = _check_source_scale(source, source_scale)
+    if source.ndim < 1:
+        raise ValueError("source must have a feature dimension")
+    k = source.shape[-1]
+    scale = _check_weight(weight, scale, 2, k)
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if source.dtype == torch.int8 else source.dtype
+    if out_dtype not in N.DTYPE_CODES:
+        raise TypeError("out_dtype must be bfloat16, float16 or float32")
+    n, lead = weight.shape[0], source.shape[:-1]
+    _check_epilogue(source, bias, activation, residual, lead, n, False, out_dtype)
+    given = [source, weight, scale, source_scale, bias, residual]
+    (a, w, s, sx, bias, residual), gpu, host = N.to_gpu([None if t is None else t.detach() for t in given])
+    a, s = _row_view(a), N.aligned(s, 4)
+    kp = -(-k // INT8_K_ALIGN) * INT8_K_ALIGN
+    w = N.aligned(_pad_codes(w, kp))
+    m = a.shape[0]
+    with N.on_device(gpu):
+        if sx is not None:
+            sx = N.aligned(sx.reshape(-1), 4)
+            a = _pad_codes(a, kp)
+            if a.data_ptr() % 16 or _row_stride(a) % 16 or _row_stride(a) > 1 << 22:
+                a = a.clone(memory_format=torch.contiguous_format)
+        elif kp != k:
+            a, sx = _quantize(a, kp)
+        if bias is not None:
+            bias = bias.contiguous()
+        if residual is not None:
+            residual = _row_view(residual)
+        code = N.DT_I8 if a.dtype == torch.int8 else N.DTYPE_CODES[a.dtype]
+        need = int(N.library().kq_int8_linear_workspace_size(code, m, n, kp))
+        ws = torch.empty(need, dtype=torch.uint8, device=gpu) if need > 0 else None
+        out = torch.empty(m, n, dtype=out_dtype, device=gpu)
+        N.call("kq_int8_linear", code, N.ptr(a), _row_stride(a), N.ptr(sx), N.ptr(w), N.ptr(s), m, n, kp,
+               N.LIN_ACTIVATIONS[activation], N.ptr(bias), N.DT_BF16 if bias is None else N.DTYPE_CODES[bias.dtype],
+               N.ptr(residual), n if residual is None else _row_stride(residual), N.DTYPE_CODES[out_dtype], N.ptr(out), n,
+               N.ptr(ws), max(need, 0), N.stream(gpu))
+    out = out.reshape(*lead, n)
     return out if host is None else out.to(host)
