@@ -355,6 +355,24 @@ int kq_int8_grouped_linear(const int8_t* x, int64_t ldx, const float* x_scale, i
                            int groups, const int8_t* w, const float* w_scale, int64_t n, int64_t k, int out_dtype,
                            void* y, int64_t ldy, void* stream);
 
+/* --------------------------------------------------------------- sampling -- */
+
+/* One token for each row of logits [rows, vocab] (dtype KQ_DT_*, row stride ld;
+ * no kquant counterpart).  With w_i = exp((l_i - max) / temperature) and the order
+ * of descending logits (ties: the lower index first), the first top_k tokens are
+ * kept (0: all), of those the shortest prefix whose weight reaches top_p of theirs
+ * (>= 1: all), of those the tokens with w_i >= min_p; the first always.  tokens[r]
+ * is the first kept token, by index, whose cumulative weight exceeds uniform[r]
+ * times the total; logprobs[r] (or NULL) the natural logarithm of its share.  A
+ * temperature that is not above 0 takes the first of the order.  A row with a NaN,
+ * or without a logit above -inf: -1 and NaN.  Each setting: a device array of one
+ * a row, or NULL and the number for all.  Weights are multiples of 2^-45 and summed
+ * as integers: deterministic.  vocab <= 262144. */
+int kq_sample_tokens(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* uniform,
+                     const float* temperature_rows, double temperature, const int* top_k_rows, int64_t top_k,
+                     const float* top_p_rows, double top_p, const float* min_p_rows, double min_p, int64_t* tokens,
+                     float* logprobs, void* stream);
+
 /* --------------------------------------------------- vocabulary head loss -- */
 
 /* Softmax cross entropy of a vocabulary head without keeping its logits (no
