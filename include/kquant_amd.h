@@ -367,11 +367,14 @@ int kq_int8_grouped_linear(const int8_t* x, int64_t ldx, const float* x_scale, i
  * temperature that is not above 0 takes the first of the order.  A row with a NaN,
  * or without a logit above -inf: -1 and NaN.  Each setting: a device array of one
  * a row, or NULL and the number for all.  Weights are multiples of 2^-45 and summed
- * as integers: deterministic.  vocab <= 262144. */
+ * as integers: deterministic.  vocab <= 262144, rows <= 2^20.  workspace:
+ * kq_sample_tokens_workspace_size bytes (filters: whether top_k or top_p may cut
+ * in some row), 16-byte aligned, written and read by this call alone. */
+int64_t kq_sample_tokens_workspace_size(int64_t rows, int64_t vocab, int filters);
 int kq_sample_tokens(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* uniform,
                      const float* temperature_rows, double temperature, const int* top_k_rows, int64_t top_k,
                      const float* top_p_rows, double top_p, const float* min_p_rows, double min_p, int64_t* tokens,
-                     float* logprobs, void* stream);
+                     float* logprobs, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* --------------------------------------------------- vocabulary head loss -- */
 

@@ -136,7 +136,9 @@ SIGNATURES: dict[str, list] = {
     "kq_int8_linear": [_INT, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _INT, _VP, _INT, _VP, _I64, _INT, _VP, _I64, _VP,
                        _I64, _VP],
     "kq_int8_grouped_linear": [_VP, _I64, _VP, _I64, _VP, _INT, _VP, _VP, _I64, _I64, _INT, _VP, _I64, _VP],
-    "kq_sample_tokens": [_INT, _VP, _I64, _I64, _I64, _VP, _VP, _F64, _VP, _I64, _VP, _F64, _VP, _F64, _VP, _VP, _VP],
+    "kq_sample_tokens_workspace_size": [_I64, _I64, _INT],
+    "kq_sample_tokens": [_INT, _VP, _I64, _I64, _I64, _VP, _VP, _F64, _VP, _I64, _VP, _F64, _VP, _F64, _VP, _VP, _VP, _I64,
+                         _VP],
     "kq_linear_cross_entropy_workspace_size": [_INT, _I64, _I64, _I64, _INT],
     "kq_linear_cross_entropy": [_INT, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _VP],
     "kq_linear_cross_entropy_backward": [_INT, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _INT, _VP,

@@ -162,6 +162,10 @@ __device__ __forceinline__ uint64_t drawn_weight(double u, uint64_t total) {
   return u > 0.0 ? share(u, total, rest) : 0;
 }
 
+__device__ __forceinline__ float logprob_of(double distance, uint64_t total) {
+  return (float)(distance - log((double)total * (1.0 / (double)(1ull << UNIT))));
+}
+
 // --------------------------------------------------------- one row, whole --
 
 constexpr int T = 1024;
@@ -250,9 +254,7 @@ __device__ __forceinline__ Cut select(const char* row, int vocab, const Scale& s
 }
 
 template <int DT>
-__global__ __launch_bounds__(T) void row_kernel(const Args a) {
-  __shared__ Shared s;
-  const int64_t r = blockIdx.x;
+__device__ __forceinline__ void whole_row(const Args& a, int64_t r, Shared& s) {
   const char* row = a.logits + r * a.ld;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // the first of the order, and whether a NaN is among the logits
@@ -339,8 +341,604 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
   before += under;
   if (w && before <= at && at < before + w) {
     a.token[r] = i;
-    if (a.logprob) a.logprob[r] = (float)(sc.distance(v) - log((double)total * (1.0 / (double)(1ull << UNIT))));
+    if (a.logprob) a.logprob[r] = logprob_of(sc.distance(v), total);
   }
+}
+
+template <int DT>
+__global__ __launch_bounds__(T) void row_kernel(const Args a) {
+  __shared__ Shared s;
+  whole_row<DT>(a, blockIdx.x, s);
+}
+
+// ------------------------------------------------------- many workgroups a row --
+
+// A row's tokens fall into bins of equal width by their distance from the top, so
+// a cut falls into one bin (of the weight's cut: a few, since the bins' weights are
+// sums of fp32 exponentials), and only what lies there has to be ordered.
+// Four launches, each a workgroup a slice of a row (the last one a row):
+//   stats      the slice's first place and least logit; clears the row's bins
+//   histogram  (with top-k or top-p) tokens and rough weight of every bin
+//   weigh      exact weight of each chunk's tokens in the bins before the cuts, of
+//              the bins that count for top-p's total only, and the list of the
+//              tokens in the cuts' bins
+//   draw       orders the list, cuts, and finds the draw's chunk and token
+// A list longer than LIST (many equal logits at a cut) leaves the row to
+// whole_row.
+// What bounds it: at one row the four launches (sums over 129280 logits take a
+// microsecond each); at many rows the exponentials, some 30 fp64 instructions a
+// logit that may be drawn or counts for a total.
+constexpr int SLICE_T = 256;
+constexpr int NBINS = 2048, FAR_BIN = NBINS - 1;  // FAR_BIN: tokens of no weight
+constexpr int LIST = 4096;
+constexpr int COUNT_SHIFT = 44;  // a bin: tokens << 44 | weight in 2^-25
+constexpr float BIN_WEIGHT = 33554432.0f;
+
+struct Part {
+  uint64_t best;
+  float least;  // of the logits above -inf
+  uint32_t pad;
+};
+struct Cuts {
+  int lo, hi;         // bins of the weight's cut (lo: those before are kept); of the count's alone both its bin
+  int kb;             // the count's bin (NBINS: none)
+  int slow;           // the list would be too long
+  int before_lo;      // tokens in the bins before lo
+  int before_kb;      // and before kb
+  int in_range;       // tokens in [lo, hi]
+  int pad;
+};
+struct RowState {
+  Cuts cuts;
+  unsigned long long sure, middle;  // weight of the bins before lo, and of those that only count for the total
+  unsigned int listed, pad[3];
+};
+
+struct Split {
+  Part* parts;                  // [rows][slices]
+  unsigned long long* bins;     // [rows][NBINS]
+  RowState* state;              // [rows]
+  unsigned long long* chunk;    // [rows][chunks]
+  unsigned long long* list;     // [rows][LIST]
+  int slices, per, chunks;      // per: chunks a slice
+  int filters;                  // top-k or top-p may cut
+};
+
+// What a row asks for.
+struct Row {
+  bool none, greedy;
+  int first, k;       // k 0: all
+  float least;
+  double p, min_p, t;
+  Scale sc;
+  float range, to_bin, to_exp;
+  __device__ __forceinline__ bool cuts() const { return k > 0 || p < 1.0; }
+};
+
+// Half the distance from the top (the whole one may not be finite).
+__device__ __forceinline__ float down(const Row& q, float v) {
+  return v == q.sc.top ? 0.0f : fmaf(-0.5f, v, 0.5f * q.sc.top);
+}
+// The bins reach as far as weights do, or the logits: below `range` they are
+// numbered from 0 to NBINS - 2.
+__device__ __forceinline__ int bin_of(const Row& q, float down) {
+  return down < q.range ? (int)(down * q.to_bin) : FAR_BIN;
+}
+
+__device__ __forceinline__ Row row_of(const Args& a, const Split& sp, int64_t r) {
+  Row q;
+  const int lane = threadIdx.x & 63;
+  uint64_t best = 0;
+  float least = __builtin_inff();
+  for (int g = lane; g < sp.slices; g += 64) {
+    const Part p = sp.parts[r * sp.slices + g];
+    best = max64(best, p.best);
+    least = fminf(least, p.least);
+  }
+  best = wave_max(best);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
+  q.sc.top = value_of((uint32_t)(best >> 32));
+  q.first = ~(int)(uint32_t)best;
+  q.t = a.temperature.of(r);
+  q.none = best == ~0ull || q.sc.top == -__builtin_inff();
+  q.greedy = !(q.t > 0.0);
+  q.sc.inv_t = 1.0 / q.t;
+  q.sc.M = (double)q.sc.top;
+  const int k = a.k_rows ? a.k_rows[r] : a.k_all;
+  q.k = k > 0 && k < a.vocab ? k : 0;
+  q.p = a.top_p.of(r);
+  q.min_p = a.min_p.of(r);
+  q.least = least;
+  // logits further than 32.25 t weigh less than 2^-46; the least one itself is within the range
+  q.range = fmaxf(fminf(16.125f * (float)q.t, down(q, least) * 1.0001f), 1e-30f);
+  q.to_bin = ((float)FAR_BIN - 0.5f) / q.range;
+  q.to_exp = (float)(-2.8853900817779268 / q.t);
+  return q;
+}
+
+// Eight logits a lane of chunk c (-inf where there is none); at(j) is the index of
+// the j-th, in pieces of 16 bytes where the rows are.
+template <int DT>
+struct Chunk {
+  float v[8];
+  int base, lane, vocab;
+  bool vec;
+  __device__ __forceinline__ int at(int j) const {
+    if (!vec) return base + 64 * j + lane;
+    return DT == KQ_DT_F32 ? base + 256 * (j >> 2) + 4 * lane + (j & 3) : base + 8 * lane + j;
+  }
+  __device__ __forceinline__ bool there(int j) const { return at(j) < vocab; }
+  __device__ __forceinline__ void load(const Args& a, const char* row, int c) {
+    base = c * CHUNK;
+    lane = threadIdx.x & 63;
+    vocab = a.vocab;
+    vec = a.vec && base + CHUNK <= vocab;
+    if (vec) {
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      if (DT == KQ_DT_F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(row + 4ll * (base + 256 * h + 4 * lane));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * h + j] = __uint_as_float(x[j]);
+        }
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(row + 2ll * (base + 8 * lane));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t h = j & 1 ? x[j >> 1] >> 16 : x[j >> 1] & 0xffffu;
+          v[j] = DT == KQ_DT_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = there(j) ? logit<DT>(row, at(j)) : -__builtin_inff();
+    }
+  }
+};
+
+template <int DT>
+__global__ __launch_bounds__(SLICE_T) void stats_kernel(const Args a, const Split sp) {
+  __shared__ Part part[SLICE_T / 64];
+  const int64_t r = blockIdx.x / sp.slices;
+  const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const char* row = a.logits + r * a.ld;
+  uint64_t best = 0;
+  float least = __builtin_inff();
+  bool nan = false;
+  const int end = min((g + 1) * sp.per, sp.chunks);
+  for (int c = g * sp.per + wave; c < end; c += SLICE_T / 64) {
+    Chunk<DT> x;
+    x.load(a, row, c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      nan |= x.v[j] != x.v[j];
+      if (x.there(j)) best = max64(best, place_of(x.v[j], x.at(j)));
+      least = x.v[j] > -__builtin_inff() ? fminf(least, x.v[j]) : least;
+    }
+  }
+  if (nan) best = ~0ull;
+  best = wave_max(best);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
+  if (lane == 0) part[wave] = Part{best, least, 0u};
+  if (sp.filters) {
+    for (int b = g * SLICE_T + threadIdx.x; b < NBINS; b += sp.slices * SLICE_T) sp.bins[r * NBINS + b] = 0;
+    if (g == 0 && threadIdx.x == 0) {
+      sp.state[r].sure = sp.state[r].middle = 0;
+      sp.state[r].listed = 0;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Part p = part[0];
+#pragma unroll
+    for (int w = 1; w < SLICE_T / 64; ++w) {
+      p.best = max64(p.best, part[w].best);
+      p.least = fminf(p.least, part[w].least);
+    }
+    sp.parts[r * sp.slices + g] = p;
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(SLICE_T) void histogram_kernel(const Args a, const Split sp) {
+  __shared__ unsigned long long bins[NBINS];
+  const int64_t r = blockIdx.x / sp.slices;
+  const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Row q = row_of(a, sp, r);
+  if (q.none || q.greedy || !q.cuts()) return;
+  for (int b = threadIdx.x; b < NBINS; b += SLICE_T) bins[b] = 0;
+  __syncthreads();
+  const char* row = a.logits + r * a.ld;
+  const int end = min((g + 1) * sp.per, sp.chunks);
+  uint64_t far = 0;
+  for (int c = g * sp.per + wave; c < end; c += SLICE_T / 64) {
+    Chunk<DT> x;
+    x.load(a, row, c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = down(q, x.v[j]);
+      const int b = bin_of(q, d);
+      if (b == FAR_BIN) {
+        far += x.there(j) ? 1 : 0;
+      } else {
+        const uint32_t w = (uint32_t)rintf(__builtin_amdgcn_exp2f(d * q.to_exp) * BIN_WEIGHT);
+        atomicAdd(&bins[b], 1ull << COUNT_SHIFT | w);
+      }
+    }
+  }
+  far = wave_sum(far);
+  if (lane == 0 && far) atomicAdd(&bins[FAR_BIN], (unsigned long long)far << COUNT_SHIFT);
+  __syncthreads();
+  for (int b = threadIdx.x; b < NBINS; b += SLICE_T)
+    if (bins[b]) atomicAdd(&sp.bins[r * NBINS + b], bins[b]);
+}
+
+// The cuts' bins from the row's histogram, by all threads of a workgroup.
+__device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const unsigned long long* bins) {
+  __shared__ uint64_t wave_total[SLICE_T / 64];
+  __shared__ int found[6];  // kb, lo, hi, tokens before kb, before lo, up to and with hi
+  __shared__ uint64_t weights[2];  // before kb, up to and with it
+  constexpr int PER = NBINS / SLICE_T;
+  constexpr uint64_t WEIGHT = (1ull << COUNT_SHIFT) - 1;
+  uint64_t v[PER], sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    v[j] = bins[threadIdx.x * PER + j];
+    sum += v[j];
+  }
+  const uint64_t upto = wave_scan(sum);
+  if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = upto;
+  if (threadIdx.x == 0) {
+    found[0] = NBINS;
+    found[1] = found[2] = FAR_BIN - 1;
+    found[3] = 0;
+  }
+  __syncthreads();
+  uint64_t before = upto - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < SLICE_T / 64; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) before += wave_total[w];
+    total += wave_total[w];
+  }
+  if (threadIdx.x == 0) weights[0] = weights[1] = total & WEIGHT;
+  __syncthreads();
+  if (q.k > 0) {
+    uint64_t at = before;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t next = at + v[j];
+      if ((int)(at >> COUNT_SHIFT) < q.k && (int)(next >> COUNT_SHIFT) >= q.k) {
+        found[0] = threadIdx.x * PER + j;
+        found[3] = (int)(at >> COUNT_SHIFT);
+        weights[0] = at & WEIGHT;
+        weights[1] = next & WEIGHT;
+      }
+      at = next;
+    }
+    __syncthreads();
+  }
+  Cuts c;
+  c.kb = found[0];
+  c.before_kb = found[3];
+  if (q.p < 1.0) {
+    // a sum of bins is off by half a unit a token, and by 2^-16 of it (the exponential and its argument in fp32)
+    const double off = 0.5 * vocab + 1.0 + ldexp((double)(total & WEIGHT), -16);
+    const double least = q.p * ((double)weights[0] - off) - off, most = q.p * ((double)weights[1] + off) + off;
+    uint64_t at = before;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t next = at + v[j];
+      const int b = threadIdx.x * PER + j;
+      const double w0 = (double)(at & WEIGHT), w1 = (double)(next & WEIGHT);
+      if (w1 >= least && (w0 < least || b == 0) && b < FAR_BIN) found[1] = b;
+      if (w1 >= most && w0 < most && b < FAR_BIN) found[2] = b;
+      at = next;
+    }
+    __syncthreads();
+    c.lo = found[1] < c.kb ? found[1] : c.kb;
+    c.hi = found[2] < c.kb ? found[2] : c.kb;
+    if (c.hi < c.lo) c.hi = c.lo;  // (equal bounds met in bins of no tokens)
+  } else {
+    c.lo = c.hi = c.kb;
+  }
+  if (c.kb == FAR_BIN) {  // tokens of no weight are not told apart
+    c.kb = NBINS;
+    if (c.lo == FAR_BIN) c.hi = FAR_BIN - 1;
+  }
+  __syncthreads();
+  uint64_t at = before;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int b = threadIdx.x * PER + j;
+    if (b == c.lo) found[4] = (int)(at >> COUNT_SHIFT);
+    at += v[j];
+    if (b == c.hi) found[5] = (int)(at >> COUNT_SHIFT);
+    if (b == c.kb) found[0] = (int)(v[j] >> COUNT_SHIFT);
+  }
+  __syncthreads();
+  c.before_lo = found[4];
+  c.in_range = c.hi >= c.lo ? found[5] - found[4] : 0;
+  c.slow = c.in_range + (c.kb < NBINS && c.kb > c.hi ? found[0] : 0) > LIST;
+  c.pad = 0;
+  return c;
+}
+
+template <int DT>
+__global__ __launch_bounds__(SLICE_T) void weigh_kernel(const Args a, const Split sp) {
+  const int64_t r = blockIdx.x / sp.slices;
+  const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Row q = row_of(a, sp, r);
+  if (q.none || q.greedy) return;
+  const bool cuts = q.cuts();
+  Cuts c{};
+  c.lo = c.kb = NBINS;
+  c.hi = NBINS - 1;
+  RowState& state = sp.state[r];
+  if (cuts) {
+    c = find_cuts(q, a.vocab, sp.bins + r * NBINS);
+    if (g == 0 && threadIdx.x == 0) state.cuts = c;
+    if (c.slow) return;
+  }
+  const char* row = a.logits + r * a.ld;
+  const int end = min((g + 1) * sp.per, sp.chunks);
+  uint64_t sure = 0, middle = 0;
+  for (int n = g * sp.per + wave; n < end; n += SLICE_T / 64) {
+    Chunk<DT> x;
+    x.load(a, row, n);
+    uint64_t kept = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = x.v[j];
+      const int b = cuts ? bin_of(q, down(q, v)) : 0;
+      const bool listed = cuts && ((b >= c.lo && b <= c.hi) || b == c.kb);
+      if (cuts) {
+        const uint64_t mask = __ballot(listed && x.there(j));
+        if (mask) {
+          unsigned int at = 0;
+          if (lane == 0) at = atomicAdd(&state.listed, (unsigned int)__popcll(mask));
+          at = __shfl(at, 0) + (unsigned int)__popcll(mask & ((1ull << lane) - 1));
+          if ((mask >> lane & 1) && at < LIST) sp.list[r * LIST + at] = place_of(v, x.at(j));
+        }
+      }
+      if (!listed && b < c.kb && b != FAR_BIN) {  // (what is after the count's bin is dropped)
+        const double w = q.sc.weight(v);
+        const uint64_t m = units(w);
+        if (b < c.lo) {
+          sure += m;
+          if (w >= q.min_p || x.at(j) == q.first) kept += m;
+        } else {
+          middle += m;
+        }
+      }
+    }
+    kept = wave_sum(kept);
+    if (lane == 0) sp.chunk[r * sp.chunks + n] = kept;
+  }
+  if (cuts && q.p < 1.0) {
+    sure = wave_sum(sure);
+    middle = wave_sum(middle);
+    if (lane == 0) {
+      if (sure) atomicAdd(&state.sure, (unsigned long long)sure);
+      if (middle) atomicAdd(&state.middle, (unsigned long long)middle);
+    }
+  }
+}
+
+// n (a power of two) places, largest first.
+__device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += T) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const bool down = !(lo & size);
+        const unsigned long long x = v[lo], y = v[hi];
+        if ((x < y) == down) {
+          v[lo] = y;
+          v[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+template <int DT>
+__global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
+  __shared__ union {
+    Shared s;
+    struct {
+      unsigned long long list[LIST];
+      unsigned long long chunk[CHUNKS];
+      uint64_t part[T / 64];
+      uint64_t found[4];
+      unsigned long long last;
+    } d;
+  } u;
+  const int64_t r = blockIdx.x;
+  const Row q = row_of(a, sp, r);
+  if (q.none || q.greedy) {
+    if (threadIdx.x == 0) {
+      a.token[r] = q.none ? -1 : q.first;
+      if (a.logprob) a.logprob[r] = q.none ? __builtin_nanf("") : 0.0f;
+    }
+    return;
+  }
+  Cuts c{};
+  c.lo = NBINS;
+  uint64_t last = 0;    // the place of the last token kept, or none of the list is
+  bool any = false;
+  auto& d = u.d;
+  if (q.cuts()) {
+    c = sp.state[r].cuts;
+    if (c.slow) {
+      whole_row<DT>(a, r, u.s);
+      return;
+    }
+  }
+  for (int i = threadIdx.x; i < sp.chunks; i += T) d.chunk[i] = sp.chunk[r * sp.chunks + i];
+  if (threadIdx.x == 0) d.last = ~0ull;
+  __syncthreads();
+  auto scan = [&](uint64_t v, uint64_t& before) {
+    const uint64_t upto = wave_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) d.part[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    uint64_t total = 0, below = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+      if (w < (int)(threadIdx.x >> 6)) below += d.part[w];
+      total += d.part[w];
+    }
+    before = below + upto - v;
+    return total;
+  };
+  const int listed = q.cuts() ? (int)min(sp.state[r].listed, (unsigned int)LIST) : 0;
+  if (listed) {
+    int n = 2;
+    while (n < listed) n <<= 1;
+    for (int i = threadIdx.x; i < n; i += T) d.list[i] = i < listed ? sp.list[r * LIST + i] : 0ull;
+    sort_down(d.list, n);
+    // thread t holds places PER t .. in the order
+    const int per = n > T ? n / T : 1;
+    uint64_t m[LIST / T], sum = 0;
+    double w[LIST / T];
+    auto position = [&](int j) { return j < c.in_range ? c.before_lo + j : c.before_kb + j - c.in_range; };
+#pragma unroll
+    for (int i = 0; i < LIST / T; ++i) {
+      const int j = (int)threadIdx.x * per + i;
+      m[i] = 0;
+      w[i] = 0.0;
+      if (i < per && j < listed) {
+        w[i] = q.sc.weight(value_of((uint32_t)(d.list[j] >> 32)));
+        if (q.k == 0 || position(j) < q.k) m[i] = units(w[i]);
+        sum += m[i];
+      }
+    }
+    uint64_t before;
+    const uint64_t allowed = scan(sum, before);
+    uint64_t target = ~0ull, at = before;
+    if (q.p < 1.0) {
+      target = nucleus(q.p, sp.state[r].sure + sp.state[r].middle + allowed);
+      at += sp.state[r].sure;
+    }
+#pragma unroll
+    for (int i = 0; i < LIST / T; ++i) {
+      const int j = (int)threadIdx.x * per + i;
+      if (i < per && j < listed) {
+        const int pos = position(j);
+        const bool keep = pos == 0 || ((q.k == 0 || pos < q.k) && at < target && (q.p >= 1.0 || j < c.in_range));
+        if (keep) {
+          const uint64_t place = d.list[j];
+          const int index = ~(int)(uint32_t)place;
+          atomicMin(&d.last, (unsigned long long)place);
+          if (m[i] && (w[i] >= q.min_p || index == q.first)) atomicAdd(&d.chunk[index / CHUNK], (unsigned long long)m[i]);
+        }
+        at += m[i];
+      }
+    }
+    __syncthreads();
+    last = d.last;
+    any = last != ~0ull;
+  }
+  auto kept = [&](float v, int i, double w) {
+    const bool in = any ? place_of(v, i) >= last : c.lo >= NBINS || bin_of(q, down(q, v)) < c.lo;
+    return in && (w >= q.min_p || i == q.first);
+  };
+  uint64_t before;
+  const uint64_t mine = (int)threadIdx.x < sp.chunks ? d.chunk[threadIdx.x] : 0;
+  const uint64_t total = scan(mine, before);
+  const uint64_t at = drawn_weight((double)a.uniform[r], total);
+  __syncthreads();
+  if (mine && before <= at && at < before + mine) {
+    d.found[0] = threadIdx.x;
+    d.found[1] = before;
+  }
+  __syncthreads();
+  const int i = (int)d.found[0] * CHUNK + (int)threadIdx.x;
+  const uint64_t under = d.found[1];
+  uint64_t w = 0;
+  float v = 0.0f;
+  if ((int)threadIdx.x < CHUNK && i < a.vocab) {
+    v = logit<DT>(a.logits + r * a.ld, i);
+    const double e = q.sc.weight(v);
+    if (kept(v, i, e)) w = units(e);
+  }
+  scan(w, before);
+  before += under;
+  if (w && before <= at && at < before + w) {
+    a.token[r] = i;
+    if (a.logprob) a.logprob[r] = logprob_of(q.sc.distance(v), total);
+  }
+}
+
+constexpr int WHOLE_VOCAB = 4096;  // rows of at most this many tokens take one workgroup
+
+struct Plan {
+  int chunks, per, slices;
+  int64_t parts, bins, state, chunk, list, bytes;  // offsets of the workspace's pieces
+};
+
+// Slices of a row: some four workgroups a CU in all, and a chunk a wave at least.
+static Plan plan(int64_t rows, int64_t vocab, bool filters) {
+  Plan p{};
+  p.chunks = (int)((vocab + CHUNK - 1) / CHUNK);
+  const int waves = SLICE_T / 64;
+  const int64_t most = 1024 / rows < 1 ? 1 : 1024 / rows;
+  int64_t slices = (p.chunks + waves - 1) / waves;
+  if (slices > most) slices = most;
+  p.per = (int)((p.chunks + slices - 1) / slices);
+  p.per = (p.per + waves - 1) / waves * waves;
+  p.slices = (p.chunks + p.per - 1) / p.per;
+  int64_t at = 0;
+  auto take = [&](int64_t n) {
+    const int64_t was = at;
+    at += (n + 255) & ~(int64_t)255;
+    return was;
+  };
+  p.parts = take(rows * p.slices * (int64_t)sizeof(Part));
+  p.chunk = take(rows * p.chunks * 8);
+  p.state = take(rows * (int64_t)sizeof(RowState));
+  p.bins = take(filters ? rows * NBINS * 8 : 0);
+  p.list = take(filters ? rows * LIST * 8 : 0);
+  p.bytes = at;
+  return p;
+}
+
+template <int DT>
+static hipError_t launch(const Args& a, int64_t rows, bool filters, char* ws, hipStream_t st) {
+  if (!ws) {
+    row_kernel<DT><<<(unsigned)rows, T, 0, st>>>(a);
+    return hipGetLastError();
+  }
+  const Plan p = plan(rows, a.vocab, filters);
+  const Split sp{(Part*)(ws + p.parts),
+                 (unsigned long long*)(ws + p.bins),
+                 (RowState*)(ws + p.state),
+                 (unsigned long long*)(ws + p.chunk),
+                 (unsigned long long*)(ws + p.list),
+                 p.slices,
+                 p.per,
+                 p.chunks,
+                 filters};
+  const unsigned grid = (unsigned)(rows * p.slices);
+  stats_kernel<DT><<<grid, SLICE_T, 0, st>>>(a, sp);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && filters) {
+    histogram_kernel<DT><<<grid, SLICE_T, 0, st>>>(a, sp);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess) {
+    weigh_kernel<DT><<<grid, SLICE_T, 0, st>>>(a, sp);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess) {
+    draw_kernel<DT><<<(unsigned)rows, T, 0, st>>>(a, sp);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 }  // namespace sample
@@ -348,25 +946,35 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
 
 using namespace kq;
 
+extern "C" int64_t kq_sample_tokens_workspace_size(int64_t rows, int64_t vocab, int filters) {
+  if (rows < 0 || vocab < 1 || vocab > sample::MAX_VOCAB) return -1;
+  if (rows == 0 || vocab <= sample::WHOLE_VOCAB) return 0;
+  return sample::plan(rows, vocab, filters != 0).bytes;
+}
+
 extern "C" int kq_sample_tokens(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* uniform,
                                 const float* temperature_rows, double temperature, const int* top_k_rows, int64_t top_k,
                                 const float* top_p_rows, double top_p, const float* min_p_rows, double min_p,
-                                int64_t* tokens, float* logprobs, void* stream) {
+                                int64_t* tokens, float* logprobs, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* fn = "kq_sample_tokens";
   if (dtype != KQ_DT_BF16 && dtype != KQ_DT_F16 && dtype != KQ_DT_F32)
     return kq_fail(KQ_ERR_INVALID, "%s: dtype must be bf16, f16 or f32", fn);
   if (rows < 0 || vocab < 1 || ld < vocab)
     return kq_fail(KQ_ERR_INVALID, "%s: need rows >= 0, vocab >= 1, a row stride of at least vocab (rows=%lld vocab=%lld ld=%lld)",
                    fn, (long long)rows, (long long)vocab, (long long)ld);
-  if (vocab > sample::MAX_VOCAB || rows > INT32_MAX)
-    return kq_fail(KQ_ERR_LIMIT, "%s: at most %d tokens in the vocabulary and 2^31 - 1 rows", fn, sample::MAX_VOCAB);
+  if (vocab > sample::MAX_VOCAB || rows > (1 << 20))
+    return kq_fail(KQ_ERR_LIMIT, "%s: at most %d tokens in the vocabulary and 2^20 rows", fn, sample::MAX_VOCAB);
   if (rows == 0) return KQ_OK;
   if (!logits || !uniform || !tokens) return kq_fail(KQ_ERR_INVALID, "%s: null buffer", fn);
   const int es = dtype == KQ_DT_F32 ? 4 : 2;
   if (kq_misaligned(logits, es) || kq_misaligned(uniform, 4) || kq_misaligned(tokens, 8) || kq_misaligned(logprobs, 4) ||
       kq_misaligned(temperature_rows, 4) || kq_misaligned(top_k_rows, 4) || kq_misaligned(top_p_rows, 4) ||
-      kq_misaligned(min_p_rows, 4))
-    return kq_fail(KQ_ERR_INVALID, "%s: buffers must be aligned to their type", fn);
+      kq_misaligned(min_p_rows, 4) || kq_misaligned(workspace, 16))
+    return kq_fail(KQ_ERR_INVALID, "%s: buffers must be aligned to their type, the workspace 16", fn);
+  const bool filters = top_k_rows || top_k > 0 || top_p_rows || top_p < 1.0;
+  const int64_t need = kq_sample_tokens_workspace_size(rows, vocab, filters);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes", fn, (long long)need);
   sample::Args a{};
   a.logits = (const char*)logits;
   a.ld = ld * es;
@@ -381,8 +989,9 @@ extern "C" int kq_sample_tokens(int dtype, const void* logits, int64_t ld, int64
   a.token = tokens;
   a.logprob = logprobs;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == KQ_DT_BF16) sample::row_kernel<KQ_DT_BF16><<<(unsigned)rows, sample::T, 0, st>>>(a);
-  else if (dtype == KQ_DT_F16) sample::row_kernel<KQ_DT_F16><<<(unsigned)rows, sample::T, 0, st>>>(a);
-  else sample::row_kernel<KQ_DT_F32><<<(unsigned)rows, sample::T, 0, st>>>(a);
-  return kq_check_launch(hipGetLastError(), fn);
+  char* ws = need > 0 ? (char*)workspace : nullptr;
+  const hipError_t e = dtype == KQ_DT_BF16  ? sample::launch<KQ_DT_BF16>(a, rows, filters, ws, st)
+                       : dtype == KQ_DT_F16 ? sample::launch<KQ_DT_F16>(a, rows, filters, ws, st)
+                                            : sample::launch<KQ_DT_F32>(a, rows, filters, ws, st);
+  return kq_check_launch(e, fn);
 }

@@ -95,9 +95,13 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
             k_rows = k_rows.clamp(0, MAX_VOCAB).to(torch.int32)
         tokens = torch.empty(rows, dtype=torch.int64, device=gpu)
         logprobs = torch.empty(rows, dtype=torch.float32, device=gpu) if return_logprobs else None
+        filters = k_rows is not None or k > 0 or p_rows is not None or p < 1
+        need = int(N.library().kq_sample_tokens_workspace_size(rows, vocab, filters))
+        ws = torch.empty(need, dtype=torch.uint8, device=gpu) if need > 0 else None
         N.call("kq_sample_tokens", N.DTYPE_CODES[z.dtype], N.ptr(z), max(z.stride(0), vocab), rows, vocab, N.ptr(u),
                N.ptr(t_rows), float(t), N.ptr(k_rows), max(0, min(int(k), MAX_VOCAB)), N.ptr(p_rows), float(p),
-               N.ptr(m_rows), float(m), N.ptr(tokens), N.ptr(logprobs), N.stream(gpu))
+               N.ptr(m_rows), float(m), N.ptr(tokens), N.ptr(logprobs), N.ptr(ws), max(need, 0),
+               N.stream(gpu))
     tokens = tokens.reshape(lead)
     if not return_logprobs:
         return tokens if host is None else tokens.to(host)

@@ -206,3 +206,40 @@ def test_strides_and_shapes(gpu):
     assert sample_tokens(base[0], u[0]).shape == ()
     assert sample_tokens(base[:0], u[:0]).shape == (0,)
     assert torch.equal(sample_tokens(base.cpu(), u.cpu(), top_k=9), sample_tokens(base, u, top_k=9).cpu())
+
+
+@pytest.mark.parametrize("m", [1, 3, 70, 1100])
+@pytest.mark.parametrize("vocab", [4097, 5003, 8192])
+def test_many_slices(gpu, m, vocab):
+    """One slice a row and many; chunks and pieces that end inside the row."""
+    for dtype in DTYPES[:2]:
+        z, u = rows(m, vocab, dtype, gpu, m)
+        for settings in ({"top_k": 40, "top_p": 0.9}, {"temperature": 0.8, "min_p": 0.001}):
+            check(z[:70], u[:70], **settings)
+            all_rows = sample_tokens(z, u, **settings)
+            assert torch.equal(all_rows[-70:], sample_tokens(z[-70:], u[-70:], **settings))
+
+
+@pytest.mark.parametrize("settings", [{"top_k": 5000}, {"top_p": 0.5}, {"top_k": 20000, "top_p": 0.7}, {"top_k": 9000, "min_p": 0.1}],
+                         ids=str)
+def test_long_lists(gpu, settings):
+    """More equal logits at a cut than a list holds."""
+    g = torch.Generator(device=gpu).manual_seed(11)
+    z = torch.zeros(6, 40001, device=gpu)
+    z[1, ::2] = -1.0
+    z[2] = torch.randint(-1, 2, (40001,), generator=g, device=gpu).float()
+    z[3, :8000] = -1e-7
+    z[4] = -torch.arange(40001, device=gpu) // 4096
+    z[5, 30000:] = 9.0
+    check(z, torch.rand(6, generator=g, device=gpu), **settings)
+
+
+def test_cuts_at_every_place(gpu):
+    """Every top_k around a list's and a bin's ends, and a row of shares for top_p."""
+    z, _ = rows(1, 6000, torch.bfloat16, gpu, 13)
+    k = torch.cat([torch.arange(1, 300, device=gpu), torch.arange(5900, 6002, device=gpu)])
+    u = torch.rand(k.numel(), generator=torch.Generator(device=gpu).manual_seed(1), device=gpu)
+    check(z.expand(k.numel(), 6000), u, top_k=k)
+    p = torch.linspace(0.0005, 0.9995, 301, device=gpu)
+    check(z.expand(301, 6000), u[:301], top_p=p)
+    check(z.expand(301, 6000), u[:301], top_p=p, top_k=k[:301] * 3)

@@ -187,7 +187,7 @@ def test_grouped_c_entry():
 
 
 def test_sample_c_entry():
-    ok = [N.DT_F32, P, 100, 4, 100, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None]
+    ok = [N.DT_F32, P, 100, 4, 100, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None, 0, None]
     cases = [(0, N.DT_I8, INVALID, b"dtype"), (2, 99, INVALID, b"row stride"), (3, -1, INVALID, b"rows >= 0"),
              (4, 0, INVALID, b"vocab >= 1"), (1, None, INVALID, b"null"), (5, None, INVALID, b"null"), (14, None, INVALID, b"null"),
              (1, ODD, INVALID, b"aligned"), (6, ODD, INVALID, b"aligned"), (8, ODD, INVALID, b"aligned"), (10, ODD, INVALID, b"aligned"),
@@ -195,4 +195,11 @@ def test_sample_c_entry():
     refused("kq_sample_tokens", ok, cases)
     wide = list(ok)
     wide[2] = wide[4] = (1 << 18) + 1
-    refused("kq_sample_tokens", wide, [(3, 4, LIMIT, b"262144")])
+    refused("kq_sample_tokens", wide, [(3, 4, LIMIT, b"262144"), (3, (1 << 20) + 1, LIMIT, b"2^20 rows")])
+    wide[2] = wide[4] = 50257
+    lib = N.library()
+    small, large = (lib.kq_sample_tokens_workspace_size(4, 50257, f) for f in (0, 1))
+    assert 0 < small < large and lib.kq_sample_tokens_workspace_size(4, 100, 1) == 0
+    wide[16], wide[17] = P, small
+    refused("kq_sample_tokens", wide, [(9, 5, INVALID, b"workspace needs"), (11, 0.5, INVALID, b"workspace needs"),
+                                       (17, small - 1, INVALID, b"workspace needs"), (16, ODD, INVALID, b"aligned")])
