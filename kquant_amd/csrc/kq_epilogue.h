@@ -58,6 +58,28 @@ __device__ __forceinline__ float epi_activate(const Epilogue& e, float x) {
   return x;
 }
 
+// The same for results in 16 bits: the hardware's exponential and reciprocal as
+// they are (a few 2^-24 of |x|; epi_activate corrects the exponential's argument).
+template <int KIND>
+__device__ __forceinline__ float epi_activate16(const Epilogue& e, float x) {
+  if (KIND == EPI_SIGMOID) {
+    constexpr float L2E = -1.44269502f;
+    const float t = x * fmaf(e.c3 * L2E, fminf(x * x, 1e30f), e.c1 * L2E);
+    return x * rcp_act(1.0f + __builtin_amdgcn_exp2f(t));
+  }
+  if (KIND == EPI_ERF) {  // as epi_activate
+    const float a = fabsf(x) * 0.70710678f;
+    const float t = rcp_act(fmaf(0.3275911f, a, 1.0f));
+    float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = fmaf(p, t, 0.5f * 1.421413741f);
+    p = fmaf(p, t, 0.5f * -0.284496736f);
+    p = fmaf(p, t, 0.5f * 0.254829592f);
+    const float tail = p * t * __builtin_amdgcn_exp2f(-1.44269502f * fminf(a * a, 200.0f));
+    return x * (x < 0.0f ? tail : 1.0f - tail);
+  }
+  return epi_activate<KIND>(e, x);
+}
+
 // the class decided at run time
 __device__ __forceinline__ float epi_activate_any(const Epilogue& e, float x) {
   return e.kind == EPI_SIGMOID ? epi_activate<EPI_SIGMOID>(e, x)

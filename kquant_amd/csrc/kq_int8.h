@@ -160,7 +160,8 @@ __device__ __forceinline__ void finish(const Finish& f, int rows, int cols, int 
   // of element (i, j, r) with row scale s
   auto value = [&](float a, float s, int j) {
     const float v = (float)__float_as_int(a) * s * sw[j];
-    return EPI != EPI_OFF ? epi_activate<EPI>(f.epi, v + bias[j]) : v;
+    if (EPI == EPI_OFF) return v;
+    return OUT == KQ_DT_F32 ? epi_activate<EPI>(f.epi, v + bias[j]) : epi_activate16<EPI>(f.epi, v + bias[j]);
   };
   auto scale_of = [&](int i, int r) { return __shfl(sx[i / 2], 32 * (i & 1) + 8 * (r >> 2) + (r & 3) + half); };
   const bool residual = EPI != EPI_OFF && f.epi.residual;

@@ -87,9 +87,19 @@ static hipError_t dense(DenseArgs g, hipStream_t st) {
   if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   if (e != hipSuccess) return e;
   const int grid = cus >= 8 ? cus / 8 * 8 : 8;
-  g.tm = 256;
-  g.mtiles = (g.m + g.tm - 1) / g.tm;
+  // A step of a tile takes its loads' way from L2 besides its products: at K = 7168 a round of tiles of 32 / 64 / 128 /
+  // 256 rows takes 28 / 35 / 52 / 77 us, so 88 + rows.  The height with the shortest rounds in all (256 x 12288: 80 us in
+  // 48 tiles of 256 rows, 39 in 192 of 64; 512 rows 93 and 57 of 128; 1024 rows 94, 107 and 109).
   g.ntiles = (g.n + mm16::BN - 1) / mm16::BN;
+  int64_t least = 0;
+  for (int tm : {32, 64, 96, 128, 256}) {
+    const int64_t tiles = ((int64_t)g.m + tm - 1) / tm * g.ntiles, cost = (tiles + grid - 1) / grid * (88 + tm);
+    if (least == 0 || cost <= least) {
+      least = cost;
+      g.tm = tm;
+    }
+  }
+  g.mtiles = (g.m + g.tm - 1) / g.tm;
   auto kern = g.epi.kind == EPI_OFF       ? dense_kernel<OUT, EPI_OFF>
               : g.epi.kind == EPI_CLAMP   ? dense_kernel<OUT, EPI_CLAMP>
               : g.epi.kind == EPI_SIGMOID ? dense_kernel<OUT, EPI_SIGMOID>

@@ -580,6 +580,7 @@ struct Core {
         if (tl.rows <= 128) {
           if (tl.rows <= 32) item<1, 2>(tl, i, 0, 64 * lw);
           else if (tl.rows <= 64) item<2, 2>(tl, i, 0, 64 * lw);
+          else if (KIND == I8 && tl.rows <= 96) item<KIND == I8 ? 3 : 4, 2>(tl, i, 0, 64 * lw);
           else item<4, 2>(tl, i, 0, 64 * lw);
           continue;
         }
