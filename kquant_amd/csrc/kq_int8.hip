@@ -355,15 +355,43 @@ static hipError_t launch_few(FewArgs f, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Row blocks of weights a workgroup (R) and windows in flight a wave.  Cold weights, K = 7168, us by N:
+//   rows       N = 12288             24576             129280
+//   1     R 1  20.4          R 1, 2  28.8, 28.8        135, 132     (R 4: 20, 33, 142)
+//   16    R 1  21.8          R 1, 2  39.0, 33.0        202, 160     (R 4, one window: 20.7, 37, 153)
+//   32    R 1, 4  32.6, 24.8         61.0, 46.8        304, 191
+//   64    R 1, 4  61.3, 34.5         119, 65.6         617, 275
+// A block's reads of the activations (from L2) are shared by its R blocks; four need
+// enough workgroups to cover the CUs (N = 4096: 19.7 and 23.0 at 32 rows).
 template <int DT, int OUT, bool TAIL>
 static hipError_t few_rows(const FewArgs& f, hipStream_t st) {
   if constexpr (DT != DT_CODES) {
+    if (f.n >= 24576) return launch_few<DT, OUT, 1, 2, 2, TAIL>(f, st);
     return launch_few<DT, OUT, 1, 1, 2, TAIL>(f, st);
   } else {
-    if (f.m <= 16) return launch_few<DT, OUT, 1, 1, 2, TAIL>(f, st);
-    if (f.m <= 32) return launch_few<DT, OUT, 2, 1, 2, TAIL>(f, st);
+    if (f.m <= 16) {
+      if (f.n >= 24576) return launch_few<DT, OUT, 1, 2, 2, TAIL>(f, st);
+      return launch_few<DT, OUT, 1, 1, 2, TAIL>(f, st);
+    }
+    if (f.m <= 32) {
+      if (f.n >= 8192) return launch_few<DT, OUT, 2, 4, 2, TAIL>(f, st);
+      return launch_few<DT, OUT, 2, 1, 2, TAIL>(f, st);
+    }
+    if (f.n >= 8192) return launch_few<DT, OUT, 4, 4, 1, TAIL>(f, st);
     return launch_few<DT, OUT, 4, 1, 2, TAIL>(f, st);
   }
+}
+
+// Whether up to FEW rows take the one-pass kernel or the tiles, where the weights
+// are wide: the first reads them at 4.8 (32 rows) or 3.4 TB/s (64), the activations'
+// reads beside them; the tiles at 5.9, in rounds of 0.9 us a step while they come
+// from memory (N = 129280, 32 / 64 rows: 191 / 275 and 158 / 161 us; 24576 47 / 66 and 55 / 51).
+static bool takes_few(int64_t m, int64_t n, int64_t k, int64_t cus) {
+  if (m > FEW) return false;
+  if (m <= 16) return true;
+  const double bytes = (double)n * (double)k, few = bytes / (m <= 32 ? 4.8e6 : 3.4e6);
+  const double rounds = (double)(((n + mm16::BN - 1) / mm16::BN + cus - 1) / cus) * 0.9 * (double)((k + 127) / 128);
+  return few <= (rounds > bytes / 5.9e6 ? rounds : bytes / 5.9e6);
 }
 
 static inline int64_t up16(int64_t v) { return (v + 15) & ~(int64_t)15; }
@@ -468,7 +496,14 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
   } else if (!codes) {
     ld = lda * (a_dtype == KQ_DT_F32 ? 4 : 2);
   }
-  if (m <= FEW) {
+  int cus = 0;
+  if (m > 16 && m <= FEW) {
+    int dev = 0;
+    hipError_t err = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
+    if (err == hipSuccess) err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+    if (err != hipSuccess) return kq_check_launch(err, fn);
+  }
+  if (takes_few(m, n, k, cus > 0 ? cus : 1)) {
     const FewArgs f{rows, ld, sx, w, w_scale, c, ldc, (int)m, (int)n, (int)k, 1, e};
     const int dt = fused ? a_dtype : KQ_DT_I8;
     const hipError_t err = out_dtype == KQ_DT_BF16  ? few<KQ_DT_BF16>(dt, f, st)

@@ -156,8 +156,7 @@ def int8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tens
         raise TypeError("out_dtype must be bfloat16, float16 or float32")
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("int8_grouped_linear carries no gradient: detach x or call it under torch.no_grad()")
-    given = [x, weight, scale, x_scale, offsets]
-    (a, w, s, sx, offsets), gpu, host = N.to_gpu([None if t is None else t.detach() for t in given])
+    (a, w, s, sx, offsets), gpu, host = N.to_gpu((x, weight, scale, x_scale, offsets))
     a, s = _row_view(a), N.aligned(s, 4)
     kp = -(-k // INT8_K_ALIGN) * INT8_K_ALIGN
     w = N.aligned(_pad_k(w, kp))

@@ -17,7 +17,7 @@ INT8_K_ALIGN = 16            # the products' K granule
 
 def _row_view(x: torch.Tensor) -> torch.Tensor:
     """[..., K] as [rows, K] with unit column stride and rows that do not overlap (copied where they do)."""
-    a = x.reshape(-1, x.shape[-1])
+    a = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
     if a.stride(1) != 1 or (a.shape[0] > 1 and a.stride(0) < a.shape[1]):
         a = a.contiguous()
     return a
@@ -55,11 +55,12 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
     if x.ndim < 1 or x.shape[-1] == 0:
         raise ValueError("x must have a feature dimension")
-    (a,), gpu, host = N.to_gpu([x.detach()])
+    (a,), gpu, host = N.to_gpu([x])
     a = _row_view(a)
     with N.on_device(gpu):
         q, scale = _quantize(a, a.shape[1])
-    q, scale = q.reshape(x.shape), scale.reshape(x.shape[:-1])
+    if x.ndim != 2:
+        q, scale = q.reshape(x.shape), scale.reshape(x.shape[:-1])
     return (q, scale) if host is None else (q.to(host), scale.to(host))
 
 

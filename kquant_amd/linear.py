@@ -274,31 +274,34 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
         raise TypeError("out_dtype must be bfloat16, float16 or float32")
     n, lead = weight.shape[0], source.shape[:-1]
     _check_epilogue(source, bias, activation, residual, lead, n, False, out_dtype)
-    given = [source, weight, scale, source_scale, bias, residual]
-    (a, w, s, sx, bias, residual), gpu, host = N.to_gpu([None if t is None else t.detach() for t in given])
+    (a, w, s, sx, bias, residual), gpu, host = N.to_gpu((source, weight, scale, source_scale, bias, residual))
     a, s = _row_view(a), N.aligned(s, 4)
     kp = -(-k // INT8_K_ALIGN) * INT8_K_ALIGN
     w = N.aligned(_pad_codes(w, kp))
     m = a.shape[0]
     with N.on_device(gpu):
+        ws, need = None, 0
         if sx is not None:
-            sx = N.aligned(sx.reshape(-1), 4)
+            sx = N.aligned(sx if sx.ndim == 1 else sx.reshape(-1), 4)
             a = _pad_codes(a, kp)
             if a.data_ptr() % 16 or _row_stride(a) % 16 or _row_stride(a) > 1 << 22:
                 a = a.clone(memory_format=torch.contiguous_format)
         elif kp != k:
             a, sx = _quantize(a, kp)
+        code = N.DT_I8 if sx is not None else N.DTYPE_CODES[a.dtype]
+        if sx is None:
+            need = N.library().kq_int8_linear_workspace_size(code, m, n, kp)
+            if need > 0:
+                ws = torch.empty(need, dtype=torch.uint8, device=gpu)
         if bias is not None:
             bias = bias.contiguous()
         if residual is not None:
             residual = _row_view(residual)
-        code = N.DT_I8 if a.dtype == torch.int8 else N.DTYPE_CODES[a.dtype]
-        need = int(N.library().kq_int8_linear_workspace_size(code, m, n, kp))
-        ws = torch.empty(need, dtype=torch.uint8, device=gpu) if need > 0 else None
-        out = torch.empty(m, n, dtype=out_dtype, device=gpu)
-        N.call("kq_int8_linear", code, N.ptr(a), _row_stride(a), N.ptr(sx), N.ptr(w), N.ptr(s), m, n, kp,
-               N.LIN_ACTIVATIONS[activation], N.ptr(bias), N.DT_BF16 if bias is None else N.DTYPE_CODES[bias.dtype],
-               N.ptr(residual), n if residual is None else _row_stride(residual), N.DTYPE_CODES[out_dtype], N.ptr(out), n,
-               N.ptr(ws), max(need, 0), N.stream(gpu))
-    out = out.reshape(*lead, n)
+        out = torch.empty((m, n), dtype=out_dtype, device=gpu)
+        N.call("kq_int8_linear", code, a.data_ptr(), _row_stride(a), N.ptr(sx), w.data_ptr(), s.data_ptr(), m, n, kp,
+               N.LIN_ACTIVATIONS[activation], N.ptr(bias), 0 if bias is None else N.DTYPE_CODES[bias.dtype],
+               N.ptr(residual), n if residual is None else _row_stride(residual), N.DTYPE_CODES[out_dtype],
+               out.data_ptr(), n, N.ptr(ws), need, N.stream(gpu))
+    if source.ndim != 2:
+        out = out.reshape(*lead, n)
     return out if host is None else out.to(host)

@@ -16,6 +16,10 @@ from . import _native as N
 MAX_VOCAB = 1 << 18
 
 
+def _flat(v: torch.Tensor) -> torch.Tensor:
+    return N.aligned(v if v.ndim == 1 else v.reshape(-1), 4)
+
+
 def _setting(name: str, value, lead, default: float, check) -> tuple[torch.Tensor | None, float]:
     """(one value a row or None, one for all)."""
     if value is None:
@@ -81,29 +85,30 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
     k_rows, k = _setting("top_k", top_k, lead, 0, lambda v: v == int(v))
     p_rows, p = _setting("top_p", top_p, lead, 1.0, lambda v: 0 < v <= 1)
     m_rows, m = _setting("min_p", min_p, lead, 0.0, lambda v: 0 <= v <= 1)
+    k = max(0, min(int(k), MAX_VOCAB))
     if temperature is None:
         raise TypeError("temperature must be a number or a tensor with a value for each row")
-    z = logits.detach().reshape(-1, vocab)
-    (z, u, t_rows, k_rows, p_rows, m_rows), gpu, host = N.to_gpu([z, uniform, t_rows, k_rows, p_rows, m_rows])
-    rows = z.shape[0]
-    if z.stride(1) != 1 or (rows > 1 and z.stride(0) < vocab):
-        z = z.contiguous()
+    (z, u, t_rows, k_rows, p_rows, m_rows), gpu, host = N.to_gpu((logits, uniform, t_rows, k_rows, p_rows, m_rows))
+    if z.ndim != 2:
+        z = z.reshape(-1, vocab)
+    rows, ld = z.shape[0], z.stride(0)
+    if z.stride(1) != 1 or ld < vocab:
+        if rows > 1 or z.stride(1) != 1:
+            z = z.contiguous()
+        ld = vocab
     with N.on_device(gpu):
-        flat = [None if v is None else N.aligned(v.reshape(-1), 4) for v in (u, t_rows, k_rows, p_rows, m_rows)]
-        u, t_rows, k_rows, p_rows, m_rows = flat
-        if k_rows is not None and k_rows.dtype != torch.int32:
-            k_rows = k_rows.clamp(0, MAX_VOCAB).to(torch.int32)
-        tokens = torch.empty(rows, dtype=torch.int64, device=gpu)
-        logprobs = torch.empty(rows, dtype=torch.float32, device=gpu) if return_logprobs else None
+        u = _flat(u)
+        if k_rows is not None:
+            k_rows = _flat(k_rows if k_rows.dtype == torch.int32 else k_rows.clamp(0, MAX_VOCAB).to(torch.int32))
+        t_rows, p_rows, m_rows = (None if v is None else _flat(v) for v in (t_rows, p_rows, m_rows))
         filters = k_rows is not None or k > 0 or p_rows is not None or p < 1
-        need = int(N.library().kq_sample_tokens_workspace_size(rows, vocab, filters))
+        need = N.library().kq_sample_tokens_workspace_size(rows, vocab, filters)
         ws = torch.empty(need, dtype=torch.uint8, device=gpu) if need > 0 else None
-        N.call("kq_sample_tokens", N.DTYPE_CODES[z.dtype], N.ptr(z), max(z.stride(0), vocab), rows, vocab, N.ptr(u),
-               N.ptr(t_rows), float(t), N.ptr(k_rows), max(0, min(int(k), MAX_VOCAB)), N.ptr(p_rows), float(p),
-               N.ptr(m_rows), float(m), N.ptr(tokens), N.ptr(logprobs), N.ptr(ws), max(need, 0),
-               N.stream(gpu))
-    tokens = tokens.reshape(lead)
-    if not return_logprobs:
-        return tokens if host is None else tokens.to(host)
-    logprobs = logprobs.reshape(lead)
-    return (tokens, logprobs) if host is None else (tokens.to(host), logprobs.to(host))
+        tokens = torch.empty(lead, dtype=torch.int64, device=gpu)
+        logprobs = torch.empty(lead, dtype=torch.float32, device=gpu) if return_logprobs else None
+        N.call("kq_sample_tokens", N.DTYPE_CODES[z.dtype], z.data_ptr(), ld, rows, vocab, u.data_ptr(), N.ptr(t_rows), t,
+               N.ptr(k_rows), k, N.ptr(p_rows), p, N.ptr(m_rows), m, tokens.data_ptr(), N.ptr(logprobs), N.ptr(ws),
+               max(need, 0), N.stream(gpu))
+    if host is not None:
+        tokens, logprobs = tokens.to(host), None if logprobs is None else logprobs.to(host)
+    return (tokens, logprobs) if return_logprobs else tokens
