@@ -23,9 +23,8 @@ namespace sample {
 
 constexpr int MAX_VOCAB = 1 << 18;  // sums of weights stay below 2^63
 constexpr int UNIT = 45;            // a weight of 1 is 2^UNIT
-constexpr double FAR = -33.0;       // exp(FAR) rounds to 0 units
 constexpr int CHUNK = 512;          // tokens whose kept weight is summed on its own
-constexpr int CHUNKS = MAX_VOCAB / CHUNK;
+constexpr int CHUNKS = MAX_VOCAB / CHUNK;  // no more than a workgroup's threads
 
 // One number for all rows, or one for each.
 struct Setting {
@@ -67,43 +66,46 @@ __device__ __forceinline__ float logit(const char* row, int i) {
   return DT == KQ_DT_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
 }
 
-// exp(d) for FAR <= d <= 0 (0 below): 2^k times the Taylor sum of the rest,
-// |rest| <= ln 2 / 2, to the 12th power (the next term is below 2e-16).
-__device__ __forceinline__ double exp64(double d) {
-  if (!(d >= FAR)) return 0.0;
-  const double k = rint(d * 1.4426950408889634);
-  double r = fma(-k, 0.6931471805598903, d);  // ln 2 in two parts, the first of 43 bits: k times it is exact
-  r = fma(-k, 5.497923018708371e-14, r);
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return ldexp(p, (int)k);
-}
-
-__device__ __forceinline__ uint64_t units(double w) {
-  // the sum's mantissa is w in units, rounded to nearest
-  return (uint64_t)__double_as_longlong(fma(w, (double)(1ull << UNIT), 4503599627370496.0)) & 0xfffffffffffffull;
+// A constant in scalar registers: as an FMA's addend it needs no copy into the result's.
+__device__ __forceinline__ double scalar(double c) {
+  asm("" : "+s"(c));
+  return c;
 }
 
 // A row's logits as weights.
 struct Scale {
-  float top;        // M
-  double inv_t, M;
-  __device__ __forceinline__ double distance(float v) const {
-    return v == top ? 0.0 : ((double)v - M) * inv_t;  // (an infinite M: 0 or -inf)
+  float top;
+  double M, a;  // the top (1e300 for an infinite one) and log2(e) / t
+  __device__ __forceinline__ Scale() {}
+  __device__ __forceinline__ Scale(float m, double t)
+      : top(m), M(m == __builtin_inff() ? 1e300 : (double)m), a(fmin(1.4426950408889634 / t, 1e300)) {}
+  // log2 of a weight: 0 for the top (an infinite one too), no less than -60, which is no weight
+  __device__ __forceinline__ double log2_weight(float v) const { return fmin(fmax(((double)v - M) * a, -60.0), 0.0); }
+  // The weight in units, not rounded: 2^(k + UNIT) 2^f with |f| <= 1/2, 2^f by the polynomial of degree 10 that meets
+  // it at the Chebyshev points (within 3e-16).  Only additions, products and FMAs: they run at the full fp64 rate.
+  __device__ __forceinline__ double weight(float v) const {
+    constexpr double SHIFT = 6755399441055744.0 + UNIT;  // 1.5 2^52: k + UNIT in the low word of the sum
+    const double y = log2_weight(v), t = y + SHIFT;
+    const double f = y - (t - SHIFT);
+    double p = fma(scalar(7.072585949269223e-09), f, scalar(1.0208690299958306e-07));
+    p = fma(p, f, scalar(1.321544258792169e-06));
+    p = fma(p, f, scalar(1.5252657260200837e-05));
+    p = fma(p, f, scalar(0.0001540353044173605));
+    p = fma(p, f, scalar(0.0013333558230164974));
+    p = fma(p, f, scalar(0.009618129107606888));
+    p = fma(p, f, scalar(0.05550410866444772));
+    p = fma(p, f, scalar(0.24022650695910097));
+    p = fma(p, f, scalar(0.69314718055995));
+    p = fma(p, f, 1.0);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
   }
-  __device__ __forceinline__ double weight(float v) const { return exp64(distance(v)); }
 };
+
+// A weight rounded to whole units: the mantissa of its sum with 2^52.
+constexpr uint64_t RAW = 0x4330000000000000ull;  // the bits of 2^52
+__device__ __forceinline__ uint64_t raw_units(double w) { return (uint64_t)__double_as_longlong(w + 4503599627370496.0); }
+__device__ __forceinline__ uint64_t units(double w) { return raw_units(w) - RAW; }
+constexpr double ONE = (double)(1ull << UNIT);
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) { return __shfl((unsigned long long)v, src); }
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
@@ -162,13 +164,13 @@ __device__ __forceinline__ uint64_t drawn_weight(double u, uint64_t total) {
   return u > 0.0 ? share(u, total, rest) : 0;
 }
 
-__device__ __forceinline__ float logprob_of(double distance, uint64_t total) {
-  return (float)(distance - log((double)total * (1.0 / (double)(1ull << UNIT))));
+__device__ __forceinline__ float logprob_of(double log2_weight, uint64_t total) {
+  return (float)(log2_weight * 0.6931471805599453 - log((double)total * (1.0 / ONE)));
 }
 
 // --------------------------------------------------------- one row, whole --
 
-constexpr int T = 1024;
+constexpr int T = 512;
 constexpr int DIGIT = 11, BINS = 1 << DIGIT;
 
 struct Shared {
@@ -225,24 +227,29 @@ __device__ __forceinline__ Cut select(const char* row, int vocab, const Scale& s
       if (w) atomicAdd(&s.mass[bin], (unsigned long long)w);
     }
     __syncthreads();
-    // two bins a thread
-    const int b0 = 2 * threadIdx.x;
-    const uint64_t c0 = s.count[b0], c1 = s.count[b0 + 1], m0 = s.mass[b0], m1 = s.mass[b0 + 1];
-    uint64_t cb, mb;
-    block_scan(c0 + c1, s, cb);
-    block_scan(m0 + m1, s, mb);
+    constexpr int PER = BINS / T;
+    uint64_t c[PER], m[PER], cs = 0, ms = 0, cb, mb;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      cs += c[j] = s.count[PER * threadIdx.x + j];
+      ms += m[j] = s.mass[PER * threadIdx.x + j];
+    }
+    block_scan(cs, s, cb);
+    block_scan(ms, s, mb);
     cb += count;
     mb += mass;
-    const uint64_t want = target;
-    const uint64_t at0 = BY_COUNT ? cb : mb, v0 = BY_COUNT ? c0 : m0, v1 = BY_COUNT ? c1 : m1;
-    // the one bin in which the target is reached
-    const bool in0 = at0 < want && at0 + v0 >= want, in1 = at0 + v0 < want && at0 + v0 + v1 >= want;
     __syncthreads();
-    if (in0 || in1) {
-      s.found[0] = in0 ? b0 : b0 + 1;
-      s.found[1] = in0 ? cb : cb + c0;
-      s.found[2] = in0 ? mb : mb + m0;
-      s.found[3] = in0 ? m0 : m1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t at = BY_COUNT ? cb : mb, v = BY_COUNT ? c[j] : m[j];
+      if (at < target && at + v >= target) {  // the one bin in which the target is reached
+        s.found[0] = PER * threadIdx.x + j;
+        s.found[1] = cb;
+        s.found[2] = mb;
+        s.found[3] = m[j];
+      }
+      cb += c[j];
+      mb += m[j];
     }
     __syncthreads();
     prefix |= (~s.found[0] & ((1u << bits) - 1)) << shift;
@@ -282,9 +289,9 @@ __device__ __forceinline__ void whole_row(const Args& a, int64_t r, Shared& s) {
     }
     return;
   }
-  const Scale sc{top, 1.0 / t, (double)top};
+  const Scale sc(top, t);
   const int k = a.k_rows ? a.k_rows[r] : a.k_all;
-  const double p = a.top_p.of(r), min_p = a.min_p.of(r);
+  const double p = a.top_p.of(r), min_p = fmin(a.min_p.of(r), 1.0) * ONE;
   uint64_t last = 0;  // the place of the last token kept
   uint64_t total = 0;
   if (k > 0 && k < a.vocab) {
@@ -299,7 +306,7 @@ __device__ __forceinline__ void whole_row(const Args& a, int64_t r, Shared& s) {
   if (p < 1.0) {
     last = max64(last, select<DT, false>(row, a.vocab, sc, nucleus(p, total), s).place);
   }
-  auto kept = [&](float v, int i, double w) { return place_of(v, i) >= last && (w >= min_p || i == first); };
+  auto kept = [&](float v, int i, double w) { return place_of(v, i) >= last && w >= min_p; };
   // the kept weight of each chunk, and where the draw falls among them
   const int chunks = (a.vocab + CHUNK - 1) / CHUNK;
   for (int c = wave; c < chunks; c += T / 64) {
@@ -341,7 +348,7 @@ __device__ __forceinline__ void whole_row(const Args& a, int64_t r, Shared& s) {
   before += under;
   if (w && before <= at && at < before + w) {
     a.token[r] = i;
-    if (a.logprob) a.logprob[r] = logprob_of(sc.distance(v), total);
+    if (a.logprob) a.logprob[r] = logprob_of(sc.log2_weight(v), total);
   }
 }
 
@@ -354,22 +361,26 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
 // ------------------------------------------------------- many workgroups a row --
 
 // A row's tokens fall into bins of equal width by their distance from the top, so
-// a cut falls into one bin (of the weight's cut: a few, since the bins' weights are
-// sums of fp32 exponentials), and only what lies there has to be ordered.
+// a cut falls into one bin (with top-k the weight's cut into a few, since the bins'
+// weights are sums of fp32 exponentials then), and only what lies there has to be
+// ordered.
 // Four launches, each a workgroup a slice of a row (the last one a row):
 //   stats      the slice's first place and least logit; clears the row's bins
-//   histogram  (with top-k or top-p) tokens and rough weight of every bin
-//   weigh      exact weight of each chunk's tokens in the bins before the cuts, of
-//              the bins that count for top-p's total only, and the list of the
-//              tokens in the cuts' bins
+//   histogram  (with top-k or top-p) every bin's weight; with top-k its tokens and a
+//              rough weight, since only the bins up to the count's matter then
+//   weigh      exact weight of each chunk's tokens in the bins before the cuts, and
+//              the list of the tokens in the cuts' bins; with top-k also the weight
+//              of the bins that count for top-p's total only
 //   draw       orders the list, cuts, and finds the draw's chunk and token
 // A list longer than LIST (many equal logits at a cut) leaves the row to
 // whole_row.
 // What bounds it: at one row the four launches (sums over 129280 logits take a
 // microsecond each); at many rows the exponentials, some 30 fp64 instructions a
 // logit that may be drawn or counts for a total.
-constexpr int SLICE_T = 256;
+constexpr int SLICE_T = 512;
+constexpr int NEAR = 1024;   // listed tokens that a workgroup gathers before they go to the list
 constexpr int NBINS = 2048, FAR_BIN = NBINS - 1;  // FAR_BIN: tokens of no weight
+constexpr int BINS_EACH = NBINS / SLICE_T;        // a thread's bins where a workgroup looks through them
 constexpr int LIST = 4096;
 constexpr int COUNT_SHIFT = 44;  // a bin: tokens << 44 | weight in 2^-25
 constexpr float BIN_WEIGHT = 33554432.0f;
@@ -390,7 +401,8 @@ struct Cuts {
 };
 struct RowState {
   Cuts cuts;
-  unsigned long long sure, middle;  // weight of the bins before lo, and of those that only count for the total
+  unsigned long long sure, middle;  // with top-k: weight of the bins before lo, and of those that only count for the total
+  unsigned long long before, total; // without: of the bins before lo, and of all
   unsigned int listed, pad[3];
 };
 
@@ -407,9 +419,9 @@ struct Split {
 // What a row asks for.
 struct Row {
   bool none, greedy;
-  int first, k;       // k 0: all
-  float least;
-  double p, min_p, t;
+  int first;          // of the order, of a greedy row
+  int k;              // 0: all
+  double p, min_p;    // min_p in units, no more than the top's weight
   Scale sc;
   float range, to_bin, to_exp;
   __device__ __forceinline__ bool cuts() const { return k > 0 || p < 1.0; }
@@ -421,9 +433,10 @@ __device__ __forceinline__ float down(const Row& q, float v) {
 }
 // The bins reach as far as weights do, or the logits: below `range` they are
 // numbered from 0 to NBINS - 2.
-__device__ __forceinline__ int bin_of(const Row& q, float down) {
-  return down < q.range ? (int)(down * q.to_bin) : FAR_BIN;
+__device__ __forceinline__ float bin_place(const Row& q, float down) {
+  return down < q.range ? down * q.to_bin : (float)FAR_BIN;
 }
+__device__ __forceinline__ int bin_of(const Row& q, float down) { return (int)bin_place(q, down); }
 
 __device__ __forceinline__ Row row_of(const Args& a, const Split& sp, int64_t r) {
   Row q;
@@ -438,22 +451,20 @@ __device__ __forceinline__ Row row_of(const Args& a, const Split& sp, int64_t r)
   best = wave_max(best);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
-  q.sc.top = value_of((uint32_t)(best >> 32));
+  const float top = value_of((uint32_t)(best >> 32));
   q.first = ~(int)(uint32_t)best;
-  q.t = a.temperature.of(r);
-  q.none = best == ~0ull || q.sc.top == -__builtin_inff();
-  q.greedy = !(q.t > 0.0);
-  q.sc.inv_t = 1.0 / q.t;
-  q.sc.M = (double)q.sc.top;
+  const double t = a.temperature.of(r);
+  q.sc = Scale(top, t);
+  q.none = best == ~0ull || top == -__builtin_inff();
+  q.greedy = !(t > 0.0);
   const int k = a.k_rows ? a.k_rows[r] : a.k_all;
   q.k = k > 0 && k < a.vocab ? k : 0;
   q.p = a.top_p.of(r);
-  q.min_p = a.min_p.of(r);
-  q.least = least;
+  q.min_p = fmin(a.min_p.of(r), 1.0) * ONE;
   // logits further than 32.25 t weigh less than 2^-46; the least one itself is within the range
-  q.range = fmaxf(fminf(16.125f * (float)q.t, down(q, least) * 1.0001f), 1e-30f);
+  q.range = fmaxf(fminf(16.125f * (float)t, down(q, least) * 1.0001f), 1e-30f);
   q.to_bin = ((float)FAR_BIN - 0.5f) / q.range;
-  q.to_exp = (float)(-2.8853900817779268 / q.t);
+  q.to_exp = (float)(-2.8853900817779268 / t);
   return q;
 }
 
@@ -498,28 +509,69 @@ struct Chunk {
   }
 };
 
+// f(chunk, its number) of a wave's chunks first, first + the workgroup's waves, ... below end, with the next D chunks'
+// logits on their way; `ready`, which may end it, runs when the first ones' are.
+template <int DT, int D, class F, class R>
+__device__ __forceinline__ void for_chunks(const Args& a, const char* row, int first, int end, F&& f, R&& ready) {
+  constexpr int STEP = SLICE_T / 64;
+  Chunk<DT> x[D];
+#pragma unroll
+  for (int i = 0; i < D; ++i)
+    if (first + i * STEP < end) x[i].load(a, row, first + i * STEP);
+  if (!ready()) return;
+  // one copy of f: a kernel's code comes from memory once a CU, and costs as its data does
+#pragma nounroll
+  for (int c = first; c < end; c += STEP) {
+    const Chunk<DT> now = x[0];
+#pragma unroll
+    for (int i = 0; i + 1 < D; ++i) x[i] = x[i + 1];
+    if (c + D * STEP < end) x[D - 1].load(a, row, c + D * STEP);
+    f(now, c);
+  }
+}
+
 template <int DT>
 __global__ __launch_bounds__(SLICE_T) void stats_kernel(const Args a, const Split sp) {
   __shared__ Part part[SLICE_T / 64];
   const int64_t r = blockIdx.x / sp.slices;
   const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const char* row = a.logits + r * a.ld;
-  uint64_t best = 0;
-  float least = __builtin_inff();
+  const float inf = __builtin_inff();
+  float high = -inf, least = inf;
+  int from = -1;  // this lane's chunk with `high` first
   bool nan = false;
   const int end = min((g + 1) * sp.per, sp.chunks);
-  for (int c = g * sp.per + wave; c < end; c += SLICE_T / 64) {
-    Chunk<DT> x;
-    x.load(a, row, c);
+  // (the median with an infinity: a maximum or minimum in one instruction, without quieting its operands first)
+  auto larger = [&](float x, float y) { return __builtin_amdgcn_fmed3f(x, y, inf); };
+  auto smaller = [&](float x, float y) { return __builtin_amdgcn_fmed3f(x, y, -inf); };
+  for_chunks<DT, 4>(a, row, g * sp.per + wave, end, [&](const Chunk<DT>& x, int c) {
+    float top = x.v[0], low = x.v[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      nan |= x.v[j] != x.v[j];
-      if (x.there(j)) best = max64(best, place_of(x.v[j], x.at(j)));
-      least = x.v[j] > -__builtin_inff() ? fminf(least, x.v[j]) : least;
+    for (int j = 1; j < 8; ++j) {
+      top = larger(top, x.v[j]);
+      low = smaller(low, x.v[j]);
+      if (j & 1) nan |= __builtin_isunordered(x.v[j - 1], x.v[j]);
     }
+    if (top > high) {
+      high = top;
+      from = c;
+    }
+    if (__any(low == -inf)) {  // masked logits, or the row's end
+#pragma unroll
+      for (int j = 0; j < 8; ++j) least = x.v[j] == -inf ? least : smaller(least, x.v[j]);
+    } else {
+      least = smaller(least, low);
+    }
+  }, [] { return true; });
+  // the place itself is asked for where it is the token: a lane's tokens come in ascending order
+  int where = -1;
+  if (!(a.temperature.of(r) > 0.0) && from >= 0) {
+    Chunk<DT> x;
+    x.load(a, row, from);
+#pragma unroll
+    for (int j = 7; j >= 0; --j) where = x.v[j] == high ? x.at(j) : where;
   }
-  if (nan) best = ~0ull;
-  best = wave_max(best);
+  const uint64_t best = wave_max(nan ? ~0ull : place_of(high, where));
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
   if (lane == 0) part[wave] = Part{best, least, 0u};
@@ -547,48 +599,105 @@ __global__ __launch_bounds__(SLICE_T) void histogram_kernel(const Args a, const 
   __shared__ unsigned long long bins[NBINS];
   const int64_t r = blockIdx.x / sp.slices;
   const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Row q = row_of(a, sp, r);
-  if (q.none || q.greedy || !q.cuts()) return;
-  for (int b = threadIdx.x; b < NBINS; b += SLICE_T) bins[b] = 0;
-  __syncthreads();
   const char* row = a.logits + r * a.ld;
   const int end = min((g + 1) * sp.per, sp.chunks);
+  Row q;
   uint64_t far = 0;
-  for (int c = g * sp.per + wave; c < end; c += SLICE_T / 64) {
-    Chunk<DT> x;
-    x.load(a, row, c);
+  bool run = false;
+  for_chunks<DT, 2>(
+      a, row, g * sp.per + wave, end,
+      [&](const Chunk<DT>& x, int) {
+        int b[8];
+        float d[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = down(q, x.v[j]);
-      const int b = bin_of(q, d);
-      if (b == FAR_BIN) {
-        far += x.there(j) ? 1 : 0;
-      } else {
-        const uint32_t w = (uint32_t)rintf(__builtin_amdgcn_exp2f(d * q.to_exp) * BIN_WEIGHT);
-        atomicAdd(&bins[b], 1ull << COUNT_SHIFT | w);
-      }
-    }
+        for (int j = 0; j < 8; ++j) {
+          d[j] = down(q, x.v[j]);
+          b[j] = bin_of(q, d[j]);
+        }
+        if (q.k > 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t w = (uint32_t)rintf(__builtin_amdgcn_exp2f(d[j] * q.to_exp) * BIN_WEIGHT);
+            if (b[j] != FAR_BIN) atomicAdd(&bins[b[j]], 1ull << COUNT_SHIFT | w);
+            else far += x.there(j) ? 1 : 0;
+          }
+        } else {
+          double w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = q.sc.weight(x.v[j]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (b[j] != FAR_BIN) atomicAdd(&bins[b[j]], (unsigned long long)units(w[j]));
+        }
+      },
+      [&] {
+        for (int b = threadIdx.x; b < NBINS; b += SLICE_T) bins[b] = 0;
+        q = row_of(a, sp, r);
+        run = !q.none && !q.greedy && q.cuts();
+        __syncthreads();
+        return run;
+      });
+  if (!run) return;
+  if (q.k > 0) {
+    far = wave_sum(far);
+    if (lane == 0 && far) atomicAdd(&bins[FAR_BIN], (unsigned long long)far << COUNT_SHIFT);
   }
-  far = wave_sum(far);
-  if (lane == 0 && far) atomicAdd(&bins[FAR_BIN], (unsigned long long)far << COUNT_SHIFT);
   __syncthreads();
   for (int b = threadIdx.x; b < NBINS; b += SLICE_T)
     if (bins[b]) atomicAdd(&sp.bins[r * NBINS + b], bins[b]);
 }
 
-// The cuts' bins from the row's histogram, by all threads of a workgroup.
-__device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const unsigned long long* bins) {
+// The bin of the weight's cut where there is no top-k: the bins' weights are exact.
+__device__ __forceinline__ Cuts find_nucleus(const Row& q, const uint64_t (&v)[BINS_EACH], RowState* state) {
+  __shared__ uint64_t wave_total[SLICE_T / 64];
+  __shared__ int found;
+  constexpr int PER = BINS_EACH;
+  uint64_t sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) sum += v[j];
+  const uint64_t upto = wave_scan(sum);
+  if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  uint64_t at = upto - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < SLICE_T / 64; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) at += wave_total[w];
+    total += wave_total[w];
+  }
+  const uint64_t target = nucleus(q.p, total);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (at < target && at + v[j] >= target) {  // one thread's
+      found = threadIdx.x * PER + j;
+      if (state) {
+        state->before = at;
+        state->total = total;
+      }
+    }
+    at += v[j];
+  }
+  __syncthreads();
+  Cuts c;
+  c.lo = c.hi = found;
+  c.kb = NBINS;
+  c.slow = 0;
+  c.before_lo = found ? 1 : 0;  // (whether the first of the order is before it)
+  c.before_kb = 0;
+  c.in_range = LIST;
+  c.pad = 0;
+  return c;
+}
+
+// The cuts' bins from the row's histogram with top-k, by all threads of a workgroup.
+__device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const uint64_t (&v)[BINS_EACH]) {
   __shared__ uint64_t wave_total[SLICE_T / 64];
   __shared__ int found[6];  // kb, lo, hi, tokens before kb, before lo, up to and with hi
   __shared__ uint64_t weights[2];  // before kb, up to and with it
-  constexpr int PER = NBINS / SLICE_T;
+  constexpr int PER = BINS_EACH;
   constexpr uint64_t WEIGHT = (1ull << COUNT_SHIFT) - 1;
-  uint64_t v[PER], sum = 0;
+  uint64_t sum = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    v[j] = bins[threadIdx.x * PER + j];
-    sum += v[j];
-  }
+  for (int j = 0; j < PER; ++j) sum += v[j];
   const uint64_t upto = wave_scan(sum);
   if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = upto;
   if (threadIdx.x == 0) {
@@ -667,57 +776,127 @@ __device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const unsigne
 }
 
 template <int DT>
-__global__ __launch_bounds__(SLICE_T) void weigh_kernel(const Args a, const Split sp) {
+__global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const Split sp) {
   const int64_t r = blockIdx.x / sp.slices;
   const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Row q = row_of(a, sp, r);
-  if (q.none || q.greedy) return;
-  const bool cuts = q.cuts();
-  Cuts c{};
-  c.lo = c.kb = NBINS;
-  c.hi = NBINS - 1;
-  RowState& state = sp.state[r];
-  if (cuts) {
-    c = find_cuts(q, a.vocab, sp.bins + r * NBINS);
-    if (g == 0 && threadIdx.x == 0) state.cuts = c;
-    if (c.slow) return;
-  }
   const char* row = a.logits + r * a.ld;
   const int end = min((g + 1) * sp.per, sp.chunks);
+  RowState& state = sp.state[r];
+  Row q;
+  Cuts c{};
+  bool cuts = false, run = false, sums = false;
+  float lo = 0.0f, hi = 0.0f, kb = 0.0f, min_far_kb = 0.0f;
   uint64_t sure = 0, middle = 0;
-  for (int n = g * sp.per + wave; n < end; n += SLICE_T / 64) {
-    Chunk<DT> x;
-    x.load(a, row, n);
-    uint64_t kept = 0;
+  __shared__ unsigned long long near[NEAR];
+  __shared__ int gathered;
+  __shared__ unsigned int base;
+  auto list_one = [&](uint64_t place) {
+    const unsigned int at = atomicAdd(&state.listed, 1u);
+    if (at < LIST) sp.list[r * LIST + at] = place;
+  };
+  if (threadIdx.x == 0) gathered = 0;
+  for_chunks<DT, 2>(
+      a, row, g * sp.per + wave, end,
+      [&](const Chunk<DT>& x, int n) {
+        // whether each of this lane's eight is kept for sure, or counts for the total only (what is after the count's bin
+        // is dropped; without one, what is after the weight's)
+        bool before[8], between[8], some = true;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = x.v[j];
-      const int b = cuts ? bin_of(q, down(q, v)) : 0;
-      const bool listed = cuts && ((b >= c.lo && b <= c.hi) || b == c.kb);
-      if (cuts) {
-        const uint64_t mask = __ballot(listed && x.there(j));
-        if (mask) {
-          unsigned int at = 0;
-          if (lane == 0) at = atomicAdd(&state.listed, (unsigned int)__popcll(mask));
-          at = __shfl(at, 0) + (unsigned int)__popcll(mask & ((1ull << lane) - 1));
-          if ((mask >> lane & 1) && at < LIST) sp.list[r * LIST + at] = place_of(v, x.at(j));
+        for (int j = 0; j < 8; ++j) {
+          before[j] = true;
+          between[j] = false;
         }
-      }
-      if (!listed && b < c.kb && b != FAR_BIN) {  // (what is after the count's bin is dropped)
-        const double w = q.sc.weight(v);
-        const uint64_t m = units(w);
-        if (b < c.lo) {
-          sure += m;
-          if (w >= q.min_p || x.at(j) == q.first) kept += m;
-        } else {
-          middle += m;
+        if (cuts) {
+          bool listed[8], any = false;
+          some = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float b = bin_place(q, down(q, x.v[j]));  // compared as it is: the bounds are whole numbers
+            before[j] = b < lo;
+            listed[j] = ((b >= lo && b < hi) || (b >= kb && b < kb + 1.0f)) && x.there(j);
+            between[j] = sums && b >= hi && b < min_far_kb;
+            some |= before[j] || between[j];
+            any |= listed[j];
+          }
+          if (__any(any)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (listed[j]) {
+                const int at = atomicAdd(&gathered, 1);
+                const uint64_t place = place_of(x.v[j], x.at(j));
+                if (at < NEAR) near[at] = place;
+                else list_one(place);
+              }
+            }
+          }
         }
-      }
-    }
-    kept = wave_sum(kept);
-    if (lane == 0) sp.chunk[r * sp.chunks + n] = kept;
+        uint64_t kept = 0;
+        if (__any(some)) {
+          // four at a time, without branches: their FMAs fill each other's latency
+#pragma unroll
+          for (int h = 0; h < 8; h += 4) {
+            double w[4];
+            if (sums) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[j] = q.sc.weight(x.v[h + j]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint64_t m = units(w[j]);
+                const bool in = before[h + j];
+                sure += in ? m : 0;
+                middle += between[h + j] ? m : 0;
+                kept += in && w[j] >= q.min_p ? m : 0;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = q.sc.weight(before[h + j] ? x.v[h + j] : -__builtin_inff());
+              if (q.min_p > 0.0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = w[j] >= q.min_p ? w[j] : 0.0;
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) kept += raw_units(w[j]);
+              kept -= 4 * RAW;
+            }
+          }
+        }
+        if (__any(kept != 0)) kept = wave_sum(kept);
+        if (lane == 0) sp.chunk[r * sp.chunks + n] = kept;
+      },
+      [&] {
+        uint64_t bins[BINS_EACH];  // on their way beside the slices' maxima
+#pragma unroll
+        for (int j = 0; j < BINS_EACH; ++j) bins[j] = sp.filters ? sp.bins[r * NBINS + threadIdx.x * BINS_EACH + j] : 0;
+        q = row_of(a, sp, r);
+        run = !q.none && !q.greedy;
+        if (!run) return false;
+        cuts = q.cuts();
+        sums = q.k > 0 && q.p < 1.0;
+        c.lo = c.kb = NBINS;
+        c.hi = NBINS - 1;
+        if (cuts) {
+          const bool writer = g == 0;
+          c = q.k > 0 ? find_cuts(q, a.vocab, bins) : find_nucleus(q, bins, writer ? &state : nullptr);
+          if (writer && threadIdx.x == 0) state.cuts = c;
+          run = !c.slow;
+          lo = (float)c.lo;
+          hi = (float)(c.hi + 1);
+          kb = (float)c.kb;
+          min_far_kb = fminf(kb, (float)FAR_BIN);
+        }
+        return run;
+      });
+  if (!run || !cuts) return;
+  __syncthreads();
+  const int here = min(gathered, NEAR);
+  if (here) {
+    if (threadIdx.x == 0) base = atomicAdd(&state.listed, (unsigned int)here);
+    __syncthreads();
+    for (int i = threadIdx.x; i < here; i += SLICE_T)
+      if (base + i < LIST) sp.list[r * LIST + base + i] = near[i];
   }
-  if (cuts && q.p < 1.0) {
+  if (sums) {
     sure = wave_sum(sure);
     middle = wave_sum(middle);
     if (lane == 0) {
@@ -727,11 +906,29 @@ __global__ __launch_bounds__(SLICE_T) void weigh_kernel(const Args a, const Spli
   }
 }
 
+// n <= T / 2 places, largest first: each one's rank is counted by a group of lanes.
+// (A step of the sort below waits for LDS twice, 0.15 us: 256 places 6 us, so 1.5.)
+__device__ __forceinline__ void rank_down(unsigned long long* v, int n, int up) {
+  const int lanes = T / up < 64 ? T / up : 64;  // of a group, a power of two as `up` >= n
+  const int e = (int)threadIdx.x / lanes;
+  __syncthreads();
+  const unsigned long long mine = e < n ? v[e] : 0ull;
+  int rank = 0;
+#pragma unroll 8
+  for (int j = (int)threadIdx.x % lanes; j < n; j += lanes) rank += v[j] > mine ? 1 : 0;
+  for (int d = 1; d < lanes; d <<= 1) rank += __shfl_xor(rank, d);
+  __syncthreads();
+  if (e < n && (int)threadIdx.x % lanes == 0) v[rank] = mine;
+  __syncthreads();
+}
+
 // n (a power of two) places, largest first.
 __device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
   for (int size = 2; size <= n; size <<= 1)
     for (int step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
+      // pairs up to 64 apart lie in a wave's own 128 places: its accesses to LDS stay in order
+      if (step > 64 || (step == 64 && size > 128) || size == 2) __syncthreads();
+      __builtin_amdgcn_wave_barrier();
       for (int i = threadIdx.x; i < n / 2; i += T) {
         const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
         const bool down = !(lo & size);
@@ -758,6 +955,24 @@ __global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
     } d;
   } u;
   const int64_t r = blockIdx.x;
+  auto& d = u.d;
+  // everything that the earlier launches left is on its way at once
+  const RowState* const state = sp.state + r;
+  const bool filters = sp.filters;
+  const uint64_t my_chunk = (int)threadIdx.x < sp.chunks ? sp.chunk[r * sp.chunks + threadIdx.x] : 0;
+  const uint64_t my_place = filters ? sp.list[r * LIST + threadIdx.x] : 0;  // (of LIST there are, if not all written)
+  Cuts c{};
+  int listed = 0;
+  uint64_t sure = 0, middle = 0, before_lo = 0, total_of = 0;
+  if (filters) {
+    c = state->cuts;
+    listed = (int)min(state->listed, (unsigned int)(LIST + 1));
+    sure = state->sure;
+    middle = state->middle;
+    before_lo = state->before;
+    total_of = state->total;
+  }
+  const double number = (double)a.uniform[r];
   const Row q = row_of(a, sp, r);
   if (q.none || q.greedy) {
     if (threadIdx.x == 0) {
@@ -766,21 +981,17 @@ __global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
     }
     return;
   }
-  Cuts c{};
-  c.lo = NBINS;
   uint64_t last = 0;    // the place of the last token kept, or none of the list is
   bool any = false;
-  auto& d = u.d;
-  if (q.cuts()) {
-    c = sp.state[r].cuts;
-    if (c.slow) {
-      whole_row<DT>(a, r, u.s);
-      return;
-    }
+  if (!q.cuts()) {
+    c.lo = NBINS;
+    listed = 0;
+  } else if (c.slow || listed > LIST) {
+    whole_row<DT>(a, r, u.s);
+    return;
   }
-  for (int i = threadIdx.x; i < sp.chunks; i += T) d.chunk[i] = sp.chunk[r * sp.chunks + i];
+  d.chunk[threadIdx.x] = my_chunk;
   if (threadIdx.x == 0) d.last = ~0ull;
-  __syncthreads();
   auto scan = [&](uint64_t v, uint64_t& before) {
     const uint64_t upto = wave_scan(v);
     __syncthreads();
@@ -795,49 +1006,39 @@ __global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
     before = below + upto - v;
     return total;
   };
-  const int listed = q.cuts() ? (int)min(sp.state[r].listed, (unsigned int)LIST) : 0;
   if (listed) {
     int n = 2;
     while (n < listed) n <<= 1;
-    for (int i = threadIdx.x; i < n; i += T) d.list[i] = i < listed ? sp.list[r * LIST + i] : 0ull;
-    sort_down(d.list, n);
+    if ((int)threadIdx.x < n) d.list[threadIdx.x] = (int)threadIdx.x < listed ? my_place : 0ull;
+    for (int i = threadIdx.x + T; i < n; i += T) d.list[i] = i < listed ? sp.list[r * LIST + i] : 0ull;
+    if (n <= T / 2) rank_down(d.list, listed, n);
+    else sort_down(d.list, n);
     // thread t holds places PER t .. in the order
     const int per = n > T ? n / T : 1;
-    uint64_t m[LIST / T], sum = 0;
-    double w[LIST / T];
+    const int j0 = (int)threadIdx.x * per, j1 = min(j0 + per, listed);
     auto position = [&](int j) { return j < c.in_range ? c.before_lo + j : c.before_kb + j - c.in_range; };
-#pragma unroll
-    for (int i = 0; i < LIST / T; ++i) {
-      const int j = (int)threadIdx.x * per + i;
-      m[i] = 0;
-      w[i] = 0.0;
-      if (i < per && j < listed) {
-        w[i] = q.sc.weight(value_of((uint32_t)(d.list[j] >> 32)));
-        if (q.k == 0 || position(j) < q.k) m[i] = units(w[i]);
-        sum += m[i];
-      }
-    }
-    uint64_t before;
+    auto weight = [&](int j) { return q.sc.weight(value_of((uint32_t)(d.list[j] >> 32))); };
+    uint64_t sum = 0, before;
+#pragma nounroll
+    for (int j = j0; j < j1; ++j)
+      if (q.k == 0 || position(j) < q.k) sum += units(weight(j));
     const uint64_t allowed = scan(sum, before);
     uint64_t target = ~0ull, at = before;
     if (q.p < 1.0) {
-      target = nucleus(q.p, sp.state[r].sure + sp.state[r].middle + allowed);
-      at += sp.state[r].sure;
+      target = nucleus(q.p, q.k > 0 ? sure + middle + allowed : total_of);
+      at += q.k > 0 ? sure : before_lo;
     }
-#pragma unroll
-    for (int i = 0; i < LIST / T; ++i) {
-      const int j = (int)threadIdx.x * per + i;
-      if (i < per && j < listed) {
-        const int pos = position(j);
-        const bool keep = pos == 0 || ((q.k == 0 || pos < q.k) && at < target && (q.p >= 1.0 || j < c.in_range));
-        if (keep) {
-          const uint64_t place = d.list[j];
-          const int index = ~(int)(uint32_t)place;
-          atomicMin(&d.last, (unsigned long long)place);
-          if (m[i] && (w[i] >= q.min_p || index == q.first)) atomicAdd(&d.chunk[index / CHUNK], (unsigned long long)m[i]);
-        }
-        at += m[i];
+#pragma nounroll
+    for (int j = j0; j < j1; ++j) {
+      const int pos = position(j);
+      const double w = weight(j);
+      const uint64_t m = units(w), place = d.list[j];
+      const int index = ~(int)(uint32_t)place;
+      if (pos == 0 || ((q.k == 0 || pos < q.k) && at < target && (q.p >= 1.0 || j < c.in_range))) {
+        atomicMin(&d.last, (unsigned long long)place);
+        if (m && w >= q.min_p) atomicAdd(&d.chunk[index / CHUNK], (unsigned long long)m);
       }
+      at += m;
     }
     __syncthreads();
     last = d.last;
@@ -845,12 +1046,13 @@ __global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
   }
   auto kept = [&](float v, int i, double w) {
     const bool in = any ? place_of(v, i) >= last : c.lo >= NBINS || bin_of(q, down(q, v)) < c.lo;
-    return in && (w >= q.min_p || i == q.first);
+    return in && w >= q.min_p;
   };
   uint64_t before;
-  const uint64_t mine = (int)threadIdx.x < sp.chunks ? d.chunk[threadIdx.x] : 0;
+  if (!listed) __syncthreads();
+  const uint64_t mine = d.chunk[threadIdx.x];
   const uint64_t total = scan(mine, before);
-  const uint64_t at = drawn_weight((double)a.uniform[r], total);
+  const uint64_t at = drawn_weight(number, total);
   __syncthreads();
   if (mine && before <= at && at < before + mine) {
     d.found[0] = threadIdx.x;
@@ -870,7 +1072,7 @@ __global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
   before += under;
   if (w && before <= at && at < before + w) {
     a.token[r] = i;
-    if (a.logprob) a.logprob[r] = logprob_of(q.sc.distance(v), total);
+    if (a.logprob) a.logprob[r] = logprob_of(q.sc.log2_weight(v), total);
   }
 }
 
@@ -886,7 +1088,7 @@ static Plan plan(int64_t rows, int64_t vocab, bool filters) {
   Plan p{};
   p.chunks = (int)((vocab + CHUNK - 1) / CHUNK);
   const int waves = SLICE_T / 64;
-  const int64_t most = 1024 / rows < 1 ? 1 : 1024 / rows;
+  const int64_t all = 4096 / waves, most = all / rows < 1 ? 1 : all / rows;
   int64_t slices = (p.chunks + waves - 1) / waves;
   if (slices > most) slices = most;
   p.per = (int)((p.chunks + slices - 1) / slices);

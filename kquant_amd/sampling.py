@@ -57,8 +57,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
     index, up to and with which the kept weight exceeds uniform times the total;
     a number from 1 up draws the last kept token, one below 0 the first.  A
     temperature of 0 takes the largest logit.  Each setting is a number or a
-    tensor [...] with a row's own (fp32; top_k int32 or int64, where a value that
-    is no number above 0 means none, as does a temperature).
+    tensor [...] with a row's own (fp32; top_k int32 or int64), where a top_k of 0
+    or fewer and a top_p of 1 or more keep all, a top_p of 0 or less and a min_p
+    of 1 or more the first token and its equals at most, and a temperature that is
+    not above 0 takes the largest logit.
 
     Logits of -inf are never drawn; logits of +inf share the draw among them.  A
     row with a NaN, or with nothing above -inf, gives -1.
