@@ -364,20 +364,25 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
 // a cut falls into one bin (with top-k the weight's cut into a few, since the bins'
 // weights are sums of fp32 exponentials then), and only what lies there has to be
 // ordered.
-// Four launches, each a workgroup a slice of a row (the last one a row):
+// Three launches, a workgroup a slice of a row:
 //   stats      the slice's first place and least logit; clears the row's bins
 //   histogram  (with top-k or top-p) every bin's weight; with top-k its tokens and a
-//              rough weight, since only the bins up to the count's matter then
+//              rough weight, since only the bins up to the count's matter then.  The
+//              row's last workgroup finds the cuts' bins
 //   weigh      exact weight of each chunk's tokens in the bins before the cuts, and
 //              the list of the tokens in the cuts' bins; with top-k also the weight
-//              of the bins that count for top-p's total only
-//   draw       orders the list, cuts, and finds the draw's chunk and token
+//              of the bins that count for top-p's total only.  The row's last
+//              workgroup orders the list, cuts, and finds the draw's chunk and token
+// No workgroup waits for another: the last one is who finds that all others of its
+// row have counted themselves.  What it reads of theirs goes to memory and comes
+// from there in agent-scope accesses, all of which end before the count (a fence
+// would write each workgroup's L2 back).
 // A list longer than LIST (many equal logits at a cut) leaves the row to
 // whole_row.
-// What bounds it: at one row the four launches (sums over 129280 logits take a
-// microsecond each); at many rows the exponentials, some 30 fp64 instructions a
-// logit that may be drawn or counts for a total.
-constexpr int SLICE_T = 512;
+// What bounds it: at one row the launches and each one's chain of loads; at many
+// rows three passes over the logits, of 8 us each at 33 MB, and where many tokens
+// have weight their exponentials, some 26 instructions each.
+constexpr int SLICE_T = T;
 constexpr int NEAR = 1024;   // listed tokens that a workgroup gathers before they go to the list
 constexpr int NBINS = 2048, FAR_BIN = NBINS - 1;  // FAR_BIN: tokens of no weight
 constexpr int BINS_EACH = NBINS / SLICE_T;        // a thread's bins where a workgroup looks through them
@@ -403,7 +408,9 @@ struct RowState {
   Cuts cuts;
   unsigned long long sure, middle;  // with top-k: weight of the bins before lo, and of those that only count for the total
   unsigned long long before, total; // without: of the bins before lo, and of all
-  unsigned int listed, pad[3];
+  unsigned int listed;
+  unsigned int arrived[2];          // workgroups that are through with the histogram, and with weighing
+  unsigned int pad;
 };
 
 struct Split {
@@ -415,6 +422,23 @@ struct Split {
   int slices, per, chunks;      // per: chunks a slice
   int filters;                  // top-k or top-p may cut
 };
+
+__device__ __forceinline__ uint64_t shared_load(const unsigned long long* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void shared_store(unsigned long long* p, uint64_t v) {
+  __hip_atomic_store(p, (unsigned long long)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether this workgroup is the last of `all` to come here; its shared accesses have ended.
+__device__ __forceinline__ bool last_of(unsigned int* counter, int all) {
+  __shared__ bool last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned int)(all - 1);
+  __syncthreads();
+  return last;
+}
 
 // What a row asks for.
 struct Row {
@@ -582,6 +606,7 @@ __global__ __launch_bounds__(SLICE_T) void stats_kernel(const Args a, const Spli
       sp.state[r].listed = 0;
     }
   }
+  if (g == 0 && threadIdx.x == 0) sp.state[r].arrived[0] = sp.state[r].arrived[1] = 0;
   __syncthreads();
   if (threadIdx.x == 0) {
     Part p = part[0];
@@ -594,61 +619,8 @@ __global__ __launch_bounds__(SLICE_T) void stats_kernel(const Args a, const Spli
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(SLICE_T) void histogram_kernel(const Args a, const Split sp) {
-  __shared__ unsigned long long bins[NBINS];
-  const int64_t r = blockIdx.x / sp.slices;
-  const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const char* row = a.logits + r * a.ld;
-  const int end = min((g + 1) * sp.per, sp.chunks);
-  Row q;
-  uint64_t far = 0;
-  bool run = false;
-  for_chunks<DT, 2>(
-      a, row, g * sp.per + wave, end,
-      [&](const Chunk<DT>& x, int) {
-        int b[8];
-        float d[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          d[j] = down(q, x.v[j]);
-          b[j] = bin_of(q, d[j]);
-        }
-        if (q.k > 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t w = (uint32_t)rintf(__builtin_amdgcn_exp2f(d[j] * q.to_exp) * BIN_WEIGHT);
-            if (b[j] != FAR_BIN) atomicAdd(&bins[b[j]], 1ull << COUNT_SHIFT | w);
-            else far += x.there(j) ? 1 : 0;
-          }
-        } else {
-          double w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = q.sc.weight(x.v[j]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (b[j] != FAR_BIN) atomicAdd(&bins[b[j]], (unsigned long long)units(w[j]));
-        }
-      },
-      [&] {
-        for (int b = threadIdx.x; b < NBINS; b += SLICE_T) bins[b] = 0;
-        q = row_of(a, sp, r);
-        run = !q.none && !q.greedy && q.cuts();
-        __syncthreads();
-        return run;
-      });
-  if (!run) return;
-  if (q.k > 0) {
-    far = wave_sum(far);
-    if (lane == 0 && far) atomicAdd(&bins[FAR_BIN], (unsigned long long)far << COUNT_SHIFT);
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < NBINS; b += SLICE_T)
-    if (bins[b]) atomicAdd(&sp.bins[r * NBINS + b], bins[b]);
-}
-
 // The bin of the weight's cut where there is no top-k: the bins' weights are exact.
-__device__ __forceinline__ Cuts find_nucleus(const Row& q, const uint64_t (&v)[BINS_EACH], RowState* state) {
+__device__ __forceinline__ Cuts find_nucleus(const Row& q, const uint64_t (&v)[BINS_EACH], RowState& state) {
   __shared__ uint64_t wave_total[SLICE_T / 64];
   __shared__ int found;
   constexpr int PER = BINS_EACH;
@@ -669,10 +641,8 @@ __device__ __forceinline__ Cuts find_nucleus(const Row& q, const uint64_t (&v)[B
   for (int j = 0; j < PER; ++j) {
     if (at < target && at + v[j] >= target) {  // one thread's
       found = threadIdx.x * PER + j;
-      if (state) {
-        state->before = at;
-        state->total = total;
-      }
+      state.before = at;
+      state.total = total;
     }
     at += v[j];
   }
@@ -776,6 +746,224 @@ __device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const uint64_
 }
 
 template <int DT>
+__global__ __launch_bounds__(SLICE_T) void histogram_kernel(const Args a, const Split sp) {
+  __shared__ unsigned long long bins[NBINS];
+  const int64_t r = blockIdx.x / sp.slices;
+  const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const char* row = a.logits + r * a.ld;
+  const int end = min((g + 1) * sp.per, sp.chunks);
+  Row q;
+  uint64_t far = 0;
+  bool run = false;
+  for_chunks<DT, 2>(
+      a, row, g * sp.per + wave, end,
+      [&](const Chunk<DT>& x, int) {
+        int b[8];
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          d[j] = down(q, x.v[j]);
+          b[j] = bin_of(q, d[j]);
+        }
+        if (q.k > 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t w = (uint32_t)rintf(__builtin_amdgcn_exp2f(d[j] * q.to_exp) * BIN_WEIGHT);
+            if (b[j] != FAR_BIN) atomicAdd(&bins[b[j]], 1ull << COUNT_SHIFT | w);
+            else far += x.there(j) ? 1 : 0;
+          }
+        } else {
+          double w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = q.sc.weight(x.v[j]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (b[j] != FAR_BIN) atomicAdd(&bins[b[j]], (unsigned long long)units(w[j]));
+        }
+      },
+      [&] {
+        for (int b = threadIdx.x; b < NBINS; b += SLICE_T) bins[b] = 0;
+        q = row_of(a, sp, r);
+        run = !q.none && !q.greedy && q.cuts();
+        __syncthreads();
+        return run;
+      });
+  if (!run) return;
+  if (q.k > 0) {
+    far = wave_sum(far);
+    if (lane == 0 && far) atomicAdd(&bins[FAR_BIN], (unsigned long long)far << COUNT_SHIFT);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < NBINS; b += SLICE_T)
+    if (bins[b]) atomicAdd(&sp.bins[r * NBINS + b], bins[b]);
+  RowState& state = sp.state[r];
+  if (!last_of(&state.arrived[0], sp.slices)) return;
+  uint64_t v[BINS_EACH];
+#pragma unroll
+  for (int j = 0; j < BINS_EACH; ++j) v[j] = shared_load(&sp.bins[r * NBINS + threadIdx.x * BINS_EACH + j]);
+  const Cuts c = q.k > 0 ? find_cuts(q, a.vocab, v) : find_nucleus(q, v, state);
+  if (threadIdx.x == 0) state.cuts = c;
+}
+
+// n <= T / 2 places, largest first: each one's rank is counted by a group of lanes.
+// (A step of the sort below waits for LDS twice, 0.15 us: 256 places 6 us, so 1.5.)
+__device__ __forceinline__ void rank_down(unsigned long long* v, int n, int up) {
+  const int lanes = T / up < 64 ? T / up : 64;  // of a group, a power of two as `up` >= n
+  const int e = (int)threadIdx.x / lanes;
+  __syncthreads();
+  const unsigned long long mine = e < n ? v[e] : 0ull;
+  int rank = 0;
+#pragma unroll 8
+  for (int j = (int)threadIdx.x % lanes; j < n; j += lanes) rank += v[j] > mine ? 1 : 0;
+  for (int d = 1; d < lanes; d <<= 1) rank += __shfl_xor(rank, d);
+  __syncthreads();
+  if (e < n && (int)threadIdx.x % lanes == 0) v[rank] = mine;
+  __syncthreads();
+}
+
+// n (a power of two) places, largest first.
+__device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      // pairs up to 64 apart lie in a wave's own 128 places: its accesses to LDS stay in order
+      if (step > 64 || (step == 64 && size > 128) || size == 2) __syncthreads();
+      __builtin_amdgcn_wave_barrier();
+      for (int i = threadIdx.x; i < n / 2; i += T) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const bool down = !(lo & size);
+        const unsigned long long x = v[lo], y = v[hi];
+        if ((x < y) == down) {
+          v[lo] = y;
+          v[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+union DrawShared {
+  Shared s;
+  struct {
+    unsigned long long list[LIST];
+    unsigned long long chunk[CHUNKS];
+    uint64_t part[T / 64];
+    uint64_t found[4];
+    unsigned long long last;
+  } d;
+};
+
+// A row's token, from what its workgroups left.
+template <int DT>
+__device__ __forceinline__ void draw(const Args& a, const Split& sp, int64_t r, const Row& q, const Cuts& c, DrawShared& u) {
+  auto& d = u.d;
+  RowState* const state = sp.state + r;
+  const bool cuts = q.cuts();
+  // all on its way at once
+  const uint64_t my_chunk = (int)threadIdx.x < sp.chunks ? shared_load(&sp.chunk[r * sp.chunks + threadIdx.x]) : 0;
+  const uint64_t my_place = cuts ? shared_load(&sp.list[r * LIST + threadIdx.x]) : 0;  // (of LIST there are, if not all written)
+  int listed = 0;
+  uint64_t sure = 0, middle = 0, before_lo = 0, total_of = 0;
+  if (cuts) {
+    listed = (int)min(__hip_atomic_load(&state->listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), (unsigned int)(LIST + 1));
+    sure = shared_load(&state->sure);
+    middle = shared_load(&state->middle);
+    before_lo = state->before;
+    total_of = state->total;
+  }
+  const double number = (double)a.uniform[r];
+  uint64_t last = 0;    // the place of the last token kept, or none of the list is
+  bool any = false;
+  if (c.slow || listed > LIST) {
+    whole_row<DT>(a, r, u.s);
+    return;
+  }
+  d.chunk[threadIdx.x] = my_chunk;
+  if (threadIdx.x == 0) d.last = ~0ull;
+  auto scan = [&](uint64_t v, uint64_t& before) {
+    const uint64_t upto = wave_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) d.part[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    uint64_t total = 0, below = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+      if (w < (int)(threadIdx.x >> 6)) below += d.part[w];
+      total += d.part[w];
+    }
+    before = below + upto - v;
+    return total;
+  };
+  if (listed) {
+    int n = 2;
+    while (n < listed) n <<= 1;
+    if ((int)threadIdx.x < n) d.list[threadIdx.x] = (int)threadIdx.x < listed ? my_place : 0ull;
+    for (int i = threadIdx.x + T; i < n; i += T) d.list[i] = i < listed ? shared_load(&sp.list[r * LIST + i]) : 0ull;
+    if (n <= T / 2) rank_down(d.list, listed, n);
+    else sort_down(d.list, n);
+    // thread t holds places PER t .. in the order
+    const int per = n > T ? n / T : 1;
+    const int j0 = (int)threadIdx.x * per, j1 = min(j0 + per, listed);
+    auto position = [&](int j) { return j < c.in_range ? c.before_lo + j : c.before_kb + j - c.in_range; };
+    auto weight = [&](int j) { return q.sc.weight(value_of((uint32_t)(d.list[j] >> 32))); };
+    uint64_t sum = 0, before;
+#pragma nounroll
+    for (int j = j0; j < j1; ++j)
+      if (q.k == 0 || position(j) < q.k) sum += units(weight(j));
+    const uint64_t allowed = scan(sum, before);
+    uint64_t target = ~0ull, at = before;
+    if (q.p < 1.0) {
+      target = nucleus(q.p, q.k > 0 ? sure + middle + allowed : total_of);
+      at += q.k > 0 ? sure : before_lo;
+    }
+#pragma nounroll
+    for (int j = j0; j < j1; ++j) {
+      const int pos = position(j);
+      const double w = weight(j);
+      const uint64_t m = units(w), place = d.list[j];
+      const int index = ~(int)(uint32_t)place;
+      if (pos == 0 || ((q.k == 0 || pos < q.k) && at < target && (q.p >= 1.0 || j < c.in_range))) {
+        atomicMin(&d.last, (unsigned long long)place);
+        if (m && w >= q.min_p) atomicAdd(&d.chunk[index / CHUNK], (unsigned long long)m);
+      }
+      at += m;
+    }
+    __syncthreads();
+    last = d.last;
+    any = last != ~0ull;
+  }
+  auto kept = [&](float v, int i, double w) {
+    const bool in = any ? place_of(v, i) >= last : c.lo >= NBINS || bin_of(q, down(q, v)) < c.lo;
+    return in && w >= q.min_p;
+  };
+  uint64_t before;
+  if (!listed) __syncthreads();
+  const uint64_t mine = d.chunk[threadIdx.x];
+  const uint64_t total = scan(mine, before);
+  const uint64_t at = drawn_weight(number, total);
+  __syncthreads();
+  if (mine && before <= at && at < before + mine) {
+    d.found[0] = threadIdx.x;
+    d.found[1] = before;
+  }
+  __syncthreads();
+  const int i = (int)d.found[0] * CHUNK + (int)threadIdx.x;
+  const uint64_t under = d.found[1];
+  uint64_t w = 0;
+  float v = 0.0f;
+  if ((int)threadIdx.x < CHUNK && i < a.vocab) {
+    v = logit<DT>(a.logits + r * a.ld, i);
+    const double e = q.sc.weight(v);
+    if (kept(v, i, e)) w = units(e);
+  }
+  scan(w, before);
+  before += under;
+  if (w && before <= at && at < before + w) {
+    a.token[r] = i;
+    if (a.logprob) a.logprob[r] = logprob_of(q.sc.log2_weight(v), total);
+  }
+}
+
+template <int DT>
 __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const Split sp) {
   const int64_t r = blockIdx.x / sp.slices;
   const int g = (int)(blockIdx.x - r * sp.slices), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -784,15 +972,16 @@ __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const S
   RowState& state = sp.state[r];
   Row q;
   Cuts c{};
-  bool cuts = false, run = false, sums = false;
+  bool cuts = false, run = true, sums = false;
   float lo = 0.0f, hi = 0.0f, kb = 0.0f, min_far_kb = 0.0f;
   uint64_t sure = 0, middle = 0;
+  __shared__ DrawShared u;
   __shared__ unsigned long long near[NEAR];
   __shared__ int gathered;
   __shared__ unsigned int base;
   auto list_one = [&](uint64_t place) {
     const unsigned int at = atomicAdd(&state.listed, 1u);
-    if (at < LIST) sp.list[r * LIST + at] = place;
+    if (at < LIST) shared_store(&sp.list[r * LIST + at], place);
   };
   if (threadIdx.x == 0) gathered = 0;
   for_chunks<DT, 2>(
@@ -862,23 +1051,19 @@ __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const S
           }
         }
         if (__any(kept != 0)) kept = wave_sum(kept);
-        if (lane == 0) sp.chunk[r * sp.chunks + n] = kept;
+        if (lane == 0) shared_store(&sp.chunk[r * sp.chunks + n], kept);
       },
       [&] {
-        uint64_t bins[BINS_EACH];  // on their way beside the slices' maxima
-#pragma unroll
-        for (int j = 0; j < BINS_EACH; ++j) bins[j] = sp.filters ? sp.bins[r * NBINS + threadIdx.x * BINS_EACH + j] : 0;
+        if (sp.filters) c = state.cuts;  // (on its way beside the slices' maxima)
         q = row_of(a, sp, r);
         run = !q.none && !q.greedy;
         if (!run) return false;
         cuts = q.cuts();
         sums = q.k > 0 && q.p < 1.0;
-        c.lo = c.kb = NBINS;
-        c.hi = NBINS - 1;
-        if (cuts) {
-          const bool writer = g == 0;
-          c = q.k > 0 ? find_cuts(q, a.vocab, bins) : find_nucleus(q, bins, writer ? &state : nullptr);
-          if (writer && threadIdx.x == 0) state.cuts = c;
+        if (!cuts) {
+          c.slow = 0;
+          c.lo = NBINS;
+        } else {
           run = !c.slow;
           lo = (float)c.lo;
           hi = (float)(c.hi + 1);
@@ -887,193 +1072,32 @@ __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const S
         }
         return run;
       });
-  if (!run || !cuts) return;
-  __syncthreads();
-  const int here = min(gathered, NEAR);
-  if (here) {
-    if (threadIdx.x == 0) base = atomicAdd(&state.listed, (unsigned int)here);
-    __syncthreads();
-    for (int i = threadIdx.x; i < here; i += SLICE_T)
-      if (base + i < LIST) sp.list[r * LIST + base + i] = near[i];
-  }
-  if (sums) {
-    sure = wave_sum(sure);
-    middle = wave_sum(middle);
-    if (lane == 0) {
-      if (sure) atomicAdd(&state.sure, (unsigned long long)sure);
-      if (middle) atomicAdd(&state.middle, (unsigned long long)middle);
-    }
-  }
-}
-
-// n <= T / 2 places, largest first: each one's rank is counted by a group of lanes.
-// (A step of the sort below waits for LDS twice, 0.15 us: 256 places 6 us, so 1.5.)
-__device__ __forceinline__ void rank_down(unsigned long long* v, int n, int up) {
-  const int lanes = T / up < 64 ? T / up : 64;  // of a group, a power of two as `up` >= n
-  const int e = (int)threadIdx.x / lanes;
-  __syncthreads();
-  const unsigned long long mine = e < n ? v[e] : 0ull;
-  int rank = 0;
-#pragma unroll 8
-  for (int j = (int)threadIdx.x % lanes; j < n; j += lanes) rank += v[j] > mine ? 1 : 0;
-  for (int d = 1; d < lanes; d <<= 1) rank += __shfl_xor(rank, d);
-  __syncthreads();
-  if (e < n && (int)threadIdx.x % lanes == 0) v[rank] = mine;
-  __syncthreads();
-}
-
-// n (a power of two) places, largest first.
-__device__ __forceinline__ void sort_down(unsigned long long* v, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      // pairs up to 64 apart lie in a wave's own 128 places: its accesses to LDS stay in order
-      if (step > 64 || (step == 64 && size > 128) || size == 2) __syncthreads();
-      __builtin_amdgcn_wave_barrier();
-      for (int i = threadIdx.x; i < n / 2; i += T) {
-        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const bool down = !(lo & size);
-        const unsigned long long x = v[lo], y = v[hi];
-        if ((x < y) == down) {
-          v[lo] = y;
-          v[hi] = x;
-        }
-      }
-    }
-  __syncthreads();
-}
-
-template <int DT>
-__global__ __launch_bounds__(T) void draw_kernel(const Args a, const Split sp) {
-  __shared__ union {
-    Shared s;
-    struct {
-      unsigned long long list[LIST];
-      unsigned long long chunk[CHUNKS];
-      uint64_t part[T / 64];
-      uint64_t found[4];
-      unsigned long long last;
-    } d;
-  } u;
-  const int64_t r = blockIdx.x;
-  auto& d = u.d;
-  // everything that the earlier launches left is on its way at once
-  const RowState* const state = sp.state + r;
-  const bool filters = sp.filters;
-  const uint64_t my_chunk = (int)threadIdx.x < sp.chunks ? sp.chunk[r * sp.chunks + threadIdx.x] : 0;
-  const uint64_t my_place = filters ? sp.list[r * LIST + threadIdx.x] : 0;  // (of LIST there are, if not all written)
-  Cuts c{};
-  int listed = 0;
-  uint64_t sure = 0, middle = 0, before_lo = 0, total_of = 0;
-  if (filters) {
-    c = state->cuts;
-    listed = (int)min(state->listed, (unsigned int)(LIST + 1));
-    sure = state->sure;
-    middle = state->middle;
-    before_lo = state->before;
-    total_of = state->total;
-  }
-  const double number = (double)a.uniform[r];
-  const Row q = row_of(a, sp, r);
   if (q.none || q.greedy) {
-    if (threadIdx.x == 0) {
+    if (g == 0 && threadIdx.x == 0) {
       a.token[r] = q.none ? -1 : q.first;
       if (a.logprob) a.logprob[r] = q.none ? __builtin_nanf("") : 0.0f;
     }
     return;
   }
-  uint64_t last = 0;    // the place of the last token kept, or none of the list is
-  bool any = false;
-  if (!q.cuts()) {
-    c.lo = NBINS;
-    listed = 0;
-  } else if (c.slow || listed > LIST) {
-    whole_row<DT>(a, r, u.s);
-    return;
-  }
-  d.chunk[threadIdx.x] = my_chunk;
-  if (threadIdx.x == 0) d.last = ~0ull;
-  auto scan = [&](uint64_t v, uint64_t& before) {
-    const uint64_t upto = wave_scan(v);
+  if (run && cuts) {
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) d.part[threadIdx.x >> 6] = upto;
-    __syncthreads();
-    uint64_t total = 0, below = 0;
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) {
-      if (w < (int)(threadIdx.x >> 6)) below += d.part[w];
-      total += d.part[w];
+    const int here = min(gathered, NEAR);
+    if (here) {
+      if (threadIdx.x == 0) base = atomicAdd(&state.listed, (unsigned int)here);
+      __syncthreads();
+      for (int i = threadIdx.x; i < here; i += SLICE_T)
+        if (base + i < LIST) shared_store(&sp.list[r * LIST + base + i], near[i]);
     }
-    before = below + upto - v;
-    return total;
-  };
-  if (listed) {
-    int n = 2;
-    while (n < listed) n <<= 1;
-    if ((int)threadIdx.x < n) d.list[threadIdx.x] = (int)threadIdx.x < listed ? my_place : 0ull;
-    for (int i = threadIdx.x + T; i < n; i += T) d.list[i] = i < listed ? sp.list[r * LIST + i] : 0ull;
-    if (n <= T / 2) rank_down(d.list, listed, n);
-    else sort_down(d.list, n);
-    // thread t holds places PER t .. in the order
-    const int per = n > T ? n / T : 1;
-    const int j0 = (int)threadIdx.x * per, j1 = min(j0 + per, listed);
-    auto position = [&](int j) { return j < c.in_range ? c.before_lo + j : c.before_kb + j - c.in_range; };
-    auto weight = [&](int j) { return q.sc.weight(value_of((uint32_t)(d.list[j] >> 32))); };
-    uint64_t sum = 0, before;
-#pragma nounroll
-    for (int j = j0; j < j1; ++j)
-      if (q.k == 0 || position(j) < q.k) sum += units(weight(j));
-    const uint64_t allowed = scan(sum, before);
-    uint64_t target = ~0ull, at = before;
-    if (q.p < 1.0) {
-      target = nucleus(q.p, q.k > 0 ? sure + middle + allowed : total_of);
-      at += q.k > 0 ? sure : before_lo;
-    }
-#pragma nounroll
-    for (int j = j0; j < j1; ++j) {
-      const int pos = position(j);
-      const double w = weight(j);
-      const uint64_t m = units(w), place = d.list[j];
-      const int index = ~(int)(uint32_t)place;
-      if (pos == 0 || ((q.k == 0 || pos < q.k) && at < target && (q.p >= 1.0 || j < c.in_range))) {
-        atomicMin(&d.last, (unsigned long long)place);
-        if (m && w >= q.min_p) atomicAdd(&d.chunk[index / CHUNK], (unsigned long long)m);
+    if (sums) {
+      sure = wave_sum(sure);
+      middle = wave_sum(middle);
+      if (lane == 0) {
+        if (sure) atomicAdd(&state.sure, (unsigned long long)sure);
+        if (middle) atomicAdd(&state.middle, (unsigned long long)middle);
       }
-      at += m;
     }
-    __syncthreads();
-    last = d.last;
-    any = last != ~0ull;
   }
-  auto kept = [&](float v, int i, double w) {
-    const bool in = any ? place_of(v, i) >= last : c.lo >= NBINS || bin_of(q, down(q, v)) < c.lo;
-    return in && w >= q.min_p;
-  };
-  uint64_t before;
-  if (!listed) __syncthreads();
-  const uint64_t mine = d.chunk[threadIdx.x];
-  const uint64_t total = scan(mine, before);
-  const uint64_t at = drawn_weight(number, total);
-  __syncthreads();
-  if (mine && before <= at && at < before + mine) {
-    d.found[0] = threadIdx.x;
-    d.found[1] = before;
-  }
-  __syncthreads();
-  const int i = (int)d.found[0] * CHUNK + (int)threadIdx.x;
-  const uint64_t under = d.found[1];
-  uint64_t w = 0;
-  float v = 0.0f;
-  if ((int)threadIdx.x < CHUNK && i < a.vocab) {
-    v = logit<DT>(a.logits + r * a.ld, i);
-    const double e = q.sc.weight(v);
-    if (kept(v, i, e)) w = units(e);
-  }
-  scan(w, before);
-  before += under;
-  if (w && before <= at && at < before + w) {
-    a.token[r] = i;
-    if (a.logprob) a.logprob[r] = logprob_of(q.sc.log2_weight(v), total);
-  }
+  if (last_of(&state.arrived[1], sp.slices)) draw<DT>(a, sp, r, q, c, u);
 }
 
 constexpr int WHOLE_VOCAB = 4096;  // rows of at most this many tokens take one workgroup
@@ -1134,10 +1158,6 @@ static hipError_t launch(const Args& a, int64_t rows, bool filters, char* ws, hi
   }
   if (e == hipSuccess) {
     weigh_kernel<DT><<<grid, SLICE_T, 0, st>>>(a, sp);
-    e = hipGetLastError();
-  }
-  if (e == hipSuccess) {
-    draw_kernel<DT><<<(unsigned)rows, T, 0, st>>>(a, sp);
     e = hipGetLastError();
   }
   return e;

@@ -297,7 +297,7 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
             bias = bias.contiguous()
         if residual is not None:
             residual = _row_view(residual)
-        out = torch.empty((m, n), dtype=out_dtype, device=gpu)
+        out = torch.empty(m, n, dtype=out_dtype, device=gpu)
         N.call("kq_int8_linear", code, a.data_ptr(), _row_stride(a), N.ptr(sx), w.data_ptr(), s.data_ptr(), m, n, kp,
                N.LIN_ACTIVATIONS[activation], N.ptr(bias), 0 if bias is None else N.DTYPE_CODES[bias.dtype],
                N.ptr(residual), n if residual is None else _row_stride(residual), N.DTYPE_CODES[out_dtype],

@@ -106,11 +106,13 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
         filters = k_rows is not None or k > 0 or p_rows is not None or p < 1
         need = N.library().kq_sample_tokens_workspace_size(rows, vocab, filters)
         ws = torch.empty(need, dtype=torch.uint8, device=gpu) if need > 0 else None
-        tokens = torch.empty(lead, dtype=torch.int64, device=gpu)
-        logprobs = torch.empty(lead, dtype=torch.float32, device=gpu) if return_logprobs else None
+        tokens = torch.empty(rows, dtype=torch.int64, device=gpu)  # (a torch.Size would cost a microsecond)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=gpu) if return_logprobs else None
         N.call("kq_sample_tokens", N.DTYPE_CODES[z.dtype], z.data_ptr(), ld, rows, vocab, u.data_ptr(), N.ptr(t_rows), t,
                N.ptr(k_rows), k, N.ptr(p_rows), p, N.ptr(m_rows), m, tokens.data_ptr(), N.ptr(logprobs), N.ptr(ws),
                max(need, 0), N.stream(gpu))
+    if len(lead) != 1:
+        tokens, logprobs = tokens.reshape(lead), None if logprobs is None else logprobs.reshape(lead)
     if host is not None:
         tokens, logprobs = tokens.to(host), None if logprobs is None else logprobs.to(host)
     return (tokens, logprobs) if return_logprobs else tokens
