@@ -206,14 +206,14 @@ struct Problem {
   }
 };
 
-// Rows that belong to no group are zeros.
+// Rows that belong to no group are zeros (workgroup w of `of` clears its share).
 template <int ES = 2>
-__device__ __forceinline__ void zero_rows(const Args& g, int cols) {
+__device__ __forceinline__ void zero_rows(const Args& g, int cols, int w, int of) {
   const int64_t beg = clamped(g.offsets[0], 0, g.rows), end = clamped(g.offsets[g.groups], beg, g.rows);
   const int64_t before = beg, after = g.rows - end;
-  for (int64_t i = blockIdx.x; i < before + after; i += gridDim.x) {
+  for (int64_t i = w; i < before + after; i += of) {
     char* p = g.out + (i < before ? i : end + i - before) * g.ld_out;
-    for (int c = (int)threadIdx.x * (16 / ES); c < cols; c += mm16::THREADS * (16 / ES))
+    for (int c = (int)threadIdx.x * (16 / ES); c < cols; c += (int)blockDim.x * (16 / ES))
       *reinterpret_cast<mm16::u32x4_t*>(p + ES * (int64_t)c) = mm16::u32x4_t{0u, 0u, 0u, 0u};
   }
 }
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void grouped_kernel(Args g) {
   Mine p;
   p.g = g;
   p.setup(lds);
-  if (MODE != DW) zero_rows<KIND == mm16::I8 && OUT == KQ_DT_F32 ? 4 : 2>(g, MODE == FORWARD ? g.n : g.k);
+  if (MODE != DW) zero_rows<KIND == mm16::I8 && OUT == KQ_DT_F32 ? 4 : 2>(g, MODE == FORWARD ? g.n : g.k, (int)blockIdx.x, (int)gridDim.x);
   mm16::Core<MODE == DW, MODE != FORWARD, KIND, MODE == DW ? mm16::WHOLE : mm16::SMALL_ROWS, true, STREAM, Mine> core(p, lds);
   core.run();
 }

@@ -1,7 +1,61 @@
 // 8-bit integers grouped by expert: y[r] = sx[r] sw_g (W_g q[r]) for the rows r of
 // group g, on the tiles of the 16-bit grouped product with the int8 matrix
 // instructions (kq_grouped.h, kq_int8.h).
+//
+// Few rows in all (FEW_EACH a group on average) take one pass over the weights of
+// each group that has rows (kq_int8_few.h), 16 rows at a time.
 #include "kq_grouped.h"
+#include "kq_int8_few.h"
+
+namespace kq {
+namespace int8 {
+
+// Workgroups: 16 R weight rows of a group each, then those that clear the rows of
+// no group.  Group sizes are device data: a group without rows is left at once, one of more
+// than 16 reads its weights again (from the caches) for the next 16.
+template <int OUT, int R, int P, bool TAIL>
+__global__ __launch_bounds__(512) void grouped_few_kernel(const grouped::Args g, int k, int tiles) {
+  constexpr int ES = OUT == KQ_DT_F32 ? 4 : 2;
+  const int e = (int)blockIdx.x / tiles;
+  if (e >= g.groups) {
+    grouped::zero_rows<ES>(g, g.n, (int)blockIdx.x - g.groups * tiles, (int)gridDim.x - g.groups * tiles);
+    return;
+  }
+  const int64_t beg = grouped::clamped(g.offsets[e], 0, g.rows), end = grouped::clamped(g.offsets[e + 1], beg, g.rows);
+  FewArgs f{};
+  f.a = g.rows_in + beg * g.ld_in;
+  f.lda = g.ld_in;
+  f.sx = g.sx + beg;
+  f.w = (const int8_t*)g.other + (int64_t)e * g.n * g.ld_other;
+  f.sw = g.sw + (int64_t)e * g.n;
+  f.c = g.out + beg * g.ld_out;
+  f.ldc = g.ld_out / ES;
+  f.m = (int)(end - beg);
+  f.n = g.n;
+  f.k = k;
+  f.epi.kind = EPI_OFF;
+  const int n0 = ((int)blockIdx.x - e * tiles) * 16 * R;
+  for (int m0 = 0; m0 < f.m; m0 += 16) {
+    few_rows<DT_CODES, OUT, 1, R, P, TAIL>(f, n0, m0);
+    __syncthreads();  // the sums have been read
+  }
+}
+
+template <int OUT>
+static hipError_t grouped_few(const grouped::Args& g, int k, hipStream_t st) {
+  constexpr int R = 2, P = 2;
+  const int tiles = (g.n + 16 * R - 1) / (16 * R), nwin = (k + WIN - 1) / WIN, waves = nwin < 8 ? nwin : 8;
+  const unsigned grid = (unsigned)(g.groups * tiles + 64);
+  const size_t lds = (size_t)waves * wave_lds(1, R);
+  if (k % WIN) grouped_few_kernel<OUT, R, P, true><<<grid, waves * 64, lds, st>>>(g, k, tiles);
+  else grouped_few_kernel<OUT, R, P, false><<<grid, waves * 64, lds, st>>>(g, k, tiles);
+  return hipGetLastError();
+}
+
+constexpr int FEW_EACH = 4;
+
+}  // namespace int8
+}  // namespace kq
 
 using namespace kq;
 
@@ -32,9 +86,16 @@ extern "C" int kq_int8_grouped_linear(const int8_t* x, int64_t ldx, const float*
                         (uint32_t)(es * ldy), offsets,        rows,     groups,        (int)n,
                         (int)(k / 2),         x_scale,        w_scale};
   hipStream_t st = (hipStream_t)stream;
+  hipError_t e;
+  if (rows <= (int64_t)int8::FEW_EACH * groups && (int64_t)groups * ((n + 31) / 32) < INT32_MAX / 2) {
+    e = out_dtype == KQ_DT_BF16  ? int8::grouped_few<KQ_DT_BF16>(g, (int)k, st)
+        : out_dtype == KQ_DT_F16 ? int8::grouped_few<KQ_DT_F16>(g, (int)k, st)
+                                 : int8::grouped_few<KQ_DT_F32>(g, (int)k, st);
+    return kq_check_launch(e, fn);
+  }
   int64_t grid;
   bool stream_weights;
-  hipError_t e = grouped::plan<grouped::FORWARD>(g, st, grid, stream_weights);
+  e = grouped::plan<grouped::FORWARD>(g, st, grid, stream_weights);
   if (e != hipSuccess) return kq_check_launch(e, fn);
   auto run = [&](auto out) {
     constexpr int OUT = decltype(out)::value;
