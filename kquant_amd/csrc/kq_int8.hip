@@ -124,7 +124,8 @@ static hipError_t launch_few(FewArgs f, hipStream_t st) {
 template <int DT, int OUT, bool TAIL>
 static hipError_t launch_few_rows(const FewArgs& f, hipStream_t st) {
   if constexpr (DT != DT_CODES) {
-    if (f.n >= 24576) return launch_few<DT, OUT, 1, 2, 2, TAIL>(f, st);
+    // (blocks share a workgroup's quantization too: N = 24576, 1 / 2 rows 33.6 / 38.7 us with one, 29.9 / 32.4 with three)
+    if (f.n >= 24576) return launch_few<DT, OUT, 1, 3, 2, TAIL>(f, st);
     return launch_few<DT, OUT, 1, 1, 2, TAIL>(f, st);
   } else {
     if (f.m <= 16) {
@@ -156,9 +157,11 @@ static bool takes_few(int64_t m, int64_t n, int64_t k, int64_t cus) {
 
 static inline int64_t up16(int64_t v) { return (v + 15) & ~(int64_t)15; }
 
-// Rows that the few-row kernel quantizes itself.
-static bool fuses(int a_dtype, int64_t m, int64_t k) {
-  return a_dtype != KQ_DT_I8 && m <= FUSED && k <= FUSED_K;
+// Whether the few-row kernel quantizes the rows itself.  Every workgroup does so
+// then, beside its first weights; a launch of its own takes 4.5 us.  K = 7168, us
+// over the product of codes: N = 12288, 1 / 2 / 4 rows 1.0 / 2.4 / 5.6, 24576 1.3 / 3.3 / 6.5, 129280 6 / 17 / 35.
+static bool fuses(int a_dtype, int64_t m, int64_t n, int64_t k) {
+  return a_dtype != KQ_DT_I8 && m <= FUSED && k <= FUSED_K && (double)m * (double)n * (double)k <= 3.5e8;
 }
 
 template <int OUT>
@@ -197,7 +200,7 @@ extern "C" int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t r
 
 extern "C" int64_t kq_int8_linear_workspace_size(int a_dtype, int64_t m, int64_t n, int64_t k) {
   if (m < 0 || n < 0 || k < 1) return -1;
-  if (a_dtype == KQ_DT_I8 || fuses(a_dtype, m, k)) return 0;
+  if (a_dtype == KQ_DT_I8 || fuses(a_dtype, m, n, k)) return 0;
   return up16(m * up16(k)) + 4 * m;  // the rows' codes and scales
 }
 
@@ -244,7 +247,7 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
   const char* rows = (const char*)a;
   int64_t ld = lda;
   const float* sx = a_scale;
-  const bool fused = fuses(a_dtype, m, k);
+  const bool fused = fuses(a_dtype, m, n, k);
   if (!codes && !fused) {
     int8_t* q = (int8_t*)workspace;
     float* s = (float*)((char*)workspace + up16(m * k));

@@ -124,8 +124,10 @@ def check(got, q, sx, w, sw, bias, kind, residual, dtype):
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} outside, first at {bad.nonzero()[0].tolist()}"
 
 
-# fused few rows, few rows, the same with 32 and 64 rows, tiles of every height, each ragged
-SHAPES = [(1, 264, 256), (3, 77, 144), (4, 129, 7168), (5, 129, 512), (16, 1000, 208), (17, 264, 192), (33, 129, 512),
+# fused few rows (one and three weight blocks, and past the size that is fused), few rows (one to four blocks), the
+# same with 32 and 64 rows, tiles of every height, each ragged
+SHAPES = [(1, 24600, 144), (2, 24577, 400), (4, 129, 8192), (2, 129, 8208), (3, 40100, 3056), (6, 12300, 80), (13, 41000, 80),
+          (7, 41000, 48), (20, 8200, 144), (50, 8200, 144), (1, 264, 256), (3, 77, 144), (4, 129, 7168), (5, 129, 512), (16, 1000, 208), (17, 264, 192), (33, 129, 512),
           (64, 40, 1040), (65, 264, 128), (100, 520, 2048), (130, 1033, 16), (300, 777, 192), (257, 300, 64),
           (700, 512, 272), (4100, 4104, 256)]
 
