@@ -323,7 +323,7 @@ int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x,
 /* ---------------------------------------------------------- 8-bit integers -- */
 
 /* Rows as 8-bit integers with one scale a row (no kquant counterpart):
- *   scale[r] = max(fl(max_k |x[r][k]| / 127), 2^-126),
+ *   scale[r] = max(fl(max_k |x[r][k]| fl(1 / 127)), 2^-126) in fp32,
  *   q[r][k] = the integer nearest to x[r][k] / scale[r], of two the even one,
  * of the exact quotient.  A row with an infinity or a NaN: scale NaN, codes 0.
  * dtype: KQ_DT_*; x [rows, k] (row stride ldx elements) and q (row stride ldq)

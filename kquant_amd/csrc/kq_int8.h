@@ -16,16 +16,16 @@ namespace int8 {
 
 constexpr int64_t MAX_K = (1 << 17) - 16;  // the sums' bound, in whole 16-byte pieces
 
-// A row's scale from the largest magnitude's bits: a 127th of it, rounded once,
-// and at least 2^-126, so that quotients by it need no subnormal scale.  A row
-// with an infinity or a NaN has scale NaN (and codes 0): what it multiplies is
-// NaN, and no other row is.
+// A row's scale from the largest magnitude's bits: its product with the fp32 number
+// nearest to 1 / 127, rounded once, and at least 2^-126, so that quotients by it
+// need no subnormal scale.  A row with an infinity or a NaN has scale NaN (and
+// codes 0): what it multiplies is NaN, and no other row is.
 __device__ __forceinline__ float row_scale(uint32_t magnitude) {
   if (magnitude >= 0x7f800000u) return __builtin_nanf("");
-  return fmaxf(__fdiv_rn(__uint_as_float(magnitude), 127.0f), 0x1p-126f);
+  return fmaxf(__uint_as_float(magnitude) * 0x1.0204080000000p-7f, 0x1p-126f);
 }
 
-// The integer nearest to x / s, the even one of two, for |x| <= 127 s (1 + 2^-23)
+// The integer nearest to x / s, the even one of two, for |x| <= 127 s (1 + 2^-22)
 // and inv near 1 / s.  n is off by one at most, and r = x - n s shows it: with
 // s = S 2^e (S of 24 bits) r is a multiple of 2^(e-1), so every r with
 // |r| <= s / 2 + 2^(e-1) is exact in fp32, a tie included, and a larger one is

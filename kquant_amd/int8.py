@@ -43,9 +43,9 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes (int8 [..., K]) and scales (fp32 [...]) of the rows of x [..., K],
     bf16, fp16 or fp32:
 
-        scale = max(fp32(max |x| / 127), 2^-126),  q = round(x / scale)
+        scale = max(max |x| * fp32(1 / 127), 2^-126),  q = round(x / scale)
 
-    with the exact quotient rounded to nearest, ties to even, so the codes do
+    with the product rounded to fp32 and the exact quotient rounded to nearest, ties to even, so the codes do
     not depend on how the division is carried out.  A row with an infinity or a
     NaN has scale NaN and codes 0: whatever it is multiplied with is NaN, and no
     other row is.  A row of zeros has codes 0.  The results carry no gradient.

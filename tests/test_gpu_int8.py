@@ -1,8 +1,8 @@
 """8-bit integers: quantized rows, the dense linear and the products grouped by
 expert, against their definitions in float64.
 
-Tolerances.  Codes and int32 sums are exact.  A scale is one fp32 division,
-within half a step.  A product's sum is rounded to fp32 (2^-24) and multiplied
+Tolerances.  Codes and int32 sums are exact.  A scale is one fp32 product,
+rounded once.  A product's sum is rounded to fp32 (2^-24) and multiplied
 by two scales (2^-24 each): 3.01 2^-24 of the value.  The epilogue's steps are
 those of tests/test_gpu_linear_epilogue.py: a bias addition (2^-24), activations
 no steeper than 1.13 and within 16 2^-24 |x| (the exact GELU 0.8e-7 more), the
@@ -32,7 +32,8 @@ def codes64(x):
     x = x.double()
     finite = torch.isfinite(x).all(-1)
     top = torch.where(finite, torch.nan_to_num(x).abs().amax(-1), torch.ones((), dtype=torch.float64, device=x.device))
-    scale = (top / 127).float().double().clamp(min=2.0 ** -126)
+    part = torch.tensor(1.0, dtype=torch.float32) / 127  # the fp32 number nearest to a 127th
+    scale = (top * float(part)).float().double().clamp(min=2.0 ** -126)  # (48 bits: exact before its rounding)
     q = torch.round(torch.nan_to_num(x) / scale[..., None])
     q = torch.where(finite[..., None], q, torch.zeros_like(q))
     return q, torch.where(finite, scale, torch.full_like(scale, float("nan")))
@@ -44,7 +45,7 @@ def check_codes(q, scale, x):
     assert torch.equal(q.double(), want)
     assert torch.equal(torch.isnan(scale), torch.isnan(s))
     fine = ~torch.isnan(s)
-    assert torch.equal(scale[fine].double(), s[fine])  # one division, rounded once
+    assert torch.equal(scale[fine].double(), s[fine])  # one product, rounded once
 
 
 def rows(m, k, dtype, gpu, seed=0):
