@@ -338,8 +338,10 @@ int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
  * kq_int8_quantize does (a_scale is not read).  activation, bias, residual as
  * kq_mx_linear_epilogue takes them, the residual of out_dtype (row stride ldr).
  * k % 16 == 0, k <= 131056; w and codes 16-byte aligned, lda of codes a multiple
- * of 16.  workspace: kq_int8_linear_workspace_size bytes (the rows' codes; 0 for
- * codes and a few rows), 16-byte aligned, written and read by this call alone. */
+ * of 16.  workspace: kq_int8_linear_workspace_size bytes on the device current then
+ * (the rows' codes, and sums of slices of k where the output has few tiles; 0 for codes
+ * and for few rows), 16-byte aligned, written and read by this call alone; one that
+ * holds the codes but not the slices runs without them. */
 int64_t kq_int8_linear_workspace_size(int a_dtype, int64_t m, int64_t n, int64_t k);
 int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const float* a_scale, const int8_t* w, const float* w_scale,
                    int64_t m, int64_t n, int64_t k, int activation, const void* bias, int bias_dtype,

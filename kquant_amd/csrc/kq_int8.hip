@@ -157,6 +157,19 @@ static bool takes_few(int64_t m, int64_t n, int64_t k, int64_t cus) {
 
 static inline int64_t up16(int64_t v) { return (v + 15) & ~(int64_t)15; }
 
+// CUs of the stream's device (of the current one without a stream); 0 where there is none.
+static int64_t device_cus(hipStream_t st) {
+  int dev = 0, cus = 0;
+  hipError_t e = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
+  if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return cus;
+}
+static int workers(int64_t cus) { return cus >= 8 ? (int)(cus / 8 * 8) : 8; }
+
 // Whether the few-row kernel quantizes the rows itself.  Every workgroup does so
 // then, beside its first weights; a launch of its own takes 4.5 us.  K = 7168, us
 // over the product of codes: N = 12288, 1 / 2 / 4 rows 1.0 / 2.4 / 5.6, 24576 1.3 / 3.3 / 6.5, 129280 6 / 17 / 35.
@@ -198,10 +211,18 @@ extern "C" int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t r
   return kq_check_launch(quantize(dtype, x, ldx, rows, k, q, ldq, k, scale, (hipStream_t)stream), fn);
 }
 
+// The rows' codes and scales.
+static int64_t codes_bytes(int a_dtype, int64_t m, int64_t n, int64_t k) {
+  return a_dtype == KQ_DT_I8 || fuses(a_dtype, m, n, k) ? 0 : up16(m * up16(k)) + up16(4 * m);
+}
+
 extern "C" int64_t kq_int8_linear_workspace_size(int a_dtype, int64_t m, int64_t n, int64_t k) {
   if (m < 0 || n < 0 || k < 1) return -1;
-  if (a_dtype == KQ_DT_I8 || fuses(a_dtype, m, n, k)) return 0;
-  return up16(m * up16(k)) + 4 * m;  // the rows' codes and scales
+  int64_t bytes = codes_bytes(a_dtype, m, n, k);
+  if (m == 0 || n == 0 || m <= 16) return bytes;
+  const int64_t cus = device_cus(nullptr);
+  if (cus > 0 && !takes_few(m, n, k, cus)) bytes += dense_plan(m, n, k, workers(cus), true).bytes;
+  return bytes;
 }
 
 extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const float* a_scale, const int8_t* w,
@@ -234,7 +255,7 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
       kq_misaligned(a_scale, 4) || kq_misaligned(c, os) || kq_misaligned(residual, os) ||
       kq_misaligned(bias, bias_dtype == KQ_DT_F32 ? 4 : 2) || kq_misaligned(workspace, 16))
     return kq_fail(KQ_ERR_INVALID, "%s: weights, codes and workspace must be 16-byte aligned, the others to their type", fn);
-  const int64_t need = kq_int8_linear_workspace_size(a_dtype, m, n, k);
+  const int64_t need = codes_bytes(a_dtype, m, n, k);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return kq_fail(KQ_ERR_INVALID, "%s: workspace needs %lld bytes", fn, (long long)need);
   hipStream_t st = (hipStream_t)stream;
@@ -259,14 +280,9 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
   } else if (!codes) {
     ld = lda * (a_dtype == KQ_DT_F32 ? 4 : 2);
   }
-  int cus = 0;
-  if (m > 16 && m <= FEW) {
-    int dev = 0;
-    hipError_t err = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
-    if (err == hipSuccess) err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-    if (err != hipSuccess) return kq_check_launch(err, fn);
-  }
-  if (takes_few(m, n, k, cus > 0 ? cus : 1)) {
+  const int64_t cus = m > 16 ? device_cus(st) : 1;
+  if (cus <= 0) return kq_fail(KQ_ERR_HIP, "%s: no device", fn);
+  if (takes_few(m, n, k, cus)) {
     const FewArgs f{rows, ld, sx, w, w_scale, c, ldc, (int)m, (int)n, (int)k, 1, e};
     const int dt = fused ? a_dtype : KQ_DT_I8;
     const hipError_t err = out_dtype == KQ_DT_BF16  ? few<KQ_DT_BF16>(dt, f, st)
@@ -289,7 +305,19 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
   g.epi = e;
   g.pieces = os == 2 && n % 8 == 0 && ldc % 8 == 0 && !kq_misaligned(c, 16) &&
              (!residual || (ldr % 8 == 0 && !kq_misaligned(residual, 16)));
-  return kq_check_launch(out_dtype == KQ_DT_BF16  ? dense_bf16(g, st)
-                         : out_dtype == KQ_DT_F16 ? dense_f16(g, st)
-                                                  : dense_f32(g, st), fn);
+  const int grid = workers(cus);
+  DensePlan plan = dense_plan(m, n, k, grid, true);
+  const bool split = plan.slices > 1 && workspace && workspace_bytes >= need + plan.bytes;
+  if (plan.slices > 1 && !split) plan = dense_plan(m, n, k, grid, false);  // without room for the planes
+  g.tm = plan.tm;
+  g.mtiles = (g.m + g.tm - 1) / g.tm;
+  g.ntiles = (g.n + mm16::BN - 1) / mm16::BN;
+  g.slices = plan.slices;
+  g.ks = plan.ks;
+  g.planes = split ? (int*)((char*)workspace + need) : nullptr;
+  return kq_check_launch(split                     ? dense_split(g, out_dtype, grid, st)
+                         : out_dtype == KQ_DT_BF16 ? dense_bf16(g, grid, st)
+                         : out_dtype == KQ_DT_F16  ? dense_f16(g, grid, st)
+                                                   : dense_f32(g, grid, st),
+                         fn);
 }

@@ -19,13 +19,24 @@ struct DenseArgs {
   int m, n, k;
   int tm;             // rows of a tile
   int mtiles, ntiles;
+  int slices, ks;     // of k, and the bytes of one (a multiple of 128)
+  int* planes;        // the slices' sums [slices][m][n]
   Epilogue epi;
   int pieces;
 };
 
-hipError_t dense_bf16(const DenseArgs& g, hipStream_t st);
-hipError_t dense_f16(const DenseArgs& g, hipStream_t st);
-hipError_t dense_f32(const DenseArgs& g, hipStream_t st);
+hipError_t dense_bf16(const DenseArgs& g, int grid, hipStream_t st);
+hipError_t dense_f16(const DenseArgs& g, int grid, hipStream_t st);
+hipError_t dense_f32(const DenseArgs& g, int grid, hipStream_t st);
+
+// How an m x n product over k is cut: the tiles' height, and slices of k where the
+// tiles alone leave most CUs without one; cus workgroups run.
+struct DensePlan {
+  int tm, slices, ks;
+  int64_t bytes;  // of the planes
+};
+DensePlan dense_plan(int64_t m, int64_t n, int64_t k, int64_t cus, bool split);
+hipError_t dense_split(const DenseArgs& g, int out, int grid, hipStream_t st);
 
 template <int OUT, int EPI>
 struct Dense {
@@ -81,25 +92,7 @@ __global__ __launch_bounds__(mm16::THREADS, 1) void dense_kernel(const DenseArgs
 }
 
 template <int OUT>
-static hipError_t dense(DenseArgs g, hipStream_t st) {
-  int dev = 0, cus = 0;
-  hipError_t e = st ? hipStreamGetDevice(st, &dev) : hipGetDevice(&dev);
-  if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
-  if (e != hipSuccess) return e;
-  const int grid = cus >= 8 ? cus / 8 * 8 : 8;
-  // A step of a tile takes its loads' way from L2 besides its products: at K = 7168 a round of tiles of 32 / 64 / 128 /
-  // 256 rows takes 28 / 35 / 52 / 77 us, so 88 + rows.  The height with the shortest rounds in all (256 x 12288: 80 us in
-  // 48 tiles of 256 rows, 39 in 192 of 64; 512 rows 93 and 57 of 128; 1024 rows 94, 107 and 109).
-  g.ntiles = (g.n + mm16::BN - 1) / mm16::BN;
-  int64_t least = 0;
-  for (int tm : {32, 64, 96, 128, 256}) {
-    const int64_t tiles = ((int64_t)g.m + tm - 1) / tm * g.ntiles, cost = (tiles + grid - 1) / grid * (88 + tm);
-    if (least == 0 || cost <= least) {
-      least = cost;
-      g.tm = tm;
-    }
-  }
-  g.mtiles = (g.m + g.tm - 1) / g.tm;
+static hipError_t dense(const DenseArgs& g, int grid, hipStream_t st) {
   auto kern = g.epi.kind == EPI_OFF       ? dense_kernel<OUT, EPI_OFF>
               : g.epi.kind == EPI_CLAMP   ? dense_kernel<OUT, EPI_CLAMP>
               : g.epi.kind == EPI_SIGMOID ? dense_kernel<OUT, EPI_SIGMOID>

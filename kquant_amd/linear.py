@@ -289,7 +289,7 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
         elif kp != k:
             a, sx = _quantize(a, kp)
         code = N.DT_I8 if sx is not None else N.DTYPE_CODES[a.dtype]
-        if sx is None:
+        if sx is None or m > 16:
             need = N.library().kq_int8_linear_workspace_size(code, m, n, kp)
             if need > 0:
                 ws = torch.empty(need, dtype=torch.uint8, device=gpu)

@@ -126,9 +126,9 @@ def check(got, q, sx, w, sw, bias, kind, residual, dtype):
 
 
 # fused few rows (one and three weight blocks, and past the size that is fused), few rows (one to four blocks), the
-# same with 32 and 64 rows, tiles of every height, each ragged
+# same with 32 and 64 rows, slices of k, tiles of every height, each ragged
 SHAPES = [(1, 24600, 144), (2, 24577, 400), (4, 129, 8192), (2, 129, 8208), (3, 40100, 3056), (6, 12300, 80), (13, 41000, 80),
-          (7, 41000, 48), (20, 8200, 144), (50, 8200, 144), (1, 264, 256), (3, 77, 144), (4, 129, 7168), (5, 129, 512), (16, 1000, 208), (17, 264, 192), (33, 129, 512),
+          (7, 41000, 48), (1187, 74, 4192), (83, 70, 4096), (300, 384, 7168), (65, 24, 1040), (520, 8, 16384 + 48), (20, 8200, 144), (50, 8200, 144), (1, 264, 256), (3, 77, 144), (4, 129, 7168), (5, 129, 512), (16, 1000, 208), (17, 264, 192), (33, 129, 512),
           (64, 40, 1040), (65, 264, 128), (100, 520, 2048), (130, 1033, 16), (300, 777, 192), (257, 300, 64),
           (700, 512, 272), (4100, 4104, 256)]
 
@@ -147,7 +147,7 @@ def test_linear(gpu, shape, dtype):
 
 
 @pytest.mark.parametrize("shape", [(1, 264, 256), (4, 129, 144), (16, 264, 256), (40, 77, 400), (300, 776, 192), (300, 777, 192),
-                                   (131, 1024, 128)], ids=str)
+                                   (131, 1024, 128), (100, 72, 2064)], ids=str)
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_epilogue(gpu, shape, kind, dtype):
@@ -273,3 +273,20 @@ def test_grouped_odd_k(gpu):
     y = int8_grouped_linear(x, w, sw, torch.tensor([0, 10, 30, 50], device=gpu))
     check_grouped(y, q, sx, w, sw, [0, 10, 30, 50], torch.bfloat16)
     assert torch.equal(y, int8_grouped_linear(q, w, sw, torch.tensor([0, 10, 30, 50], device=gpu), x_scale=sx))
+
+
+def test_workspace_without_slices(gpu):
+    """Room for the codes alone, and for the slices of k too: the same bits; what is behind the workspace stays."""
+    m, n, k = 200, 72, 4096
+    x, (w, sw) = rows(m, k, torch.bfloat16, gpu), weights(n, k, gpu)
+    want = int8_linear(x, w, sw)
+    need = int(N.library().kq_int8_linear_workspace_size(N.DT_BF16, m, n, k))
+    codes = m * k + (4 * m + 15) // 16 * 16
+    assert need > codes
+    for size in (codes, need - 4, need):
+        ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device=gpu)
+        y = torch.full((m + 1, n), 7.0, dtype=torch.bfloat16, device=gpu)
+        N.call("kq_int8_linear", N.DT_BF16, N.ptr(x), k, None, N.ptr(w), N.ptr(sw), m, n, k, 0, None, 0, None, n, N.DT_BF16,
+               N.ptr(y), n, N.ptr(ws), size, N.stream(x.device))
+        assert torch.equal(y[:m], want) and (y[m] == 7).all()
+        assert (ws[max(size, codes):] == 77).all()
