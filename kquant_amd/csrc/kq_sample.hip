@@ -178,7 +178,7 @@ struct Shared {
   unsigned int count[BINS];
   unsigned long long chunk[CHUNKS];
   uint64_t part[T / 64];
-  uint64_t found[4];
+  uint64_t found[5];
 };
 
 // Sum of v over the workgroup, and (before) of the threads below this one.
@@ -207,7 +207,7 @@ struct Cut {
 // tokens together reach it.
 template <int DT, bool BY_COUNT>
 __device__ __forceinline__ Cut select(const char* row, int vocab, const Scale& sc, uint64_t target, Shared& s) {
-  uint64_t prefix = 0, count = 0, mass = 0;
+  uint64_t prefix = 0, count = 0, mass = 0, own = 0;
   constexpr int SHIFTS[6] = {53, 42, 31, 20, 9, 0};
   int top = 64;
   for (int step = 0; step < 6; ++step) {
@@ -247,6 +247,7 @@ __device__ __forceinline__ Cut select(const char* row, int vocab, const Scale& s
         s.found[1] = cb;
         s.found[2] = mb;
         s.found[3] = m[j];
+        s.found[4] = c[j];
       }
       cb += c[j];
       mb += m[j];
@@ -255,9 +256,21 @@ __device__ __forceinline__ Cut select(const char* row, int vocab, const Scale& s
     prefix |= (~s.found[0] & ((1u << bits) - 1)) << shift;
     count = s.found[1];
     mass = s.found[2];
+    own = s.found[3];
     top = shift;
+    if (shift > 0 && s.found[4] == 1) {  // one token is left: its other digits are read from it
+      __syncthreads();                   // (all have read what was found)
+      for (int i = threadIdx.x; i < vocab; i += T) {
+        const uint64_t place = place_of(logit<DT>(row, i), i);
+        if (!((place ^ prefix) >> shift)) s.found[0] = place;
+      }
+      __syncthreads();
+      prefix = s.found[0];
+      break;
+    }
   }
-  return Cut{prefix, mass + s.found[3]};
+  __syncthreads();  // (the next search writes there)
+  return Cut{prefix, mass + own};
 }
 
 template <int DT>
@@ -1100,7 +1113,10 @@ __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const S
   if (last_of(&state.arrived[1], sp.slices)) draw<DT>(a, sp, r, q, c, u);
 }
 
-constexpr int WHOLE_VOCAB = 4096;  // rows of at most this many tokens take one workgroup
+// Rows of at most this many tokens take one workgroup and launch.  One row, us so and in slices: 1024 tokens without
+// filters 11, 15, with top-k 12, 21, with both 17, 23; 4096 11, 15, with top-k 16, 22, with both 25, 23; 2048 rows of
+// 4096 34, 40, 81, 103, 131, 111.
+constexpr int WHOLE_VOCAB = 4096;
 
 struct Plan {
   int chunks, per, slices;
