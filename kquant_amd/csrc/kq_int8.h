@@ -137,6 +137,31 @@ __device__ __forceinline__ float of16(uint32_t h) {
   return OUT == KQ_DT_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
 }
 
+// A value as it is in fp32.  Without this a product, sum or rounding to fp16 that
+// follows may become one instruction with the one before it, here and not there, and
+// a result would depend on the path that it took.
+__device__ __forceinline__ float settled(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
+// A sum scaled and finished up to the residual, in the same steps on every path.
+template <int OUT, int EPI>
+__device__ __forceinline__ float finished(const Epilogue& e, int sum, float sx, float sw, float bias) {
+  const float t = settled((float)sum * sx);
+  if (EPI == EPI_OFF) return settled(t * sw);
+  const float v = settled(fmaf(t, sw, bias));
+  return settled(OUT == KQ_DT_F32 ? epi_activate<EPI>(e, v) : epi_activate16<EPI>(e, v));
+}
+// the class decided at run time
+template <int OUT>
+__device__ __forceinline__ float finished_any(const Epilogue& e, int sum, float sx, float sw, float bias) {
+  return e.kind == EPI_OFF       ? finished<OUT, EPI_OFF>(e, sum, sx, sw, bias)
+         : e.kind == EPI_SIGMOID ? finished<OUT, EPI_SIGMOID>(e, sum, sx, sw, bias)
+         : e.kind == EPI_ERF     ? finished<OUT, EPI_ERF>(e, sum, sx, sw, bias)
+                                 : finished<OUT, EPI_CLAMP>(e, sum, sx, sw, bias);
+}
+
 // Scales, finishes and stores a wave's blocks: rows below `rows` and columns
 // below `cols` of the tile (element (i, j, r) as in mm16::each).  The scales of
 // the wave's rows are in two registers, a row a lane, and reach their elements
@@ -158,11 +183,7 @@ __device__ __forceinline__ void finish(const Finish& f, int rows, int cols, int 
     bias[j] = EPI != EPI_OFF ? epi_bias(f.epi, c) : 0.0f;
   }
   // of element (i, j, r) with row scale s
-  auto value = [&](float a, float s, int j) {
-    const float v = (float)__float_as_int(a) * s * sw[j];
-    if (EPI == EPI_OFF) return v;
-    return OUT == KQ_DT_F32 ? epi_activate<EPI>(f.epi, v + bias[j]) : epi_activate16<EPI>(f.epi, v + bias[j]);
-  };
+  auto value = [&](float a, float s, int j) { return finished<OUT, EPI>(f.epi, __float_as_int(a), s, sw[j], bias[j]); };
   auto scale_of = [&](int i, int r) { return __shfl(sx[i / 2], 32 * (i & 1) + 8 * (r >> 2) + (r & 3) + half); };
   const bool residual = EPI != EPI_OFF && f.epi.residual;
   if (OUT != KQ_DT_F32 && f.pieces) {
@@ -200,7 +221,7 @@ __device__ __forceinline__ void finish(const Finish& f, int rows, int cols, int 
             const uint32_t h = res[j][(r & 3) >> 1];
             v += of16<OUT>(r & 1 ? h >> 16 : h & 0xffffu);
           }
-          return v;
+          return residual ? settled(v) : v;
         });
         const int at = row + 32 * i + 8 * g;
         char* p = f.out + (int64_t)min(at, rows - 1) * f.ld + 2 * (int64_t)col;
@@ -237,7 +258,7 @@ __device__ __forceinline__ void finish(const Finish& f, int rows, int cols, int 
         char* p = f.out + (int64_t)at * f.ld + (int64_t)col * ES;
 #pragma unroll
         for (int j = 0; j < WN; ++j) {
-          const float v = value(acc[i][j][4 * g + r], s, j) + epi_residual_value<OUT>(res[r][j]);
+          const float v = settled(value(acc[i][j][4 * g + r], s, j) + epi_residual_value<OUT>(res[r][j]));
           if (col + 32 * j >= cols) continue;
           if (OUT == KQ_DT_F32) *reinterpret_cast<float*>(p + 32 * ES * j) = v;
           else *reinterpret_cast<uint16_t*>(p + 32 * ES * j) = (uint16_t)mm16::pack16<OUT == KQ_DT_F16>(v, 0.0f);

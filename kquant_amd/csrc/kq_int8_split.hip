@@ -6,9 +6,9 @@
 namespace kq {
 namespace int8 {
 
-// A step of a tile takes its loads' way from L2 besides its products: at K = 7168
-// (56 steps) a round of tiles of 32 / 64 / 128 / 256 rows takes 28 / 35 / 52 / 77 us,
-// so 88 + rows.  The cut with the least rounds in all (256 x 12288: 80 us in 48 tiles
+// A step of a tile is bounded by its reads of LDS, in which the 256 columns' share is
+// the same for every tile: at K = 7168 (56 steps) a round of tiles of 32 / 64 / 128 /
+// 256 rows takes 28 / 35 / 52 / 77 us, so 88 + rows.  The cut with the least rounds in all (256 x 12288: 80 us in 48 tiles
 // of 256 rows, 39 in 192 of 64; 512 rows 93 and 57 of 128; 1024 rows 94, 107 and 109).
 // Planes cost a launch and their bytes.
 DensePlan dense_plan(int64_t m, int64_t n, int64_t k, int64_t cus, bool split) {
@@ -88,10 +88,9 @@ __global__ __launch_bounds__(256) void join_kernel(const DenseArgs g) {
     const int64_t m = i / g.n, n = i - m * g.n;
     int sum = 0;
     for (int s = 0; s < g.slices; ++s) sum += g.planes[s * all + i];
-    float y = (float)sum * g.sx[m] * g.sw[n];
     constexpr int RES = OUT == KQ_DT_F32 ? KQ_DT_F32 : KQ_DT_BF16;
-    if (g.epi.kind != EPI_OFF)
-      y = epi_activate_any(g.epi, y + epi_bias(g.epi, n)) + epi_residual_value<OUT>(epi_residual_bits<RES>(g.epi, m, n));
+    const float y = settled(finished_any<OUT>(g.epi, sum, g.sx[m], g.sw[n], epi_bias(g.epi, n)) +
+                            epi_residual_value<OUT>(epi_residual_bits<RES>(g.epi, m, n)));
     char* p = g.out + m * g.ld + n * (OUT == KQ_DT_F32 ? 4 : 2);
     if (OUT == KQ_DT_F32) *reinterpret_cast<float*>(p) = y;
     else *reinterpret_cast<uint16_t*>(p) = (uint16_t)mm16::pack16<OUT == KQ_DT_F16>(y, 0.0f);

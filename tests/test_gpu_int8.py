@@ -290,3 +290,25 @@ def test_workspace_without_slices(gpu):
                N.ptr(y), n, N.ptr(ws), size, N.stream(x.device))
         assert torch.equal(y[:m], want) and (y[m] == 7).all()
         assert (ws[max(size, codes):] == 77).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m", [3, 40, 100, 300])
+def test_rows_are_independent(gpu, m, dtype):
+    """A row's bits depend neither on the path that its batch takes nor on the alignment of what it is written to."""
+    x, (w, sw) = rows(m, 272, dtype, gpu, m), weights(264, 272, gpu)
+    g = torch.Generator(device=gpu).manual_seed(4)
+    bias, residual = torch.randn(264, generator=g, device=gpu), torch.randn(m, 264, generator=g, device=gpu).to(dtype)
+    for keywords in ({}, {"bias": bias}, {"residual": residual}, *({"bias": bias, "activation": kind, "residual": residual}
+                                                                  for kind in KINDS)):
+        y = int8_linear(x, w, sw, **keywords)
+        one = dict(keywords)
+        for r in (0, m - 1):
+            if "residual" in one:
+                one["residual"] = residual[r:r + 1]
+            assert torch.equal(int8_linear(x[r:r + 1], w, sw, **one), y[r:r + 1])
+        cut = dict(keywords)
+        for name in ("bias", "residual"):
+            if name in cut:
+                cut[name] = cut[name][..., 1:]
+        assert torch.equal(int8_linear(x, w[1:], sw[1:], **cut), y[:, 1:])  # 263 columns: no whole 16-byte pieces
