@@ -78,7 +78,9 @@ struct Scale {
   double M, a;  // the top (1e300 for an infinite one) and log2(e) / t
   __device__ __forceinline__ Scale() {}
   __device__ __forceinline__ Scale(float m, double t)
-      : top(m), M(m == __builtin_inff() ? 1e300 : (double)m), a(fmin(1.4426950408889634 / t, 1e300)) {}
+      : top(m),
+        M(m == __builtin_inff() ? 1e300 : (double)m),
+        a(fmax(fmin(1.4426950408889634 / t, 1e300), m == __builtin_inff() ? 1.0 : 0.0)) {}  // (t may be infinite)
   // log2 of a weight: 0 for the top (an infinite one too), no less than -60, which is no weight
   __device__ __forceinline__ double log2_weight(float v) const { return fmin(fmax(((double)v - M) * a, -60.0), 0.0); }
   // The weight in units, not rounded: 2^(k + UNIT) 2^f with |f| <= 1/2, 2^f by the polynomial of degree 10 that meets
@@ -396,6 +398,7 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
 // rows three passes over the logits, of 8 us each at 33 MB, and where many tokens
 // have weight their exponentials, some 26 instructions each.
 constexpr int SLICE_T = T;
+static_assert(CHUNKS <= SLICE_T && CHUNK <= SLICE_T, "a thread for each chunk and each token of one");
 constexpr int NEAR = 1024;   // listed tokens that a workgroup gathers before they go to the list
 constexpr int NBINS = 2048, FAR_BIN = NBINS - 1;  // FAR_BIN: tokens of no weight
 constexpr int BINS_EACH = NBINS / SLICE_T;        // a thread's bins where a workgroup looks through them
@@ -1069,6 +1072,7 @@ __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const S
       [&] {
         if (sp.filters) c = state.cuts;  // (on its way beside the slices' maxima)
         q = row_of(a, sp, r);
+        __syncthreads();  // (`gathered` is 0)
         run = !q.none && !q.greedy;
         if (!run) return false;
         cuts = q.cuts();

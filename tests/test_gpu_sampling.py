@@ -243,3 +243,21 @@ def test_cuts_at_every_place(gpu):
     p = torch.linspace(0.0005, 0.9995, 301, device=gpu)
     check(z.expand(301, 6000), u[:301], top_p=p)
     check(z.expand(301, 6000), u[:301], top_p=p, top_k=k[:301] * 3)
+
+
+@pytest.mark.parametrize("vocab", [1000, 20000])
+@pytest.mark.parametrize("settings", [{}, {"top_k": 50}, {"top_p": 0.9}, {"top_k": 50, "top_p": 0.9}, {"min_p": 0.5}], ids=str)
+def test_infinite_temperatures(gpu, vocab, settings):
+    """A row's own temperature may be infinite: its finite logits share the draw, or its infinite ones where there are."""
+    m = 24
+    z, u = rows(m, vocab, torch.float32, gpu, 21)
+    z[:, ::3] = -math.inf
+    z[::2, 7] = z[::2, vocab - 2 - (vocab - 2) % 3 + 1] = math.inf
+    t = torch.full((m,), math.inf, device=gpu)
+    tokens, logprobs = sample_tokens(z, u, temperature=t, return_logprobs=True, **settings)
+    picked = z.gather(1, tokens[:, None])[:, 0]
+    assert torch.equal(picked == math.inf, torch.arange(m, device=gpu) % 2 == 0) and not (picked == -math.inf).any()
+    if "top_p" not in settings:  # logarithms of whole numbers, in fp64 rounded once
+        odd = min(settings.get("top_k", vocab), int((z[1] > -math.inf).sum()))
+        for r in range(m):
+            assert abs(logprobs[r].item() + math.log(odd if r % 2 else 2)) <= 2.0 ** -24 * 12 + 1e-12
