@@ -337,7 +337,7 @@ int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
  * codes with a_scale [m]; otherwise rows of that type, quantized as
  * kq_int8_quantize does (a_scale is not read).  activation, bias, residual as
  * kq_mx_linear_epilogue takes them, the residual of out_dtype (row stride ldr).
- * k % 16 == 0, k <= 131056; w and codes 16-byte aligned, lda of codes a multiple
+ * k % 16 == 0, k <= 131056, n <= 2^26; w and codes 16-byte aligned, lda of codes a multiple
  * of 16.  workspace: kq_int8_linear_workspace_size bytes on the device current then
  * (the rows' codes, and sums of slices of k where the output has few tiles; 0 for codes
  * and for few rows), 16-byte aligned, written and read by this call alone; one that

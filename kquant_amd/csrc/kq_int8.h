@@ -162,6 +162,12 @@ __device__ __forceinline__ float finished_any(const Epilogue& e, int sum, float 
                                  : finished<OUT, EPI_CLAMP>(e, sum, sx, sw, bias);
 }
 
+// With the residual's bits, where there is one.
+template <int OUT>
+__device__ __forceinline__ float added(const Epilogue& e, float v, uint32_t bits) {
+  return e.residual ? settled(v + epi_residual_value<OUT>(bits)) : v;
+}
+
 // Scales, finishes and stores a wave's blocks: rows below `rows` and columns
 // below `cols` of the tile (element (i, j, r) as in mm16::each).  The scales of
 // the wave's rows are in two registers, a row a lane, and reach their elements
@@ -258,7 +264,7 @@ __device__ __forceinline__ void finish(const Finish& f, int rows, int cols, int 
         char* p = f.out + (int64_t)at * f.ld + (int64_t)col * ES;
 #pragma unroll
         for (int j = 0; j < WN; ++j) {
-          const float v = settled(value(acc[i][j][4 * g + r], s, j) + epi_residual_value<OUT>(res[r][j]));
+          const float v = added<OUT>(f.epi, value(acc[i][j][4 * g + r], s, j), res[r][j]);
           if (col + 32 * j >= cols) continue;
           if (OUT == KQ_DT_F32) *reinterpret_cast<float*>(p + 32 * ES * j) = v;
           else *reinterpret_cast<uint16_t*>(p + 32 * ES * j) = (uint16_t)mm16::pack16<OUT == KQ_DT_F16>(v, 0.0f);

@@ -80,12 +80,17 @@ static hipError_t quantize(int dtype, const void* x, int64_t ldx, int64_t rows, 
   const int vec_out = !kq_misaligned(q, 8) && ldq % 8 == 0;
   auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (k <= 2048)
-      quantize_kernel<DT, 64, 4><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(
-          (const char*)x, ldx * es, rows, k, q, ldq, kp, scale, vec_in, vec_out);
-    else
-      quantize_kernel<DT, 256, 4><<<(unsigned)rows, 256, 0, st>>>((const char*)x, ldx * es, rows, k, q, ldq, kp, scale,
-                                                                  vec_in, vec_out);
+    constexpr int64_t MOST = 1 << 23;  // rows of a launch, which has less than 2^32 threads
+    for (int64_t r = 0; r < rows; r += MOST) {
+      const int64_t some = rows - r < MOST ? rows - r : MOST;
+      const char* xr = (const char*)x + r * ldx * es;
+      if (k <= 2048)
+        quantize_kernel<DT, 64, 4><<<(unsigned)((some + 3) / 4), 256, 0, st>>>(xr, ldx * es, some, k, q + r * ldq, ldq, kp,
+                                                                               scale + r, vec_in, vec_out);
+      else
+        quantize_kernel<DT, 256, 4><<<(unsigned)some, 256, 0, st>>>(xr, ldx * es, some, k, q + r * ldq, ldq, kp, scale + r,
+                                                                    vec_in, vec_out);
+    }
   };
   if (dtype == KQ_DT_BF16) run(std::integral_constant<int, KQ_DT_BF16>{});
   else if (dtype == KQ_DT_F16) run(std::integral_constant<int, KQ_DT_F16>{});
@@ -94,6 +99,8 @@ static hipError_t quantize(int dtype, const void* x, int64_t ldx, int64_t rows, 
 }
 
 // ---------------------------------------------------------------- few rows --
+
+constexpr int64_t MAX_N = 1 << 26;  // a launch of 512 threads for 16 columns has less than 2^32
 
 template <int DT, int OUT, int MB, int R, int P, bool TAIL>
 static hipError_t launch_few(FewArgs f, hipStream_t st) {
@@ -244,9 +251,9 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
     return kq_fail(KQ_ERR_INVALID, "%s: unknown activation %d", fn, activation);
   if (bias && bias_dtype != KQ_DT_BF16 && bias_dtype != KQ_DT_F32)
     return kq_fail(KQ_ERR_INVALID, "%s: bias dtype must be bf16 or f32", fn);
-  if (k > MAX_K || m > INT32_MAX / 2 || n > INT32_MAX / 2 || (codes && lda > mm16::MAX_LD) ||
+  if (k > MAX_K || m > INT32_MAX / 2 || n > MAX_N || (codes && lda > mm16::MAX_LD) ||
       ((m + 255) / 256) * ((n + 255) / 256) > INT32_MAX / 2)
-    return kq_fail(KQ_ERR_LIMIT, "%s: at most k = %lld (the int32 sums), 2^30 rows, columns and tiles, code rows 2^22 apart",
+    return kq_fail(KQ_ERR_LIMIT, "%s: at most k = %lld (the int32 sums), 2^30 rows and tiles, 2^26 columns, code rows 2^22 apart",
                    fn, (long long)MAX_K);
   if (m == 0 || n == 0) return KQ_OK;
   if (!a || !w || !w_scale || !c || (codes && !a_scale)) return kq_fail(KQ_ERR_INVALID, "%s: null buffer", fn);

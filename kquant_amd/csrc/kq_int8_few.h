@@ -239,8 +239,8 @@ __device__ __forceinline__ void few_rows(const FewArgs& f, int n0, int m0) {
     } else {
       s = f.sx[m0 + m];
     }
-    const float y = settled(finished_any<OUT>(f.epi, sum, s, sw0, epi_bias_value(f.epi, bias_bits)) +
-                            epi_residual_value<OUT>(residual_bits));
+    const float y =
+        added<OUT>(f.epi, finished_any<OUT>(f.epi, sum, s, sw0, epi_bias_value(f.epi, bias_bits)), residual_bits);
     const int64_t to = (int64_t)(m0 + m) * f.ldc + n0 + n;
     if (OUT == KQ_DT_F32) static_cast<float*>(f.c)[to] = y;
     else static_cast<uint16_t*>(f.c)[to] = (uint16_t)mm16::pack16<OUT == KQ_DT_F16>(y, 0.0f);

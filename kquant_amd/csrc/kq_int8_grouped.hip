@@ -88,7 +88,7 @@ extern "C" int kq_int8_grouped_linear(const int8_t* x, int64_t ldx, const float*
                         (int)(k / 2),         x_scale,        w_scale};
   hipStream_t st = (hipStream_t)stream;
   hipError_t e;
-  if (rows <= (int64_t)int8::FEW_EACH * groups && (int64_t)groups * ((n + 31) / 32) < INT32_MAX / 2) {
+  if (rows <= (int64_t)int8::FEW_EACH * groups && (int64_t)groups * ((n + 31) / 32) < 1 << 22) {  // (less than 2^32 threads)
     e = out_dtype == KQ_DT_BF16  ? int8::grouped_few<KQ_DT_BF16>(g, (int)k, st)
         : out_dtype == KQ_DT_F16 ? int8::grouped_few<KQ_DT_F16>(g, (int)k, st)
                                  : int8::grouped_few<KQ_DT_F32>(g, (int)k, st);

@@ -89,8 +89,8 @@ __global__ __launch_bounds__(256) void join_kernel(const DenseArgs g) {
     int sum = 0;
     for (int s = 0; s < g.slices; ++s) sum += g.planes[s * all + i];
     constexpr int RES = OUT == KQ_DT_F32 ? KQ_DT_F32 : KQ_DT_BF16;
-    const float y = settled(finished_any<OUT>(g.epi, sum, g.sx[m], g.sw[n], epi_bias(g.epi, n)) +
-                            epi_residual_value<OUT>(epi_residual_bits<RES>(g.epi, m, n)));
+    const float y = added<OUT>(g.epi, finished_any<OUT>(g.epi, sum, g.sx[m], g.sw[n], epi_bias(g.epi, n)),
+                               epi_residual_bits<RES>(g.epi, m, n));
     char* p = g.out + m * g.ld + n * (OUT == KQ_DT_F32 ? 4 : 2);
     if (OUT == KQ_DT_F32) *reinterpret_cast<float*>(p) = y;
     else *reinterpret_cast<uint16_t*>(p) = (uint16_t)mm16::pack16<OUT == KQ_DT_F16>(y, 0.0f);

@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from .int8 import INT8_K_ALIGN, _check_source_scale, _check_weight, _pad_k, _quantize, _row_stride, _row_view
+from .int8 import INT8_K_ALIGN, _check_no_gradient, _check_source_scale, _check_weight, _pad_k, _quantize, _row_stride, _row_view
 
 MAX_GROUPS = 4096
 MAX_STRIDE = 1 << 22  # elements from row to row
@@ -133,7 +133,7 @@ def int8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tens
     ``grouped_linear``.  N is a multiple of 8; a K that is no multiple of 16 is
     padded with zeros (a copy of the weight in every call).  The sums are exact;
     the scaled result is rounded once to ``out_dtype`` (x's type, bf16 for codes).
-    No gradient: an x that requires one is refused while autograd records.
+    No gradient: an x or a scale that requires one is refused while autograd records.
     """
 
     x_scale = _check_source_scale(x, x_scale)
@@ -154,8 +154,7 @@ def int8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tens
         out_dtype = torch.bfloat16 if x.dtype == torch.int8 else x.dtype
     if out_dtype not in N.DTYPE_CODES:
         raise TypeError("out_dtype must be bfloat16, float16 or float32")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError("int8_grouped_linear carries no gradient: detach x or call it under torch.no_grad()")
+    _check_no_gradient("int8_grouped_linear", x, scale, x_scale)
     (a, w, s, sx, offsets), gpu, host = N.to_gpu((x, weight, scale, x_scale, offsets))
     a, s = _row_view(a), N.aligned(s, 4)
     kp = -(-k // INT8_K_ALIGN) * INT8_K_ALIGN

@@ -30,7 +30,8 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .int8 import INT8_K_ALIGN, _check_source_scale, _check_weight, _pad_k as _pad_codes, _quantize, _row_stride, _row_view
+from .int8 import (INT8_K_ALIGN, _check_no_gradient, _check_source_scale, _check_weight, _pad_k as _pad_codes, _quantize,
+                   _row_stride, _row_view)
 
 
 def _check_epilogue(source, bias, activation, residual, lead, n: int, f32: bool, out_dtype: torch.dtype) -> None:
@@ -261,7 +262,7 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
     infinity or a NaN is NaN.  K is at most 131056; a K that is no multiple of 16
     is padded with zeros (a copy of the weight in every call: pad it once to skip
     that).  Results do not change from call to call.  They carry no gradient: a
-    source, bias or residual that requires one is refused while autograd records.
+    source, bias, residual or scale that requires one is refused while autograd records.
     """
     source_scale = _check_source_scale(source, source_scale)
     if source.ndim < 1:
@@ -274,6 +275,7 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
         raise TypeError("out_dtype must be bfloat16, float16 or float32")
     n, lead = weight.shape[0], source.shape[:-1]
     _check_epilogue(source, bias, activation, residual, lead, n, False, out_dtype)
+    _check_no_gradient("int8_linear", scale, source_scale)
     (a, w, s, sx, bias, residual), gpu, host = N.to_gpu((source, weight, scale, source_scale, bias, residual))
     a, s = _row_view(a), N.aligned(s, 4)
     kp = -(-k // INT8_K_ALIGN) * INT8_K_ALIGN
@@ -296,7 +298,7 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
         if bias is not None:
             bias = bias.contiguous()
         if residual is not None:
-            residual = _row_view(residual)
+            residual = _row_view(residual if residual.ndim == 2 else residual.reshape(m, n))
         out = torch.empty(m, n, dtype=out_dtype, device=gpu)
         N.call("kq_int8_linear", code, a.data_ptr(), _row_stride(a), N.ptr(sx), w.data_ptr(), s.data_ptr(), m, n, kp,
                N.LIN_ACTIVATIONS[activation], N.ptr(bias), 0 if bias is None else N.DTYPE_CODES[bias.dtype],

@@ -77,6 +77,13 @@ def test_quantize_many_rows(gpu):
         check_codes(*int8_quantize(x), x)
 
 
+def test_quantize_more_rows_than_a_launch(gpu):
+    x = torch.randn((1 << 26) + 5, device=gpu, dtype=torch.float16)[:, None]
+    q, scale = int8_quantize(x)
+    assert torch.equal(q, 127 * torch.sign(x).to(torch.int8))
+    assert torch.equal(scale, torch.clamp(x[:, 0].float().abs() * (1.0 / 127.0), min=2.0 ** -126))
+
+
 def test_quantize_ties_and_borders(gpu):
     """Quotients that are halves, and the fp32 numbers next to them."""
     half = torch.arange(-126, 127, device=gpu).float() + 0.5
@@ -312,3 +319,23 @@ def test_rows_are_independent(gpu, m, dtype):
             if name in cut:
                 cut[name] = cut[name][..., 1:]
         assert torch.equal(int8_linear(x, w[1:], sw[1:], **cut), y[:, 1:])  # 263 columns: no whole 16-byte pieces
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_signs_of_zeros(gpu, dtype):
+    """Rows of zeros with negative channel scales: -0 without a bias or residual, whatever the batch."""
+    w, sw = weights(264, 256, gpu)
+    for m in (1, 40, 100, 300):
+        y = int8_linear(torch.zeros(m, 256, device=gpu, dtype=dtype), w, -sw)
+        assert not y.any() and torch.signbit(y).all(), m
+        z = int8_linear(torch.zeros(m, 256, device=gpu, dtype=dtype), w, -sw, residual=torch.zeros_like(y))
+        assert not z.any() and not torch.signbit(z).any(), m
+
+
+def test_empty_results(gpu):
+    w, sw = weights(0, 256, gpu)
+    x = torch.ones(2, 3, 256, device=gpu, dtype=torch.bfloat16)
+    y = int8_linear(x, w, sw, residual=torch.zeros(2, 3, 0, device=gpu, dtype=torch.bfloat16))
+    assert y.shape == (2, 3, 0)
+    w, sw = weights(24, 256, gpu)
+    assert int8_linear(x[:, :0], w, sw, activation="relu").shape == (2, 0, 24)

@@ -65,6 +65,8 @@ LINEAR = [
     (dict(residual=torch.zeros(4, 23, dtype=BF16)), ValueError, "residual shape"),
     (dict(source=torch.zeros(4, 32, dtype=BF16, requires_grad=True)), RuntimeError, "carries no gradient"),
     (dict(bias=torch.zeros(24, requires_grad=True)), RuntimeError, "carries no gradient"),
+    (dict(scale=torch.zeros(24, requires_grad=True)), RuntimeError, "carries no gradient"),
+    (dict(source=i8(4, 32), source_scale=torch.zeros(4, requires_grad=True)), RuntimeError, "carries no gradient"),
 ]
 
 
@@ -90,6 +92,7 @@ def test_linear(change, error, text):
     (dict(scale=torch.zeros(2, 23)), ValueError, "scale shape"),
     (dict(out_dtype=torch.int8), TypeError, "out_dtype"),
     (dict(x=torch.zeros(4, 32, dtype=BF16, requires_grad=True)), RuntimeError, "carries no gradient"),
+    (dict(scale=torch.zeros(2, 24, requires_grad=True)), RuntimeError, "carries no gradient"),
 ])
 def test_grouped(change, error, text):
     args = dict(x=torch.zeros(4, 32, dtype=BF16), w=i8(2, 24, 32), scale=torch.zeros(2, 24),
@@ -121,6 +124,7 @@ def test_grouped(change, error, text):
     (dict(top_p=torch.ones(4, dtype=torch.float64)), TypeError, "must be float32"),
     (dict(min_p=-0.1), ValueError, "min_p"),
     (dict(min_p=1.5), ValueError, "min_p"),
+    (dict(logits=torch.zeros(4, 9, requires_grad=True), return_logprobs=True), RuntimeError, "carries no gradient"),
 ])
 def test_sample(change, error, text):
     args = dict(logits=torch.zeros(4, 9), uniform=torch.zeros(4)) | change
@@ -158,6 +162,9 @@ def test_linear_c_entry():
         (8, 56, INVALID, b"k % 16"), (8, 0, INVALID, b"k % 16"), (9, 5, INVALID, b"activation"), (14, N.DT_I8, INVALID, b"output"),
         (16, 23, INVALID, b"ldc"), (1, ctypes.c_void_p(264), INVALID, b"16-byte"), (4, ctypes.c_void_p(264), INVALID, b"16-byte"),
         (2, (1 << 22) + 16, LIMIT, b"2^22"), (6, 1 << 31, LIMIT, b"2^30")])
+    wide = list(ok)
+    wide[7] = wide[13] = wide[16] = (1 << 26) + 8
+    refused("kq_int8_linear", wide, [(9, 0, LIMIT, b"2^26")])
     long = list(ok)
     long[2] = long[8] = INT8_MAX_K + 16
     refused("kq_int8_linear", long, [(9, 0, LIMIT, b"131056")])
