@@ -7,6 +7,8 @@ Drop-in modules mirroring kquant's API:
   kquant_amd.constants        <- kquant/constants.py (format block)
   kquant_amd.grouped          products grouped by expert, with gradients (absent from kquant)
   kquant_amd.loss             cross entropy of a vocabulary head, with gradients (absent from kquant)
+  kquant_amd.int8             rows in 8-bit integers for linear and grouped (absent from kquant)
+  kquant_amd.sampling         the next token from a head's logits (absent from kquant)
 
 Every compute call runs a HIP kernel of libkquant_amd.so (C ABI in
 include/kquant_amd.h) on the GPU.

@@ -6,11 +6,13 @@
 namespace kq {
 namespace int8 {
 
-// A step of a tile is bounded by its reads of LDS, in which the 256 columns' share is
-// the same for every tile: at K = 7168 (56 steps) a round of tiles of 32 / 64 / 128 /
-// 256 rows takes 28 / 35 / 52 / 77 us, so 88 + rows.  The cut with the least rounds in all (256 x 12288: 80 us in 48 tiles
-// of 256 rows, 39 in 192 of 64; 512 rows 93 and 57 of 128; 1024 rows 94, 107 and 109).
-// Planes cost a launch and their bytes.
+// A step of a narrow tile is bounded by its loads, in which the 256 columns' share is
+// the same for every tile (256 x 12288 in tiles of 64 rows: 42 us, 33 without fragment
+// reads and MFMAs; 1024 rows in tiles of 256: 94 and 49): at K = 7168 (56 steps) a round
+// of tiles of 32 / 64 / 128 / 256 rows takes 28 / 35 / 52 / 77 us, so 88 + rows.
+// The cut with the least rounds in all (256 x 12288: 80 us in 48 tiles of 256 rows, 39
+// in 192 of 64; 512 rows 93 and 57 of 128; 1024 rows 94, 107 and 109).  Planes cost a
+// launch and their bytes.
 DensePlan dense_plan(int64_t m, int64_t n, int64_t k, int64_t cus, bool split) {
   DensePlan best{};
   double least = 0.0;
