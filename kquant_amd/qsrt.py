@@ -315,7 +315,7 @@ def qsrt_linear(
         ws = None
     elif m <= FUSED_MAX_ROWS:
         # the fused kernel's counters and polled partials: zeroed once, back at zero after every call
-        ws = _workspace(_LINEAR_WORKSPACES, (gpu, stream.value, m, k_tiles, n_tiles), need, gpu)
+        ws = _workspace(_LINEAR_WORKSPACES, (gpu, stream, m, k_tiles, n_tiles), need, gpu)
     else:
         # the prefill form keeps no state between calls: a buffer from torch's
         # caching allocator, released with this call, so prompts of many
@@ -429,7 +429,7 @@ def qsrt_expert_forward(
         if need < 0:
             raise RuntimeError("kq_qsrt_moe_workspace_size: no HIP device")
         stream = N.stream(gpu)
-        ws = _workspace(_MOE_WORKSPACES, (gpu, stream.value, tokens, topk, h_tiles, i_tiles), need, gpu)
+        ws = _workspace(_MOE_WORKSPACES, (gpu, stream, tokens, topk, h_tiles, i_tiles), need, gpu)
         act = N.ACT_SITU if activation == "situ" else N.ACT_SWIGLU
         N.call("kq_qsrt_moe_decode", act, float(beta), float(linear_beta), N.ptr(xg), N.DTYPE_CODES[xg.dtype],
                tokens, xg.stride(0), N.ptr(ids), N.ptr(wts), topk, N.ptr(experts.descriptors), experts.experts,
