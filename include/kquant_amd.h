@@ -371,7 +371,8 @@ int kq_int8_grouped_linear(const int8_t* x, int64_t ldx, const float* x_scale, i
  * a row, or NULL and the number for all.  Weights are multiples of 2^-45 and summed
  * as integers: deterministic.  vocab <= 262144, rows <= 2^20.  workspace:
  * kq_sample_tokens_workspace_size bytes (filters: whether top_k or top_p may cut
- * in some row), 16-byte aligned, written and read by this call alone. */
+ * in some row; some 49 KiB a row, of 8192 rows at most), 16-byte aligned, written and
+ * read by this call alone. */
 int64_t kq_sample_tokens_workspace_size(int64_t rows, int64_t vocab, int filters);
 int kq_sample_tokens(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* uniform,
                      const float* temperature_rows, double temperature, const int* top_k_rows, int64_t top_k,

@@ -1122,6 +1122,9 @@ __global__ __launch_bounds__(SLICE_T, 4) void weigh_kernel(const Args a, const S
 // 4096 34, 40, 81, 103, 131, 111.
 constexpr int WHOLE_VOCAB = 4096;
 
+// Rows of one set of launches, each set after the last one in the same workspace: 49 KiB a row of it.
+constexpr int64_t MOST_ROWS = 8192;
+
 struct Plan {
   int chunks, per, slices;
   int64_t parts, bins, state, chunk, list, bytes;  // offsets of the workspace's pieces
@@ -1160,6 +1163,22 @@ static hipError_t launch(const Args& a, int64_t rows, bool filters, char* ws, hi
     row_kernel<DT><<<(unsigned)rows, T, 0, st>>>(a);
     return hipGetLastError();
   }
+  if (rows > MOST_ROWS) {
+    for (int64_t r = 0; r < rows; r += MOST_ROWS) {
+      Args b = a;
+      b.logits += r * a.ld;
+      b.uniform += r;
+      if (a.temperature.rows) b.temperature.rows += r;
+      if (a.top_p.rows) b.top_p.rows += r;
+      if (a.min_p.rows) b.min_p.rows += r;
+      if (a.k_rows) b.k_rows += r;
+      b.token += r;
+      if (a.logprob) b.logprob += r;
+      const hipError_t e = launch<DT>(b, rows - r < MOST_ROWS ? rows - r : MOST_ROWS, filters, ws, st);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   const Plan p = plan(rows, a.vocab, filters);
   const Split sp{(Part*)(ws + p.parts),
                  (unsigned long long*)(ws + p.bins),
@@ -1192,7 +1211,7 @@ using namespace kq;
 extern "C" int64_t kq_sample_tokens_workspace_size(int64_t rows, int64_t vocab, int filters) {
   if (rows < 0 || vocab < 1 || vocab > sample::MAX_VOCAB) return -1;
   if (rows == 0 || vocab <= sample::WHOLE_VOCAB) return 0;
-  return sample::plan(rows, vocab, filters != 0).bytes;
+  return sample::plan(rows < sample::MOST_ROWS ? rows : sample::MOST_ROWS, vocab, filters != 0).bytes;
 }
 
 extern "C" int kq_sample_tokens(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const float* uniform,

@@ -261,3 +261,17 @@ def test_infinite_temperatures(gpu, vocab, settings):
         odd = min(settings.get("top_k", vocab), int((z[1] > -math.inf).sum()))
         for r in range(m):
             assert abs(logprobs[r].item() + math.log(odd if r % 2 else 2)) <= 2.0 ** -24 * 12 + 1e-12
+
+
+@pytest.mark.parametrize("settings", [{}, {"top_k": 20, "top_p": 0.9, "min_p": 0.01}], ids=str)
+def test_more_rows_than_a_set_of_launches(gpu, settings):
+    m, vocab = 8192 + 300, 4100
+    z, u = rows(m, vocab, torch.bfloat16, gpu, 31)
+    own = {name: torch.full((m,), value, device=gpu, dtype=torch.int32 if name == "top_k" else torch.float32)
+           for name, value in (settings | {"temperature": 0.9}).items()}
+    own["temperature"][1::2] = 1.3
+    tokens, logprobs = sample_tokens(z, u, return_logprobs=True, **own)
+    for a, b in ((0, 700), (8000, 8400), (8192, m)):
+        part = sample_tokens(z[a:b], u[a:b], return_logprobs=True, **{name: v[a:b] for name, v in own.items()})
+        assert torch.equal(part[0], tokens[a:b]) and torch.equal(part[1], logprobs[a:b])
+    check(z[8190:8195], u[8190:8195], **{name: v[8190:8195] for name, v in own.items()})
