@@ -14,6 +14,7 @@ import ctypes
 from collections.abc import Iterable
 
 import torch
+from torch.autograd import forward_ad
 
 from ._build import LIB_PATH
 
@@ -272,6 +273,17 @@ def to_gpu(tensors: Iterable[torch.Tensor | None]) -> tuple[list, torch.device, 
         library()
     moved = [None if t is None else t.to(gpu) for t in tensors]
     return moved, gpu, host
+
+
+def carries_gradient(*tensors: torch.Tensor | None) -> bool:
+    """Whether a derivative of one of them is asked for: autograd records and it
+    requires a gradient, or it has a tangent (which no_grad leaves in force)."""
+
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return True
+    # (outside forward mode a tensor has no tangent: 0.1 us instead of 1 a tensor)
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given)
 
 
 _LEAF_STREAM = "kquant_amd.stream"

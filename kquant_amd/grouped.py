@@ -133,7 +133,7 @@ def int8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tens
     ``grouped_linear``.  N is a multiple of 8; a K that is no multiple of 16 is
     padded with zeros (a copy of the weight in every call).  The sums are exact;
     the scaled result is rounded once to ``out_dtype`` (x's type, bf16 for codes).
-    No gradient: an x or a scale that requires one is refused while autograd records.
+    No gradient: an x or a scale that requires one (while autograd records) or has a tangent is refused.
     """
 
     x_scale = _check_source_scale(x, x_scale)

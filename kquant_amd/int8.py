@@ -97,8 +97,9 @@ def _check_weight(weight: torch.Tensor, scale: torch.Tensor, dims: int, k: int) 
 
 
 def _check_no_gradient(name: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} carries no gradient: detach its arguments or call it under torch.no_grad()")
+    if N.carries_gradient(*tensors):
+        raise RuntimeError(f"{name} carries no gradient: detach its arguments, or call it under "
+                           "torch.no_grad() where none has a tangent")
 
 
 def _check_source_scale(source: torch.Tensor, scale: torch.Tensor | None) -> torch.Tensor | None:

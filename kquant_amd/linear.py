@@ -49,9 +49,9 @@ def _check_epilogue(source, bias, activation, residual, lead, n: int, f32: bool,
             raise TypeError(f"residual must have the result's type {out_dtype}, got {residual.dtype}")
         if tuple(residual.shape) != (*lead, n):
             raise ValueError(f"residual shape {tuple(residual.shape)} != {(*lead, n)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (source, bias, residual)):
-        raise RuntimeError("a linear with bias, activation or residual carries no gradient: detach its inputs or call it "
-                           "under torch.no_grad()")
+    if N.carries_gradient(source, bias, residual):
+        raise RuntimeError("a linear with bias, activation or residual carries no gradient: detach its inputs, or call it "
+                           "under torch.no_grad() where none has a tangent")
 
 
 def _linear(fmt: int, source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
@@ -138,8 +138,8 @@ def mxfp8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor
     type) are applied in the kernel's epilogue on the fp32 sums, which are then
     rounded once: ``activation(source @ W.T + bias) + residual``.  The result
     carries no gradient: with any of the three, a source, bias or residual that
-    requires one is refused while autograd records (a skip connection inside
-    the call would leave the graph unseen).
+    requires one (while autograd records) or has a tangent is refused (a skip
+    connection inside the call would leave the graph unseen).
     """
     if weight.dtype not in (torch.float8_e4m3fn, torch.uint8):
         raise TypeError(f"MXFP8 weight must be float8_e4m3fn, got {weight.dtype}")
@@ -262,7 +262,8 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
     infinity or a NaN is NaN.  K is at most 131056; a K that is no multiple of 16
     is padded with zeros (a copy of the weight in every call: pad it once to skip
     that).  Results do not change from call to call.  They carry no gradient: a
-    source, bias, residual or scale that requires one is refused while autograd records.
+    source, bias, residual or scale that requires one (while autograd records) or has a
+    tangent is refused.
     """
     source_scale = _check_source_scale(source, source_scale)
     if source.ndim < 1:

@@ -71,8 +71,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
 
     ``return_logprobs`` returns also the natural logarithm of the probability
     with which each token was drawn, among those kept (fp32 [...]; NaN where the
-    token is -1); they carry no gradient: logits that require one are refused
-    then while autograd records.
+    token is -1); they carry no gradient: logits that require one
+    (while autograd records) or have a tangent are refused then.
     """
 
     if logits.dtype not in N.DTYPE_CODES:
@@ -81,8 +81,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: f
         raise TypeError(f"uniform must be float32, got {uniform.dtype}")
     if logits.ndim < 1 or not 0 < logits.shape[-1] <= MAX_VOCAB:
         raise ValueError(f"logits must be [..., V] with V between 1 and {MAX_VOCAB}, got {tuple(logits.shape)}")
-    if return_logprobs and torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("sample_tokens carries no gradient: detach the logits or call it under torch.no_grad()")
+    if return_logprobs and N.carries_gradient(logits):
+        raise RuntimeError("sample_tokens carries no gradient: detach the logits, or call it under "
+                           "torch.no_grad() where they have no tangent")
     vocab, lead = logits.shape[-1], logits.shape[:-1]
     if tuple(uniform.shape) != tuple(lead):
         raise ValueError(f"uniform has shape {tuple(uniform.shape)}, the rows {tuple(lead)}")
