@@ -71,7 +71,23 @@ def int8_dequantize(q: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype 
         raise TypeError(f"expected int8 codes and float32 scales, got {q.dtype} and {scale.dtype}")
     if q.ndim < 1 or tuple(scale.shape) != tuple(q.shape[:-1]):
         raise ValueError(f"scale shape {tuple(scale.shape)} != {tuple(q.shape[:-1])}")
-    return (q.float() * scale.unsqueeze(-1)).to(dtype)
+    s, codes = scale.unsqueeze(-1), q.float()
+    if dtype == torch.float64:
+        return q.double() * s.double()
+    values = codes * s
+    if dtype not in (torch.bfloat16, torch.float16):
+        return values.to(dtype)
+    # Rounded to fp32 and then to 16 bits a product can end on the far side of a border between two results that its
+    # fp32 value lies on.  A product that is not an fp32 number is therefore taken as the neighbour with an odd last bit,
+    # which no border has.  Its rest is exact: the scale's upper 16 and lower 8 bits times a code are fp32 numbers.
+    s, v = s.detach(), values.detach()
+    high = (s.contiguous().view(torch.int32) & ~0xff).view(torch.float32)
+    rest = torch.addcmul(-v, codes, high).addcmul_(codes, s - high)
+    bits = v.view(torch.int32)
+    even = (bits & 1 == 0) & (rest != 0) & torch.isfinite(v)
+    outward = torch.where((rest > 0) == (v > 0), 1, -1).to(torch.int32)
+    odd = (bits + outward).view(torch.float32)
+    return (values + torch.where(even, odd - v, 0.0)).to(dtype)
 
 
 def _pad_k(q: torch.Tensor, width: int) -> torch.Tensor:
