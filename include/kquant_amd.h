@@ -338,10 +338,13 @@ int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
  * kq_int8_quantize does (a_scale is not read).  activation, bias, residual as
  * kq_mx_linear_epilogue takes them, the residual of out_dtype (row stride ldr).
  * k % 16 == 0, k <= 131056, n <= 2^26; w and codes 16-byte aligned, lda of codes a multiple
- * of 16.  workspace: kq_int8_linear_workspace_size bytes on the device current then
- * (the rows' codes, and sums of slices of k where the output has few tiles; 0 for codes
- * and for few rows), 16-byte aligned, written and read by this call alone; one that
- * holds the codes but not the slices runs without them. */
+ * of 16.  workspace: kq_int8_linear_workspace_size bytes, asked for with the device
+ * current that the call runs on; 16-byte aligned, written and read by this call alone.
+ * It holds the codes of rows that are quantized here (m k and 4 m bytes, each rounded up
+ * to 16; a call without that room is refused), but none for a_dtype KQ_DT_I8 and for up to
+ * 4 rows of at most 8192 elements with m n k <= 3.5e8, and the sums of slices of k where
+ * more than 16 rows make an output of few tiles, of any a_dtype (a call without that room,
+ * or with workspace NULL where no codes are held, runs without slices: the same bits, slower). */
 int64_t kq_int8_linear_workspace_size(int a_dtype, int64_t m, int64_t n, int64_t k);
 int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const float* a_scale, const int8_t* w, const float* w_scale,
                    int64_t m, int64_t n, int64_t k, int activation, const void* bias, int bias_dtype,
