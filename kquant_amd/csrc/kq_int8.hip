@@ -103,7 +103,7 @@ static hipError_t quantize(int dtype, const void* x, int64_t ldx, int64_t rows, 
 constexpr int64_t MAX_N = 1 << 26;  // a launch of 512 threads for 16 columns has less than 2^32
 
 template <int DT, int OUT, int MB, int R, int P, bool TAIL>
-static hipError_t launch_few(FewArgs f, hipStream_t st) {
+static hipError_t launch_few(const FewArgs& f, hipStream_t st) {
   const int nwin = (f.k + WIN - 1) / WIN, waves = nwin < 8 ? nwin : 8;
   const size_t lds = (size_t)waves * wave_lds(MB, R) + (DT != DT_CODES ? (size_t)f.m * (nwin * WIN + 16) : 0);
   auto kern = few_rows_kernel<DT, OUT, MB, R, P, TAIL>;
@@ -111,9 +111,7 @@ static hipError_t launch_few(FewArgs f, hipStream_t st) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  f.mtiles = (f.m + 16 * MB - 1) / (16 * MB);
-  const int64_t ntiles = ((int64_t)f.n + 16 * R - 1) / (16 * R);
-  kern<<<(unsigned)(f.mtiles * ((ntiles + 7) / 8 * 8)), waves * 64, lds, st>>>(f);
+  kern<<<(unsigned)((f.n + 16 * R - 1) / (16 * R)), waves * 64, lds, st>>>(f);
   return hipGetLastError();
 }
 
@@ -290,7 +288,7 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
   const int64_t cus = m > 16 ? device_cus(st) : 1;
   if (cus <= 0) return kq_fail(KQ_ERR_HIP, "%s: no device", fn);
   if (takes_few(m, n, k, cus)) {
-    const FewArgs f{rows, ld, sx, w, w_scale, c, ldc, (int)m, (int)n, (int)k, 1, e};
+    const FewArgs f{rows, ld, sx, w, w_scale, c, ldc, (int)m, (int)n, (int)k, e};
     const int dt = fused ? a_dtype : KQ_DT_I8;
     const hipError_t err = out_dtype == KQ_DT_BF16  ? few<KQ_DT_BF16>(dt, f, st)
                            : out_dtype == KQ_DT_F16 ? few<KQ_DT_F16>(dt, f, st)

@@ -47,7 +47,7 @@ struct FewArgs {
   const float* sw;
   void* c;
   int64_t ldc;
-  int m, n, k, mtiles;
+  int m, n, k;
   Epilogue epi;
 };
 
@@ -249,10 +249,7 @@ __device__ __forceinline__ void few_rows(const FewArgs& f, int n0, int m0) {
 
 template <int DT, int OUT, int MB, int R, int P, bool TAIL>
 __global__ __launch_bounds__(512) void few_rows_kernel(const FewArgs f) {
-  // row tiles of one column tile run on one XCD, one after the other, and share its weights in that L2
-  const int idx = (int)blockIdx.x / 8, xcd = (int)blockIdx.x % 8;
-  const int n0 = ((idx / f.mtiles) * 8 + xcd) * 16 * R, m0 = (idx % f.mtiles) * 16 * MB;
-  if (n0 < f.n) few_rows<DT, OUT, MB, R, P, TAIL>(f, n0, m0);
+  few_rows<DT, OUT, MB, R, P, TAIL>(f, (int)blockIdx.x * 16 * R, 0);  // (at most 16 MB rows)
 }
 
 }  // namespace int8
