@@ -15,8 +15,8 @@ namespace int8 {
 // longer row has besides is read again (from L2).
 template <int DT, int T, int NV>
 __global__ __launch_bounds__(256) void quantize_kernel(const char* __restrict__ x, int64_t ldx, int64_t rows, int64_t k,
-                                                       int8_t* __restrict__ q, int64_t ldq, int64_t kp,
-                                                       float* __restrict__ scale, int vec_in, int vec_out) {
+                                                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
+                                                       int vec_in, int vec_out) {
   __shared__ uint32_t part[4];
   const int t = threadIdx.x % T;
   const int64_t row = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T;
@@ -51,30 +51,28 @@ __global__ __launch_bounds__(256) void quantize_kernel(const char* __restrict__ 
   auto store = [&](const Eight<DT>& e, int64_t at) {
     u32x2_t c = {0u, 0u};
     if (finite) c = e.codes(s, inv);
-    if (vec_out && at + 8 <= kp) {
+    if (vec_out && at + 8 <= k) {
       *reinterpret_cast<u32x2_t*>(qr + at) = c;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (at + i < kp) qr[at + i] = (int8_t)(c[i >> 2] >> 8 * (i & 3));
+        if (at + i < k) qr[at + i] = (int8_t)(c[i >> 2] >> 8 * (i & 3));
     }
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t at = (int64_t)(t + i * T) * 8;
-    if (at < kp) store(v[i], at);
+    if (at < k) store(v[i], at);
   }
-  for (int64_t at = (int64_t)(t + NV * T) * 8; at < kp; at += T * 8) {
+  for (int64_t at = (int64_t)(t + NV * T) * 8; at < k; at += T * 8) {
     Eight<DT> more;
-    if (at < k) more.load(xr, at, k, vec_in);
-    else more.clear();
+    more.load(xr, at, k, vec_in);
     store(more, at);
   }
 }
 
-// Columns [k, kp) of q are written as zeros.
 static hipError_t quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t k, int8_t* q, int64_t ldq,
-                           int64_t kp, float* scale, hipStream_t st) {
+                           float* scale, hipStream_t st) {
   const int es = dtype == KQ_DT_F32 ? 4 : 2;
   const int vec_in = !kq_misaligned(x, 16) && ldx * es % 16 == 0;
   const int vec_out = !kq_misaligned(q, 8) && ldq % 8 == 0;
@@ -85,10 +83,10 @@ static hipError_t quantize(int dtype, const void* x, int64_t ldx, int64_t rows, 
       const int64_t some = rows - r < MOST ? rows - r : MOST;
       const char* xr = (const char*)x + r * ldx * es;
       if (k <= 2048)
-        quantize_kernel<DT, 64, 4><<<(unsigned)((some + 3) / 4), 256, 0, st>>>(xr, ldx * es, some, k, q + r * ldq, ldq, kp,
+        quantize_kernel<DT, 64, 4><<<(unsigned)((some + 3) / 4), 256, 0, st>>>(xr, ldx * es, some, k, q + r * ldq, ldq,
                                                                                scale + r, vec_in, vec_out);
       else
-        quantize_kernel<DT, 256, 4><<<(unsigned)some, 256, 0, st>>>(xr, ldx * es, some, k, q + r * ldq, ldq, kp, scale + r,
+        quantize_kernel<DT, 256, 4><<<(unsigned)some, 256, 0, st>>>(xr, ldx * es, some, k, q + r * ldq, ldq, scale + r,
                                                                     vec_in, vec_out);
     }
   };
@@ -213,7 +211,7 @@ extern "C" int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t r
   if (!x || !q || !scale) return kq_fail(KQ_ERR_INVALID, "%s: null buffer", fn);
   if (kq_misaligned(x, dtype == KQ_DT_F32 ? 4 : 2) || kq_misaligned(scale, 4))
     return kq_fail(KQ_ERR_INVALID, "%s: x and scale must be aligned to their type", fn);
-  return kq_check_launch(quantize(dtype, x, ldx, rows, k, q, ldq, k, scale, (hipStream_t)stream), fn);
+  return kq_check_launch(quantize(dtype, x, ldx, rows, k, q, ldq, scale, (hipStream_t)stream), fn);
 }
 
 // The rows' codes and scales.
@@ -277,7 +275,7 @@ extern "C" int kq_int8_linear(int a_dtype, const void* a, int64_t lda, const flo
   if (!codes && !fused) {
     int8_t* q = (int8_t*)workspace;
     float* s = (float*)((char*)workspace + up16(m * k));
-    const hipError_t err = quantize(a_dtype, a, lda, m, k, q, k, k, s, st);
+    const hipError_t err = quantize(a_dtype, a, lda, m, k, q, k, s, st);
     if (err != hipSuccess) return kq_check_launch(err, "kq_int8_linear/quantize");
     rows = (const char*)q;
     ld = k;
