@@ -686,11 +686,7 @@ __device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const uint64_
   for (int j = 0; j < PER; ++j) sum += v[j];
   const uint64_t upto = wave_scan(sum);
   if ((threadIdx.x & 63) == 63) wave_total[threadIdx.x >> 6] = upto;
-  if (threadIdx.x == 0) {
-    found[0] = NBINS;
-    found[1] = found[2] = FAR_BIN - 1;
-    found[3] = 0;
-  }
+  if (threadIdx.x == 0) found[1] = found[2] = FAR_BIN - 1;
   __syncthreads();
   uint64_t before = upto - sum, total = 0;
 #pragma unroll
@@ -698,23 +694,19 @@ __device__ __forceinline__ Cuts find_cuts(const Row& q, int vocab, const uint64_
     if (w < (int)(threadIdx.x >> 6)) before += wave_total[w];
     total += wave_total[w];
   }
-  if (threadIdx.x == 0) weights[0] = weights[1] = total & WEIGHT;
-  __syncthreads();
-  if (q.k > 0) {
-    uint64_t at = before;
+  uint64_t up = before;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint64_t next = at + v[j];
-      if ((int)(at >> COUNT_SHIFT) < q.k && (int)(next >> COUNT_SHIFT) >= q.k) {
-        found[0] = threadIdx.x * PER + j;
-        found[3] = (int)(at >> COUNT_SHIFT);
-        weights[0] = at & WEIGHT;
-        weights[1] = next & WEIGHT;
-      }
-      at = next;
+  for (int j = 0; j < PER; ++j) {
+    const uint64_t next = up + v[j];
+    if ((int)(up >> COUNT_SHIFT) < q.k && (int)(next >> COUNT_SHIFT) >= q.k) {  // one thread's: 0 < k < the bins' tokens
+      found[0] = threadIdx.x * PER + j;
+      found[3] = (int)(up >> COUNT_SHIFT);
+      weights[0] = up & WEIGHT;
+      weights[1] = next & WEIGHT;
     }
-    __syncthreads();
+    up = next;
   }
+  __syncthreads();
   Cuts c;
   c.kb = found[0];
   c.before_kb = found[3];
