@@ -331,6 +331,12 @@ int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x,
 int kq_int8_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t k, int8_t* q, int64_t ldq,
                      float* scale, void* stream);
 
+/* out[r][k] = scale[r] q[r][k], the exact product rounded once to out_dtype
+ * (KQ_DT_*); q [rows, k] (row stride ldq) and out (row stride ldo) at any alignment
+ * of their types. */
+int kq_int8_dequantize(const int8_t* q, int64_t ldq, const float* scale, int64_t rows, int64_t k, int out_dtype, void* out,
+                       int64_t ldo, void* stream);
+
 /* c = act(a_scale[m] w_scale[n] sum_k a[m][k] w[n][k] + bias) + residual over
  * 8-bit integers w [n, k] with an fp32 scale a row; int32 sums (exact), fp32
  * after them, rounded once to out_dtype (KQ_DT_*).  a_dtype KQ_DT_I8: a holds

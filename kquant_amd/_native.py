@@ -133,6 +133,7 @@ SIGNATURES: dict[str, list] = {
     "kq_grouped_linear_dx": [_INT, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _I64, _VP, _I64, _VP],
     "kq_grouped_linear_dw": [_INT, _VP, _I64, _VP, _I64, _I64, _VP, _INT, _I64, _I64, _VP, _VP],
     "kq_int8_quantize": [_INT, _VP, _I64, _I64, _I64, _VP, _I64, _VP, _VP],
+    "kq_int8_dequantize": [_VP, _I64, _VP, _I64, _I64, _INT, _VP, _I64, _VP],
     "kq_int8_linear_workspace_size": [_INT, _I64, _I64, _I64],
     "kq_int8_linear": [_INT, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _INT, _VP, _INT, _VP, _I64, _INT, _VP, _I64, _VP,
                        _I64, _VP],

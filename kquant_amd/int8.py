@@ -65,12 +65,24 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def int8_dequantize(q: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """``q * scale`` of codes [..., K] and their rows' scales [...], rounded once to ``dtype``."""
+    """``q * scale`` of codes [..., K] and their rows' scales [...], rounded once to ``dtype``.
+
+    Differentiable in the scales.  On the GPU, in bf16, fp16 or fp32 and without a derivative, one kernel; else
+    elementwise torch operations with the same results, on the tensors' own device.
+    """
 
     if q.dtype != torch.int8 or scale.dtype != torch.float32:
         raise TypeError(f"expected int8 codes and float32 scales, got {q.dtype} and {scale.dtype}")
     if q.ndim < 1 or tuple(scale.shape) != tuple(q.shape[:-1]):
         raise ValueError(f"scale shape {tuple(scale.shape)} != {tuple(q.shape[:-1])}")
+    if (q.is_cuda and scale.device == q.device and dtype in N.DTYPE_CODES and q.shape[-1] and not N.carries_gradient(scale)
+            and not any(map(torch._C._functorch.is_functorch_wrapped_tensor, (q, scale)))):
+        a = _row_view(q)
+        with N.on_device(q.device):
+            out = torch.empty(a.shape, dtype=dtype, device=q.device)
+            N.call("kq_int8_dequantize", N.ptr(a), _row_stride(a), N.ptr(N.aligned(scale.reshape(-1), 4)), *a.shape,
+                   N.DTYPE_CODES[dtype], N.ptr(out), a.shape[1], N.stream(q.device))
+        return out.reshape(q.shape)
     s, codes = scale.unsqueeze(-1), q.float()
     if dtype == torch.float64:
         return q.double() * s.double()
@@ -79,15 +91,13 @@ def int8_dequantize(q: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype 
         return values.to(dtype)
     # Rounded to fp32 and then to 16 bits a product can end on the far side of a border between two results that its
     # fp32 value lies on.  A product that is not an fp32 number is therefore taken as the neighbour with an odd last bit,
-    # which no border has.  Its rest is exact: the scale's upper 16 and lower 8 bits times a code are fp32 numbers.
-    s, v = s.detach(), values.detach()
-    high = (s.contiguous().view(torch.int32) & ~0xff).view(torch.float32)
-    rest = torch.addcmul(-v, codes, high).addcmul_(codes, s - high)
-    bits = v.view(torch.int32)
-    even = (bits & 1 == 0) & (rest != 0) & torch.isfinite(v)
-    outward = torch.where((rest > 0) == (v > 0), 1, -1).to(torch.int32)
-    odd = (bits + outward).view(torch.float32)
-    return (values + torch.where(even, odd - v, 0.0)).to(dtype)
+    # which no border has.  (What lies below fp32's normal numbers is exact: no rest.)
+    v = values.detach()
+    rest = codes.double() * s.detach().double() - v.double()
+    beyond = torch.nextafter(v, torch.where(rest > 0, torch.inf, -torch.inf).to(v.dtype))
+    half = torch.frexp(v).mantissa * 2.0 ** 23  # of an odd last bit: no whole number
+    even = (half == torch.floor(half)) & (rest != 0) & torch.isfinite(v)
+    return (values + torch.where(even, beyond - v, 0.0)).to(dtype)
 
 
 def _pad_k(q: torch.Tensor, width: int) -> torch.Tensor:
