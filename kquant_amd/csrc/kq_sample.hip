@@ -504,7 +504,7 @@ __device__ __forceinline__ Row row_of(const Args& a, const Split& sp, int64_t r)
   // logits further than 32.25 t weigh less than 2^-46; the least one itself is within the range
   q.range = fmaxf(fminf(16.125f * (float)t, down(q, least) * 1.0001f), 1e-30f);
   q.to_bin = ((float)FAR_BIN - 0.5f) / q.range;
-  q.to_exp = (float)(-2.8853900817779268 / t);
+  q.to_exp = fmaxf((float)(-2.8853900817779268 / t), -3e38f);  // (the top's distance of 0 times an infinity were NaN)
   return q;
 }
 
