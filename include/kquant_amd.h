@@ -323,7 +323,8 @@ int kq_grouped_linear_dw(int dtype, const void* dy, int64_t lddy, const void* x,
 /* ---------------------------------------------------------- 8-bit integers -- */
 
 /* Rows as 8-bit integers with one scale a row (no kquant counterpart):
- *   scale[r] = max(fl(max_k |x[r][k]| fl(1 / 127)), 2^-126) in fp32,
+ *   scale[r] = max(fl(max_k |x[r][k]| fl(1 / 127)), 2^-126) in fp32 (at most one
+ *     step below the number nearest to max_k |x[r][k]| / 127),
  *   q[r][k] = the integer nearest to x[r][k] / scale[r], of two the even one,
  * of the exact quotient.  A row with an infinity or a NaN: scale NaN, codes 0.
  * dtype: KQ_DT_*; x [rows, k] (row stride ldx elements) and q (row stride ldq)
@@ -339,7 +340,7 @@ int kq_int8_dequantize(const int8_t* q, int64_t ldq, const float* scale, int64_t
 
 /* c = act(a_scale[m] w_scale[n] sum_k a[m][k] w[n][k] + bias) + residual over
  * 8-bit integers w [n, k] with an fp32 scale a row; int32 sums (exact), fp32
- * after them, rounded once to out_dtype (KQ_DT_*).  a_dtype KQ_DT_I8: a holds
+ * after them (times a_scale, then w_scale), rounded once to out_dtype (KQ_DT_*).  a_dtype KQ_DT_I8: a holds
  * codes with a_scale [m]; otherwise rows of that type, quantized as
  * kq_int8_quantize does (a_scale is not read).  activation, bias, residual as
  * kq_mx_linear_epilogue takes them, the residual of out_dtype (row stride ldr).

@@ -191,6 +191,8 @@ static hipError_t launch_few(const FewArgs& f, hipStream_t st) {
 //   64    1, 2 / 4, 1    61.3 / 34.5        119  / 65.6        617 / 275
 // The activations' reads (from L2) are shared by a workgroup's R blocks; its
 // workgroups have to cover the CUs (N = 4096: 19.7 with R 1 and 23.0 with R 4 at 32 rows).
+// (Results in bf16; 16 rows of 129280 in fp32 take 162.)  The borders in N are measured ones at K = 7168, not
+// sought between these columns: a shorter K gives each wave fewer windows, which no row of the table has.
 template <int DT, int OUT, bool TAIL>
 static hipError_t launch_few_rows(const FewArgs& f, hipStream_t st) {
   if constexpr (DT != DT_CODES) {

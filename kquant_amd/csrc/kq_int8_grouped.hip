@@ -52,7 +52,7 @@ static hipError_t grouped_few(const grouped::Args& g, int k, hipStream_t st) {
   return hipGetLastError();
 }
 
-// (48 groups of 4096 x 7168, us, and the tiles: 1 row 14, 45; 16 rows 75, 73; 64 rows 165, 193; 128 rows 183, 201; 192 rows 199, 204.)
+// (48 groups of 4096 x 7168, whole calls of bf16 rows, us, and the tiles; of the 165 the kernel is 154: 1 row 14, 45; 16 rows 75, 73; 64 rows 165, 193; 128 rows 183, 201; 192 rows 199, 204.)
 constexpr int FEW_EACH = 4;
 
 }  // namespace int8

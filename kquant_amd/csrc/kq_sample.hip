@@ -393,10 +393,16 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
 // from there in agent-scope accesses, all of which end before the count (a fence
 // would write each workgroup's L2 back).
 // A list longer than LIST (many equal logits at a cut) leaves the row to
-// whole_row.
-// What bounds it: at one row the launches and each one's chain of loads; at many
-// rows three passes over the logits, of 8 us each at 33 MB, and where many tokens
-// have weight their exponentials, some 26 instructions each.
+// whole_row, in one workgroup after the three launches: a bf16 row of 129280 equal
+// logits 1.25 ms with top-k or top-p, 2.4 with both (64 rows 2.5, 4.7); logits of 20
+// with a spread of 0.3, which are 1/8 apart, 0.65 ms with top-p (64 rows 1.2).
+// What bounds it, kernels in us.  One row of 129280: without cuts 3.5 + 8.9, with
+// 3.5 + 8 + 12 - 17, nearly all of the last ones the chain of dependent reads,
+// barriers and LDS steps of the row's last workgroup.  64 such rows (33 MB, 8 us to
+// read): stats 8.6; histogram 16 - 18; weigh 20 without cuts, 23 - 24 with lists of
+// some 50 tokens, 28 - 32 with longer ones, which the last workgroup sorts.  256 rows
+// of 65536 in bf16 without cuts 10 + 28, of which 16.8 M exponentials of some 26
+// instructions are about 11.
 constexpr int SLICE_T = T;
 static_assert(CHUNKS <= SLICE_T && CHUNK <= SLICE_T, "a thread for each chunk and each token of one");
 constexpr int NEAR = 1024;   // listed tokens that a workgroup gathers before they go to the list

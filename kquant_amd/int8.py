@@ -45,8 +45,8 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
         scale = max(max |x| * fp32(1 / 127), 2^-126),  q = round(x / scale)
 
-    with the product rounded to fp32 and the exact quotient rounded to nearest, ties to even, so the codes do
-    not depend on how the division is carried out.  A row with an infinity or a
+    with the product rounded to fp32 (at most one fp32 step below max |x| / 127 rounded once) and the exact quotient
+    rounded to nearest, ties to even, so the codes do not depend on how the division is carried out.  A row with an infinity or a
     NaN has scale NaN and codes 0: whatever it is multiplied with is NaN, and no
     other row is.  A row of zeros has codes 0.  The results carry no gradient.
     """

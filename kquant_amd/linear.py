@@ -255,7 +255,7 @@ def int8_linear(source: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor,
     once for all layers that read the rows) or bf16, fp16 or fp32 rows, which are
     quantized in the call by the same rule.
 
-    The integer sums are exact; scaling, bias [N] (bf16 or fp32), activation
+    The integer sums are exact; scaling (by the row's scale, then the channel's), bias [N] (bf16 or fp32), activation
     ("relu", "silu", "gelu", "gelu_tanh") and residual (of the result's shape and
     type) are fp32, rounded once.  The result is bf16, fp16 or fp32: ``out_dtype``,
     else the source's type, else (codes) bf16.  A row whose source holds an
