@@ -18,7 +18,8 @@ constexpr int64_t MAX_K = (1 << 17) - 16;  // the sums' bound, in whole 16-byte 
 
 // A row's scale from the largest magnitude's bits: its product with the fp32 number
 // nearest to 1 / 127, which is (1 - 2^-28) / 127, rounded once (within 9/16 of a step of
-// a 127th of the magnitude, one step below the nearest in some 4.5 % of rows), and at least 2^-126, so that quotients by it
+// a 127th of the magnitude, one step below the nearest in some 4.5 % of rows), and at
+// least 2^-126, so that quotients by it
 // need no subnormal scale.  A row with an infinity or a NaN has scale NaN (and
 // codes 0): what it multiplies is NaN, and no other row is.
 __device__ __forceinline__ float row_scale(uint32_t magnitude) {

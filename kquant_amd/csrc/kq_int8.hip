@@ -291,7 +291,6 @@ extern "C" int kq_int8_dequantize(const int8_t* q, int64_t ldq, const float* sca
   if (rows < 0 || k < 1 || ldq < k || ldo < k)
     return kq_fail(KQ_ERR_INVALID, "%s: need rows >= 0, k >= 1, row strides of at least k (rows=%lld k=%lld strides %lld, %lld)",
                    fn, (long long)rows, (long long)k, (long long)ldq, (long long)ldo);
-  if (rows > INT32_MAX / 2 || k > INT32_MAX / 2) return kq_fail(KQ_ERR_LIMIT, "%s: at most 2^30 rows and columns", fn);
   if (rows == 0) return KQ_OK;
   if (!q || !scale || !out) return kq_fail(KQ_ERR_INVALID, "%s: null buffer", fn);
   if (kq_misaligned(out, out_dtype == KQ_DT_F32 ? 4 : 2) || kq_misaligned(scale, 4))
