@@ -398,11 +398,12 @@ __global__ __launch_bounds__(T) void row_kernel(const Args a) {
 // with a spread of 0.3, which are 1/8 apart, 0.65 ms with top-p (64 rows 1.2).
 // What bounds it, kernels in us.  One row of 129280: without cuts 3.5 + 8.9, with
 // 3.5 + 8 + 12 - 17, nearly all of the last ones the chain of dependent reads,
-// barriers and LDS steps of the row's last workgroup.  64 such rows (33 MB, 8 us to
-// read): stats 8.6; histogram 16 - 18; weigh 20 without cuts, 23 - 24 with lists of
-// some 50 tokens, 28 - 32 with longer ones, which the last workgroup sorts.  256 rows
-// of 65536 in bf16 without cuts 10 + 28, of which 16.8 M exponentials of some 26
-// instructions are about 11.
+// barriers and LDS steps of the row's last workgroup.  64 such rows (33 MB, 8 to
+// read): stats 8.6; histogram 16 - 18; weigh 20 without cuts, 23 - 24 with top-k 50,
+// where few chunks hold a token that counts, 28 - 32 with top-k 1000 or top-p, where
+// most do: by difference some 5 are the exponentials (26 instructions each), 6 the last
+// workgroup's sums and draw, and 4 - 9 more its list.  256 rows of 65536 in bf16
+// without cuts 10 + 28, of which 16.8 M exponentials are about 11.
 constexpr int SLICE_T = T;
 static_assert(CHUNKS <= SLICE_T && CHUNK <= SLICE_T, "a thread for each chunk and each token of one");
 constexpr int NEAR = 1024;   // listed tokens that a workgroup gathers before they go to the list
